@@ -14,6 +14,7 @@ from .attention import (  # noqa: F401
     flash_attention_forward,
     qk_norm_rope,
 )
+from .cache import KVCache, cached_attention  # noqa: F401
 from .model import OlmoModel, ce_loss  # noqa: F401
 from ._capi import DTError, LIB_PATH  # noqa: F401
 
@@ -21,9 +22,11 @@ __all__ = [
     "Context",
     "DTError",
     "FlashAttentionResult",
+    "KVCache",
     "LIB_PATH",
     "OlmoAttention",
     "OlmoModel",
+    "cached_attention",
     "ce_loss",
     "default_context",
     "flash_attention_backward",

@@ -25,6 +25,10 @@ DT_BF16 = 1
 DT_MEM_DEVICE = 0
 DT_MEM_HOST = 1
 
+DT_KV_INT8 = 0
+DT_KV_FP8 = 1
+DT_KV_BF16 = 2
+
 DT_OPT_QKV_FUSED = 1
 DT_QKV_GEMM = 0
 DT_QKV_FUSED = 1
@@ -44,6 +48,7 @@ N_HEADS = 16
 
 _c_int = ctypes.c_int
 _vp = ctypes.c_void_p
+_i64 = ctypes.c_int64
 _fp = ctypes.POINTER(ctypes.c_float)
 _i32p = ctypes.POINTER(ctypes.c_int32)
 
@@ -82,6 +87,15 @@ SIGNATURES = {
     "dt_model_bwd": (_c_int, [_vp, _vp, _c_int, _vp]),
     "dt_model_step": (_c_int, [_vp, ctypes.c_float, _vp]),
     "dt_model_zero_grad": (_c_int, [_vp, _vp]),
+    "dt_kv_cache_create": (_c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, ctypes.POINTER(_vp)]),
+    "dt_kv_cache_destroy": (_c_int, [_vp]),
+    "dt_kv_cache_lengths": (_c_int, [_vp, _vp]),
+    "dt_kv_cache_truncate": (_c_int, [_vp, _c_int, _vp, _vp]),
+    "dt_kv_cache_append": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _i64, _i64, _vp, _vp, _c_int, _c_int, _vp]),
+    "dt_kv_cache_read": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _vp, _vp, _c_int, _c_int, _vp]),
+    "dt_cached_attn_workspace": (_c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _c_int, _c_int, _vp]),
+    "dt_cached_attn_fwd": (_c_int, [_vp] * 5 + [_c_int] * 4 + [_i64, ctypes.c_float, _c_int, _vp, _vp, _vp, _c_int, _vp,
+                                    _i64, _c_int, _c_int, _vp]),
     "dt_ce_loss": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _c_int, _vp]),
 }
 

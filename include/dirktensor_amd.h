@@ -375,6 +375,75 @@ int dt_model_zero_grad(dt_model* model, void* stream);
 int dt_ce_loss(dt_ctx* ctx, const float* logits, const int32_t* tokens, int B, int T, int V, int ignore_index,
                float* loss, float* d_logits, int mem, void* stream);
 
+/*
+ * Key/value cache: the keys and values of tokens that a program has answered with, kept on the device for
+ * dt_cached_attn_fwd. No reference counterpart (the reference recomputes whole sequences, OlmoModel.cpp:25-48).
+ *
+ * A cache has `slots` sequences of at most `capacity` (<= 1048576) tokens, n_heads key/value heads of 128 values. A
+ * row (the 128 values of one token and head) is held in the cache's format with one fp32 scale and stands for
+ * value * scale:
+ *   DT_KV_INT8  scale = amax / 127; value = x / scale to the nearest whole number, ties to even
+ *   DT_KV_FP8   scale = the smallest power of two >= 2^-126 with amax / scale <= 448; value = x / scale as OCP
+ *               e4m3, ties to even (where that would stand for more than fp32's range, the largest that does not)
+ *   DT_KV_BF16  x as bf16
+ * A row that holds an infinity or a NaN (DT_KV_BF16: also one whose rounding is infinite) reads back as NaN in all its
+ * places, and a query that sees it gets NaN. Rows of zeros are held exactly.
+ * The lengths of the slots are host state of the handle: the calls below read and advance them when they are made,
+ * whether or not their stream has run. A captured graph repeats the positions that held at its capture, and does not
+ * advance them. Calls on one cache must be ordered, like those on a context (dt_ctx); attention calls that only
+ * read a cache (as their own or as prefix) may run at the same time, each with a workspace of its own. Destroy a cache
+ * before its context.
+ */
+#define DT_KV_INT8 0
+#define DT_KV_FP8 1
+#define DT_KV_BF16 2
+typedef struct dt_kv_cache dt_kv_cache;
+int dt_kv_cache_create(dt_ctx* ctx, int slots, int capacity, int n_heads, int D, int format, dt_kv_cache** out);
+int dt_kv_cache_destroy(dt_kv_cache* cache);
+/* the tokens held by each slot, [slots] */
+int dt_kv_cache_lengths(const dt_kv_cache* cache, int32_t* lengths);
+/* shortens B slots (slots NULL: 0 .. B-1) to lengths[b], at most what they hold; 0 frees a slot for another sequence */
+int dt_kv_cache_truncate(dt_kv_cache* cache, int B, const int32_t* slots, const int32_t* lengths);
+/*
+ * Quantises T tokens' keys and values and writes them behind what the slots hold.
+ *   k, v    : B x T tokens of n_heads*128 values in dtype, tokens ldk / ldv elements apart (a column block of a
+ *             projection's output may be passed as it is)
+ *   slots   : the slot of each batch row (host, B distinct values), or NULL for 0 .. B-1
+ *   counts  : how many of its T tokens each batch row appends (host, 0 .. T), or NULL for all T
+ * 1 <= B <= 256. Tokens that do not fit the capacity are refused (DT_ERR_INVALID_ARG) before anything is written.
+ */
+int dt_kv_cache_append(dt_kv_cache* cache, const void* k, const void* v, int B, int T, int64_t ldk, int64_t ldv,
+                       const int32_t* slots, const int32_t* counts, int dtype, int mem, void* stream);
+/* Reads T tokens from position starts[b] (NULL: 0) of B slots back as the values they stand for, rounded to dtype:
+ * k, v [B, T, n_heads, 128]. All of them must be held. */
+int dt_kv_cache_read(dt_kv_cache* cache, void* k, void* v, int B, int T, const int32_t* slots, const int32_t* starts,
+                     int dtype, int mem, void* stream);
+
+/*
+ * Attention of the newest tokens over a cache (the cached form of flash_attention_forward, FlashAttention.h:15-21).
+ *   q, o    : [B, T, H, 128] in dtype, q's tokens ldq elements apart; H a multiple of the cache's heads: query head h
+ *             reads key/value head h / (H / n_heads)
+ *   m, l    : [B, T, H] fp32 as in dt_flash_attn_fwd, or NULL
+ *   causal  : 1: the counts[b] query tokens of batch row b are the newest of its slot, token t sees the keys at
+ *             positions < length - counts[b] + t + 1; 0: every query sees all keys of the slot
+ *   slots   : the slot of each batch row (host; the same slot may serve several rows), or NULL for 0 .. B-1
+ *   counts  : query tokens of each batch row (host, 0 .. T), NULL for all T; rows t >= counts[b] are written as the
+ *             empty row (O = 0, m = -inf, l = 0), like every row that sees no key
+ *   prefix  : NULL, or a cache (of the same context, format and heads; may be `cache` itself) whose slot prefix_slot
+ *             holds tokens that come before every sequence of the batch: each query sees all of them. They are read
+ *             once for the whole batch.
+ *   ws      : a device workspace of at least dt_cached_attn_workspace bytes for the same arguments (0: none is needed),
+ *             16-byte aligned, not shared with a call that may run at the same time. Ignored with DT_MEM_HOST.
+ * 1 <= B <= 256, 1 <= T <= 8192. Deterministic: the same call gives the same bits.
+ */
+int dt_cached_attn_workspace(const dt_kv_cache* cache, int B, int T, int H, int D, const int32_t* slots,
+                             const int32_t* counts, const dt_kv_cache* prefix, int prefix_slot, int dtype,
+                             int64_t* bytes);
+int dt_cached_attn_fwd(dt_kv_cache* cache, const void* q, void* o, float* m, float* l, int B, int T, int H, int D,
+                       int64_t ldq, float scale, int causal, const int32_t* slots, const int32_t* counts,
+                       const dt_kv_cache* prefix, int prefix_slot, void* ws, int64_t ws_bytes, int dtype, int mem,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif
