@@ -15,6 +15,7 @@ from .attention import (  # noqa: F401
     qk_norm_rope,
 )
 from .cache import KVCache, cached_attention  # noqa: F401
+from .logprobs import TokenLogprobs, token_logprobs, token_logprobs_backward  # noqa: F401
 from .model import OlmoModel, ce_loss  # noqa: F401
 from ._capi import DTError, LIB_PATH  # noqa: F401
 
@@ -26,10 +27,13 @@ __all__ = [
     "LIB_PATH",
     "OlmoAttention",
     "OlmoModel",
+    "TokenLogprobs",
     "cached_attention",
     "ce_loss",
     "default_context",
     "flash_attention_backward",
     "flash_attention_forward",
     "qk_norm_rope",
+    "token_logprobs",
+    "token_logprobs_backward",
 ]

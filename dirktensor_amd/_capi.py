@@ -25,6 +25,8 @@ DT_BF16 = 1
 DT_MEM_DEVICE = 0
 DT_MEM_HOST = 1
 
+DT_NO_IGNORE = -(2**63)
+
 DT_KV_INT8 = 0
 DT_KV_FP8 = 1
 DT_KV_BF16 = 2
@@ -96,6 +98,11 @@ SIGNATURES = {
     "dt_cached_attn_workspace": (_c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _c_int, _c_int, _vp]),
     "dt_cached_attn_fwd": (_c_int, [_vp] * 5 + [_c_int] * 4 + [_i64, ctypes.c_float, _c_int, _vp, _vp, _vp, _c_int, _vp,
                                     _i64, _c_int, _c_int, _vp]),
+    "dt_token_logprobs_workspace": (_c_int, [_c_int, _c_int, _c_int, _c_int, _vp]),
+    "dt_token_logprobs": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _i64, _i64, _c_int, _i64, _c_int] + [_vp] * 7
+                          + [_i64, _c_int, _c_int, _vp]),
+    "dt_token_logprobs_bwd": (_c_int, [_vp] * 8 + [_c_int, _c_int, _c_int, _i64, _i64, _c_int, _i64, _vp, _i64, _i64, _c_int,
+                                                   _c_int, _vp]),
     "dt_ce_loss": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _c_int, _vp]),
 }
 

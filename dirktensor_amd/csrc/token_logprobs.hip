@@ -1,0 +1,738 @@
+// Log probabilities of given tokens, with each row's entropy and most likely tokens, and the gradient of the
+// log probabilities and entropies with respect to the logits.
+//
+// For a row x of V logits and its token y, with m = max x, e_j = exp(x_j - m), l = sum e_j:
+//   logprob = (x_y - m) - log l
+//   entropy = log l - sum e_j (x_j - m) / l      (both terms >= 0: no difference of large numbers)
+//   dx_j    = g (delta_jy - p_j) - h p_j (log p_j + entropy),   p_j = exp((x_j - m) - log l)
+// for d logprob = g, d entropy = h. The top alternatives are the k largest logits, the lower index first of equals.
+//
+// Both are bound by HBM: the forward reads the logits once, the backward reads them and writes as many.
+//
+// Forward: a workgroup of 256 threads streams a row (or, where there are few rows, a segment of one) with 16-byte loads;
+// a thread keeps its own running maximum, sum and weighted sum and remembers which of its batches of 16 values the
+// maximum came from, so the loop has no exchange between lanes. The statistics meet once at the end. The alternatives cost
+// no second pass: with the threads' maxima ranked, the k-th largest is a bound that the k largest values reach, and
+// every value that reaches it belongs to one of those k threads. Only these threads' values are read again (about k of 256
+// runs, from L2), those that reach the bound (a few more than k) are collected in LDS, and each takes the place
+// that the number of larger ones gives it. Keys are (value, index) pairs, so no two are equal, ties go to the lower index and the
+// order of the collection does not matter. A row cut into segments leaves (m, l, sum, k keys) of each in the workspace and a
+// second kernel joins them by the same selection.
+
+#include "dt_internal.h"
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+namespace dt {
+namespace {
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
+typedef u32x4 u32x4_at4 __attribute__((aligned(4)));
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int kMaxTop = 64;
+constexpr int kList = 1024;          // values that may reach the bound before the slow selection takes over
+constexpr int kBatch = 16;           // values a thread takes at a time
+constexpr int kMinSegment = 2048;    // values of a segment at least
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2eLo = 1.92596303e-8f;  // log2 e - kLog2e
+constexpr float kLn2 = 0.693147180559945f;
+constexpr float kNegInf = -__builtin_huge_valf();
+
+struct LogprobArgs {
+    const void* x;
+    const void* tok;
+    int64_t ldb, ldt;     // strides of x, elements
+    int64_t ignore;
+    int tok64;
+    int T, V, k;
+    int segments, seg_len;
+    float* logprob;
+    float* entropy;       // nullable
+    float* m;
+    float* l;
+    int32_t* top_index;   // [rows][k]
+    float* top_logprob;
+    float* part;          // [rows][segments][4]: m, l, weighted sum
+    uint64_t* part_key;   // [rows][segments][k], sorted
+};
+
+__device__ __forceinline__ int64_t token_at(const void* tok, int tok64, int64_t row) {
+    return tok64 ? static_cast<const int64_t*>(tok)[row] : static_cast<const int32_t*>(tok)[row];
+}
+
+// (value, index) as a number that orders like the pair, the lower index above; NaN counts as -inf. Never 0.
+__device__ __forceinline__ uint32_t order_of(float x) {
+    x = x != x ? kNegInf : x + 0.0f;  // (-0 and 0 are equal)
+    const uint32_t u = __float_as_uint(x);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t key_of(float x, int index) {
+    return static_cast<uint64_t>(order_of(x)) << 32 | static_cast<uint32_t>(~index);
+}
+__device__ __forceinline__ float key_value(uint64_t key) {
+    const uint32_t u = static_cast<uint32_t>(key >> 32);
+    return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+__device__ __forceinline__ int key_index(uint64_t key) { return static_cast<int>(~static_cast<uint32_t>(key)); }
+
+// A run of n values of a row in 16-byte pieces from its first value on, whatever its alignment (global 16-byte accesses
+// take any, and a row's bits then do not depend on where it lies), single values after the last whole piece. Piece p belongs to
+// thread p % 256; a thread's batch j is its pieces 256 (j kPer + 0 .. kPer - 1) + tid; value tid of those behind the
+// pieces is its batch `batches`. A thread's batches ascend in index.
+template <bool kBf16>
+struct Run {
+    static constexpr int kEs = kBf16 ? 2 : 4, kPiece = 16 / kEs, kPer = kBatch / kPiece;
+    using Piece = std::conditional_t<kBf16, u32x4_at2, u32x4_at4>;
+    const uint8_t* x;  // the run's first value
+    int n, pieces, batches;
+    __device__ __forceinline__ Run(const void* p, int n_) : x(static_cast<const uint8_t*>(p)), n(n_) {
+        pieces = n / kPiece;
+        batches = (pieces + kThreads * kPer - 1) / (kThreads * kPer);
+    }
+    __device__ __forceinline__ float one(int i) const {
+        if constexpr (kBf16) return __uint_as_float(static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(x)[i]) << 16);
+        return reinterpret_cast<const float*>(x)[i];
+    }
+    __device__ __forceinline__ int tail() const { return pieces * kPiece; }
+    __device__ __forceinline__ u32x4 load(int p) const { return *reinterpret_cast<const Piece*>(x + p * 16); }
+    static __device__ __forceinline__ void unpack(const u32x4& w, float* v) {
+        if constexpr (kBf16) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
+        }
+    }
+};
+
+struct Stats {
+    float m = kNegInf, s = 0.0f, d = 0.0f;  // maximum; sum e; sum e (x - m)
+    int batch = -1;                         // where the maximum was first met
+};
+
+template <int kN>
+__device__ __forceinline__ void take(Stats& st, const float (&v)[kN], int n, int batch) {
+    float bm = kNegInf;
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+        if (i < n) bm = fmaxf(bm, v[i]);
+    if (st.batch == -1) st.batch = batch;  // (a thread whose values are all -inf has its first one as its best)
+    if (bm > st.m) {
+        const float f = __builtin_amdgcn_exp2f((st.m - bm) * kLog2e);
+        st.d = (st.d + st.s * fmaxf(st.m - bm, -1e4f)) * f;  // (further down f is 0: the sum must not become an infinity)
+        st.s *= f;
+        st.m = bm;
+        st.batch = batch;
+    }
+    const float base = st.m == kNegInf ? 0.0f : st.m;
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+        if (i < n) {
+            const float t = v[i] - base;
+            // (log2 e in two parts: the first alone is off by 1.3e-8, the same way for every term)
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(t, kLog2e, t * kLog2eLo));
+            st.s += e;
+            st.d += e * fmaxf(t, -1e4f);  // (0 for -inf; a NaN shows in s)
+        }
+}
+
+// a's statistics and b's; the batch is a's
+__device__ __forceinline__ void join(Stats& a, float m, float s, float d) {
+    const float mx = fmaxf(a.m, m), base = mx == kNegInf ? 0.0f : mx;
+    const float fa = __builtin_amdgcn_exp2f((a.m - base) * kLog2e), fb = __builtin_amdgcn_exp2f((m - base) * kLog2e);
+    a.d = (a.d + a.s * fmaxf(a.m - base, -1e4f)) * fa + (d + s * fmaxf(m - base, -1e4f)) * fb;
+    a.s = a.s * fa + s * fb;
+    a.m = mx;
+}
+
+// the same total in every thread of the workgroup
+__device__ __forceinline__ Stats join_block(Stats st, float (*buf)[3]) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        // (both lanes of a pair join lower first, so they agree to the bit)
+        const float m = __shfl_xor(st.m, o, 64), s = __shfl_xor(st.s, o, 64), d = __shfl_xor(st.d, o, 64);
+        if (threadIdx.x & o) {
+            Stats lower;
+            lower.m = m, lower.s = s, lower.d = d;
+            join(lower, st.m, st.s, st.d);
+            st.m = lower.m, st.s = lower.s, st.d = lower.d;
+        } else {
+            join(st, m, s, d);
+        }
+    }
+    if ((threadIdx.x & 63) == 0) {
+        float* b = buf[threadIdx.x >> 6];
+        b[0] = st.m, b[1] = st.s, b[2] = st.d;
+    }
+    __syncthreads();
+    Stats all;
+    all.m = buf[0][0], all.s = buf[0][1], all.d = buf[0][2];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) join(all, buf[w][0], buf[w][1], buf[w][2]);
+    return all;
+}
+
+struct Finish {
+    float m, l, logl, nan;
+};
+// (a row of nothing but -inf has no distribution: NaN)
+__device__ __forceinline__ Finish finish(const LogprobArgs& a, int64_t row, const void* xrow, bool bf16, const Stats& st, bool write) {
+    Finish f;
+    f.m = st.m;
+    f.l = st.m == kNegInf ? __builtin_nanf("") : st.s;
+    f.logl = logf(f.l);
+    if (f.l != f.l) f.m = f.l;  // (a maximum passes NaN over)
+    if (!write) return f;
+    a.m[row] = f.m;
+    a.l[row] = f.l;
+    if (a.entropy) a.entropy[row] = f.logl - st.d / f.l;
+    const int64_t y = token_at(a.tok, a.tok64, row);
+    float lp = 0.0f;
+    if (y != a.ignore) {
+        if (y < 0 || y >= a.V) lp = __builtin_nanf("");
+        else {
+            const float x = bf16 ? __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(xrow)[y]) << 16)
+                                 : static_cast<const float*>(xrow)[y];
+            lp = (x - f.m) - f.logl;
+        }
+    }
+    a.logprob[row] = lp;
+    return f;
+}
+
+struct SelectBuf {
+    union {
+        uint64_t rank[kThreads];
+        uint64_t list[kList];
+    };
+    int owner[kMaxTop];
+    uint64_t best[kWaves];
+    int count;
+    uint64_t bound;
+};
+
+// The k largest keys of the workgroup's values, in order, through out(place, key); places past the last value get key 0. `mine` is
+// the thread's largest key (0: none); each(owner, lane, f) calls f(key) for the values of thread `owner` that fall to a
+// lane of the wave that asks, and all lanes of a wave call it together.
+template <class Each, class Out>
+__device__ __forceinline__ void select(SelectBuf& b, uint64_t mine, int k, Each each, Out out) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __syncthreads();
+    b.rank[tid] = mine;
+    if (tid == 0) b.count = 0, b.bound = 0;
+    if (tid < kMaxTop) b.owner[tid] = -1;
+    __syncthreads();
+    if (mine != 0) {
+        int larger = 0;
+#pragma unroll 8
+        for (int i = 0; i < kThreads; ++i) larger += b.rank[i] > mine;
+        if (larger < k) b.owner[larger] = tid;
+        if (larger == k - 1) b.bound = mine;
+    }
+    __syncthreads();
+    const uint64_t bound = b.bound;
+    for (int r = wave; r < k; r += kWaves) {
+        const int o = b.owner[r];
+        if (o < 0) continue;
+        each(o, lane, [&](uint64_t key) {
+            if (key < bound) return;
+            const int at = atomicAdd(&b.count, 1);
+            if (at < kList) b.list[at] = key;
+        });
+    }
+    __syncthreads();
+    const int c = b.count;
+    if (c <= kList) {
+        for (int i = tid; i < c; i += kThreads) {
+            const uint64_t key = b.list[i];
+            int larger = 0;
+#pragma unroll 4
+            for (int j = 0; j < c; ++j) larger += b.list[j] > key;
+            if (larger < k) out(larger, key);
+        }
+        for (int i = c + tid; i < k; i += kThreads) out(i, 0);
+        return;
+    }
+    // one after another: the largest key below the last
+    uint64_t last = ~uint64_t(0);
+    for (int r = 0; r < k; ++r) {
+        uint64_t top = 0;
+        for (int i = wave; i < k; i += kWaves) {
+            const int o = b.owner[i];
+            if (o < 0) continue;
+            each(o, lane, [&](uint64_t key) {
+                if (key < last && key > top) top = key;
+            });
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint64_t other = __shfl_xor(static_cast<unsigned long long>(top), o, 64);
+            top = other > top ? other : top;
+        }
+        __syncthreads();
+        if (lane == 0) b.best[wave] = top;
+        __syncthreads();
+        last = b.best[0];
+        for (int w = 1; w < kWaves; ++w) last = b.best[w] > last ? b.best[w] : last;
+        if (tid == 0) out(r, last);
+    }
+}
+
+__device__ __forceinline__ void write_top(const LogprobArgs& a, int64_t row, int place, uint64_t key, const Finish& f) {
+    a.top_index[row * a.k + place] = key_index(key);
+    a.top_logprob[row * a.k + place] = (key_value(key) - f.m) - f.logl;
+}
+
+template <bool kBf16, bool kTop>
+__global__ __launch_bounds__(kThreads) void logprob_rows_kernel(LogprobArgs a) {
+    __shared__ float sbuf[kWaves][3];
+    __shared__ SelectBuf buf;
+    using R = Run<kBf16>;
+    const int tid = threadIdx.x;
+    const int64_t row = blockIdx.x / a.segments;
+    const int seg = static_cast<int>(blockIdx.x - row * a.segments);
+    const uint8_t* xrow = static_cast<const uint8_t*>(a.x) + ((row / a.T) * a.ldb + (row % a.T) * a.ldt) * R::kEs;
+    const int first = seg * a.seg_len;
+    const R run(xrow + static_cast<int64_t>(first) * R::kEs, min(a.V - first, a.seg_len));
+
+    Stats st;
+    int j = 0;
+    // whole batches, the next one's loads in flight while one is summed
+    const int whole = run.pieces / (kThreads * R::kPer);
+    u32x4 w[R::kPer];
+    if (whole > 0) {
+#pragma unroll
+        for (int i = 0; i < R::kPer; ++i) w[i] = run.load(i * kThreads + tid);
+    }
+    for (; j < whole; ++j) {
+        float v[kBatch];
+#pragma unroll
+        for (int i = 0; i < R::kPer; ++i) R::unpack(w[i], v + i * R::kPiece);
+        if (j + 1 < whole) {
+#pragma unroll
+            for (int i = 0; i < R::kPer; ++i) w[i] = run.load(((j + 1) * R::kPer + i) * kThreads + tid);
+        }
+        take(st, v, kBatch, j);
+    }
+    for (; j < run.batches; ++j) {
+        float v[kBatch];
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < R::kPer; ++i) {
+            const int p = (j * R::kPer + i) * kThreads + tid;
+            if (p < run.pieces) {
+                R::unpack(run.load(p), v + i * R::kPiece);
+                n = (i + 1) * R::kPiece;
+            }
+        }
+        if (n > 0) take(st, v, n, j);
+    }
+    if (run.tail() + tid < run.n) {
+        const float v[1] = {run.one(run.tail() + tid)};
+        take(st, v, 1, run.batches);
+    }
+
+    uint64_t mine = 0;
+    if constexpr (kTop) {
+        // the first value of the thread's best batch that equals its maximum
+        const uint32_t top = order_of(st.m);
+        if (st.batch == run.batches) mine = key_of(st.m, first + run.tail() + tid);
+        else if (st.batch >= 0) {
+#pragma unroll
+            for (int i = R::kPer - 1; i >= 0; --i) {
+                const int p = (st.batch * R::kPer + i) * kThreads + tid;
+                if (p < run.pieces) {
+                    float v[R::kPiece];
+                    R::unpack(run.load(p), v);
+#pragma unroll
+                    for (int q = R::kPiece - 1; q >= 0; --q)
+                        if (order_of(v[q]) == top) mine = key_of(st.m, first + p * R::kPiece + q);
+                }
+            }
+        }
+    }
+    const Stats all = join_block(st, sbuf);
+    Finish f{};
+    if (a.segments == 1) f = finish(a, row, xrow, kBf16, all, tid == 0);
+    else if (tid == 0) {
+        float* p = a.part + (row * a.segments + seg) * 4;
+        p[0] = all.m, p[1] = all.s, p[2] = all.d;
+    }
+    if constexpr (kTop) {
+        select(
+            buf, mine, a.k,
+            [&](int o, int lane, auto&& use) {
+                for (int p = o + lane * kThreads; p < run.pieces; p += 64 * kThreads) {
+                    float v[R::kPiece];
+                    R::unpack(run.load(p), v);
+#pragma unroll
+                    for (int q = 0; q < R::kPiece; ++q) use(key_of(v[q], first + p * R::kPiece + q));
+                }
+                if (lane == 0 && run.tail() + o < run.n) use(key_of(run.one(run.tail() + o), first + run.tail() + o));
+            },
+            [&](int place, uint64_t key) {
+                if (a.segments == 1) write_top(a, row, place, key, f);
+                else a.part_key[(row * a.segments + seg) * a.k + place] = key;
+            });
+    }
+}
+
+// Joins a row's segments.
+template <bool kBf16>
+__global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
+    __shared__ float sbuf[kWaves][3];
+    __shared__ SelectBuf buf;
+    const int tid = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    const uint8_t* xrow = static_cast<const uint8_t*>(a.x) + ((row / a.T) * a.ldb + (row % a.T) * a.ldt) * (kBf16 ? 2 : 4);
+    Stats st;
+    if (tid < a.segments) {  // (at most kThreads of them)
+        const float* p = a.part + (row * a.segments + tid) * 4;
+        st.m = p[0], st.s = p[1], st.d = p[2];
+    }
+    const Stats all = join_block(st, sbuf);
+    const Finish f = finish(a, row, xrow, kBf16, all, tid == 0);
+    if (a.k == 0) return;
+    const uint64_t* keys = a.part_key + row * a.segments * a.k;
+    const int n = a.segments * a.k;
+    uint64_t mine = 0;
+    for (int i = tid; i < n; i += kThreads) mine = keys[i] > mine ? keys[i] : mine;
+    select(
+        buf, mine, a.k,
+        [&](int o, int lane, auto&& use) {
+            for (int i = o + lane * kThreads; i < n; i += 64 * kThreads)
+                if (keys[i] != 0) use(keys[i]);
+        },
+        [&](int place, uint64_t key) { write_top(a, row, place, key, f); });
+}
+
+// Segments a row: enough workgroups to fill the CUs several times, none shorter than kMinSegment, their keys a few a thread.
+void cut(int64_t rows, int V, int k, int* segments, int* seg_len) {
+    constexpr int64_t kTarget = 2048;
+    int64_t s = std::min<int64_t>((kTarget + rows - 1) / rows, (V + kMinSegment - 1) / kMinSegment);
+    s = std::min<int64_t>(s, kThreads);
+    if (k > 0) s = std::min<int64_t>(s, 4096 / k);
+    s = std::max<int64_t>(s, 1);
+    *seg_len = static_cast<int>(((V + s - 1) / s + 7) / 8 * 8);
+    *segments = (V + *seg_len - 1) / *seg_len;
+}
+
+int64_t workspace_bytes(int64_t rows, int V, int k) {
+    int segments = 0, len = 0;
+    cut(rows, V, k, &segments, &len);
+    return segments == 1 ? 0 : rows * segments * (4 * static_cast<int64_t>(sizeof(float)) + k * static_cast<int64_t>(sizeof(uint64_t)));
+}
+
+int launch_logprobs(LogprobArgs a, int64_t rows, bool bf16, void* ws, hipStream_t s) {
+    cut(rows, a.V, a.k, &a.segments, &a.seg_len);
+    // (keys first: they are the wider)
+    a.part_key = static_cast<uint64_t*>(ws);
+    a.part = reinterpret_cast<float*>(a.part_key + rows * a.segments * a.k);
+    const dim3 g(static_cast<unsigned>(rows * a.segments)), t(kThreads);
+    if (bf16) {
+        if (a.k) hipLaunchKernelGGL((logprob_rows_kernel<true, true>), g, t, 0, s, a);
+        else hipLaunchKernelGGL((logprob_rows_kernel<true, false>), g, t, 0, s, a);
+    } else {
+        if (a.k) hipLaunchKernelGGL((logprob_rows_kernel<false, true>), g, t, 0, s, a);
+        else hipLaunchKernelGGL((logprob_rows_kernel<false, false>), g, t, 0, s, a);
+    }
+    DT_HIP_TRY(hipGetLastError());
+    if (a.segments > 1) {
+        if (bf16) hipLaunchKernelGGL((logprob_join_kernel<true>), dim3(static_cast<unsigned>(rows)), t, 0, s, a);
+        else hipLaunchKernelGGL((logprob_join_kernel<false>), dim3(static_cast<unsigned>(rows)), t, 0, s, a);
+        DT_HIP_TRY(hipGetLastError());
+    }
+    return DT_OK;
+}
+
+struct LogprobBwdArgs {
+    const void* x;
+    void* dx;
+    const void* tok;
+    const float* g;
+    const float* h;  // nullable
+    const float* m;
+    const float* l;
+    const float* entropy;
+    int64_t ldb, ldt, ldb_out, ldt_out;
+    int64_t ignore;
+    int tok64;
+    int T, V;
+    int segments, seg_len;
+};
+
+// One workgroup a segment of a row; each value is read and written by one thread, so dx may be x.
+template <bool kBf16>
+__global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(LogprobBwdArgs a) {
+    using R = Run<kBf16>;
+    const int tid = threadIdx.x;
+    const int64_t row = blockIdx.x / a.segments;
+    const int first = static_cast<int>(blockIdx.x - row * a.segments) * a.seg_len;
+    const int n = min(a.V - first, a.seg_len);
+    const int64_t b = row / a.T, t = row % a.T;
+    const uint8_t* x = static_cast<const uint8_t*>(a.x) + (b * a.ldb + t * a.ldt + first) * R::kEs;
+    uint8_t* dx = static_cast<uint8_t*>(a.dx) + (b * a.ldb_out + t * a.ldt_out + first) * R::kEs;
+    const int64_t y = token_at(a.tok, a.tok64, row);
+    float g = a.g[row];
+    int hit = -1;
+    if (y == a.ignore) g = 0.0f;
+    else if (y < 0 || y >= a.V) g = __builtin_nanf("");
+    else if (y >= first && y < first + n) hit = static_cast<int>(y) - first;
+    const float h = a.h ? a.h[row] : 0.0f;
+    const float m = a.m[row], logl = logf(a.l[row]);
+    const float ent = a.h ? a.entropy[row] : 0.0f;
+    auto grad = [&](float v, int i) {
+        const float lp = (v - m) - logl;
+        // exp(lp) with what the product with log2 e rounds away (2^-24 of it: 2e-6 of p at lp = -20) put back
+        const float t2 = lp * kLog2e;
+        const float lo = __builtin_fmaf(lp, kLog2eLo, __builtin_fmaf(lp, kLog2e, -t2));
+        const float e = __builtin_amdgcn_exp2f(t2);
+        const float p = lp < -200.0f ? 0.0f : __builtin_fmaf(e, lo * kLn2, e);  // (-inf, and where the remainder would be none)
+        float d = -p * (g + h * (lp + ent));
+        if (p == 0.0f && g == g) d = 0.0f;  // (log p may be -inf)
+        if (i == hit) d += g;
+        return d;
+    };
+    auto put = [&](int i, float d) {
+        if constexpr (kBf16) reinterpret_cast<uint16_t*>(dx)[i] = static_cast<uint16_t>(__builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2){d, 0.0f}, bf16x2)));
+        else reinterpret_cast<float*>(dx)[i] = d;
+    };
+    const R run(x, n);
+    const int tl = run.tail() + tid;
+    if (tl < n) put(tl, grad(run.one(tl), tl));
+#pragma unroll 4
+    for (int p = tid; p < run.pieces; p += kThreads) {
+        const u32x4 w = run.load(p);
+        const int at = p * R::kPiece;
+        float v[R::kPiece];
+        R::unpack(w, v);
+        u32x4 o;
+#pragma unroll
+        for (int i = 0; i < R::kPiece; ++i) v[i] = grad(v[i], at + i);
+        if constexpr (kBf16) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2){v[2 * i], v[2 * i + 1]}, bf16x2));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = __float_as_uint(v[i]);
+        }
+        *reinterpret_cast<typename R::Piece*>(dx + p * 16) = o;
+    }
+}
+
+int launch_logprobs_bwd(LogprobBwdArgs a, int64_t rows, bool bf16, hipStream_t s) {
+    // segments of 8192 values, so that few rows fill the CUs too and many leave no long tail
+    a.seg_len = 8192;
+    a.segments = (a.V + a.seg_len - 1) / a.seg_len;
+    const int64_t grid = rows * a.segments;
+    if (grid > 0x7fffff) return set_error(DT_ERR_UNSUPPORTED, "%lld rows of %d logits need %lld workgroups", (long long)rows, a.V, (long long)grid);
+    if (bf16) hipLaunchKernelGGL((logprob_bwd_kernel<true>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, s, a);
+    else hipLaunchKernelGGL((logprob_bwd_kernel<false>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, s, a);
+    DT_HIP_TRY(hipGetLastError());
+    return DT_OK;
+}
+
+int check_logits(int B, int T, int V, int64_t ldb, int64_t ldt, int token_bytes, int dtype, int mem) {
+    if (B < 1 || T < 1 || V < 1) return set_error(DT_ERR_INVALID_ARG, "B=%d, T=%d, V=%d must be >= 1", B, T, V);
+    if (V > (1 << 24)) return set_error(DT_ERR_UNSUPPORTED, "V=%d exceeds %d", V, 1 << 24);
+    if (static_cast<int64_t>(B) * T > 0x7fffff) return set_error(DT_ERR_UNSUPPORTED, "%lld rows", (long long)B * T);
+    if (ldb < 0 || ldt < 0) return set_error(DT_ERR_INVALID_ARG, "strides %lld, %lld must be >= 0", (long long)ldb, (long long)ldt);
+    if (token_bytes != 4 && token_bytes != 8) return set_error(DT_ERR_INVALID_ARG, "token_bytes=%d must be 4 or 8", token_bytes);
+    if (dtype != DT_FP32_EXACT && dtype != DT_BF16) return set_error(DT_ERR_INVALID_ARG, "unknown dtype %d", dtype);
+    if (mem != DT_MEM_DEVICE && mem != DT_MEM_HOST) return set_error(DT_ERR_INVALID_ARG, "unknown mem %d", mem);
+    return DT_OK;
+}
+
+int check_host_tokens(const void* tok, int token_bytes, int64_t rows, int V, int64_t ignore) {
+    for (int64_t i = 0; i < rows; ++i) {
+        const int64_t y = token_bytes == 8 ? static_cast<const int64_t*>(tok)[i] : static_cast<const int32_t*>(tok)[i];
+        if (y != ignore && (y < 0 || y >= V))
+            return set_error(DT_ERR_INVALID_ARG, "token %lld of row %lld outside [0, %d)", (long long)y, (long long)i, V);
+    }
+    return DT_OK;
+}
+
+// copies B x T rows of host logits into a staging buffer, densely
+int stage_rows(void* dst, const void* src, int B, int T, int V, int64_t ldb, int64_t ldt, size_t es, hipStream_t s) {
+    if ((T == 1 || ldt == V) && (B == 1 || ldb == static_cast<int64_t>(T) * V)) {
+        DT_HIP_TRY(hipMemcpyAsync(dst, src, static_cast<size_t>(B) * T * V * es, hipMemcpyHostToDevice, s));
+        return DT_OK;
+    }
+    for (int b = 0; b < B; ++b)
+        for (int t = 0; t < T; ++t)
+            DT_HIP_TRY(hipMemcpyAsync(static_cast<uint8_t*>(dst) + (static_cast<size_t>(b) * T + t) * V * es,
+                                      static_cast<const uint8_t*>(src) + (b * ldb + t * ldt) * es, V * es, hipMemcpyHostToDevice, s));
+    return DT_OK;
+}
+
+}  // namespace
+}  // namespace dt
+
+using namespace dt;
+
+extern "C" {
+
+int dt_token_logprobs_workspace(int B, int T, int V, int top_k, int64_t* bytes) {
+    clear_error();
+    if (!bytes) return set_error(DT_ERR_INVALID_ARG, "bytes is NULL");
+    DT_TRY(check_logits(B, T, V, 0, 0, 4, DT_BF16, DT_MEM_DEVICE));
+    if (top_k < 0 || top_k > kMaxTop || top_k > V)
+        return set_error(DT_ERR_INVALID_ARG, "top_k=%d outside [0, %d]", top_k, std::min(kMaxTop, V));
+    *bytes = workspace_bytes(static_cast<int64_t>(B) * T, V, top_k);
+    return DT_OK;
+}
+
+int dt_token_logprobs(dt_ctx* ctx, const void* logits, const void* tokens, int B, int T, int V, int64_t ldb, int64_t ldt,
+                      int token_bytes, int64_t ignore_index, int top_k, float* logprob, float* entropy, float* m, float* l,
+                      int32_t* top_index, float* top_logprob, void* ws, int64_t ws_bytes, int dtype, int mem, void* stream) {
+    clear_error();
+    if (!logits || !tokens || !logprob || !m || !l)
+        return set_error(DT_ERR_INVALID_ARG, "logits, tokens, logprob, m and l must be non-NULL");
+    DT_TRY(check_logits(B, T, V, ldb, ldt, token_bytes, dtype, mem));
+    if (top_k < 0 || top_k > kMaxTop || top_k > V)
+        return set_error(DT_ERR_INVALID_ARG, "top_k=%d outside [0, %d]", top_k, std::min(kMaxTop, V));
+    if (top_k > 0 && (!top_index || !top_logprob))
+        return set_error(DT_ERR_INVALID_ARG, "top_index and top_logprob must be non-NULL with top_k=%d", top_k);
+    const int64_t rows = static_cast<int64_t>(B) * T;
+    const int64_t need = workspace_bytes(rows, V, top_k);
+    const size_t es = dtype == DT_BF16 ? 2 : 4;
+    if (mem == DT_MEM_DEVICE) {
+        if (reinterpret_cast<uintptr_t>(logits) % es) return set_error(DT_ERR_INVALID_ARG, "logits are not aligned to their type");
+        if (!aligned16(ws)) return set_error(DT_ERR_INVALID_ARG, "the workspace must be 16-byte aligned");
+        if (need > 0 && (!ws || ws_bytes < need))
+            return set_error(DT_ERR_INVALID_ARG, "the workspace has %lld bytes, the call needs %lld", (long long)(ws ? ws_bytes : 0), (long long)need);
+    } else {
+        DT_TRY(check_host_tokens(tokens, token_bytes, rows, V, ignore_index));
+    }
+    if (!ctx) return set_error(DT_ERR_INVALID_ARG, "ctx is NULL");
+    DT_TRY(check_device_binding(ctx));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    LogprobArgs a{};
+    a.x = logits;
+    a.tok = tokens;
+    a.ldb = ldb;
+    a.ldt = ldt;
+    a.ignore = ignore_index;
+    a.tok64 = token_bytes == 8;
+    a.T = T;
+    a.V = V;
+    a.k = top_k;
+    a.logprob = logprob;
+    a.entropy = entropy;
+    a.m = m;
+    a.l = l;
+    a.top_index = top_index;
+    a.top_logprob = top_logprob;
+    if (mem == DT_MEM_DEVICE) return launch_logprobs(a, rows, dtype == DT_BF16, ws, s);
+
+    const size_t nk = static_cast<size_t>(rows) * top_k;
+    DT_TRY(ctx->stage[0].ensure(rows * V * es));
+    DT_TRY(ctx->stage[1].ensure(rows * token_bytes));
+    DT_TRY(ctx->stage[2].ensure(rows * 4 * sizeof(float)));
+    DT_TRY(ctx->stage[3].ensure(nk * 8 + 16));
+    if (need > 0) DT_TRY(ctx->stage[4].ensure(need));
+    DT_TRY(stage_rows(ctx->stage[0].ptr, logits, B, T, V, ldb, ldt, es, s));
+    DT_HIP_TRY(hipMemcpyAsync(ctx->stage[1].ptr, tokens, rows * token_bytes, hipMemcpyHostToDevice, s));
+    a.x = ctx->stage[0].ptr;
+    a.tok = ctx->stage[1].ptr;
+    a.ldt = V;
+    a.ldb = static_cast<int64_t>(T) * V;
+    a.logprob = static_cast<float*>(ctx->stage[2].ptr);
+    a.entropy = a.logprob + rows;
+    a.m = a.logprob + 2 * rows;
+    a.l = a.logprob + 3 * rows;
+    a.top_index = static_cast<int32_t*>(ctx->stage[3].ptr);
+    a.top_logprob = reinterpret_cast<float*>(a.top_index + nk);
+    DT_TRY(launch_logprobs(a, rows, dtype == DT_BF16, ctx->stage[4].ptr, s));
+    DT_HIP_TRY(hipMemcpyAsync(logprob, a.logprob, rows * 4, hipMemcpyDeviceToHost, s));
+    if (entropy) DT_HIP_TRY(hipMemcpyAsync(entropy, a.entropy, rows * 4, hipMemcpyDeviceToHost, s));
+    DT_HIP_TRY(hipMemcpyAsync(m, a.m, rows * 4, hipMemcpyDeviceToHost, s));
+    DT_HIP_TRY(hipMemcpyAsync(l, a.l, rows * 4, hipMemcpyDeviceToHost, s));
+    if (nk) {
+        DT_HIP_TRY(hipMemcpyAsync(top_index, a.top_index, nk * 4, hipMemcpyDeviceToHost, s));
+        DT_HIP_TRY(hipMemcpyAsync(top_logprob, a.top_logprob, nk * 4, hipMemcpyDeviceToHost, s));
+    }
+    DT_HIP_TRY(hipStreamSynchronize(s));
+    return DT_OK;
+}
+
+int dt_token_logprobs_bwd(dt_ctx* ctx, const float* d_logprob, const float* d_entropy, const void* logits, const void* tokens,
+                          const float* m, const float* l, const float* entropy, int B, int T, int V, int64_t ldb, int64_t ldt,
+                          int token_bytes, int64_t ignore_index, void* d_logits, int64_t ldb_out, int64_t ldt_out, int dtype,
+                          int mem, void* stream) {
+    clear_error();
+    if (!d_logprob || !logits || !tokens || !m || !l || !d_logits)
+        return set_error(DT_ERR_INVALID_ARG, "d_logprob, logits, tokens, m, l and d_logits must be non-NULL");
+    if (d_entropy && !entropy) return set_error(DT_ERR_INVALID_ARG, "entropy must be non-NULL with d_entropy");
+    DT_TRY(check_logits(B, T, V, ldb, ldt, token_bytes, dtype, mem));
+    if ((T > 1 && ldt_out < V) || (B > 1 && ldb_out < (T - 1) * ldt_out + V) || ldb_out < 0 || ldt_out < 0)
+        return set_error(DT_ERR_INVALID_ARG, "rows of d_logits %lld and %lld apart overlap", (long long)ldb_out, (long long)ldt_out);
+    const int64_t rows = static_cast<int64_t>(B) * T;
+    const size_t es = dtype == DT_BF16 ? 2 : 4;
+    if (mem == DT_MEM_DEVICE) {
+        if (reinterpret_cast<uintptr_t>(logits) % es || reinterpret_cast<uintptr_t>(d_logits) % es)
+            return set_error(DT_ERR_INVALID_ARG, "logits or d_logits are not aligned to their type");
+    } else {
+        DT_TRY(check_host_tokens(tokens, token_bytes, rows, V, ignore_index));
+    }
+    if (!ctx) return set_error(DT_ERR_INVALID_ARG, "ctx is NULL");
+    DT_TRY(check_device_binding(ctx));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    LogprobBwdArgs a{};
+    a.x = logits;
+    a.dx = d_logits;
+    a.tok = tokens;
+    a.g = d_logprob;
+    a.h = d_entropy;
+    a.m = m;
+    a.l = l;
+    a.entropy = entropy;
+    a.ldb = ldb;
+    a.ldt = ldt;
+    a.ldb_out = ldb_out;
+    a.ldt_out = ldt_out;
+    a.ignore = ignore_index;
+    a.tok64 = token_bytes == 8;
+    a.T = T;
+    a.V = V;
+    if (mem == DT_MEM_DEVICE) return launch_logprobs_bwd(a, rows, dtype == DT_BF16, s);
+
+    DT_TRY(ctx->stage[0].ensure(rows * V * es));
+    DT_TRY(ctx->stage[1].ensure(rows * token_bytes));
+    DT_TRY(ctx->stage[2].ensure(rows * 5 * sizeof(float)));
+    DT_TRY(stage_rows(ctx->stage[0].ptr, logits, B, T, V, ldb, ldt, es, s));
+    DT_HIP_TRY(hipMemcpyAsync(ctx->stage[1].ptr, tokens, rows * token_bytes, hipMemcpyHostToDevice, s));
+    float* st = static_cast<float*>(ctx->stage[2].ptr);
+    const float* src[5] = {d_logprob, m, l, d_entropy, d_entropy ? entropy : nullptr};
+    for (int i = 0; i < 5; ++i)
+        if (src[i]) DT_HIP_TRY(hipMemcpyAsync(st + i * rows, src[i], rows * 4, hipMemcpyHostToDevice, s));
+    a.x = a.dx = ctx->stage[0].ptr;  // (in place)
+    a.tok = ctx->stage[1].ptr;
+    a.g = st;
+    a.m = st + rows;
+    a.l = st + 2 * rows;
+    a.h = d_entropy ? st + 3 * rows : nullptr;
+    a.entropy = st + 4 * rows;
+    a.ldt = a.ldt_out = V;
+    a.ldb = a.ldb_out = static_cast<int64_t>(T) * V;
+    DT_TRY(launch_logprobs_bwd(a, rows, dtype == DT_BF16, s));
+    for (int b = 0; b < B; ++b)
+        for (int t = 0; t < T; ++t)
+            DT_HIP_TRY(hipMemcpyAsync(static_cast<uint8_t*>(d_logits) + (b * ldb_out + t * ldt_out) * es,
+                                      static_cast<uint8_t*>(ctx->stage[0].ptr) + (static_cast<size_t>(b) * T + t) * V * es, V * es,
+                                      hipMemcpyDeviceToHost, s));
+    DT_HIP_TRY(hipStreamSynchronize(s));
+    return DT_OK;
+}
+
+}  // extern "C"

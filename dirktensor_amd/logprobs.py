@@ -1,0 +1,196 @@
+"""Scores of given tokens and their gradient, on the HIP path (beside ce_loss, which gives their mean over a batch): every
+call goes to libdirktensor_amd.so; nothing here computes.
+
+    token_logprobs(logits, tokens, top_k=0) -> TokenLogprobs
+        log probabilities of the tokens, the rows' entropies and their top_k most likely tokens
+    token_logprobs_backward(d_logprob, logits, tokens, result, d_entropy=None) -> d_logits
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+from typing import Optional
+
+import numpy as np
+
+from . import _capi as C
+from .attention import Context, _is_torch, _mode_of, _stream_of, default_context, torch
+
+
+@dataclass
+class TokenLogprobs:
+    """logprob, entropy (nats), softmax_m (row maximum) and softmax_l (sum exp(x - m)) [...], fp32; with top_k > 0 top_index
+    (int32) and top_logprob [..., top_k], descending, the lower index first of equals. ``ignore_index`` is the call's."""
+
+    logprob: object
+    entropy: object
+    softmax_m: object
+    softmax_l: object
+    top_index: object = None
+    top_logprob: object = None
+    ignore_index: Optional[int] = None
+
+
+def _two_strides(shape, strides):
+    """Leading dimensions as B x T of two strides: (B, T, ldb, ldt), or None where they are none."""
+    dims = [(n, s) for n, s in zip(shape, strides) if n != 1]
+    merged = []
+    for n, s in dims:
+        if merged and merged[-1][1] == n * s:
+            merged[-1] = (merged[-1][0] * n, s)
+        else:
+            merged.append((n, s))
+    if len(merged) > 2:
+        return None
+    while len(merged) < 2:
+        merged.insert(0, (1, 0))
+    (B, ldb), (T, ldt) = merged
+    return B, T, ldb, ldt
+
+
+def _check_tokens(tokens, lead, like):
+    if tuple(tokens.shape) != tuple(lead):
+        raise ValueError(f"tokens have shape {tuple(tokens.shape)}, expected {tuple(lead)}")
+    if _is_torch(like):
+        if not _is_torch(tokens) or tokens.device != like.device:
+            raise ValueError("tokens must be a torch tensor on the logits' device")
+        if tokens.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"unsupported token dtype {tokens.dtype}: int32 or int64")
+        t = tokens.contiguous()
+        return t, t.data_ptr(), t.element_size()
+    t = np.asarray(tokens.cpu() if _is_torch(tokens) else tokens)
+    if t.dtype not in (np.int32, np.int64):
+        raise TypeError(f"unsupported token dtype {t.dtype}: int32 or int64")
+    t = np.ascontiguousarray(t)
+    return t, t.ctypes.data, t.itemsize
+
+
+def _check_logits(logits, ctx):
+    if len(logits.shape) < 1:
+        raise ValueError("logits need a vocabulary dimension")
+    if _is_torch(logits):
+        if not logits.is_cuda:
+            raise ValueError("torch inputs must be on a ROCm device; use numpy arrays for host memory")
+        ctx = ctx or default_context(logits.device.index or 0)
+        if logits.device.index != ctx.device:
+            raise ValueError(f"logits are on {logits.device}, the context on cuda:{ctx.device}")
+        return ctx
+    return ctx or default_context(0)
+
+
+def _rows(logits):
+    """The logits' rows as the library takes them: the tensor itself where its leading dimensions have at most two strides
+    (a slice [:, :-1] is one), else a copy."""
+    V = int(logits.shape[-1])
+    if logits.stride(-1) == 1 or V == 1:
+        r = _two_strides(logits.shape[:-1], logits.stride()[:-1])
+        if r is not None:
+            return logits, r
+    logits = logits.contiguous()
+    return logits, _two_strides(logits.shape[:-1], logits.stride()[:-1])
+
+
+def token_logprobs(logits, tokens, *, top_k: int = 0, ignore_index: Optional[int] = None,
+                   ctx: Optional[Context] = None) -> TokenLogprobs:
+    """Scores tokens [...] by the rows of logits [..., V] (fp32 or bf16, torch device tensors, strided views such as
+    logits[:, :-1] among them, or numpy arrays). For next-token scores pass logits[:, :-1] and tokens[:, 1:].
+
+    Positions whose token is ``ignore_index`` get logprob 0 (and no gradient from it). A token outside the vocabulary is refused
+    with numpy arrays and gives NaN on the device. Logits of -inf are tokens of probability 0; a row with a NaN or +inf, or with
+    nothing but -inf, gives NaN. top_k: 0 to 64."""
+    ctx = _check_logits(logits, ctx)
+    lead, V, k = tuple(logits.shape[:-1]), int(logits.shape[-1]), int(top_k)
+    dtype = _mode_of(logits, None)
+    tok, tok_p, tok_bytes = _check_tokens(tokens, lead, logits)
+    ign = C.DT_NO_IGNORE if ignore_index is None else int(ignore_index)
+    if _is_torch(logits):
+        x, (B, T, ldb, ldt) = _rows(logits)
+        nbytes = ctypes.c_int64()
+        C.call("dt_token_logprobs_workspace", B, T, V, k, ctypes.byref(nbytes))
+        # a workspace of the call's own: torch's allocator keeps it for this stream, or for the graph being captured
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=x.device) if nbytes.value else None
+        lp, ent, m, l = (torch.empty(lead, dtype=torch.float32, device=x.device) for _ in range(4))
+        idx = torch.empty((*lead, k), dtype=torch.int32, device=x.device) if k else None
+        top = torch.empty((*lead, k), dtype=torch.float32, device=x.device) if k else None
+        C.call("dt_token_logprobs", ctx.handle, x.data_ptr(), tok_p, B, T, V, ldb, ldt, tok_bytes, ign, k, lp.data_ptr(),
+               ent.data_ptr(), m.data_ptr(), l.data_ptr(), idx.data_ptr() if k else None, top.data_ptr() if k else None,
+               ws.data_ptr() if ws is not None else None, nbytes.value, dtype, C.DT_MEM_DEVICE, _stream_of(x))
+        return TokenLogprobs(lp, ent, m, l, idx, top, ignore_index)
+    x = np.ascontiguousarray(logits)
+    rows = int(np.prod(lead, dtype=np.int64))
+    lp, ent, m, l = (np.empty(lead, np.float32) for _ in range(4))
+    idx = np.empty((*lead, k), np.int32) if k else None
+    top = np.empty((*lead, k), np.float32) if k else None
+    C.call("dt_token_logprobs", ctx.handle, x.ctypes.data, tok_p, 1, rows, V, rows * V, V, tok_bytes, ign, k, lp.ctypes.data,
+           ent.ctypes.data, m.ctypes.data, l.ctypes.data, idx.ctypes.data if k else None, top.ctypes.data if k else None, None,
+           0, dtype, C.DT_MEM_HOST, None)
+    return TokenLogprobs(lp, ent, m, l, idx, top, ignore_index)
+
+
+def _span(t):
+    """The addresses that a tensor's elements lie in."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def token_logprobs_backward(d_logprob, logits, tokens, result: TokenLogprobs, *, d_entropy=None, out=None,
+                            ctx: Optional[Context] = None):
+    """The gradient with respect to the logits, in their dtype, of d_logprob [...] and (optionally) d_entropy [...], fp32, for
+    the forward's ``result`` on the same logits and tokens. ``out`` (torch): where to write it, a tensor of the logits' shape and
+    dtype, or the logits themselves to overwrite them."""
+    ctx = _check_logits(logits, ctx)
+    lead, V = tuple(logits.shape[:-1]), int(logits.shape[-1])
+    dtype = _mode_of(logits, None)
+    tok, tok_p, tok_bytes = _check_tokens(tokens, lead, logits)
+    ign = C.DT_NO_IGNORE if result.ignore_index is None else int(result.ignore_index)
+    per_row = dict(d_logprob=d_logprob, softmax_m=result.softmax_m, softmax_l=result.softmax_l, entropy=result.entropy)
+    if d_entropy is not None:
+        per_row["d_entropy"] = d_entropy
+    for name, t in per_row.items():
+        if tuple(t.shape) != lead:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {lead}")
+        if _is_torch(t) != _is_torch(logits) or (_is_torch(t) and t.device != logits.device):
+            raise ValueError(f"{name} must be where the logits are")
+    if _is_torch(logits):
+        p = {k: t.contiguous().float() for k, t in per_row.items()}
+        x, (B, T, ldb, ldt) = _rows(logits)
+        if out is None:
+            out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+            raise ValueError("out must have the logits' shape, dtype and device")
+        elif out.stride(-1) != 1 and V != 1:
+            raise ValueError("out's vocabulary dimension must be contiguous")
+        r = _two_strides(out.shape[:-1], out.stride()[:-1])
+        same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
+        if not same and out.numel():
+            (a0, a1), (b0, b1) = _span(out), _span(x)
+            if a0 < b1 and b0 < a1:
+                raise ValueError("out overlaps the logits without being them")
+        # (both row orders must have the same two strides' extents)
+        if r is None or (r[:2] != (B, T) and not (r[0] == 1 or B == 1)):
+            raise ValueError("out's leading dimensions must have at most two strides, split like the logits'")
+        if r[:2] != (B, T):
+            if B == 1:  # the logits' rows have one stride: they split like out's
+                ldb, B, T = r[1] * ldt, r[0], r[1]
+                bo, to = r[2], r[3]
+            else:
+                bo, to = T * r[3], r[3]
+        else:
+            bo, to = r[2], r[3]
+        C.call("dt_token_logprobs_bwd", ctx.handle, p["d_logprob"].data_ptr(),
+               p["d_entropy"].data_ptr() if d_entropy is not None else None, x.data_ptr(), tok_p, p["softmax_m"].data_ptr(),
+               p["softmax_l"].data_ptr(), p["entropy"].data_ptr(), B, T, V, ldb, ldt, tok_bytes, ign, out.data_ptr(), bo, to,
+               dtype, C.DT_MEM_DEVICE, _stream_of(x))
+        return out
+    if out is not None:
+        raise ValueError("out is for torch tensors")
+    x = np.ascontiguousarray(logits)
+    p = {k: np.ascontiguousarray(t, dtype=np.float32) for k, t in per_row.items()}
+    g = np.empty_like(x)
+    rows = int(np.prod(lead, dtype=np.int64))
+    C.call("dt_token_logprobs_bwd", ctx.handle, p["d_logprob"].ctypes.data,
+           p["d_entropy"].ctypes.data if d_entropy is not None else None, x.ctypes.data, tok_p, p["softmax_m"].ctypes.data,
+           p["softmax_l"].ctypes.data, p["entropy"].ctypes.data, 1, rows, V, rows * V, V, tok_bytes, ign, g.ctypes.data,
+           rows * V, V, dtype, C.DT_MEM_HOST, None)
+    return g

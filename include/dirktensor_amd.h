@@ -444,6 +444,39 @@ int dt_cached_attn_fwd(dt_kv_cache* cache, const void* q, void* o, float* m, flo
                        const dt_kv_cache* prefix, int prefix_slot, void* ws, int64_t ws_bytes, int dtype, int mem,
                        void* stream);
 
+/*
+ * Log probabilities of given tokens, with entropies and the most likely alternatives (beside dt_ce_loss, which
+ * gives their mean over a batch; the per-token terms are CrossEntropyLoss.cpp:25-37's).
+ *   logits      : B x T rows of V (<= 2^24) logits in dtype, row (b, t) at element b*ldb + t*ldt
+ *   tokens      : [B, T], token_bytes 4 (int32) or 8 (int64) each, in the same memory as logits: the token scored by each
+ *                 row (for next-token scores: logits [:, :-1] with tokens [:, 1:])
+ *   ignore_index: tokens equal to it are skipped (logprob 0, no gradient; entropy and alternatives are still the row's);
+ *                 DT_NO_IGNORE: none. Any other token outside [0, V) is refused with DT_MEM_HOST; on the device its
+ *                 logprob, and its row of the gradient, is NaN.
+ *   logprob, entropy, m, l : [B, T] fp32; entropy (nats) may be NULL; m = row maximum, l = sum exp(x - m)
+ *   top_index, top_logprob : [B, T, top_k]: the top_k (0 .. 64, at most V) largest logits, descending, the lower index
+ *                 first of equals (a NaN counts as -inf); NULL with top_k 0
+ *   ws          : device workspace of at least dt_token_logprobs_workspace bytes (0: none is needed), 16-byte aligned, not
+ *                 shared with a call that may run at the same time. Ignored with DT_MEM_HOST.
+ * Logits of -inf (masked tokens) have probability 0. A row with a NaN or +inf, or with nothing but -inf, gives NaN. B*T <=
+ * 8388607. Deterministic.
+ */
+#define DT_NO_IGNORE (-INT64_MAX - 1)
+int dt_token_logprobs_workspace(int B, int T, int V, int top_k, int64_t* bytes);
+int dt_token_logprobs(dt_ctx* ctx, const void* logits, const void* tokens, int B, int T, int V, int64_t ldb, int64_t ldt,
+                      int token_bytes, int64_t ignore_index, int top_k, float* logprob, float* entropy, float* m,
+                      float* l, int32_t* top_index, float* top_logprob, void* ws, int64_t ws_bytes, int dtype, int mem,
+                      void* stream);
+/*
+ * Its gradient: d_logprob [B, T] and d_entropy [B, T] (or NULL: 0) fp32 -> d_logits, B x T rows in dtype at b*ldb_out +
+ * t*ldt_out, rows not overlapping: g (1[j = token] - p_j) - h p_j (log p_j + entropy). m, l and (with d_entropy) entropy are
+ * the forward's. d_logits may be logits themselves (the same address and strides). The alternatives have no gradient.
+ */
+int dt_token_logprobs_bwd(dt_ctx* ctx, const float* d_logprob, const float* d_entropy, const void* logits,
+                          const void* tokens, const float* m, const float* l, const float* entropy, int B, int T, int V,
+                          int64_t ldb, int64_t ldt, int token_bytes, int64_t ignore_index, void* d_logits,
+                          int64_t ldb_out, int64_t ldt_out, int dtype, int mem, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

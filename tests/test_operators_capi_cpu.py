@@ -94,3 +94,76 @@ def test_cached_attn_workspace():
     refused(lib.dt_cached_attn_workspace(None, 1, 1, 2, 128, None, None, None, 0, 0, None), C.DT_ERR_INVALID_ARG, "bytes")
     refused(lib.dt_cached_attn_workspace(None, 1, 1, 2, 128, None, None, None, 0, 0, ctypes.byref(n)), C.DT_ERR_INVALID_ARG,
             "cache is NULL")
+
+
+@pytest.mark.parametrize("kw,code,msg", [
+    (dict(logits=None), C.DT_ERR_INVALID_ARG, "non-NULL"),
+    (dict(m=None), C.DT_ERR_INVALID_ARG, "non-NULL"),
+    (dict(B=0), C.DT_ERR_INVALID_ARG, ">= 1"),
+    (dict(V=(1 << 24) + 1), C.DT_ERR_UNSUPPORTED, "V="),
+    (dict(T=1 << 24), C.DT_ERR_UNSUPPORTED, "rows"),
+    (dict(ldt=-1), C.DT_ERR_INVALID_ARG, "strides"),
+    (dict(token_bytes=2), C.DT_ERR_INVALID_ARG, "token_bytes"),
+    (dict(top_k=65), C.DT_ERR_INVALID_ARG, "top_k"),
+    (dict(top_k=3, top_index=None), C.DT_ERR_INVALID_ARG, "top_index"),
+    (dict(logits=FAKE + 2), C.DT_ERR_INVALID_ARG, "aligned"),
+    (dict(ws=FAKE + 8), C.DT_ERR_INVALID_ARG, "aligned"),
+    (dict(V=100352, ws=None), C.DT_ERR_INVALID_ARG, "the workspace has 0"),
+    (dict(dtype=9), C.DT_ERR_INVALID_ARG, "dtype"),
+    (dict(mem=9), C.DT_ERR_INVALID_ARG, "mem"),
+    ({}, C.DT_ERR_INVALID_ARG, "ctx is NULL"),
+])
+def test_token_logprobs(kw, code, msg):
+    a = dict(ctx=None, logits=FAKE, tokens=FAKE, B=1, T=1, V=100, ldb=0, ldt=0, token_bytes=4, ignore=C.DT_NO_IGNORE, top_k=0,
+             logprob=FAKE, entropy=None, m=FAKE, l=FAKE, top_index=FAKE, top_logprob=FAKE, ws=FAKE, ws_bytes=0,
+             dtype=C.DT_FP32_EXACT, mem=C.DT_MEM_DEVICE, stream=None)
+    a.update(kw)
+    refused(C.lib().dt_token_logprobs(*a.values()), code, msg)
+
+
+@pytest.mark.parametrize("kw,code,msg", [
+    (dict(g=None), C.DT_ERR_INVALID_ARG, "non-NULL"),
+    (dict(h=FAKE, entropy=None), C.DT_ERR_INVALID_ARG, "entropy"),
+    (dict(T=2, ldt_out=99), C.DT_ERR_INVALID_ARG, "overlap"),
+    (dict(B=2, T=2, ldt_out=100, ldb_out=199), C.DT_ERR_INVALID_ARG, "overlap"),
+    (dict(dx=FAKE + 1), C.DT_ERR_INVALID_ARG, "aligned"),
+    (dict(token_bytes=0), C.DT_ERR_INVALID_ARG, "token_bytes"),
+    ({}, C.DT_ERR_INVALID_ARG, "ctx is NULL"),
+])
+def test_token_logprobs_bwd(kw, code, msg):
+    a = dict(ctx=None, g=FAKE, h=None, logits=FAKE, tokens=FAKE, m=FAKE, l=FAKE, entropy=FAKE, B=1, T=1, V=100, ldb=0, ldt=0,
+             token_bytes=4, ignore=0, dx=FAKE, ldb_out=0, ldt_out=0, dtype=C.DT_BF16, mem=C.DT_MEM_DEVICE, stream=None)
+    a.update(kw)
+    refused(C.lib().dt_token_logprobs_bwd(*a.values()), code, msg)
+
+
+def test_token_logprobs_host_tokens_are_checked():
+    tok = np.array([3, 100], np.int64)
+    args = [None, FAKE, tok.ctypes.data, 1, 2, 100, 200, 100, 8, C.DT_NO_IGNORE, 0, FAKE, None, FAKE, FAKE, None, None, None, 0, 0,
+            C.DT_MEM_HOST, None]
+    refused(C.lib().dt_token_logprobs(*args), C.DT_ERR_INVALID_ARG, "token 100 of row 1")
+    args[9] = 100  # ignored
+    refused(C.lib().dt_token_logprobs(*args), C.DT_ERR_INVALID_ARG, "ctx is NULL")
+
+
+def test_token_logprobs_workspace():
+    n = ctypes.c_int64(-1)
+    lib = C.lib()
+    assert lib.dt_token_logprobs_workspace(2048, 2, 100352, 5, ctypes.byref(n)) == C.DT_OK and n.value == 0  # rows enough
+    assert lib.dt_token_logprobs_workspace(1, 1, 100352, 20, ctypes.byref(n)) == C.DT_OK and n.value > 0
+    refused(lib.dt_token_logprobs_workspace(1, 1, 10, 11, ctypes.byref(n)), C.DT_ERR_INVALID_ARG, "top_k")
+    refused(lib.dt_token_logprobs_workspace(1, 1, 10, 1, None), C.DT_ERR_INVALID_ARG, "bytes")
+
+
+def test_leading_dimensions_as_two_strides():
+    from dirktensor_amd.logprobs import _two_strides
+
+    assert _two_strides((), ()) == (1, 1, 0, 0)
+    assert _two_strides((5,), (7,)) == (1, 5, 0, 7)
+    assert _two_strides((3, 5), (35, 7)) == (1, 15, 0, 7)
+    assert _two_strides((3, 5), (42, 7)) == (3, 5, 42, 7)
+    assert _two_strides((3, 1, 5), (42, 9, 7)) == (3, 5, 42, 7)
+    assert _two_strides((2, 3, 5), (105, 35, 7)) == (1, 30, 0, 7)
+    assert _two_strides((2, 3, 5), (126, 42, 7)) == (6, 5, 42, 7)
+    assert _two_strides((2, 3, 5), (200, 42, 7)) is None
+    assert _two_strides((4, 5), (0, 7)) == (4, 5, 0, 7)
