@@ -10,14 +10,14 @@
 // Both are bound by HBM: the forward reads the logits once, the backward reads them and writes as many.
 //
 // Forward: a workgroup of 256 threads streams a row (or, where there are few rows, a segment of one) with 16-byte loads;
-// a thread keeps its own running maximum, sum and weighted sum and remembers which of its batches of 16 values the
-// maximum came from, so the loop has no exchange between lanes. The statistics meet once at the end. The alternatives cost
-// no second pass: with the threads' maxima ranked, the k-th largest is a bound that the k largest values reach, and
-// every value that reaches it belongs to one of those k threads. Only these threads' values are read again (about k of 256
-// runs, from L2), those that reach the bound (a few more than k) are collected in LDS, and each takes the place
-// that the number of larger ones gives it. Keys are (value, index) pairs, so no two are equal, ties go to the lower index and the
-// order of the collection does not matter. A row cut into segments leaves (m, l, sum, k keys) of each in the workspace and a
-// second kernel joins them by the same selection.
+// a thread keeps its own running maximum, sum and weighted sum, so the loop has no exchange between lanes, and the statistics
+// meet once at the end. The alternatives cost no second pass: after the first fifth of the row the k-th largest of the
+// threads' maxima is a bound that at least k values reach. The threads whose maximum reaches it look at their share of that fifth again
+// (from L2), and the rest of the row is compared with the bound as it streams by, one comparison for 16 values; what reaches
+// it (about 5 k values) is collected in LDS, and each takes the place that the number of larger ones gives it. Keys are
+// (value, index) pairs, so no two are equal, ties go to the lower index and the order of the collection does not matter. Where more values
+// reach the bound than the list holds (rows of many equal values) they are selected one after another in passes over the
+// row. A row cut into segments leaves (m, l, sum, k keys) of each in the workspace and a second kernel joins them.
 
 #include "dt_internal.h"
 
@@ -36,7 +36,8 @@ typedef u32x4 u32x4_at4 __attribute__((aligned(4)));
 
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kMaxTop = 64;
-constexpr int kList = 1024;          // values that may reach the bound before the slow selection takes over
+constexpr int kList = 1024;          // values that may reach the bound before the selection goes one by one
+constexpr uint32_t kOrderNegInf = 0x007fffffu;  // order_of(-inf): the least there is
 constexpr int kBatch = 16;           // values a thread takes at a time
 constexpr int kMinSegment = 2048;    // values of a segment at least
 constexpr float kLog2e = 1.4426950408889634f;
@@ -83,8 +84,7 @@ __device__ __forceinline__ int key_index(uint64_t key) { return static_cast<int>
 
 // A run of n values of a row in 16-byte pieces from its first value on, whatever its alignment (global 16-byte accesses
 // take any, and a row's bits then do not depend on where it lies), single values after the last whole piece. Piece p belongs to
-// thread p % 256; a thread's batch j is its pieces 256 (j kPer + 0 .. kPer - 1) + tid; value tid of those behind the
-// pieces is its batch `batches`. A thread's batches ascend in index.
+// thread p % 256; a thread's batch j is its pieces 256 (j kPer + 0 .. kPer - 1) + tid.
 template <bool kBf16>
 struct Run {
     static constexpr int kEs = kBf16 ? 2 : 4, kPiece = 16 / kEs, kPer = kBatch / kPiece;
@@ -101,6 +101,8 @@ struct Run {
     }
     __device__ __forceinline__ int tail() const { return pieces * kPiece; }
     __device__ __forceinline__ u32x4 load(int p) const { return *reinterpret_cast<const Piece*>(x + p * 16); }
+    // a value that is not read again: past the caches (large reads reach 7.0 TB/s so, 6.1 through them)
+    __device__ __forceinline__ u32x4 load_once(int p) const { return __builtin_nontemporal_load(reinterpret_cast<const Piece*>(x + p * 16)); }
     static __device__ __forceinline__ void unpack(const u32x4& w, float* v) {
         if constexpr (kBf16) {
 #pragma unroll
@@ -117,22 +119,20 @@ struct Run {
 
 struct Stats {
     float m = kNegInf, s = 0.0f, d = 0.0f;  // maximum; sum e; sum e (x - m)
-    int batch = -1;                         // where the maximum was first met
 };
 
+// takes n of the values, and returns their maximum
 template <int kN>
-__device__ __forceinline__ void take(Stats& st, const float (&v)[kN], int n, int batch) {
+__device__ __forceinline__ float take(Stats& st, const float (&v)[kN], int n) {
     float bm = kNegInf;
 #pragma unroll
     for (int i = 0; i < kN; ++i)
         if (i < n) bm = fmaxf(bm, v[i]);
-    if (st.batch == -1) st.batch = batch;  // (a thread whose values are all -inf has its first one as its best)
     if (bm > st.m) {
         const float f = __builtin_amdgcn_exp2f((st.m - bm) * kLog2e);
         st.d = (st.d + st.s * fmaxf(st.m - bm, -1e4f)) * f;  // (further down f is 0: the sum must not become an infinity)
         st.s *= f;
         st.m = bm;
-        st.batch = batch;
     }
     const float base = st.m == kNegInf ? 0.0f : st.m;
 #pragma unroll
@@ -144,9 +144,10 @@ __device__ __forceinline__ void take(Stats& st, const float (&v)[kN], int n, int
             st.s += e;
             st.d += e * fmaxf(t, -1e4f);  // (0 for -inf; a NaN shows in s)
         }
+    return bm;
 }
 
-// a's statistics and b's; the batch is a's
+// a's statistics and b's
 __device__ __forceinline__ void join(Stats& a, float m, float s, float d) {
     const float mx = fmaxf(a.m, m), base = mx == kNegInf ? 0.0f : mx;
     const float fa = __builtin_amdgcn_exp2f((a.m - base) * kLog2e), fb = __builtin_amdgcn_exp2f((m - base) * kLog2e);
@@ -211,69 +212,63 @@ __device__ __forceinline__ Finish finish(const LogprobArgs& a, int64_t row, cons
 }
 
 struct SelectBuf {
-    union {
-        uint64_t rank[kThreads];
-        uint64_t list[kList];
-    };
-    int owner[kMaxTop];
+    uint32_t top[kThreads];
+    uint64_t list[kList];
     uint64_t best[kWaves];
     int count;
-    uint64_t bound;
 };
 
-// The k largest keys of the workgroup's values, in order, through out(place, key); places past the last value get key 0. `mine` is
-// the thread's largest key (0: none); each(owner, lane, f) calls f(key) for the values of thread `owner` that fall to a
-// lane of the wave that asks, and all lanes of a wave call it together.
+// A bound that the k-th largest of the threads' `mine` (order_of their maximum; 0: none) reaches, to 20 bits, the same for all;
+// empties the list. Each wave finds it for itself, bit by bit, from four of the 256 a lane.
+__device__ __forceinline__ uint32_t find_bound(SelectBuf& b, uint32_t mine, int k) {
+    __syncthreads();
+    b.top[threadIdx.x] = mine;
+    if (threadIdx.x == 0) b.count = 0;
+    __syncthreads();
+    uint32_t v[kWaves];
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) v[i] = b.top[i * 64 + (threadIdx.x & 63)];
+    uint32_t bound = 0;
+    for (int bit = 31; bit >= 12; --bit) {
+        const uint32_t trial = bound | 1u << bit;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) n += __popcll(__ballot(v[i] >= trial));
+        if (n >= k) bound = trial;
+    }
+    return bound;
+}
+
+__device__ __forceinline__ void push(SelectBuf& b, uint64_t key) {
+    if (*static_cast<volatile int*>(&b.count) >= kList + kThreads) return;  // (the list has long run over)
+    const int at = atomicAdd(&b.count, 1);
+    if (at < kList) b.list[at] = key;
+}
+
+// The k largest of the collected keys, in order, through out(place, key); places past the last get key 0. Where the list ran
+// over, the k largest of all: each(f) calls f(key) for every value of the thread.
 template <class Each, class Out>
-__device__ __forceinline__ void select(SelectBuf& b, uint64_t mine, int k, Each each, Out out) {
+__device__ __forceinline__ void select(SelectBuf& b, int k, Each each, Out out) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    __syncthreads();
-    b.rank[tid] = mine;
-    if (tid == 0) b.count = 0, b.bound = 0;
-    if (tid < kMaxTop) b.owner[tid] = -1;
-    __syncthreads();
-    if (mine != 0) {
-        int larger = 0;
-#pragma unroll 8
-        for (int i = 0; i < kThreads; ++i) larger += b.rank[i] > mine;
-        if (larger < k) b.owner[larger] = tid;
-        if (larger == k - 1) b.bound = mine;
-    }
-    __syncthreads();
-    const uint64_t bound = b.bound;
-    for (int r = wave; r < k; r += kWaves) {
-        const int o = b.owner[r];
-        if (o < 0) continue;
-        each(o, lane, [&](uint64_t key) {
-            if (key < bound) return;
-            const int at = atomicAdd(&b.count, 1);
-            if (at < kList) b.list[at] = key;
-        });
-    }
     __syncthreads();
     const int c = b.count;
     if (c <= kList) {
         for (int i = tid; i < c; i += kThreads) {
             const uint64_t key = b.list[i];
             int larger = 0;
-#pragma unroll 4
+#pragma unroll 8
             for (int j = 0; j < c; ++j) larger += b.list[j] > key;
             if (larger < k) out(larger, key);
         }
         for (int i = c + tid; i < k; i += kThreads) out(i, 0);
         return;
     }
-    // one after another: the largest key below the last
     uint64_t last = ~uint64_t(0);
-    for (int r = 0; r < k; ++r) {
+    for (int r = 0; r < k; ++r) {  // the largest key below the last
         uint64_t top = 0;
-        for (int i = wave; i < k; i += kWaves) {
-            const int o = b.owner[i];
-            if (o < 0) continue;
-            each(o, lane, [&](uint64_t key) {
-                if (key < last && key > top) top = key;
-            });
-        }
+        each([&](uint64_t key) {
+            if (key < last && key > top) top = key;
+        });
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const uint64_t other = __shfl_xor(static_cast<unsigned long long>(top), o, 64);
@@ -306,60 +301,71 @@ __global__ __launch_bounds__(kThreads) void logprob_rows_kernel(LogprobArgs a) {
     const R run(xrow + static_cast<int64_t>(first) * R::kEs, min(a.V - first, a.seg_len));
 
     Stats st;
-    int j = 0;
-    // whole batches, the next one's loads in flight while one is summed
-    const int whole = run.pieces / (kThreads * R::kPer);
-    u32x4 w[R::kPer];
-    if (whole > 0) {
-#pragma unroll
-        for (int i = 0; i < R::kPer; ++i) w[i] = run.load(i * kThreads + tid);
+    uint32_t bound = 0;
+    const int tail = run.tail() + tid;
+    float last[1] = {kNegInf};
+    if (tail < run.n) {
+        last[0] = run.one(tail);
+        take(st, last, 1);
     }
-    for (; j < whole; ++j) {
-        float v[kBatch];
+    // f(batch's values, how many) for batches from .. to - 1, the next one's loads in flight while one is taken
+    auto stream = [&](int from, int to, auto load, auto f) {
+        const int whole = min(to, run.pieces / (kThreads * R::kPer));
+        u32x4 w[R::kPer];
+        if (from < whole) {
 #pragma unroll
-        for (int i = 0; i < R::kPer; ++i) R::unpack(w[i], v + i * R::kPiece);
-        if (j + 1 < whole) {
-#pragma unroll
-            for (int i = 0; i < R::kPer; ++i) w[i] = run.load(((j + 1) * R::kPer + i) * kThreads + tid);
+            for (int i = 0; i < R::kPer; ++i) w[i] = load((from * R::kPer + i) * kThreads + tid);
         }
-        take(st, v, kBatch, j);
-    }
-    for (; j < run.batches; ++j) {
-        float v[kBatch];
-        int n = 0;
+        int j = from;
+        for (; j < whole; ++j) {
+            float v[kBatch];
 #pragma unroll
-        for (int i = 0; i < R::kPer; ++i) {
-            const int p = (j * R::kPer + i) * kThreads + tid;
-            if (p < run.pieces) {
-                R::unpack(run.load(p), v + i * R::kPiece);
-                n = (i + 1) * R::kPiece;
+            for (int i = 0; i < R::kPer; ++i) R::unpack(w[i], v + i * R::kPiece);
+            if (j + 1 < whole) {
+#pragma unroll
+                for (int i = 0; i < R::kPer; ++i) w[i] = load(((j + 1) * R::kPer + i) * kThreads + tid);
             }
+            f(v, kBatch, j);
         }
-        if (n > 0) take(st, v, n, j);
-    }
-    if (run.tail() + tid < run.n) {
-        const float v[1] = {run.one(run.tail() + tid)};
-        take(st, v, 1, run.batches);
-    }
-
-    uint64_t mine = 0;
-    if constexpr (kTop) {
-        // the first value of the thread's best batch that equals its maximum
-        const uint32_t top = order_of(st.m);
-        if (st.batch == run.batches) mine = key_of(st.m, first + run.tail() + tid);
-        else if (st.batch >= 0) {
+        for (; j < to; ++j) {  // (the run's last batch at most)
+            float v[kBatch];
+            int n = 0;
 #pragma unroll
-            for (int i = R::kPer - 1; i >= 0; --i) {
-                const int p = (st.batch * R::kPer + i) * kThreads + tid;
+            for (int i = 0; i < R::kPer; ++i) {
+                const int p = (j * R::kPer + i) * kThreads + tid;
                 if (p < run.pieces) {
-                    float v[R::kPiece];
-                    R::unpack(run.load(p), v);
-#pragma unroll
-                    for (int q = R::kPiece - 1; q >= 0; --q)
-                        if (order_of(v[q]) == top) mine = key_of(st.m, first + p * R::kPiece + q);
+                    R::unpack(load(p), v + i * R::kPiece);
+                    n = (i + 1) * R::kPiece;
                 }
             }
+            if (n > 0) f(v, n, j);
         }
+    };
+    auto index_of = [&](int j, int i) { return first + ((j * R::kPer + i / R::kPiece) * kThreads + tid) * R::kPiece + i % R::kPiece; };
+    const auto cached = [&](int p) { return run.load(p); };
+    const auto once = [&](int p) { return run.load_once(p); };
+    if constexpr (kTop) {
+        // (runs of a few batches give their bound from all of them)
+        const int part = run.batches <= 4 ? run.batches : (run.batches + 4) / 5;
+        stream(0, part, cached, [&](const float(&v)[kBatch], int n, int) { take(st, v, n); });
+        const bool any = tail < run.n || tid < run.pieces;
+        const uint32_t mine = any ? order_of(st.m) : 0;
+        bound = find_bound(buf, mine, a.k);
+        const auto look = [&](const float(&v)[kBatch], int n, int j) {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+                if (i < n && order_of(v[i]) >= bound) push(buf, key_of(v[i], index_of(j, i)));
+        };
+        if (any && mine >= bound) {
+            if (tail < run.n && order_of(last[0]) >= bound) push(buf, key_of(last[0], first + tail));
+            stream(0, part, cached, look);
+        }
+        const float least = bound <= kOrderNegInf ? kNegInf : key_value(static_cast<uint64_t>(bound) << 32);
+        stream(part, run.batches, once, [&](const float(&v)[kBatch], int n, int j) {
+            if (take(st, v, n) >= least) look(v, n, j);
+        });
+    } else {
+        stream(0, run.batches, once, [&](const float(&v)[kBatch], int n, int) { take(st, v, n); });
     }
     const Stats all = join_block(st, sbuf);
     Finish f{};
@@ -370,15 +376,14 @@ __global__ __launch_bounds__(kThreads) void logprob_rows_kernel(LogprobArgs a) {
     }
     if constexpr (kTop) {
         select(
-            buf, mine, a.k,
-            [&](int o, int lane, auto&& use) {
-                for (int p = o + lane * kThreads; p < run.pieces; p += 64 * kThreads) {
-                    float v[R::kPiece];
-                    R::unpack(run.load(p), v);
+            buf, a.k,
+            [&](auto&& use) {
+                if (tail < run.n) use(key_of(last[0], first + tail));
+                stream(0, run.batches, cached, [&](const float(&v)[kBatch], int n, int j) {
 #pragma unroll
-                    for (int q = 0; q < R::kPiece; ++q) use(key_of(v[q], first + p * R::kPiece + q));
-                }
-                if (lane == 0 && run.tail() + o < run.n) use(key_of(run.one(run.tail() + o), first + run.tail() + o));
+                    for (int i = 0; i < kBatch; ++i)
+                        if (i < n) use(key_of(v[i], index_of(j, i)));
+                });
             },
             [&](int place, uint64_t key) {
                 if (a.segments == 1) write_top(a, row, place, key, f);
@@ -407,13 +412,15 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
     const int n = a.segments * a.k;
     uint64_t mine = 0;
     for (int i = tid; i < n; i += kThreads) mine = keys[i] > mine ? keys[i] : mine;
-    select(
-        buf, mine, a.k,
-        [&](int o, int lane, auto&& use) {
-            for (int i = o + lane * kThreads; i < n; i += 64 * kThreads)
-                if (keys[i] != 0) use(keys[i]);
-        },
-        [&](int place, uint64_t key) { write_top(a, row, place, key, f); });
+    const uint32_t bound = find_bound(buf, static_cast<uint32_t>(mine >> 32), a.k);
+    const auto each = [&](auto&& use) {
+        for (int i = tid; i < n; i += kThreads)
+            if (keys[i] != 0) use(keys[i]);
+    };
+    each([&](uint64_t key) {
+        if (static_cast<uint32_t>(key >> 32) >= bound) push(buf, key);
+    });
+    select(buf, a.k, each, [&](int place, uint64_t key) { write_top(a, row, place, key, f); });
 }
 
 // Segments a row: enough workgroups to fill the CUs several times, none shorter than kMinSegment, their keys a few a thread.
