@@ -10,13 +10,17 @@
 // Work decomposition
 //   * Query rows that share a key/value head's keys go together, 16 to a matrix tile: the tokens and the query heads of
 //     its group for a batch row's own keys; for a shared prefix those of the whole batch, so that the prefix is read
-//     once for all of them. One kernel does both, in two launches.
-//   * A workgroup takes kNT tiles of 16 query rows and one chunk of the keys; chunks are as long as leaves a few
-//     workgroups a CU, and at least 128 keys. Each of its four waves takes every fourth block of 32 keys and keeps its
-//     own running maximum, sum and O; they meet in LDS once at the end. No wave waits for another in the loop, and no key
-//     passes through LDS: the cache lies in memory in the order in which the matrix instructions read it (kv_cache.h).
-//   * A chunk leaves its (m, l, unnormalised O) in the workspace, and a second kernel joins a row's chunks, the prefix's
-//     and its own, in a fixed order. Where one chunk has all of a row's keys it writes the result itself.
+//     once for all of them.
+//   * A workgroup has eight waves: kWq of them (1, 2, 4 or 8, as many as there are tiles) take a tile of 16 query rows each and
+//     the rest is spread over the keys, 32 at a time. Every wave keeps its own running maximum, sum and O; those of one
+//     tile meet in LDS once at the end. No wave waits for another in the loop, and no key passes through LDS: the cache lies
+//     in memory in the order in which the matrix instructions read it (kv_cache.h).
+//   * The keys of all (head, batch row, query tile) triples form one list, cut into as many equal shares as workgroups fit the
+//     CUs (two each), so ragged lengths leave no CU idle; a share may end within a triple and go on in the next. Short
+//     lists are not cut within a triple: a workgroup then has all keys of one, and no second kernel is needed.
+//     The prefix's keys are cut into chunks for workgroups of the same launch.
+//   * A workgroup that has all of a triple's keys writes the result itself; otherwise it leaves (m, l, unnormalised O) in the
+//     workspace, and a second kernel joins a row's parts, the prefix's and its own, in a fixed order.
 //
 // Arithmetic: S^T = K Q^T with v_mfma_f32_16x16x32_bf16 on the held values, which bf16 holds exactly (int8 and e4m3
 // alike); the key's scale multiplies the 32-bit score. P times the value's scale is rounded to bf16 (half a step,
@@ -39,14 +43,26 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 256, kWaves = 4;
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kJoinThreads = 256;
 constexpr int kD = DT_HEAD_DIM;
-constexpr int kMinChunk = kWaves * kKvBlock;
+constexpr int kObufRow = kD + 4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_huge_valf();
 
+// blocks in flight a wave: what 256 registers a lane hold, which leave two workgroups a CU
+constexpr int stages(int format) { return format == DT_KV_BF16 ? 1 : 2; }
+
+// The batch rows, by value in the kernel's arguments.
+struct AttnRows {
+    int32_t len[kMaxRaggedBatch];       // tokens held
+    int32_t cum[kMaxRaggedBatch];       // steps of one head before this row's, all query tiles
+    uint16_t slot[kMaxRaggedBatch];
+    uint16_t cnt[kMaxRaggedBatch];      // query tokens
+};
+
 struct CachedAttnArgs {
-    KvView c;
+    KvView own, pre;
     const void* q;
     void* o;
     float* m;  // nullable
@@ -57,14 +73,31 @@ struct CachedAttnArgs {
     int B, T, H, G;  // G: query heads a key/value head
     int causal;
     float scale;
-    int chunk;       // keys a workgroup
     int parts;       // partial results a row at most
-    int part0;       // the first of this launch's
-    int direct;      // one chunk has all keys: write the result
-    int prefix;      // the slot of the prefix whose keys all query rows share, or -1: each batch row its own
-    int prefix_len;
-    int tiles;       // workgroups over the query rows
+    // own keys: steps of 32 keys a key wave
+    int own_wq, own_tiles;
+    int head_steps;     // steps of one head: all batch rows and tiles
+    int own_groups;     // workgroups
+    int aligned;        // one (head, batch row, tile) each; otherwise shares of the list:
+    int share, extra;
+    // prefix
+    int pre_slot, pre_len, pre_wq, pre_tiles, pre_chunk;  // pre_chunk: keys a workgroup
+    int pre_parts, pre_groups;
 };
+
+// steps of a batch row's keys for a query tile (0: there is nothing to see)
+__host__ __device__ __forceinline__ int steps_of(int len, int cnt, int wq) {
+    const int keys = kKvBlock * kWaves / wq;
+    return cnt == 0 ? 0 : (len + keys - 1) / keys;
+}
+// The list's steps in equal shares: the first `extra` workgroups have one more than `share`. group_of: whose share step s is in.
+__host__ __device__ __forceinline__ int share_start(const CachedAttnArgs& a, int w) {
+    return w * a.share + (w < a.extra ? w : a.extra);
+}
+__host__ __device__ __forceinline__ int group_of(const CachedAttnArgs& a, int s) {
+    const int longer = a.extra * (a.share + 1);
+    return s < longer ? s / (a.share + 1) : a.extra + (s - longer) / a.share;
+}
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2){lo, hi}, bf16x2));
@@ -86,6 +119,10 @@ __device__ __forceinline__ float sum_groups(float x) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// keeps the compiler from widening a whole block at once, which would take 64 registers more than there are for two
+// workgroups a CU
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0); }
+
 // 8 held values (two words of 8-bit ones) as the bf16 operand of a matrix instruction
 template <int kFormat>
 __device__ __forceinline__ bf16x8 widen(uint32_t a, uint32_t b) {
@@ -106,33 +143,43 @@ __device__ __forceinline__ bf16x8 widen(uint32_t a, uint32_t b) {
     return r.v;
 }
 
-// A block's K (two tiles of 16 keys) or V (eight tiles of 16 values) as loaded: 16-byte pieces of a lane
-template <int kFormat>
+// A block as loaded: 16-byte pieces of K (two tiles of 16 keys) and V (eight tiles of 16 values), and the scales of the lane's
+// keys. kOnce: no other wave reads these keys, so they pass the caches by.
+template <int kFormat, bool kOnce>
 struct Block {
     static constexpr int kPieces = kFormat == DT_KV_BF16 ? 8 : 4;
-    u32x4 w[kPieces];
+    u32x4 k[kPieces], v[kPieces];
+    floatx4 ks[2], vs[2];
+    static __device__ __forceinline__ u32x4 load16(const uint8_t* p) {
+        if constexpr (kOnce) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+        return *reinterpret_cast<const u32x4*>(p);
+    }
+    __device__ __forceinline__ void load_k(const uint8_t* block, int lane) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) k[i] = load16(block + i * kKvRun + lane * 16);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) ks[t] = *reinterpret_cast<const floatx4*>(block + kv_scale_at(kFormat) + t * 64 + (lane >> 4) * 16);
+    }
+    __device__ __forceinline__ void load_v(const uint8_t* block, int lane) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) v[i] = load16(block + kv_tensor_bytes(kFormat) + i * kKvRun + lane * 16);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) vs[t] = *reinterpret_cast<const floatx4*>(block + kv_scale_at(kFormat) + 128 + t * 64 + (lane >> 4) * 16);
+    }
+    // the pieces as values of their own: else the compiler carries them through the loop widened, in twice or four times the
+    // registers
+    static __device__ __forceinline__ void settle(u32x4 (&w)[kPieces]) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) asm volatile("" : "+v"(w[i]));
+    }
     // operand i of 8: K tile i / 4, step i % 4; V tile i
-    __device__ __forceinline__ bf16x8 operand(int i) const {
+    static __device__ __forceinline__ bf16x8 operand(const u32x4 (&w)[kPieces], int i) {
         if constexpr (kFormat == DT_KV_BF16) return __builtin_bit_cast(bf16x8, w[i]);
         else return widen<kFormat>(w[i >> 1][(i & 1) * 2], w[i >> 1][(i & 1) * 2 + 1]);
     }
 };
 
-template <int kFormat>
-__device__ __forceinline__ void load_k(Block<kFormat>& r, const uint8_t* k, int lane) {
-    constexpr int kEs = kv_elem_bytes(kFormat), kPer = Block<kFormat>::kPieces / 2;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            r.w[t * kPer + i] = *reinterpret_cast<const u32x4*>(k + (t * 16 + (lane & 15)) * kD * kEs + i * 64 + (lane >> 4) * 16);
-}
-template <int kFormat>
-__device__ __forceinline__ void load_v(Block<kFormat>& r, const uint8_t* v, int lane) {
-#pragma unroll
-    for (int i = 0; i < Block<kFormat>::kPieces; ++i) r.w[i] = *reinterpret_cast<const u32x4*>(v + i * 1024 + lane * 16);
-}
-// the first of the 8 values that a lane group's operand of step s covers, in load_k's order
+// the first of the 8 values that a lane group's operand of step s covers, in k_offset's order
 template <int kFormat>
 __device__ __forceinline__ int k_dim(int s, int g) {
     if constexpr (kFormat == DT_KV_BF16) return s * 32 + g * 8;
@@ -143,319 +190,391 @@ struct QueryRow {
     int b, t, hq;
 };
 // row r of those that share key/value head hk's keys: tokens, then the group's heads; for the prefix the batch first
-__device__ __forceinline__ QueryRow query_row(const CachedAttnArgs& a, int r, int b, int hk) {
+__device__ __forceinline__ QueryRow query_row(const CachedAttnArgs& a, int r, int b, int hk, bool prefix) {
     const int g = r % a.G, bt = r / a.G;
-    if (a.prefix >= 0) return {bt / a.T, bt % a.T, hk * a.G + g};
+    if (prefix) return {bt / a.T, bt % a.T, hk * a.G + g};
     return {b, bt, hk * a.G + g};
 }
 
-template <int kFormat, bool kF32, int kNT>
-__global__ __launch_bounds__(kThreads) void cached_attn_kernel(CachedAttnArgs a, KvRows rows) {
+// One workgroup's stretch of keys for one (head, batch row, tile), or of the prefix for one (head, tile).
+struct Work {
+    int hk, b, tile;
+    int k0, k1;      // keys
+    int slot, len, cnt;  // cnt: the batch row's query tokens
+    int wq;
+    int part;        // where the partial result goes, or -1: the result is written
+    bool prefix;
+};
+
+// The thread's index as a value of its own: what is derived from it is then not worked out ahead of the loops around and held in
+// registers through them.
+__device__ __forceinline__ int thread_here() {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+
+struct Shared {
+    float o[kWaves][16][kObufRow];
+    float ml[kWaves][2][16];
+};
+
+template <int kFormat, bool kF32, bool kOnce>
+__device__ __forceinline__ void attend(const CachedAttnArgs& a, const AttnRows& rows, const Work& w, Shared& sh) {
     constexpr int kQS = kF32 ? 3 : 1;
-    __shared__ __align__(16) float obuf[2][kNT * 16][kD + 4];
-    __shared__ float ml[kWaves][2][kNT * 16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int tid = thread_here();
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
+    const int qw = wave % w.wq, kw = wave / w.wq, step = kKvBlock * kWaves / w.wq;
+    const uint8_t* base_block = (w.prefix ? a.pre : a.own).block<kFormat>(w.slot, w.hk, 0);
+    const auto block_at = [&](int key) { return base_block + static_cast<int64_t>(key / kKvBlock) * kv_block_bytes(kFormat); };
+    const int nrows = (w.prefix ? a.B : 1) * a.T * a.G;
+    const int row0 = w.tile * 16 * w.wq;
+    const int r = row0 + qw * 16 + n;
+    const bool have = r < nrows;
+    const QueryRow qr = query_row(a, have ? r : row0, w.b, w.hk, w.prefix);
 
-    // workgroups in launch order: eight (chunk, head, batch row) triples, one an XCD, all their query tiles before
-    // the next eight, so that the tiles which read the same keys run beside each other on one XCD's L2
-    int64_t id = blockIdx.x;
-    const int64_t chunks_total = gridDim.x / a.tiles;
-    int64_t item;
-    int tile;
-    {
-        const int64_t full = chunks_total / 8 * 8 * a.tiles;
-        if (id < full) {
-            const int64_t oct = id / (8 * a.tiles);
-            const int rem = static_cast<int>(id - oct * 8 * a.tiles);
-            tile = rem >> 3;
-            item = oct * 8 + (rem & 7);
-        } else {
-            id -= full;
-            const int left = static_cast<int>(chunks_total % 8);
-            tile = static_cast<int>(id / left);
-            item = chunks_total / 8 * 8 + id % left;
+    // the first blocks are under way before anything else
+    constexpr int kStages = stages(kFormat);
+    Block<kFormat, kOnce> st[kStages];
+    int kb = w.k0 + kw * kKvBlock;
+#pragma unroll
+    for (int i = 0; i < kStages; ++i)
+        if (kb + i * step < w.k1) {
+            st[i].load_k(block_at(kb + i * step), lane);
+            st[i].load_v(block_at(kb + i * step), lane);
         }
+
+    // Q fragment; keys below lim are seen by the lane's query, keys below minlim by all of the wave's
+    int lim = w.len;
+    if (have && !w.prefix && a.causal) {
+        if (qr.t < w.cnt) lim = max(0, min(w.len, w.len - w.cnt + qr.t + 1));
     }
-    const int hk = static_cast<int>(item % a.c.heads);
-    item /= a.c.heads;
-    const int nb = a.prefix >= 0 ? 1 : a.B;
-    const int b = static_cast<int>(item % nb), chunk = static_cast<int>(item / nb);
-
-    const int len = a.prefix >= 0 ? a.prefix_len : rows.len[b];
-    const int slot = a.prefix >= 0 ? a.prefix : rows.slot[b];
-    const int k0 = chunk * a.chunk;
-    if (k0 >= len && !(a.direct && chunk == 0)) return;  // (whole workgroups)
-    const int k1 = min(len, k0 + a.chunk);
-    const int nrows = (a.prefix >= 0 ? a.B : 1) * a.T * a.G;
-    const int row0 = tile * kNT * 16;
-
-    // Q fragments and each lane's query: keys below lim are seen
-    int lim[kNT];
-    bf16x8 qf[kNT][kQS][4];
-    float qscale[kNT];
-    int minlim = len;
-#pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
-        const int r = row0 + nt * 16 + n;
-        lim[nt] = len;
-        qscale[nt] = a.scale;
-        const bool have = r < nrows;
-        const QueryRow qr = query_row(a, have ? r : row0, b, hk);
-        const int64_t at = (static_cast<int64_t>(qr.b) * a.T + qr.t) * a.ldq + qr.hq * kD;
-        if (have && a.prefix < 0 && a.causal) {
-            const int cnt = rows.cnt[b];
-            if (qr.t < cnt) lim[nt] = max(0, min(len, len - cnt + qr.t + 1));
-        }
-        minlim = min(minlim, lim[nt]);
-        if constexpr (!kF32) {
-            const uint16_t* q = static_cast<const uint16_t*>(a.q) + at;
-#pragma unroll
-            for (int s = 0; s < 4; ++s) qf[nt][0][s] = *reinterpret_cast<const bf16x8*>(q + k_dim<kFormat>(s, g));
-        } else {
-            const float* q = static_cast<const float*>(a.q) + at;
-            float x[4][8];
-            uint32_t top = 0;
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const floatx4 lo = *reinterpret_cast<const floatx4*>(q + k_dim<kFormat>(s, g));
-                const floatx4 hi = *reinterpret_cast<const floatx4*>(q + k_dim<kFormat>(s, g) + 4);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[s][j] = lo[j], x[s][4 + j] = hi[j];
-            }
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[s][j]) & 0x7f800000u);
-            top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, 64)));
-            top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, 64)));
-            // exponents from 2^-126 to 2^126 have a reciprocal; rows beyond (and with infinities, NaN) stay as they are
-            const bool norm = top >= 0x00800000u && top <= 0x7e800000u;
-            const float inv = norm ? __uint_as_float(0x7f000000u - top) : 1.0f;
-            qscale[nt] = norm ? a.scale * __uint_as_float(top) : a.scale;
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float v = x[s][j] * inv, h = bf16_round(v), m = bf16_round(v - h);
-                    qf[nt][0][s][j] = static_cast<__bf16>(h);
-                    qf[nt][1][s][j] = static_cast<__bf16>(m);
-                    qf[nt][2][s][j] = static_cast<__bf16>(v - h - m);
-                }
-        }
-    }
+    int minlim = lim;
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) minlim = min(minlim, __shfl_xor(minlim, o, 64));
-
-    const int64_t head = static_cast<int64_t>(slot) * a.c.heads + hk;
-    constexpr int kEs = kv_elem_bytes(kFormat);
-    const uint8_t* kp = a.c.k + head * a.c.keys * kD * kEs;
-    const uint8_t* vp = a.c.v + head * a.c.keys * kD * kEs;
-    const float* ksp = a.c.ks + head * a.c.keys;
-    const float* vsp = a.c.vs + head * a.c.keys;
-
-    floatx4 acc[kNT][8];
-    float mrun[kNT], lrun[kNT];
+    float qscale = a.scale;
+    bf16x8 qf[kQS][4];
+    const int64_t qat = (static_cast<int64_t>(qr.b) * a.T + qr.t) * a.ldq + qr.hq * kD;
+    if constexpr (!kF32) {
+        const uint16_t* q = static_cast<const uint16_t*>(a.q) + qat;
 #pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
-        mrun[nt] = kNegInf;
-        lrun[nt] = 0.0f;
+        for (int s = 0; s < 4; ++s) qf[0][s] = *reinterpret_cast<const bf16x8*>(q + k_dim<kFormat>(s, g));
+    } else {
+        const float* q = static_cast<const float*>(a.q) + qat;
+        float x[4][8];
+        uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[nt][i] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s = 0; s < 4; ++s) {
+            const floatx4 lo = *reinterpret_cast<const floatx4*>(q + k_dim<kFormat>(s, g));
+            const floatx4 hi = *reinterpret_cast<const floatx4*>(q + k_dim<kFormat>(s, g) + 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[s][j] = lo[j], x[s][4 + j] = hi[j];
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[s][j]) & 0x7f800000u);
+        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, 64)));
+        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, 64)));
+        // exponents from 2^-126 to 2^126 have a reciprocal; rows beyond (and with infinities, NaN) stay as they are
+        const bool norm = top >= 0x00800000u && top <= 0x7e800000u;
+        const float inv = norm ? __uint_as_float(0x7f000000u - top) : 1.0f;
+        qscale = norm ? a.scale * __uint_as_float(top) : a.scale;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float v = x[s][j] * inv, h = bf16_round(v), m = bf16_round(v - h);
+                qf[0][s][j] = static_cast<__bf16>(h);
+                qf[1][s][j] = static_cast<__bf16>(m);
+                qf[2][s][j] = static_cast<__bf16>(v - h - m);
+            }
     }
 
-    for (int kb = k0 + wave * kKvBlock; kb < k1; kb += kWaves * kKvBlock) {
-        Block<kFormat> kr, vr;
-        load_k<kFormat>(kr, kp + static_cast<int64_t>(kb) * kD * kEs, lane);
-        floatx4 ks[2], vs[2];
+    floatx4 acc[8];
+    float mrun = kNegInf, lrun = 0.0f;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) ks[t] = *reinterpret_cast<const floatx4*>(ksp + kb + t * 16 + g * 4);
-        load_v<kFormat>(vr, vp + static_cast<int64_t>(kb) * kD * kEs, lane);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) vs[t] = *reinterpret_cast<const floatx4*>(vsp + kb + t * 16 + g * 4);
+    for (int i = 0; i < 8; ++i) acc[i] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
 
-        floatx4 s[kNT][2];
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) s[nt][0] = s[nt][1] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+    // one block: scores, probabilities, O; its registers are filled again, K's behind the scores and V's behind O, with the block
+    // kStages steps on
+    auto take = [&](Block<kFormat, kOnce>& blk) {
+        const int next = kb + kStages * step;
+        const bool more = next < w.k1;
+        blk.settle(blk.k);
+        floatx4 s[2];
+        s[0] = s[1] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const bf16x8 kf = kr.operand(i);
+            const bf16x8 kf = blk.operand(blk.k, i);
 #pragma unroll
-            for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-                for (int x = kQS - 1; x >= 0; --x)
-                    s[nt][i >> 2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[nt][x][i & 3], s[nt][i >> 2], 0, 0, 0);
+            for (int x = kQS - 1; x >= 0; --x) s[i >> 2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[x][i & 3], s[i >> 2], 0, 0, 0);
+            keep_order();
         }
-
+        float mx = kNegInf;
         const bool mask = kb + kKvBlock > minlim;  // (the same for the whole wave)
-        bf16x8 pf[kNT][kQS];
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) {
-            float mx = kNegInf;
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float v = s[nt][t][i] * (ks[t][i] * qscale[nt]);
-                    if (mask && kb + t * 16 + g * 4 + i >= lim[nt]) v = kNegInf;
-                    s[nt][t][i] = v;
-                    mx = fmaxf(mx, v);
-                }
-            mx = fmaxf(max_groups(mx), mrun[nt]);
-            const float base = mx == kNegInf ? 0.0f : mx;  // (nothing seen yet: every p is 0)
-            if (__any(mx != mrun[nt])) {
-                const float f = __builtin_amdgcn_exp2f((mrun[nt] - base) * kLog2e);
-                lrun[nt] *= f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) acc[nt][i] *= f;
-                mrun[nt] = mx;
+            for (int i = 0; i < 4; ++i) {
+                s[t][i] *= blk.ks[t][i] * qscale;
+                mx = fmaxf(mx, s[t][i]);
             }
-            float p[8], sum = 0.0f;
+        if (mask) {
+            mx = kNegInf;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float e = __builtin_amdgcn_exp2f((s[nt][t][i] - base) * kLog2e);
-                    sum += e;
-                    p[t * 4 + i] = e * vs[t][i];
-                    // a masked key's scale may be anything, NaN too
-                    if (mask && kb + t * 16 + g * 4 + i >= lim[nt]) p[t * 4 + i] = 0.0f;
+                    if (kb + t * 16 + g * 4 + i >= lim) s[t][i] = kNegInf;
+                    mx = fmaxf(mx, s[t][i]);
                 }
-            lrun[nt] += sum;
+        }
+        keep_order();
+        if (more) blk.load_k(block_at(next), lane);
+        keep_order();
+        mx = fmaxf(max_groups(mx), mrun);
+        const float base = mx == kNegInf ? 0.0f : mx;  // (nothing seen yet: every p is 0)
+        if (__any(mx != mrun)) {
+            const float f = __builtin_amdgcn_exp2f((mrun - base) * kLog2e);
+            lrun *= f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] *= f;
+            mrun = mx;
+        }
+        float p[8], sum = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float e = __builtin_amdgcn_exp2f((s[t][i] - base) * kLog2e);
+                sum += e;
+                p[t * 4 + i] = e * blk.vs[t][i];
+            }
+        if (mask) {  // (a masked key's scale may be anything, NaN too)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (kb + (i >> 2) * 16 + g * 4 + (i & 3) >= lim) p[i] = 0.0f;
+        }
+        lrun += sum;
+        blk.settle(blk.v);
+        bf16x8 pf[kQS];
+#pragma unroll
+        for (int x = 0; x < kQS; ++x) {
             union { uint32_t u[4]; bf16x8 v; } f;
 #pragma unroll
-            for (int x = 0; x < kQS; ++x) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    f.u[j] = pack2(p[2 * j], p[2 * j + 1]);
-                    if (x + 1 < kQS) {
-                        p[2 * j] -= __uint_as_float(f.u[j] << 16);
-                        p[2 * j + 1] -= __uint_as_float(f.u[j] & 0xffff0000u);
-                    }
+            for (int j = 0; j < 4; ++j) {
+                f.u[j] = pack2(p[2 * j], p[2 * j + 1]);
+                if (x + 1 < kQS) {
+                    p[2 * j] -= __uint_as_float(f.u[j] << 16);
+                    p[2 * j + 1] -= __uint_as_float(f.u[j] & 0xffff0000u);
                 }
-                pf[nt][x] = f.v;
             }
+            pf[x] = f.v;
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const bf16x8 vf = vr.operand(i);
+            const bf16x8 vf = blk.operand(blk.v, i);
 #pragma unroll
-            for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-                for (int x = kQS - 1; x >= 0; --x)
-                    acc[nt][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[nt][x], acc[nt][i], 0, 0, 0);
+            for (int x = kQS - 1; x >= 0; --x) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[x], acc[i], 0, 0, 0);
+            keep_order();
+        }
+        if (more) blk.load_v(block_at(next), lane);
+        kb += step;
+    };
+    while (kb < w.k1) {
+        take(st[0]);
+        if constexpr (kStages > 1) {
+            if (kb >= w.k1) break;
+            take(st[1]);
         }
     }
 
-    // the four waves' results: scaled to the common maximum, waves 2 and 3 onto 0 and 1, then 1 onto 0
-#pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
-        lrun[nt] = sum_groups(lrun[nt]);
-        if (g == 0) {
-            ml[wave][0][nt * 16 + n] = mrun[nt];
-            ml[wave][1][nt * 16 + n] = lrun[nt];
-        }
+    // the waves' results meet: a thread sums four values of a row over the key waves, scaled to their common maximum
+    lrun = sum_groups(lrun);
+    if (g == 0) {
+        sh.ml[wave][0][n] = mrun;
+        sh.ml[wave][1][n] = lrun;
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) *reinterpret_cast<floatx4*>(&sh.o[wave][n][i * 16 + g * 4]) = acc[i];
     __syncthreads();
-    float mall[kNT], lall[kNT];
-#pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
+    const int wk = kWaves / w.wq;
+    for (int it = thread_here(); it < w.wq * 16 * (kD / 4); it += kThreads) {
+        const int d = (it & 31) * 4, rt = it >> 5;  // (row within the workgroup's tiles)
+        const int tq = rt >> 4, rn = rt & 15;
+        if (row0 + rt >= nrows) continue;
         float mx = kNegInf;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, ml[w][0][nt * 16 + n]);
+        for (int k = 0; k < wk; ++k) mx = fmaxf(mx, sh.ml[k * w.wq + tq][0][rn]);
         const float base = mx == kNegInf ? 0.0f : mx;
-        float sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const float f = __builtin_amdgcn_exp2f((ml[w][0][nt * 16 + n] - base) * kLog2e);
-            sum += f * ml[w][1][nt * 16 + n];
-            if (w == wave) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) acc[nt][i] *= f;
-            }
+        float l = 0.0f;
+        floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 0; k < wk; ++k) {
+            const int from = k * w.wq + tq;
+            const float f = __builtin_amdgcn_exp2f((sh.ml[from][0][rn] - base) * kLog2e);
+            l += f * sh.ml[from][1][rn];
+            v += f * *reinterpret_cast<const floatx4*>(&sh.o[from][rn][d]);
         }
-        mall[nt] = mx;
-        lall[nt] = sum;
-    }
-#pragma unroll
-    for (int step = 2; step >= 1; step >>= 1) {
-        if (wave >= step && wave < 2 * step) {
-#pragma unroll
-            for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    *reinterpret_cast<floatx4*>(&obuf[wave - step][nt * 16 + n][i * 16 + g * 4]) = acc[nt][i];
-        }
-        __syncthreads();
-        if (wave < step) {
-#pragma unroll
-            for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    acc[nt][i] += *reinterpret_cast<const floatx4*>(&obuf[wave][nt * 16 + n][i * 16 + g * 4]);
-        }
-        __syncthreads();
-    }
-    if (wave != 0) return;
-#pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
-        const int r = row0 + nt * 16 + n;
-        if (r >= nrows) continue;
-        const QueryRow qr = query_row(a, r, b, hk);
-        const int64_t row = (static_cast<int64_t>(qr.b) * a.T + qr.t) * a.H + qr.hq;
-        if (a.direct) {
-            const bool nan = lall[nt] != lall[nt];  // (a maximum passes NaN scores over: they show in the sum)
-            const bool empty = qr.t >= rows.cnt[qr.b] || (mall[nt] == kNegInf && !nan);
-            const float inv = empty ? 0.0f : 1.0f / lall[nt];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int64_t at = row * kD + i * 16 + g * 4;
-                floatx4 v = acc[nt][i] * inv;
-                if (empty) v = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
-                if constexpr (kF32) *reinterpret_cast<floatx4*>(static_cast<float*>(a.o) + at) = v;
-                else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
-            }
-            if (g == 0) {
-                if (a.m) a.m[row] = empty ? kNegInf : nan ? lall[nt] : mall[nt];
-                if (a.l) a.l[row] = empty ? 0.0f : lall[nt];
+        const QueryRow to = query_row(a, row0 + rt, w.b, w.hk, w.prefix);
+        const int64_t row = (static_cast<int64_t>(to.b) * a.T + to.t) * a.H + to.hq;
+        if (w.part < 0) {
+            const bool nan = l != l;  // (a maximum passes NaN scores over: they show in the sum)
+            const bool empty = to.t >= rows.cnt[to.b] || (mx == kNegInf && !nan);
+            v = empty ? (floatx4){0.0f, 0.0f, 0.0f, 0.0f} : v * (1.0f / l);
+            const int64_t at = row * kD + d;
+            if constexpr (kF32) *reinterpret_cast<floatx4*>(static_cast<float*>(a.o) + at) = v;
+            else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+            if (d == 0) {
+                if (a.m) a.m[row] = empty ? kNegInf : nan ? l : mx;
+                if (a.l) a.l[row] = empty ? 0.0f : l;
             }
         } else {
-            const int64_t part = row * a.parts + a.part0 + chunk;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) *reinterpret_cast<floatx4*>(a.part_o + part * kD + i * 16 + g * 4) = acc[nt][i];
-            if (g == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(mall[nt], lall[nt]);
+            const int64_t part = row * a.parts + w.part;
+            *reinterpret_cast<floatx4*>(a.part_o + part * kD + d) = v;
+            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(mx, l);
         }
+    }
+}
+
+template <int kFormat, bool kF32, bool kOnce>
+__global__ __launch_bounds__(kThreads, 2) void cached_attn_kernel(CachedAttnArgs a, AttnRows rows) {
+    __shared__ __align__(16) Shared sh;
+    __shared__ AttnRows rl;
+    // the batch rows into LDS: one trip to the arguments' memory in place of one for each dependent use
+    for (int i = threadIdx.x; i < a.B; i += kThreads) {
+        rl.len[i] = rows.len[i];
+        rl.cum[i] = rows.cum[i];
+        rl.slot[i] = rows.slot[i];
+        rl.cnt[i] = rows.cnt[i];
+    }
+    __syncthreads();
+    int id = blockIdx.x;
+    Work w;
+    w.prefix = id < a.pre_groups;
+    w.wq = w.prefix ? a.pre_wq : a.own_wq;
+    const int keys = kKvBlock * kWaves / w.wq;
+    int s = 0, end = 0;
+    if (w.prefix) {
+        // tiles of one chunk beside each other on one XCD (workgroups go to the eight XCDs in turn), which reads it once
+        const int chunks = a.pre_groups / a.pre_tiles, full = chunks / 8 * 8 * a.pre_tiles;
+        int item;
+        if (id < full) {
+            const int oct = id / (8 * a.pre_tiles), rem = id % (8 * a.pre_tiles);
+            w.tile = rem >> 3;
+            item = oct * 8 + (rem & 7);
+        } else {
+            const int left = chunks % 8;
+            w.tile = (id - full) / left;
+            item = chunks / 8 * 8 + (id - full) % left;
+        }
+        w.hk = item % a.pre.heads;
+        w.b = 0;
+        w.part = item / a.pre.heads;
+        w.k0 = w.part * a.pre_chunk;
+        w.k1 = min(a.pre_len, w.k0 + a.pre_chunk);
+        w.slot = a.pre_slot;
+        w.len = a.pre_len;
+        w.cnt = 0;
+    } else {
+        id -= a.pre_groups;
+        // the list's neighbours on one XCD: they may share keys
+        const int full = a.own_groups / 8 * 8;
+        if (id < full) id = (id & 7) * (a.own_groups / 8) + (id >> 3);
+        if (a.aligned) {
+            w.tile = id % a.own_tiles;
+            w.b = id / a.own_tiles % a.B;
+            w.hk = id / a.own_tiles / a.B;
+            w.part = a.pre_parts > 0 ? a.pre_parts : -1;
+        } else {
+            s = share_start(a, id);
+            end = share_start(a, id + 1);
+        }
+    }
+    for (;;) {
+        if (!w.prefix) {
+            int off = 0, count;
+            if (a.aligned) {
+                w.len = __builtin_amdgcn_readfirstlane(rl.len[w.b]);
+                w.cnt = __builtin_amdgcn_readfirstlane(rl.cnt[w.b]);
+                count = steps_of(w.len, w.cnt, w.wq);
+            } else {
+                w.hk = s / a.head_steps;
+                const int in_head = s - w.hk * a.head_steps;
+                // the last batch row that begins at or before this step (rows without steps begin where the next one does)
+                int below = 0;
+#pragma unroll
+                for (int i = 0; i < kMaxRaggedBatch / 64; ++i) {
+                    const int at = i * 64 + (threadIdx.x & 63);
+                    if (i * 64 < a.B) below += __popcll(__ballot(at < a.B && rl.cum[at] <= in_head));
+                }
+                w.b = __builtin_amdgcn_readfirstlane(below) - 1;
+                w.len = __builtin_amdgcn_readfirstlane(rl.len[w.b]);
+                w.cnt = __builtin_amdgcn_readfirstlane(rl.cnt[w.b]);
+                const int steps = steps_of(w.len, w.cnt, w.wq);
+                const int in_row = in_head - __builtin_amdgcn_readfirstlane(rl.cum[w.b]);
+                w.tile = in_row / steps;
+                off = in_row - w.tile * steps;
+                count = min(steps - off, end - s);
+                w.part = a.pre_parts == 0 && count == steps ? -1 : a.pre_parts + id - group_of(a, s - off);
+                s += count;
+            }
+            w.slot = __builtin_amdgcn_readfirstlane(rl.slot[w.b]);
+            w.k0 = off * keys;
+            w.k1 = min(w.len, (off + count) * keys);
+            if (a.causal) {  // nothing past the tile's newest query
+                const int t = min(a.T - 1, ((w.tile + 1) * 16 * w.wq - 1) / a.G);
+                w.k1 = min(w.k1, max(0, w.len - w.cnt + t + 1));
+            }
+        }
+        attend<kFormat, kF32, kOnce>(a, rl, w, sh);
+        if (s >= end) return;
+        __syncthreads();  // the next stretch writes the shared results
     }
 }
 
 // Joins a row's partial results: one workgroup a row, 32 threads across the 128 values, eight runs of parts.
 template <bool kF32>
-__global__ __launch_bounds__(kThreads) void cached_attn_join_kernel(CachedAttnArgs a, KvRows rows, int prefix_parts, int own_chunk) {
-    __shared__ float red[kWaves];
+__global__ __launch_bounds__(kJoinThreads) void cached_attn_join_kernel(CachedAttnArgs a, AttnRows rows) {
+    __shared__ float red[kJoinThreads / 64];
     __shared__ float lred[8];
     __shared__ __align__(16) float obuf[8][kD];
     const int64_t row = blockIdx.x;
-    const int b = static_cast<int>(row / (static_cast<int64_t>(a.T) * a.H));
-    const int t = static_cast<int>(row / a.H % a.T);
-    const int len = rows.len[b];
-    const int parts = t < rows.cnt[b] ? prefix_parts + (len + own_chunk - 1) / own_chunk : 0;
     const float* pml = a.part_ml + row * a.parts * 2;
     const float* po = a.part_o + row * a.parts * kD;
-    float mx = kNegInf;
-    for (int p = threadIdx.x; p < parts; p += kThreads) mx = fmaxf(mx, pml[2 * p]);
+    const int run = threadIdx.x >> 5, d = (threadIdx.x & 31) * 4;
+    // the first parts' values are under way before it is known how many there are
+    floatx4 v0 = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (run < a.parts) v0 = *reinterpret_cast<const floatx4*>(po + static_cast<int64_t>(run) * kD + d);
+    float2 s0 = make_float2(kNegInf, 0.0f);
+    if (static_cast<int>(threadIdx.x) < a.parts) s0 = *reinterpret_cast<const float2*>(pml + 2 * threadIdx.x);
+    const int hq = static_cast<int>(row % a.H), bt = static_cast<int>(row / a.H);
+    const int b = bt / a.T, t = bt % a.T;
+    int parts = 0;
+    if (t < rows.cnt[b]) {
+        const int steps = steps_of(rows.len[b], rows.cnt[b], a.own_wq);
+        int own = steps > 0;
+        if (own && !a.aligned) {
+            const int first = hq / a.G * a.head_steps + rows.cum[b] + (t * a.G + hq % a.G) / (16 * a.own_wq) * steps;
+            own = group_of(a, first + steps - 1) - group_of(a, first) + 1;
+        }
+        if (own == 1 && a.pre_parts == 0) return;  // (written already)
+        parts = own + a.pre_parts;
+    }
+    float mx = static_cast<int>(threadIdx.x) < parts ? s0.x : kNegInf;
+    for (int p = threadIdx.x + kJoinThreads; p < parts; p += kJoinThreads) mx = fmaxf(mx, pml[2 * p]);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mx;
     __syncthreads();
     mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const float base = mx == kNegInf ? 0.0f : mx;
-    const int run = threadIdx.x >> 5, d = (threadIdx.x & 31) * 4;
     floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     float l = 0.0f;
 #pragma unroll 4
     for (int p = run; p < parts; p += 8) {
         const float2 s = *reinterpret_cast<const float2*>(pml + 2 * p);
-        const floatx4 v = *reinterpret_cast<const floatx4*>(po + static_cast<int64_t>(p) * kD + d);
+        const floatx4 v = p == run ? v0 : *reinterpret_cast<const floatx4*>(po + static_cast<int64_t>(p) * kD + d);
         const float f = __builtin_amdgcn_exp2f((s.x - base) * kLog2e);
         l += f * s.y;
         acc += f * v;
@@ -483,114 +602,95 @@ __global__ __launch_bounds__(kThreads) void cached_attn_join_kernel(CachedAttnAr
     }
 }
 
-// How a call is cut: chunks of the batch rows' own keys and of the prefix's, partial results a row.
-struct Plan {
-    int own_chunk = kMinChunk, prefix_chunk = kMinChunk;
-    int own_parts = 0, prefix_parts = 0;  // the longest row's
-    int own_nt = 1, prefix_nt = 1;
-    bool direct = false;
-    int64_t ws_bytes = 0;
-};
+constexpr int kCus = 256;
+constexpr int kWholeSteps = 4;     // up to so many steps (of 256 keys for one query tile) a triple's keys are not cut
 
-// query tiles of 16 rows that a workgroup takes
-int tiles_for(int64_t rows, int dtype) {
-    if (dtype != DT_BF16) return 1;
-    return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-}
+// waves that take query tiles: as many as there are tiles of 16 rows
+int query_waves(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : kWaves == 4 || rows <= 64 ? 4 : 8; }
 
-// keys a chunk: about `target` workgroups over all of `keys` (times heads and query tiles), whole blocks for every wave
-int chunk_for(int64_t keys, int64_t per_key, int target) {
-    const int64_t c = (keys * per_key + target - 1) / target;
-    return static_cast<int>(std::min<int64_t>(std::max<int64_t>((c + kMinChunk - 1) / kMinChunk, 1) * kMinChunk, kMaxCacheTokens));
-}
-
-Plan make_plan(const dt_kv_cache* c, int B, int T, int H, const KvRows& rows, const dt_kv_cache* prefix, int prefix_len, int dtype) {
-    constexpr int kTarget = 1024;  // workgroups: four a CU
-    Plan p;
-    const int G = H / c->heads;
-    const int64_t own_rows = static_cast<int64_t>(T) * G, all_rows = own_rows * B;
-    p.own_nt = tiles_for(own_rows, dtype);
-    p.prefix_nt = tiles_for(all_rows, dtype);
-    int64_t keys = 0;
-    int longest = 0;
-    for (int b = 0; b < B; ++b) {
-        if (rows.cnt[b] == 0) continue;
-        keys += rows.len[b];
-        longest = std::max(longest, rows.len[b]);
-    }
-    const int64_t own_tiles = (own_rows + 16 * p.own_nt - 1) / (16 * p.own_nt);
-    p.own_chunk = chunk_for(keys, own_tiles * c->heads, kTarget);
-    p.own_parts = (longest + p.own_chunk - 1) / p.own_chunk;
-    if (prefix && prefix_len > 0) {
-        const int64_t tiles = (all_rows + 16 * p.prefix_nt - 1) / (16 * p.prefix_nt);
-        p.prefix_chunk = chunk_for(prefix_len, tiles * c->heads, kTarget);
-        p.prefix_parts = (prefix_len + p.prefix_chunk - 1) / p.prefix_chunk;
-    }
-    p.direct = p.prefix_parts == 0 && p.own_parts <= 1;
-    if (!p.direct) p.ws_bytes = all_rows * c->heads * (p.own_parts + p.prefix_parts) * (kD + 2) * static_cast<int64_t>(sizeof(float));
-    return p;
-}
-
-template <int kFormat, bool kF32>
-int launch_tiles(CachedAttnArgs a, const KvRows& rows, int nt, int64_t items, int64_t qrows, hipStream_t s) {
-    a.tiles = static_cast<int>((qrows + 16 * nt - 1) / (16 * nt));
-    const int64_t grid = items * a.tiles;
-    if (grid == 0) return DT_OK;
-    if (grid > 0x7fffff) return set_error(DT_ERR_UNSUPPORTED, "the call needs %lld workgroups", (long long)grid);
-    const dim3 g(static_cast<unsigned>(grid)), t(kThreads);
-    if (nt == 1) hipLaunchKernelGGL((cached_attn_kernel<kFormat, kF32, 1>), g, t, 0, s, a, rows);
-    else if constexpr (!kF32) {
-        if (nt == 2) hipLaunchKernelGGL((cached_attn_kernel<kFormat, kF32, 2>), g, t, 0, s, a, rows);
-        else hipLaunchKernelGGL((cached_attn_kernel<kFormat, kF32, 4>), g, t, 0, s, a, rows);
-    }
-    DT_HIP_TRY(hipGetLastError());
-    return DT_OK;
-}
-
-int launch_part(const CachedAttnArgs& a, const KvRows& rows, int format, int dtype, int nt, int64_t items, int64_t qrows, hipStream_t s) {
-    const bool f32 = dtype != DT_BF16;
-    if (format == DT_KV_INT8)
-        return f32 ? launch_tiles<DT_KV_INT8, true>(a, rows, nt, items, qrows, s) : launch_tiles<DT_KV_INT8, false>(a, rows, nt, items, qrows, s);
-    if (format == DT_KV_FP8)
-        return f32 ? launch_tiles<DT_KV_FP8, true>(a, rows, nt, items, qrows, s) : launch_tiles<DT_KV_FP8, false>(a, rows, nt, items, qrows, s);
-    return f32 ? launch_tiles<DT_KV_BF16, true>(a, rows, nt, items, qrows, s) : launch_tiles<DT_KV_BF16, false>(a, rows, nt, items, qrows, s);
-}
-
-int run(const dt_kv_cache* c, CachedAttnArgs a, const KvRows& rows, const dt_kv_cache* prefix, int prefix_slot, int prefix_len,
-        const Plan& p, void* ws, int dtype, hipStream_t s) {
+// How a call is cut; fills rows' cum and the arguments that follow from the sizes. Returns the workspace's bytes.
+int64_t make_plan(CachedAttnArgs& a, AttnRows& rows, bool* join) {
+    constexpr int kResident = 2 * kCus;
+    const int heads = a.own.heads;
     const int64_t own_rows = static_cast<int64_t>(a.T) * a.G, all_rows = own_rows * a.B;
-    a.parts = p.own_parts + p.prefix_parts;
-    a.part_o = static_cast<float*>(ws);
-    a.part_ml = ws ? a.part_o + all_rows * c->heads * a.parts * kD : nullptr;
-    a.direct = p.direct;
-    if (p.prefix_parts > 0) {
-        CachedAttnArgs f = a;
-        f.c = prefix->view();
-        f.prefix = prefix_slot;
-        f.prefix_len = prefix_len;
-        f.chunk = p.prefix_chunk;
-        f.part0 = 0;
-        DT_TRY(launch_part(f, rows, c->format, dtype, p.prefix_nt, static_cast<int64_t>(p.prefix_parts) * c->heads, all_rows, s));
+    a.own_wq = query_waves(own_rows);
+    a.own_tiles = static_cast<int>((own_rows + 16 * a.own_wq - 1) / (16 * a.own_wq));
+    int longest = 0, shortest = kMaxCacheTokens;
+    int64_t cum = 0;
+    for (int b = 0; b < a.B; ++b) {
+        rows.cum[b] = static_cast<int>(cum);
+        const int n = steps_of(rows.len[b], rows.cnt[b], a.own_wq);
+        cum += static_cast<int64_t>(n) * a.own_tiles;
+        longest = std::max(longest, n);
+        shortest = std::min(shortest, n);
     }
-    a.c = c->view();
-    a.prefix = -1;
-    a.prefix_len = 0;
-    a.chunk = p.own_chunk;
-    a.part0 = p.prefix_parts;
-    // (a call with nothing to see still writes its empty rows)
-    const int64_t items = static_cast<int64_t>(p.direct ? 1 : p.own_parts) * a.B * c->heads;
-    DT_TRY(launch_part(a, rows, c->format, dtype, p.own_nt, items, own_rows, s));
-    if (p.direct) return DT_OK;
-    const dim3 g(static_cast<unsigned>(all_rows * c->heads)), t(kThreads);
-    if (dtype == DT_BF16) hipLaunchKernelGGL((cached_attn_join_kernel<false>), g, t, 0, s, a, rows, p.prefix_parts, p.own_chunk);
-    else hipLaunchKernelGGL((cached_attn_join_kernel<true>), g, t, 0, s, a, rows, p.prefix_parts, p.own_chunk);
+    const int64_t all = cum * heads, triples = static_cast<int64_t>(heads) * a.B * a.own_tiles;
+
+    a.pre_wq = a.pre_tiles = 1;
+    a.pre_chunk = a.pre_parts = a.pre_groups = 0;
+    if (a.pre_len > 0) {
+        // as many of the workgroups as the prefix has of the waves' work
+        a.pre_wq = query_waves(all_rows);
+        a.pre_tiles = static_cast<int>((all_rows + 16 * a.pre_wq - 1) / (16 * a.pre_wq));
+        const int unit = kKvBlock * kWaves / a.pre_wq;
+        const int64_t steps = (a.pre_len + unit - 1) / unit, per_chunk = static_cast<int64_t>(a.pre_tiles) * heads;
+        const int64_t groups = std::max<int64_t>(kResident * (steps * per_chunk) / (steps * per_chunk + all), 1);
+        // but at least four steps each: a workgroup's start and end cost about as much
+        const int64_t chunks = std::max<int64_t>(1, groups / per_chunk), each = std::max<int64_t>(4, (steps + chunks - 1) / chunks);
+        a.pre_chunk = static_cast<int>(std::min(each, steps) * unit);
+        a.pre_parts = (a.pre_len + a.pre_chunk - 1) / a.pre_chunk;
+        a.pre_groups = static_cast<int>(a.pre_parts * per_chunk);
+    }
+
+    const int64_t slots = std::max<int64_t>(kResident - a.pre_groups, kResident / 4);
+    // (a list past 2^30 steps, thousands of query tiles over the longest cache, has triples enough)
+    a.aligned = all > (1 << 30) || (longest <= kWholeSteps && (a.pre_groups == 0 || triples <= slots));
+    a.head_steps = a.aligned ? 0 : static_cast<int>(cum);
+    a.own_groups = static_cast<int>(a.aligned ? triples : std::min<int64_t>(all, slots));
+    int own_parts = 1;
+    bool whole = true;  // every triple's keys in one workgroup
+    if (!a.aligned) {
+        a.share = static_cast<int>(all / a.own_groups);
+        a.extra = static_cast<int>(all % a.own_groups);
+        own_parts = std::min(longest, (longest - 1) / a.share + 2);
+        whole = shortest == longest && a.extra == 0 && a.share % longest == 0;
+    }
+    a.parts = own_parts + a.pre_parts;
+    *join = !(whole && a.pre_parts == 0);
+    return *join ? all_rows * heads * a.parts * (kD + 2) * static_cast<int64_t>(sizeof(float)) : 0;
+}
+
+int launch(const CachedAttnArgs& a, const AttnRows& rows, bool join, int format, int dtype, hipStream_t s) {
+    const int64_t groups = static_cast<int64_t>(a.own_groups) + a.pre_groups;
+    if (groups > 0x7fffff) return set_error(DT_ERR_UNSUPPORTED, "the call needs %lld workgroups", (long long)groups);
+    const bool f32 = dtype != DT_BF16;
+    const bool once = a.own_wq == 1 && a.own_tiles == 1;
+    if (groups > 0) {
+        const dim3 g(static_cast<unsigned>(groups)), t(kThreads);
+#define DT_GO(F)                                                                                        \
+    do {                                                                                                \
+        if (f32 && once) hipLaunchKernelGGL((cached_attn_kernel<F, true, true>), g, t, 0, s, a, rows);  \
+        else if (f32) hipLaunchKernelGGL((cached_attn_kernel<F, true, false>), g, t, 0, s, a, rows);    \
+        else if (once) hipLaunchKernelGGL((cached_attn_kernel<F, false, true>), g, t, 0, s, a, rows);   \
+        else hipLaunchKernelGGL((cached_attn_kernel<F, false, false>), g, t, 0, s, a, rows);            \
+    } while (0)
+        if (format == DT_KV_INT8) DT_GO(DT_KV_INT8);
+        else if (format == DT_KV_FP8) DT_GO(DT_KV_FP8);
+        else DT_GO(DT_KV_BF16);
+#undef DT_GO
+        DT_HIP_TRY(hipGetLastError());
+    }
+    if (!join) return DT_OK;
+    const dim3 g(static_cast<unsigned>(static_cast<int64_t>(a.B) * a.T * a.H)), t(kJoinThreads);
+    if (f32) hipLaunchKernelGGL((cached_attn_join_kernel<true>), g, t, 0, s, a, rows);
+    else hipLaunchKernelGGL((cached_attn_join_kernel<false>), g, t, 0, s, a, rows);
     DT_HIP_TRY(hipGetLastError());
     return DT_OK;
 }
 
 // what dt_cached_attn_fwd and its workspace query check alike; fills rows
 int check_call(const dt_kv_cache* cache, int B, int T, int H, int D, const int32_t* slots, const int32_t* counts,
-               const dt_kv_cache* prefix, int prefix_slot, int dtype, KvRows* rows) {
+               const dt_kv_cache* prefix, int prefix_slot, int dtype, CachedAttnArgs* a, AttnRows* out) {
     if (D != DT_HEAD_DIM) return set_error(DT_ERR_UNSUPPORTED, "head_dim D=%d, kernels are built for D=%d", D, DT_HEAD_DIM);
     if (B < 1 || T < 1 || H < 1) return set_error(DT_ERR_INVALID_ARG, "B=%d, T=%d, H=%d must be >= 1", B, T, H);
     if (B > kMaxRaggedBatch) return set_error(DT_ERR_UNSUPPORTED, "B=%d > %d", B, kMaxRaggedBatch);
@@ -601,15 +701,28 @@ int check_call(const dt_kv_cache* cache, int B, int T, int H, int D, const int32
         return set_error(DT_ERR_INVALID_ARG, "H=%d is no multiple of the cache's %d heads, or above %d", H, cache->heads, kMaxCacheHeads);
     // (row and workgroup indices within a launch stay within 31 bits)
     if (static_cast<int64_t>(B) * T * H > 0x7fffff) return set_error(DT_ERR_UNSUPPORTED, "B*T*H = %lld query rows", (long long)B * T * H);
-    DT_TRY(kv_check_slots(cache, B, slots, false, rows));
-    DT_TRY(kv_check_counts(B, T, counts, rows));
-    for (int b = 0; b < B; ++b) rows->len[b] = cache->len[rows->slot[b]];
+    KvRows rows;
+    DT_TRY(kv_check_slots(cache, B, slots, false, &rows));
+    DT_TRY(kv_check_counts(B, T, counts, &rows));
+    for (int b = 0; b < B; ++b) {
+        out->slot[b] = static_cast<uint16_t>(rows.slot[b]);
+        out->cnt[b] = static_cast<uint16_t>(rows.cnt[b]);
+        out->len[b] = cache->len[rows.slot[b]];
+    }
     if (prefix) {
         if (prefix->heads != cache->heads || prefix->format != cache->format || prefix->ctx != cache->ctx)
             return set_error(DT_ERR_INVALID_ARG, "the prefix's cache has another context, format or number of heads");
         if (prefix_slot < 0 || prefix_slot >= prefix->slots)
             return set_error(DT_ERR_INVALID_ARG, "prefix_slot=%d outside [0, %d)", prefix_slot, prefix->slots);
+        a->pre = prefix->view();
+        a->pre_slot = prefix_slot;
+        a->pre_len = prefix->len[prefix_slot];
     }
+    a->own = cache->view();
+    a->B = B;
+    a->T = T;
+    a->H = H;
+    a->G = H / cache->heads;
     return DT_OK;
 }
 
@@ -624,9 +737,11 @@ int dt_cached_attn_workspace(const dt_kv_cache* cache, int B, int T, int H, int 
                              const dt_kv_cache* prefix, int prefix_slot, int dtype, int64_t* bytes) {
     clear_error();
     if (!bytes) return set_error(DT_ERR_INVALID_ARG, "bytes is NULL");
-    KvRows rows;
-    DT_TRY(check_call(cache, B, T, H, D, slots, counts, prefix, prefix_slot, dtype, &rows));
-    *bytes = make_plan(cache, B, T, H, rows, prefix, prefix ? prefix->len[prefix_slot] : 0, dtype).ws_bytes;
+    CachedAttnArgs a{};
+    AttnRows rows;
+    bool join = false;
+    DT_TRY(check_call(cache, B, T, H, D, slots, counts, prefix, prefix_slot, dtype, &a, &rows));
+    *bytes = make_plan(a, rows, &join);
     return DT_OK;
 }
 
@@ -638,33 +753,34 @@ int dt_cached_attn_fwd(dt_kv_cache* cache, const void* q, void* o, float* m, flo
     if (mem != DT_MEM_DEVICE && mem != DT_MEM_HOST) return set_error(DT_ERR_INVALID_ARG, "unknown mem %d", mem);
     if (!(scale > 0.0f) || !std::isfinite(scale)) return set_error(DT_ERR_INVALID_ARG, "scale %g must be finite and > 0", scale);
     if (causal != 0 && causal != 1) return set_error(DT_ERR_INVALID_ARG, "causal must be 0 or 1");
-    KvRows rows;
-    DT_TRY(check_call(cache, B, T, H, D, slots, counts, prefix, prefix_slot, dtype, &rows));
+    CachedAttnArgs a{};
+    AttnRows rows;
+    DT_TRY(check_call(cache, B, T, H, D, slots, counts, prefix, prefix_slot, dtype, &a, &rows));
     const size_t esz = dtype == DT_BF16 ? 2 : 4;
     const int64_t dm = static_cast<int64_t>(H) * kD;
     if (ldq < dm) return set_error(DT_ERR_INVALID_ARG, "row stride %lld is below %lld", (long long)ldq, (long long)dm);
     if (mem == DT_MEM_DEVICE && (!aligned16(q) || !aligned16(o) || !aligned16(ws) || ldq * esz % 16))
         return set_error(DT_ERR_INVALID_ARG, "device q/o/workspace and q's row stride must be 16-byte aligned");
-    const int prefix_len = prefix ? prefix->len[prefix_slot] : 0;
-    const Plan p = make_plan(cache, B, T, H, rows, prefix, prefix_len, dtype);
-    if (mem == DT_MEM_DEVICE && p.ws_bytes > 0 && (!ws || ws_bytes < p.ws_bytes))
-        return set_error(DT_ERR_INVALID_ARG, "the workspace has %lld bytes, the call needs %lld", (long long)(ws ? ws_bytes : 0), (long long)p.ws_bytes);
+    bool join = false;
+    const int64_t need = make_plan(a, rows, &join);
+    if (mem == DT_MEM_DEVICE && need > 0 && (!ws || ws_bytes < need))
+        return set_error(DT_ERR_INVALID_ARG, "the workspace has %lld bytes, the call needs %lld", (long long)(ws ? ws_bytes : 0), (long long)need);
     dt_ctx* ctx = cache->ctx;
     DT_TRY(check_device_binding(ctx));
     hipStream_t s = static_cast<hipStream_t>(stream);
-    CachedAttnArgs a{};
     a.q = q;
     a.o = o;
     a.m = m;
     a.l = l;
     a.ldq = ldq;
-    a.B = B;
-    a.T = T;
-    a.H = H;
-    a.G = H / cache->heads;
     a.causal = causal;
     a.scale = scale;
-    if (mem == DT_MEM_DEVICE) return run(cache, a, rows, prefix, prefix_slot, prefix_len, p, ws, dtype, s);
+    const int64_t part_floats = static_cast<int64_t>(B) * T * H * a.parts * kD;
+    if (mem == DT_MEM_DEVICE) {
+        a.part_o = static_cast<float*>(ws);
+        a.part_ml = a.part_o + part_floats;
+        return launch(a, rows, join, cache->format, dtype, s);
+    }
 
     // host memory: staged through the context's buffers, synchronous
     const size_t tok = static_cast<size_t>(B) * T, row = dm * esz, nst = tok * H * sizeof(float);
@@ -672,14 +788,16 @@ int dt_cached_attn_fwd(dt_kv_cache* cache, const void* q, void* o, float* m, flo
     DT_TRY(ctx->stage[1].ensure(tok * row));
     DT_TRY(ctx->stage[2].ensure(nst));
     DT_TRY(ctx->stage[3].ensure(nst));
-    if (p.ws_bytes > 0) DT_TRY(ctx->stage[4].ensure(p.ws_bytes));
+    if (need > 0) DT_TRY(ctx->stage[4].ensure(need));
     DT_HIP_TRY(hipMemcpy2DAsync(ctx->stage[0].ptr, row, q, ldq * esz, row, tok, hipMemcpyHostToDevice, s));
     a.q = ctx->stage[0].ptr;
     a.o = ctx->stage[1].ptr;
     a.m = static_cast<float*>(ctx->stage[2].ptr);
     a.l = static_cast<float*>(ctx->stage[3].ptr);
     a.ldq = dm;
-    DT_TRY(run(cache, a, rows, prefix, prefix_slot, prefix_len, p, ctx->stage[4].ptr, dtype, s));
+    a.part_o = static_cast<float*>(ctx->stage[4].ptr);
+    a.part_ml = a.part_o + part_floats;
+    DT_TRY(launch(a, rows, join, cache->format, dtype, s));
     DT_HIP_TRY(hipMemcpyAsync(o, a.o, tok * row, hipMemcpyDeviceToHost, s));
     if (m) DT_HIP_TRY(hipMemcpyAsync(m, a.m, nst, hipMemcpyDeviceToHost, s));
     if (l) DT_HIP_TRY(hipMemcpyAsync(l, a.l, nst, hipMemcpyDeviceToHost, s));

@@ -12,12 +12,13 @@
 // NaN: it reads back as NaN, and no held value is ever infinite or NaN. A masked key may then go through the
 // matrix instructions with probability 0 (0 times a held value is 0).
 //
-// Per (slot, head), keys in blocks of 32 (the k extent of one v_mfma_f32_16x16x32_bf16):
-//   K       [key][128 values], row-major: the A operand of S^T = K Q^T has 8 consecutive values a lane
-//   V       each block in the order in which the A operand of O^T = V^T P^T reads it, so a lane's fragment is one
-//           16-byte load: see v_offset
-//   scales  [key] for K and V each
-// All of it is zeroed when the cache is made, and the block that a length ends in lies whole in the buffer.
+// Per (slot, head), keys in blocks of 32 (the k extent of one v_mfma_f32_16x16x32_bf16), a block's K, V and scales behind
+// each other, so a reader streams one run of memory:
+//   K       32 x 128 values in the order in which the A operand of S^T = K Q^T reads them
+//   V       32 x 128 values in the order of the A operand of O^T = V^T P^T
+//   scales  of K [32], of V [32]
+// A lane's fragment is one 16-byte load and a wave's load one run of 1 KB: see k_offset and v_offset. All of it is zeroed
+// when the cache is made, and the block that a length ends in lies whole in the buffer.
 #pragma once
 
 #include "dt_internal.h"
@@ -37,25 +38,40 @@ struct KvRows {
 
 __host__ __device__ constexpr int kv_elem_bytes(int format) { return format == DT_KV_BF16 ? 2 : 1; }
 
-// Byte offset of value d (0..127) of key kk (0..31) in a block of V. The A operand of the 16x16x32 product takes
-// 16 values d (lane & 15) and 32 keys, 8 a lane group g = lane >> 4; which keys those are may be chosen freely as
-// long as P's fragment has the same order. P comes out of S^T's accumulators, where group g holds keys 4g..4g+3
-// of each 16-key tile: so slots 0..3 are those of the first tile, 4..7 those of the second.
+constexpr int kKvRun = 1024;  // bytes of a wave's load
+__host__ __device__ constexpr int kv_tensor_bytes(int format) { return kKvBlock * DT_HEAD_DIM * kv_elem_bytes(format); }
+__host__ __device__ constexpr int kv_scale_at(int format) { return 2 * kv_tensor_bytes(format); }  // K's; V's behind
+__host__ __device__ constexpr int kv_block_bytes(int format) { return kv_scale_at(format) + 2 * kKvBlock * 4; }
+
+// Byte offset of value d (0..127) of key kk (0..31) in a block's K. The A operand of the 16x16x32 product takes 16 keys
+// (lane & 15) and 32 values d, 8 a lane group g = lane >> 4; which those are may be chosen freely as long as Q's fragment has the
+// same order. A 16-byte piece has 16 (8 bits) or 8 (bf16) consecutive ones: two steps, or one.
 template <int kFormat>
-__device__ __forceinline__ int v_offset(int d, int kk) {
+__host__ __device__ __forceinline__ int k_offset(int d, int kk) {
+    const int tile = kk >> 4, m = kk & 15;
+    if constexpr (kFormat == DT_KV_BF16) return tile * 4096 + (d >> 5) * kKvRun + ((d >> 3 & 3) * 16 + m) * 16 + (d & 7) * 2;
+    return tile * 2048 + (d >> 6) * kKvRun + ((d >> 4 & 3) * 16 + m) * 16 + (d & 15);
+}
+
+// Byte offset of value d of key kk in a block's V. The operand takes 16 values d (lane & 15) and 32 keys, 8 a lane group.
+// P comes out of S^T's accumulators, where group g holds keys 4g..4g+3 of each 16-key tile: so slots 0..3 are those of the
+// first tile, 4..7 those of the second.
+template <int kFormat>
+__host__ __device__ __forceinline__ int v_offset(int d, int kk) {
     const int g = (kk & 15) >> 2, j = (kk >> 4) * 4 + (kk & 3);
     const int mt = d >> 4, lane = g * 16 + (d & 15);
-    if constexpr (kFormat == DT_KV_BF16) return mt * 1024 + lane * 16 + j * 2;
-    return (mt >> 1) * 1024 + lane * 16 + (mt & 1) * 8 + j;
+    if constexpr (kFormat == DT_KV_BF16) return mt * kKvRun + lane * 16 + j * 2;
+    return (mt >> 1) * kKvRun + lane * 16 + (mt & 1) * 8 + j;
 }
 
 struct KvView {
-    uint8_t* k;
-    uint8_t* v;
-    float* ks;
-    float* vs;
-    int64_t keys;  // keys allocated per (slot, head), a multiple of kKvBlock
+    uint8_t* data;
+    int blocks;  // allocated per (slot, head)
     int heads;
+    template <int kFormat>
+    __device__ __forceinline__ uint8_t* block(int slot, int head, int blk) const {
+        return data + ((static_cast<int64_t>(slot) * heads + head) * blocks + blk) * kv_block_bytes(kFormat);
+    }
 };
 
 }  // namespace dt
@@ -63,15 +79,10 @@ struct KvView {
 struct dt_kv_cache {
     dt_ctx* ctx = nullptr;
     int slots = 0, capacity = 0, heads = 0, format = 0;
-    int64_t keys = 0;
-    void* k = nullptr;
-    void* v = nullptr;
-    float* ks = nullptr;
-    float* vs = nullptr;
+    int blocks = 0;  // of 32 tokens per (slot, head)
+    void* data = nullptr;
     std::vector<int32_t> len;  // tokens held by each slot
-    dt::KvView view() const {
-        return {static_cast<uint8_t*>(k), static_cast<uint8_t*>(v), ks, vs, keys, heads};
-    }
+    dt::KvView view() const { return {static_cast<uint8_t*>(data), blocks, heads}; }
 };
 
 namespace dt {

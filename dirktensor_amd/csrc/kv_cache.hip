@@ -160,19 +160,29 @@ __device__ __forceinline__ void dequantise(const uint32_t (&w)[kFormat == DT_KV_
     }
 }
 
-// V's block in LDS: its 1 KB runs (of lane fragments) are 16 bytes further apart than in memory, which keeps the
-// eight threads of a key off one bank
-constexpr int kRun = 1024, kRunLds = kRun + 16;
+// V's block in LDS: its 1 KB runs are 16 bytes further apart than in memory, which keeps the eight threads of a key off one
+// bank
+constexpr int kRunLds = kKvRun + 16;
 template <int kFormat>
 __device__ __forceinline__ int v_lds_offset(int d, int kk) {
     const int o = v_offset<kFormat>(d, kk);
-    return (o >> 10) * kRunLds + (o & (kRun - 1));
+    return (o >> 10) * kRunLds + (o & (kKvRun - 1));
+}
+
+// K's 16 values of thread part c of key kk: one or two 16-byte pieces
+template <int kFormat>
+__device__ __forceinline__ uint4* k_piece(uint8_t* block, int c, int kk, int i) {
+    return reinterpret_cast<uint4*>(block + k_offset<kFormat>(c * 16 + i * 8, kk));
+}
+template <int kFormat>
+__device__ __forceinline__ float* scale_of(uint8_t* block, bool v, int kk) {
+    return reinterpret_cast<float*>(block + kv_scale_at(kFormat)) + (v ? kKvBlock : 0) + kk;
 }
 
 template <int kFormat, bool kBf16>
 __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvMoveArgs a, KvRows rows) {
-    constexpr int kEs = kv_elem_bytes(kFormat), kWords = 4 * kEs, kBlockBytes = kKvBlock * DT_HEAD_DIM * kEs;
-    __shared__ __align__(16) uint8_t vbuf[kBlockBytes / kRun * kRunLds];
+    constexpr int kEs = kv_elem_bytes(kFormat), kWords = 4 * kEs, kTensor = kv_tensor_bytes(kFormat);
+    __shared__ __align__(16) uint8_t vbuf[kTensor / kKvRun * kRunLds];
     const int b = blockIdx.z, h = blockIdx.y;
     const int start = rows.len[b], cnt = rows.cnt[b];
     const int blk = start / kKvBlock + static_cast<int>(blockIdx.x);
@@ -204,20 +214,16 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvMoveArgs a, KvRow
     const float sk = quantise<kFormat>(x, kmax, qk);
     const float sv = quantise<kFormat>(y, vmax, qv);
 
-    const int64_t head = static_cast<int64_t>(rows.slot[b]) * a.c.heads + h;
+    uint8_t* block = a.c.block<kFormat>(rows.slot[b], h, blk);
+    uint8_t* vd = block + kTensor;
     if (mine) {
-        const int64_t row = head * a.c.keys + first + kk;
-        uint4* kd = reinterpret_cast<uint4*>(a.c.k + (row * DT_HEAD_DIM + c * 16) * kEs);
 #pragma unroll
-        for (int i = 0; i < kEs; ++i) kd[i] = make_uint4(qk[4 * i], qk[4 * i + 1], qk[4 * i + 2], qk[4 * i + 3]);
+        for (int i = 0; i < kEs; ++i) *k_piece<kFormat>(block, c, kk, i) = make_uint4(qk[4 * i], qk[4 * i + 1], qk[4 * i + 2], qk[4 * i + 3]);
         if (c == 0) {
-            a.c.ks[row] = sk;
-            a.c.vs[row] = sv;
+            *scale_of<kFormat>(block, false, kk) = sk;
+            *scale_of<kFormat>(block, true, kk) = sv;
         }
-    }
-    uint8_t* vd = a.c.v + (head * a.c.keys + first) * DT_HEAD_DIM * kEs;
-    uint8_t* to = whole ? vbuf : vd;
-    if (mine) {
+        uint8_t* to = whole ? vbuf : vd;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int o = whole ? v_lds_offset<kFormat>(c * 16 + i, kk) : v_offset<kFormat>(c * 16 + i, kk);
@@ -230,15 +236,15 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvMoveArgs a, KvRow
 #pragma unroll
         for (int i = 0; i < kEs; ++i) {
             const int o = (i * kThreads + threadIdx.x) * 16;
-            *reinterpret_cast<uint4*>(vd + o) = *reinterpret_cast<const uint4*>(vbuf + (o >> 10) * kRunLds + (o & (kRun - 1)));
+            *reinterpret_cast<uint4*>(vd + o) = *reinterpret_cast<const uint4*>(vbuf + (o >> 10) * kRunLds + (o & (kKvRun - 1)));
         }
     }
 }
 
 template <int kFormat, bool kBf16>
 __global__ __launch_bounds__(kThreads) void kv_read_kernel(KvMoveArgs a, KvRows rows) {
-    constexpr int kEs = kv_elem_bytes(kFormat), kWords = 4 * kEs, kBlockBytes = kKvBlock * DT_HEAD_DIM * kEs;
-    __shared__ __align__(16) uint8_t vbuf[kBlockBytes / kRun * kRunLds];
+    constexpr int kEs = kv_elem_bytes(kFormat), kWords = 4 * kEs, kTensor = kv_tensor_bytes(kFormat);
+    __shared__ __align__(16) uint8_t vbuf[kTensor / kKvRun * kRunLds];
     const int b = blockIdx.z, h = blockIdx.y;
     const int start = rows.len[b], cnt = rows.cnt[b];
     const int blk = start / kKvBlock + static_cast<int>(blockIdx.x);
@@ -247,25 +253,22 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(KvMoveArgs a, KvRows 
     const int kk = threadIdx.x >> 3, c = threadIdx.x & 7;
     const int t = first + kk - start;
     const bool mine = t >= 0 && t < cnt;
-    const int64_t head = static_cast<int64_t>(rows.slot[b]) * a.c.heads + h;
-    const int64_t row = head * a.c.keys + first + kk;
+    uint8_t* block = a.c.block<kFormat>(rows.slot[b], h, blk);
 
-    const uint8_t* vd = a.c.v + (head * a.c.keys + first) * DT_HEAD_DIM * kEs;
 #pragma unroll
     for (int i = 0; i < kEs; ++i) {
         const int o = (i * kThreads + threadIdx.x) * 16;
-        *reinterpret_cast<uint4*>(vbuf + (o >> 10) * kRunLds + (o & (kRun - 1))) = *reinterpret_cast<const uint4*>(vd + o);
+        *reinterpret_cast<uint4*>(vbuf + (o >> 10) * kRunLds + (o & (kKvRun - 1))) = *reinterpret_cast<const uint4*>(block + kTensor + o);
     }
     float x[16];
     uint32_t w[kWords];
     if (mine) {
-        const uint4* ks = reinterpret_cast<const uint4*>(a.c.k + (row * DT_HEAD_DIM + c * 16) * kEs);
 #pragma unroll
         for (int i = 0; i < kEs; ++i) {
-            const uint4 u = ks[i];
+            const uint4 u = *k_piece<kFormat>(block, c, kk, i);
             w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
         }
-        dequantise<kFormat>(w, a.c.ks[row], x);
+        dequantise<kFormat>(w, *scale_of<kFormat>(block, false, kk), x);
         store16<kBf16>(a.k, b * a.bsk + t * a.ldk + h * DT_HEAD_DIM + c * 16, x);
     }
     __syncthreads();
@@ -278,7 +281,7 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(KvMoveArgs a, KvRows 
             if constexpr (kEs == 2) w[i >> 1] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(vbuf + o)) << (16 * (i & 1));
             else w[i >> 2] |= static_cast<uint32_t>(vbuf[o]) << (8 * (i & 3));
         }
-        dequantise<kFormat>(w, a.c.vs[row], x);
+        dequantise<kFormat>(w, *scale_of<kFormat>(block, true, kk), x);
         store16<kBf16>(a.v, b * a.bsv + t * a.ldv + h * DT_HEAD_DIM + c * 16, x);
     }
 }
@@ -311,10 +314,7 @@ int launch_move(const KvMoveArgs& a, const KvRows& rows, int B, int format, int 
 }
 
 void free_cache(dt_kv_cache* c) {
-    if (c->k) (void)hipFree(c->k);
-    if (c->v) (void)hipFree(c->v);
-    if (c->ks) (void)hipFree(c->ks);
-    if (c->vs) (void)hipFree(c->vs);
+    if (c->data) (void)hipFree(c->data);
     delete c;
 }
 
@@ -381,30 +381,23 @@ int dt_kv_cache_create(dt_ctx* ctx, int slots, int capacity, int n_heads, int D,
     c->capacity = capacity;
     c->heads = n_heads;
     c->format = format;
-    c->keys = (static_cast<int64_t>(capacity) + kKvBlock - 1) / kKvBlock * kKvBlock;
+    c->blocks = (capacity + kKvBlock - 1) / kKvBlock;
     try {
         c->len.assign(slots, 0);
     } catch (const std::bad_alloc&) {
         free_cache(c);
         return set_error(DT_ERR_INVALID_ARG, "out of host memory");
     }
-    const size_t rows = static_cast<size_t>(slots) * n_heads * c->keys;
-    const size_t bytes = rows * DT_HEAD_DIM * kv_elem_bytes(format);
-    struct { void** p; size_t n; } parts[] = {{&c->k, bytes}, {&c->v, bytes},
-                                              {reinterpret_cast<void**>(&c->ks), rows * sizeof(float)},
-                                              {reinterpret_cast<void**>(&c->vs), rows * sizeof(float)}};
-    hipError_t e = hipSuccess;
-    for (auto& p : parts) {
-        if (e == hipSuccess) e = hipMalloc(p.p, p.n);
-        if (e == hipSuccess) e = hipMemset(*p.p, 0, p.n);
-    }
+    const size_t bytes = static_cast<size_t>(slots) * n_heads * c->blocks * kv_block_bytes(format);
+    hipError_t e = hipMalloc(&c->data, bytes);
+    if (e == hipSuccess) e = hipMemset(c->data, 0, bytes);
     // the clearing is done before the call returns: streams that do not wait for the null stream may use the cache
     if (e == hipSuccess) e = hipStreamSynchronize(nullptr);
     if (e != hipSuccess) {
         (void)hipGetLastError();
         free_cache(c);
         return set_error(DT_ERR_HIP, "a cache of %.1f GiB cannot be had: %s",
-                         2.0 * (bytes + rows * sizeof(float)) / (1u << 30), hipGetErrorString(e));
+                         static_cast<double>(bytes) / (1u << 30), hipGetErrorString(e));
     }
     *out = c;
     return DT_OK;
