@@ -51,7 +51,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_huge_valf();
 
 // blocks in flight a wave: what 256 registers a lane hold, which leave two workgroups a CU
-constexpr int stages(int format) { return format == DT_KV_BF16 ? 1 : 2; }
+constexpr int stages(int format, bool f32) { return format == DT_KV_BF16 || f32 ? 1 : 2; }
 
 // The batch rows, by value in the kernel's arguments.
 struct AttnRows {
@@ -219,188 +219,207 @@ struct Shared {
     float ml[kWaves][2][16];
 };
 
+// A wave's part of a stretch of work: begin puts the loads of its first blocks and of its Q rows under way, attend does the work
+// and leaves the results in LDS, join (of the whole workgroup) puts the waves' results together.
 template <int kFormat, bool kF32, bool kOnce>
-__device__ __forceinline__ void attend(const CachedAttnArgs& a, const AttnRows& rows, const Work& w, Shared& sh) {
-    constexpr int kQS = kF32 ? 3 : 1;
-    const int tid = thread_here();
-    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n = lane & 15, g = lane >> 4;
-    const int qw = wave % w.wq, kw = wave / w.wq, step = kKvBlock * kWaves / w.wq;
-    const uint8_t* base_block = (w.prefix ? a.pre : a.own).block<kFormat>(w.slot, w.hk, 0);
-    const auto block_at = [&](int key) { return base_block + static_cast<int64_t>(key / kKvBlock) * kv_block_bytes(kFormat); };
-    const int nrows = (w.prefix ? a.B : 1) * a.T * a.G;
-    const int row0 = w.tile * 16 * w.wq;
-    const int r = row0 + qw * 16 + n;
-    const bool have = r < nrows;
-    const QueryRow qr = query_row(a, have ? r : row0, w.b, w.hk, w.prefix);
-
-    // the first blocks are under way before anything else
-    constexpr int kStages = stages(kFormat);
+struct Stretch {
+    static constexpr int kQS = kF32 ? 3 : 1, kStages = stages(kFormat, kF32);
     Block<kFormat, kOnce> st[kStages];
-    int kb = w.k0 + kw * kKvBlock;
-#pragma unroll
-    for (int i = 0; i < kStages; ++i)
-        if (kb + i * step < w.k1) {
-            st[i].load_k(block_at(kb + i * step), lane);
-            st[i].load_v(block_at(kb + i * step), lane);
-        }
+    u32x4 qraw[kF32 ? 8 : 4];
+    const uint8_t* base;  // the (slot, head)'s first block
+    int kb, k1, step;     // the next block's first key, the end, the distance of the wave's blocks
+    int lane, wave, lim, minlim;
 
-    // Q fragment; keys below lim are seen by the lane's query, keys below minlim by all of the wave's
-    int lim = w.len;
-    if (have && !w.prefix && a.causal) {
-        if (qr.t < w.cnt) lim = max(0, min(w.len, w.len - w.cnt + qr.t + 1));
+    __device__ __forceinline__ const uint8_t* block_at(int key) const {
+        return base + static_cast<int64_t>(key / kKvBlock) * kv_block_bytes(kFormat);
     }
-    int minlim = lim;
+
+    __device__ __forceinline__ void begin(const CachedAttnArgs& a, const Work& w) {
+        const int tid = thread_here();
+        lane = tid & 63;
+        wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int n = lane & 15, g = lane >> 4;
+        const int qw = wave % w.wq, kw = wave / w.wq;
+        step = kKvBlock * kWaves / w.wq;
+        k1 = w.k1;
+        base = (w.prefix ? a.pre : a.own).block<kFormat>(w.slot, w.hk, 0);
+        kb = w.k0 + kw * kKvBlock;
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) minlim = min(minlim, __shfl_xor(minlim, o, 64));
-    float qscale = a.scale;
-    bf16x8 qf[kQS][4];
-    const int64_t qat = (static_cast<int64_t>(qr.b) * a.T + qr.t) * a.ldq + qr.hq * kD;
-    if constexpr (!kF32) {
-        const uint16_t* q = static_cast<const uint16_t*>(a.q) + qat;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) qf[0][s] = *reinterpret_cast<const bf16x8*>(q + k_dim<kFormat>(s, g));
-    } else {
-        const float* q = static_cast<const float*>(a.q) + qat;
-        float x[4][8];
-        uint32_t top = 0;
+        for (int i = 0; i < kStages; ++i)
+            if (kb + i * step < k1) {
+                st[i].load_k(block_at(kb + i * step), lane);
+                st[i].load_v(block_at(kb + i * step), lane);
+            }
+        const int nrows = (w.prefix ? a.B : 1) * a.T * a.G;
+        const int row0 = w.tile * 16 * w.wq;
+        const int r = row0 + qw * 16 + n;
+        const bool have = r < nrows;
+        const QueryRow qr = query_row(a, have ? r : row0, w.b, w.hk, w.prefix);
+        const int64_t at = (static_cast<int64_t>(qr.b) * a.T + qr.t) * a.ldq + qr.hq * kD;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            const floatx4 lo = *reinterpret_cast<const floatx4*>(q + k_dim<kFormat>(s, g));
-            const floatx4 hi = *reinterpret_cast<const floatx4*>(q + k_dim<kFormat>(s, g) + 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[s][j] = lo[j], x[s][4 + j] = hi[j];
-        }
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[s][j]) & 0x7f800000u);
-        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, 64)));
-        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, 64)));
-        // exponents from 2^-126 to 2^126 have a reciprocal; rows beyond (and with infinities, NaN) stay as they are
-        const bool norm = top >= 0x00800000u && top <= 0x7e800000u;
-        const float inv = norm ? __uint_as_float(0x7f000000u - top) : 1.0f;
-        qscale = norm ? a.scale * __uint_as_float(top) : a.scale;
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float v = x[s][j] * inv, h = bf16_round(v), m = bf16_round(v - h);
-                qf[0][s][j] = static_cast<__bf16>(h);
-                qf[1][s][j] = static_cast<__bf16>(m);
-                qf[2][s][j] = static_cast<__bf16>(v - h - m);
+            if constexpr (kF32) {
+                const u32x4* q = reinterpret_cast<const u32x4*>(static_cast<const float*>(a.q) + at + k_dim<kFormat>(s, g));
+                qraw[2 * s] = q[0];
+                qraw[2 * s + 1] = q[1];
+            } else {
+                qraw[s] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at + k_dim<kFormat>(s, g));
             }
+        }
+        // keys below lim are seen by the lane's query, keys below minlim by all of the wave's
+        lim = w.len;
+        if (have && !w.prefix && a.causal && qr.t < w.cnt) lim = max(0, min(w.len, w.len - w.cnt + qr.t + 1));
+        minlim = lim;
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) minlim = min(minlim, __shfl_xor(minlim, o, 64));
     }
 
-    floatx4 acc[8];
-    float mrun = kNegInf, lrun = 0.0f;
+    // Q as the matrix operand: as it is, or in three parts; returns what the scores are multiplied with
+    __device__ __forceinline__ float operand_q(float scale, bf16x8 (&qf)[kQS][4]) const {
+        if constexpr (!kF32) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
-
-    // one block: scores, probabilities, O; its registers are filled again, K's behind the scores and V's behind O, with the block
-    // kStages steps on
-    auto take = [&](Block<kFormat, kOnce>& blk) {
-        const int next = kb + kStages * step;
-        const bool more = next < w.k1;
-        blk.settle(blk.k);
-        floatx4 s[2];
-        s[0] = s[1] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+            for (int s = 0; s < 4; ++s) qf[0][s] = __builtin_bit_cast(bf16x8, qraw[s]);
+            return scale;
+        } else {
+            uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const bf16x8 kf = blk.operand(blk.k, i);
+            for (int s = 0; s < 8; ++s)
 #pragma unroll
-            for (int x = kQS - 1; x >= 0; --x) s[i >> 2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[x][i & 3], s[i >> 2], 0, 0, 0);
-            keep_order();
+                for (int j = 0; j < 4; ++j) top = max(top, qraw[s][j] & 0x7f800000u);
+            top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, 64)));
+            top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, 64)));
+            // exponents from 2^-126 to 2^126 have a reciprocal; rows beyond (and with infinities, NaN) stay as they are
+            const bool norm = top >= 0x00800000u && top <= 0x7e800000u;
+            const float inv = norm ? __uint_as_float(0x7f000000u - top) : 1.0f;
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float v = __uint_as_float(qraw[2 * s + (j >> 2)][j & 3]) * inv, h = bf16_round(v), m = bf16_round(v - h);
+                    qf[0][s][j] = static_cast<__bf16>(h);
+                    qf[1][s][j] = static_cast<__bf16>(m);
+                    qf[2][s][j] = static_cast<__bf16>(v - h - m);
+                }
+            return norm ? scale * __uint_as_float(top) : scale;
         }
-        float mx = kNegInf;
-        const bool mask = kb + kKvBlock > minlim;  // (the same for the whole wave)
+    }
+
+    __device__ __forceinline__ void attend(float scale, Shared& sh) {
+        const int n = lane & 15, g = lane >> 4;
+        bf16x8 qf[kQS][4];
+        const float qscale = operand_q(scale, qf);
+        floatx4 acc[8];
+        float mrun = kNegInf, lrun = 0.0f;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int i = 0; i < 8; ++i) acc[i] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+
+        // one block: scores, probabilities, O; its registers are filled again, K's behind the scores and V's behind O, with the block
+        // kStages steps on
+        auto take = [&](Block<kFormat, kOnce>& blk) {
+            const int next = kb + kStages * step;
+            const bool more = next < k1;
+            blk.settle(blk.k);
+            floatx4 s[2];
+            s[0] = s[1] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[t][i] *= blk.ks[t][i] * qscale;
-                mx = fmaxf(mx, s[t][i]);
+            for (int i = 0; i < 8; ++i) {
+                const bf16x8 kf = blk.operand(blk.k, i);
+#pragma unroll
+                for (int x = kQS - 1; x >= 0; --x) s[i >> 2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[x][i & 3], s[i >> 2], 0, 0, 0);
+                keep_order();
             }
-        if (mask) {
-            mx = kNegInf;
+            float mx = kNegInf;
+            const bool mask = kb + kKvBlock > minlim;  // (the same for the whole wave)
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    if (kb + t * 16 + g * 4 + i >= lim) s[t][i] = kNegInf;
+                    s[t][i] *= blk.ks[t][i] * qscale;
                     mx = fmaxf(mx, s[t][i]);
                 }
-        }
-        keep_order();
-        if (more) blk.load_k(block_at(next), lane);
-        keep_order();
-        mx = fmaxf(max_groups(mx), mrun);
-        const float base = mx == kNegInf ? 0.0f : mx;  // (nothing seen yet: every p is 0)
-        if (__any(mx != mrun)) {
-            const float f = __builtin_amdgcn_exp2f((mrun - base) * kLog2e);
-            lrun *= f;
+            if (mask) {
+                mx = kNegInf;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] *= f;
-            mrun = mx;
-        }
-        float p[8], sum = 0.0f;
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float e = __builtin_amdgcn_exp2f((s[t][i] - base) * kLog2e);
-                sum += e;
-                p[t * 4 + i] = e * blk.vs[t][i];
+                    for (int i = 0; i < 4; ++i) {
+                        if (kb + t * 16 + g * 4 + i >= lim) s[t][i] = kNegInf;
+                        mx = fmaxf(mx, s[t][i]);
+                    }
             }
-        if (mask) {  // (a masked key's scale may be anything, NaN too)
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (kb + (i >> 2) * 16 + g * 4 + (i & 3) >= lim) p[i] = 0.0f;
-        }
-        lrun += sum;
-        blk.settle(blk.v);
-        bf16x8 pf[kQS];
-#pragma unroll
-        for (int x = 0; x < kQS; ++x) {
-            union { uint32_t u[4]; bf16x8 v; } f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f.u[j] = pack2(p[2 * j], p[2 * j + 1]);
-                if (x + 1 < kQS) {
-                    p[2 * j] -= __uint_as_float(f.u[j] << 16);
-                    p[2 * j + 1] -= __uint_as_float(f.u[j] & 0xffff0000u);
-                }
-            }
-            pf[x] = f.v;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const bf16x8 vf = blk.operand(blk.v, i);
-#pragma unroll
-            for (int x = kQS - 1; x >= 0; --x) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[x], acc[i], 0, 0, 0);
             keep_order();
-        }
-        if (more) blk.load_v(block_at(next), lane);
-        kb += step;
-    };
-    while (kb < w.k1) {
-        take(st[0]);
-        if constexpr (kStages > 1) {
-            if (kb >= w.k1) break;
-            take(st[1]);
-        }
-    }
-
-    // the waves' results meet: a thread sums four values of a row over the key waves, scaled to their common maximum
-    lrun = sum_groups(lrun);
-    if (g == 0) {
-        sh.ml[wave][0][n] = mrun;
-        sh.ml[wave][1][n] = lrun;
-    }
+            if (more) blk.load_k(block_at(next), lane);
+            keep_order();
+            mx = fmaxf(max_groups(mx), mrun);
+            const float base = mx == kNegInf ? 0.0f : mx;  // (nothing seen yet: every p is 0)
+            if (__any(mx != mrun)) {
+                const float f = __builtin_amdgcn_exp2f((mrun - base) * kLog2e);
+                lrun *= f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) *reinterpret_cast<floatx4*>(&sh.o[wave][n][i * 16 + g * 4]) = acc[i];
-    __syncthreads();
-    const int wk = kWaves / w.wq;
+                for (int i = 0; i < 8; ++i) acc[i] *= f;
+                mrun = mx;
+            }
+            float p[8], sum = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = __builtin_amdgcn_exp2f((s[t][i] - base) * kLog2e);
+                    sum += e;
+                    p[t * 4 + i] = e * blk.vs[t][i];
+                }
+            if (mask) {  // (a masked key's scale may be anything, NaN too)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (kb + (i >> 2) * 16 + g * 4 + (i & 3) >= lim) p[i] = 0.0f;
+            }
+            lrun += sum;
+            blk.settle(blk.v);
+            bf16x8 pf[kQS];
+#pragma unroll
+            for (int x = 0; x < kQS; ++x) {
+                union { uint32_t u[4]; bf16x8 v; } f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    f.u[j] = pack2(p[2 * j], p[2 * j + 1]);
+                    if (x + 1 < kQS) {
+                        p[2 * j] -= __uint_as_float(f.u[j] << 16);
+                        p[2 * j + 1] -= __uint_as_float(f.u[j] & 0xffff0000u);
+                    }
+                }
+                pf[x] = f.v;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const bf16x8 vf = blk.operand(blk.v, i);
+#pragma unroll
+                for (int x = kQS - 1; x >= 0; --x) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[x], acc[i], 0, 0, 0);
+                keep_order();
+            }
+            if (more) blk.load_v(block_at(next), lane);
+            kb += step;
+        };
+        while (kb < k1) {
+            take(st[0]);
+            if constexpr (kStages > 1) {
+                if (kb >= k1) break;
+                take(st[1]);
+            }
+        }
+        lrun = sum_groups(lrun);
+        if (g == 0) {
+            sh.ml[wave][0][n] = mrun;
+            sh.ml[wave][1][n] = lrun;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) *reinterpret_cast<floatx4*>(&sh.o[wave][n][i * 16 + g * 4]) = acc[i];
+    }
+};
+
+// The waves' results meet: a thread sums four values of a row over the key waves, scaled to their common maximum.
+template <bool kF32>
+__device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRows& rows, const Work& w, const Shared& sh) {
+    const int wk = kWaves / w.wq, row0 = w.tile * 16 * w.wq, nrows = (w.prefix ? a.B : 1) * a.T * a.G;
     for (int it = thread_here(); it < w.wq * 16 * (kD / 4); it += kThreads) {
         const int d = (it & 31) * 4, rt = it >> 5;  // (row within the workgroup's tiles)
         const int tq = rt >> 4, rn = rt & 15;
@@ -491,45 +510,57 @@ __global__ __launch_bounds__(kThreads, 2) void cached_attn_kernel(CachedAttnArgs
             end = share_start(a, id + 1);
         }
     }
-    for (;;) {
-        if (!w.prefix) {
-            int off = 0, count;
-            if (a.aligned) {
-                w.len = __builtin_amdgcn_readfirstlane(rl.len[w.b]);
-                w.cnt = __builtin_amdgcn_readfirstlane(rl.cnt[w.b]);
-                count = steps_of(w.len, w.cnt, w.wq);
-            } else {
-                w.hk = s / a.head_steps;
-                const int in_head = s - w.hk * a.head_steps;
-                // the last batch row that begins at or before this step (rows without steps begin where the next one does)
-                int below = 0;
+    // fills w with the next stretch of the list's share
+    const auto next = [&]() {
+        int off = 0, count;
+        if (a.aligned) {
+            w.len = __builtin_amdgcn_readfirstlane(rl.len[w.b]);
+            w.cnt = __builtin_amdgcn_readfirstlane(rl.cnt[w.b]);
+            count = steps_of(w.len, w.cnt, w.wq);
+        } else {
+            w.hk = s / a.head_steps;
+            const int in_head = s - w.hk * a.head_steps;
+            // the last batch row that begins at or before this step (rows without steps begin where the next one does)
+            int below = 0;
 #pragma unroll
-                for (int i = 0; i < kMaxRaggedBatch / 64; ++i) {
-                    const int at = i * 64 + (threadIdx.x & 63);
-                    if (i * 64 < a.B) below += __popcll(__ballot(at < a.B && rl.cum[at] <= in_head));
-                }
-                w.b = __builtin_amdgcn_readfirstlane(below) - 1;
-                w.len = __builtin_amdgcn_readfirstlane(rl.len[w.b]);
-                w.cnt = __builtin_amdgcn_readfirstlane(rl.cnt[w.b]);
-                const int steps = steps_of(w.len, w.cnt, w.wq);
-                const int in_row = in_head - __builtin_amdgcn_readfirstlane(rl.cum[w.b]);
-                w.tile = in_row / steps;
-                off = in_row - w.tile * steps;
-                count = min(steps - off, end - s);
-                w.part = a.pre_parts == 0 && count == steps ? -1 : a.pre_parts + id - group_of(a, s - off);
-                s += count;
+            for (int i = 0; i < kMaxRaggedBatch / 64; ++i) {
+                const int at = i * 64 + (threadIdx.x & 63);
+                if (i * 64 < a.B) below += __popcll(__ballot(at < a.B && rl.cum[at] <= in_head));
             }
-            w.slot = __builtin_amdgcn_readfirstlane(rl.slot[w.b]);
-            w.k0 = off * keys;
-            w.k1 = min(w.len, (off + count) * keys);
-            if (a.causal) {  // nothing past the tile's newest query
-                const int t = min(a.T - 1, ((w.tile + 1) * 16 * w.wq - 1) / a.G);
-                w.k1 = min(w.k1, max(0, w.len - w.cnt + t + 1));
-            }
+            w.b = __builtin_amdgcn_readfirstlane(below) - 1;
+            w.len = __builtin_amdgcn_readfirstlane(rl.len[w.b]);
+            w.cnt = __builtin_amdgcn_readfirstlane(rl.cnt[w.b]);
+            const int steps = steps_of(w.len, w.cnt, w.wq);
+            const int in_row = in_head - __builtin_amdgcn_readfirstlane(rl.cum[w.b]);
+            w.tile = in_row / steps;
+            off = in_row - w.tile * steps;
+            count = min(steps - off, end - s);
+            w.part = a.pre_parts == 0 && count == steps ? -1 : a.pre_parts + id - group_of(a, s - off);
+            s += count;
         }
-        attend<kFormat, kF32, kOnce>(a, rl, w, sh);
-        if (s >= end) return;
-        __syncthreads();  // the next stretch writes the shared results
+        w.slot = __builtin_amdgcn_readfirstlane(rl.slot[w.b]);
+        w.k0 = off * keys;
+        w.k1 = min(w.len, (off + count) * keys);
+        if (a.causal) {  // nothing past the tile's newest query
+            const int t = min(a.T - 1, ((w.tile + 1) * 16 * w.wq - 1) / a.G);
+            w.k1 = min(w.k1, max(0, w.len - w.cnt + t + 1));
+        }
+    };
+    if (!w.prefix) next();
+    Stretch<kFormat, kF32, kOnce> st;
+    st.begin(a, w);
+    for (;;) {
+        st.attend(a.scale, sh);
+        const Work done = w;
+        const bool more = s < end;
+        if (more) {  // the next stretch's first loads are under way while this one is put together
+            next();
+            st.begin(a, w);
+        }
+        __syncthreads();
+        join_waves<kF32>(a, rl, done, sh);
+        if (!more) return;
+        __syncthreads();
     }
 }
 
