@@ -48,7 +48,11 @@ constexpr int kJoinThreads = 256;
 constexpr int kD = DT_HEAD_DIM;
 constexpr int kObufRow = kD + 4;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -__builtin_huge_valf();
+constexpr float kLowest = -3.402823466e38f;
+constexpr float kSlack = 8.0f;
+constexpr int kBufferDword3 = 0x00020000;  // raw buffer, 32-bit data format (gfx9 family)
 
 // blocks in flight a wave: what 256 registers a lane hold, which leave two workgroups a CU
 constexpr int stages(int format, bool f32) { return format == DT_KV_BF16 || f32 ? 1 : 2; }
@@ -150,21 +154,23 @@ struct Block {
     static constexpr int kPieces = kFormat == DT_KV_BF16 ? 8 : 4;
     u32x4 k[kPieces], v[kPieces];
     floatx4 ks[2], vs[2];
-    static __device__ __forceinline__ u32x4 load16(const uint8_t* p) {
-        if constexpr (kOnce) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
-        return *reinterpret_cast<const u32x4*>(p);
+    // 16 bytes at `at` + the lane's offset of the block that begins at `from` (the immediate offset holds 12 bits)
+    template <bool kNt>
+    static __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off, int from, int at) {
+        return __builtin_amdgcn_raw_buffer_load_b128(r, off + (at & 4095), from + (at & ~4095), kNt ? 2 : 0);
     }
-    __device__ __forceinline__ void load_k(const uint8_t* block, int lane) {
+    __device__ __forceinline__ void load_k(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t scale_off, int from) {
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) k[i] = load16(block + i * kKvRun + lane * 16);
+        for (int i = 0; i < kPieces; ++i) k[i] = load16<kOnce>(r, off, from, i * kKvRun);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) ks[t] = *reinterpret_cast<const floatx4*>(block + kv_scale_at(kFormat) + t * 64 + (lane >> 4) * 16);
+        for (int t = 0; t < 2; ++t) ks[t] = __builtin_bit_cast(floatx4, load16<false>(r, scale_off, from, kv_scale_at(kFormat) + t * 64));
     }
-    __device__ __forceinline__ void load_v(const uint8_t* block, int lane) {
+    __device__ __forceinline__ void load_v(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t scale_off, int from) {
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) v[i] = load16(block + kv_tensor_bytes(kFormat) + i * kKvRun + lane * 16);
+        for (int i = 0; i < kPieces; ++i) v[i] = load16<kOnce>(r, off, from, kv_tensor_bytes(kFormat) + i * kKvRun);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) vs[t] = *reinterpret_cast<const floatx4*>(block + kv_scale_at(kFormat) + 128 + t * 64 + (lane >> 4) * 16);
+        for (int t = 0; t < 2; ++t)
+            vs[t] = __builtin_bit_cast(floatx4, load16<false>(r, scale_off, from, kv_scale_at(kFormat) + 128 + t * 64));
     }
     // the pieces as values of their own: else the compiler carries them through the loop widened, in twice or four times the
     // registers
@@ -216,7 +222,7 @@ __device__ __forceinline__ int thread_here() {
 
 struct Shared {
     float o[kWaves][16][kObufRow];
-    float ml[kWaves][2][16];
+    float ml[kWaves][3][16];  // base, sum, true maximum
 };
 
 // A wave's part of a stretch of work: begin puts the loads of its first blocks and of its Q rows under way, attend does the work
@@ -226,12 +232,22 @@ struct Stretch {
     static constexpr int kQS = kF32 ? 3 : 1, kStages = stages(kFormat, kF32);
     Block<kFormat, kOnce> st[kStages];
     u32x4 qraw[kF32 ? 8 : 4];
-    const uint8_t* base;  // the (slot, head)'s first block
-    int kb, k1, step;     // the next block's first key, the end, the distance of the wave's blocks
+    __amdgpu_buffer_rsrc_t rsrc;  // the (slot, head)'s blocks
+    int kb, k1, step;             // the next block's first key, the end, the distance of the wave's blocks
+    int at, at_step;              // the byte offset of the next block to load, the distance
     int lane, wave, lim, minlim;
 
-    __device__ __forceinline__ const uint8_t* block_at(int key) const {
-        return base + static_cast<int64_t>(key / kKvBlock) * kv_block_bytes(kFormat);
+    // Loads the wave's next block into st[i], K or V. Past its last block nothing is read: the lanes' offset is then beyond the
+    // buffer and zeros arrive. (No load is under a condition: the compiler would count it as not issued, and every wait
+    // for a block would be one for all loads.)
+    __device__ __forceinline__ void load_k(Block<kFormat, kOnce>& b, int key) {
+        const uint32_t beyond = key < k1 ? 0u : 0x80000000u;
+        b.load_k(rsrc, lane * 16 + beyond, (lane >> 4) * 16 + beyond, at);
+    }
+    __device__ __forceinline__ void load_v(Block<kFormat, kOnce>& b, int key) {
+        const uint32_t beyond = key < k1 ? 0u : 0x80000000u;
+        b.load_v(rsrc, lane * 16 + beyond, (lane >> 4) * 16 + beyond, at);
+        at += at_step;
     }
 
     __device__ __forceinline__ void begin(const CachedAttnArgs& a, const Work& w) {
@@ -242,28 +258,30 @@ struct Stretch {
         const int qw = wave % w.wq, kw = wave / w.wq;
         step = kKvBlock * kWaves / w.wq;
         k1 = w.k1;
-        base = (w.prefix ? a.pre : a.own).block<kFormat>(w.slot, w.hk, 0);
+        const KvView& c = w.prefix ? a.pre : a.own;
+        rsrc = __builtin_amdgcn_make_buffer_rsrc(c.block<kFormat>(w.slot, w.hk, 0), 0, c.blocks * kv_block_bytes(kFormat), kBufferDword3);
         kb = w.k0 + kw * kKvBlock;
+        at = kb / kKvBlock * kv_block_bytes(kFormat);
+        at_step = step / kKvBlock * kv_block_bytes(kFormat);
 #pragma unroll
-        for (int i = 0; i < kStages; ++i)
-            if (kb + i * step < k1) {
-                st[i].load_k(block_at(kb + i * step), lane);
-                st[i].load_v(block_at(kb + i * step), lane);
-            }
+        for (int i = 0; i < kStages; ++i) {
+            load_k(st[i], kb + i * step);
+            load_v(st[i], kb + i * step);
+        }
         const int nrows = (w.prefix ? a.B : 1) * a.T * a.G;
         const int row0 = w.tile * 16 * w.wq;
         const int r = row0 + qw * 16 + n;
         const bool have = r < nrows;
         const QueryRow qr = query_row(a, have ? r : row0, w.b, w.hk, w.prefix);
-        const int64_t at = (static_cast<int64_t>(qr.b) * a.T + qr.t) * a.ldq + qr.hq * kD;
+        const int64_t qat = (static_cast<int64_t>(qr.b) * a.T + qr.t) * a.ldq + qr.hq * kD;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             if constexpr (kF32) {
-                const u32x4* q = reinterpret_cast<const u32x4*>(static_cast<const float*>(a.q) + at + k_dim<kFormat>(s, g));
+                const u32x4* q = reinterpret_cast<const u32x4*>(static_cast<const float*>(a.q) + qat + k_dim<kFormat>(s, g));
                 qraw[2 * s] = q[0];
                 qraw[2 * s + 1] = q[1];
             } else {
-                qraw[s] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at + k_dim<kFormat>(s, g));
+                qraw[s] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + qat + k_dim<kFormat>(s, g));
             }
         }
         // keys below lim are seen by the lane's query, keys below minlim by all of the wave's
@@ -275,7 +293,9 @@ struct Stretch {
     }
 
     // Q as the matrix operand: as it is, or in three parts; returns what the scores are multiplied with
-    __device__ __forceinline__ float operand_q(float scale, bf16x8 (&qf)[kQS][4]) const {
+    __device__ __forceinline__ float operand_q(float scale, bf16x8 (&qf)[kQS][4]) {
+#pragma unroll
+        for (int i = 0; i < (kF32 ? 8 : 4); ++i) asm volatile("" : "+v"(qraw[i]));  // (arrived: no wait for them in the loop)
         if constexpr (!kF32) {
 #pragma unroll
             for (int s = 0; s < 4; ++s) qf[0][s] = __builtin_bit_cast(bf16x8, qraw[s]);
@@ -307,17 +327,19 @@ struct Stretch {
     __device__ __forceinline__ void attend(float scale, Shared& sh) {
         const int n = lane & 15, g = lane >> 4;
         bf16x8 qf[kQS][4];
-        const float qscale = operand_q(scale, qf);
+        const float qscale = operand_q(scale * kLog2e, qf);  // (scores in the log2 domain)
+
+        // p = exp2(score - base): base is at least the true maximum less kSlack, and moves to it only where a score exceeds it by
+        // more, so O is seldom rescaled. Each lane keeps the true maximum and the sum of its own keys.
         floatx4 acc[8];
-        float mrun = kNegInf, lrun = 0.0f;
+        float base = kLowest, top = kNegInf, sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[i] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
 
-        // one block: scores, probabilities, O; its registers are filled again, K's behind the scores and V's behind O, with the block
-        // kStages steps on
+        // one block: scores, probabilities, O; its registers are filled again, K's behind the scores and V's behind O, with the
+        // block kStages steps on
         auto take = [&](Block<kFormat, kOnce>& blk) {
             const int next = kb + kStages * step;
-            const bool more = next < k1;
             blk.settle(blk.k);
             floatx4 s[2];
             s[0] = s[1] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
@@ -328,66 +350,60 @@ struct Stretch {
                 for (int x = kQS - 1; x >= 0; --x) s[i >> 2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[x][i & 3], s[i >> 2], 0, 0, 0);
                 keep_order();
             }
-            float mx = kNegInf;
+            floatx4 f[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) f[t] = blk.ks[t] * qscale;
+            keep_order();
+            load_k(blk, next);
+            keep_order();
             const bool mask = kb + kKvBlock > minlim;  // (the same for the whole wave)
+            const int rest = lim - kb - g * 4;         // the lane's key 16 t + i is seen if it is below
+            float p[8], most = kNegInf;  // (the maximum of the scores themselves: it does not depend on how the keys are cut)
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[t][i] *= blk.ks[t][i] * qscale;
-                    mx = fmaxf(mx, s[t][i]);
-                }
+            for (int i = 0; i < 8; ++i) p[i] = s[i >> 2][i & 3] * f[i >> 2][i & 3];
             if (mask) {
-                mx = kNegInf;
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (kb + t * 16 + g * 4 + i >= lim) s[t][i] = kNegInf;
-                        mx = fmaxf(mx, s[t][i]);
-                    }
+                for (int i = 0; i < 8; ++i)
+                    if ((i >> 2) * 16 + (i & 3) >= rest) p[i] = kNegInf;
             }
-            keep_order();
-            if (more) blk.load_k(block_at(next), lane);
-            keep_order();
-            mx = fmaxf(max_groups(mx), mrun);
-            const float base = mx == kNegInf ? 0.0f : mx;  // (nothing seen yet: every p is 0)
-            if (__any(mx != mrun)) {
-                const float f = __builtin_amdgcn_exp2f((mrun - base) * kLog2e);
-                lrun *= f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) acc[i] *= f;
-                mrun = mx;
+            for (int i = 0; i < 8; ++i) most = fmaxf(most, p[i]);
+            top = fmaxf(top, most);
+            if (__any(most - base > kSlack)) {
+                const float to = max_groups(fmaxf(most, base));
+                const float by = __builtin_amdgcn_exp2f(base - to);
+                sum *= by;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[i] *= by;
+                base = to;
             }
-            float p[8], sum = 0.0f;
+            float add = 0.0f;
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e = __builtin_amdgcn_exp2f((s[t][i] - base) * kLog2e);
-                    sum += e;
-                    p[t * 4 + i] = e * blk.vs[t][i];
-                }
+            for (int i = 0; i < 8; ++i) {
+                const float e = __builtin_amdgcn_exp2f(p[i] - base);
+                add += e;
+                p[i] = e * blk.vs[i >> 2][i & 3];
+            }
+            sum += add;
             if (mask) {  // (a masked key's scale may be anything, NaN too)
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (kb + (i >> 2) * 16 + g * 4 + (i & 3) >= lim) p[i] = 0.0f;
+                    if ((i >> 2) * 16 + (i & 3) >= rest) p[i] = 0.0f;
             }
-            lrun += sum;
             blk.settle(blk.v);
             bf16x8 pf[kQS];
 #pragma unroll
             for (int x = 0; x < kQS; ++x) {
-                union { uint32_t u[4]; bf16x8 v; } f;
+                union { uint32_t u[4]; bf16x8 v; } h;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    f.u[j] = pack2(p[2 * j], p[2 * j + 1]);
+                    h.u[j] = pack2(p[2 * j], p[2 * j + 1]);
                     if (x + 1 < kQS) {
-                        p[2 * j] -= __uint_as_float(f.u[j] << 16);
-                        p[2 * j + 1] -= __uint_as_float(f.u[j] & 0xffff0000u);
+                        p[2 * j] -= __uint_as_float(h.u[j] << 16);
+                        p[2 * j + 1] -= __uint_as_float(h.u[j] & 0xffff0000u);
                     }
                 }
-                pf[x] = f.v;
+                pf[x] = h.v;
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -396,20 +412,23 @@ struct Stretch {
                 for (int x = kQS - 1; x >= 0; --x) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[x], acc[i], 0, 0, 0);
                 keep_order();
             }
-            if (more) blk.load_v(block_at(next), lane);
+            load_v(blk, next);
             kb += step;
         };
-        while (kb < k1) {
+        // (a way out of the middle of the loop would cost it the same)
+        while (kb + (kStages - 1) * step < k1) {
             take(st[0]);
-            if constexpr (kStages > 1) {
-                if (kb >= k1) break;
-                take(st[1]);
-            }
+            if constexpr (kStages > 1) take(st[1]);
         }
-        lrun = sum_groups(lrun);
+        if constexpr (kStages > 1)
+            if (kb < k1) take(st[0]);
+        // the sum and O relative to base, base, and the true maximum
+        sum = sum_groups(sum);
+        top = max_groups(top);
         if (g == 0) {
-            sh.ml[wave][0][n] = mrun;
-            sh.ml[wave][1][n] = lrun;
+            sh.ml[wave][0][n] = base;
+            sh.ml[wave][1][n] = sum;
+            sh.ml[wave][2][n] = top;
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) *reinterpret_cast<floatx4*>(&sh.o[wave][n][i * 16 + g * 4]) = acc[i];
@@ -425,13 +444,13 @@ __device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRo
         const int tq = rt >> 4, rn = rt & 15;
         if (row0 + rt >= nrows) continue;
         float mx = kNegInf;
-        for (int k = 0; k < wk; ++k) mx = fmaxf(mx, sh.ml[k * w.wq + tq][0][rn]);
+        for (int k = 0; k < wk; ++k) mx = fmaxf(mx, sh.ml[k * w.wq + tq][2][rn]);
         const float base = mx == kNegInf ? 0.0f : mx;
         float l = 0.0f;
         floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int k = 0; k < wk; ++k) {
             const int from = k * w.wq + tq;
-            const float f = __builtin_amdgcn_exp2f((sh.ml[from][0][rn] - base) * kLog2e);
+            const float f = __builtin_amdgcn_exp2f(sh.ml[from][0][rn] - base);
             l += f * sh.ml[from][1][rn];
             v += f * *reinterpret_cast<const floatx4*>(&sh.o[from][rn][d]);
         }
@@ -445,7 +464,7 @@ __device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRo
             if constexpr (kF32) *reinterpret_cast<floatx4*>(static_cast<float*>(a.o) + at) = v;
             else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
             if (d == 0) {
-                if (a.m) a.m[row] = empty ? kNegInf : nan ? l : mx;
+                if (a.m) a.m[row] = empty ? kNegInf : nan ? l : mx * kLn2;
                 if (a.l) a.l[row] = empty ? 0.0f : l;
             }
         } else {
@@ -606,7 +625,7 @@ __global__ __launch_bounds__(kJoinThreads) void cached_attn_join_kernel(CachedAt
     for (int p = run; p < parts; p += 8) {
         const float2 s = *reinterpret_cast<const float2*>(pml + 2 * p);
         const floatx4 v = p == run ? v0 : *reinterpret_cast<const floatx4*>(po + static_cast<int64_t>(p) * kD + d);
-        const float f = __builtin_amdgcn_exp2f((s.x - base) * kLog2e);
+        const float f = __builtin_amdgcn_exp2f(s.x - base);
         l += f * s.y;
         acc += f * v;
     }
@@ -628,7 +647,7 @@ __global__ __launch_bounds__(kJoinThreads) void cached_attn_join_kernel(CachedAt
     if constexpr (kF32) *reinterpret_cast<floatx4*>(static_cast<float*>(a.o) + at) = acc;
     else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = make_uint2(pack2(acc[0], acc[1]), pack2(acc[2], acc[3]));
     if (threadIdx.x == 0) {
-        if (a.m) a.m[row] = nan ? l : mx;
+        if (a.m) a.m[row] = nan ? l : mx * kLn2;
         if (a.l) a.l[row] = empty ? 0.0f : l;
     }
 }
