@@ -693,8 +693,8 @@ int64_t make_plan(CachedAttnArgs& a, AttnRows& rows, bool* join) {
     }
 
     const int64_t slots = std::max<int64_t>(kResident - a.pre_groups, kResident / 4);
-    // (a list past 2^30 steps, thousands of query tiles over the longest cache, has triples enough)
-    a.aligned = all > (1 << 30) || (longest <= kWholeSteps && (a.pre_groups == 0 || triples <= slots));
+    // (an empty list has no shares; one past 2^30 steps, thousands of query tiles over the longest cache, has triples enough)
+    a.aligned = all == 0 || all > (1 << 30) || (longest <= kWholeSteps && (a.pre_groups == 0 || triples <= slots));
     a.head_steps = a.aligned ? 0 : static_cast<int>(cum);
     a.own_groups = static_cast<int>(a.aligned ? triples : std::min<int64_t>(all, slots));
     int own_parts = 1;

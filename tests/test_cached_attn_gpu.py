@@ -164,6 +164,23 @@ def test_prefix_in_the_same_cache_and_slots_twice():
     assert torch.equal(r.output[4], r.output[0])
 
 
+def test_a_prefix_and_nothing_of_their_own():
+    """A full batch whose slots hold nothing yet, and one none of whose rows has a query."""
+    from dirktensor_amd import KVCache
+
+    B, H = 64, 16
+    c, p = KVCache(B, 10, H), KVCache(1, 500, H)
+    fill(p, [500], 700)
+    q = randn((B, 1, H, D), 701, torch.bfloat16)
+    run(q, c, prefix=p)
+    r = run(q, c, counts=[0] * B, prefix=p)
+    assert not bool(r.output.any())
+    fill(c, [1] * B, 702)
+    run(q, c, counts=[0] * B, prefix=p)
+    run(q, c, counts=[0] * B)
+    run(q, c, counts=[1] + [0] * (B - 1), prefix=p)
+
+
 def test_a_whole_sequence_is_the_causal_attention():
     """All tokens appended at once, unquantised, then attended: flash_attention_forward's results."""
     from dirktensor_amd import KVCache, cached_attention, flash_attention_forward
