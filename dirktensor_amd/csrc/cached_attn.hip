@@ -45,6 +45,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kJoinThreads = 256;
+constexpr int kKeysLog = 7;  // log2 of kKvBlock * kWaves
+static_assert(1 << kKeysLog == kKvBlock * kWaves, "a step's keys");
 constexpr int kD = DT_HEAD_DIM;
 constexpr int kObufRow = kD + 4;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -78,21 +80,21 @@ struct CachedAttnArgs {
     int causal;
     float scale;
     int parts;       // partial results a row at most
-    // own keys: steps of 32 keys a key wave
-    int own_wq, own_tiles;
+    // own keys, in steps of 32 keys a key wave; own_wl: log2 of the waves that take query tiles
+    int own_wl, own_tiles;
     int head_steps;     // steps of one head: all batch rows and tiles
     int own_groups;     // workgroups
     int aligned;        // one (head, batch row, tile) each; otherwise shares of the list:
     int share, extra;
     // prefix
-    int pre_slot, pre_len, pre_wq, pre_tiles, pre_chunk;  // pre_chunk: keys a workgroup
+    int pre_slot, pre_len, pre_wl, pre_tiles, pre_chunk;  // pre_chunk: keys a workgroup
     int pre_parts, pre_groups;
 };
 
 // steps of a batch row's keys for a query tile (0: there is nothing to see)
-__host__ __device__ __forceinline__ int steps_of(int len, int cnt, int wq) {
-    const int keys = kKvBlock * kWaves / wq;
-    return cnt == 0 ? 0 : (len + keys - 1) / keys;
+__host__ __device__ __forceinline__ int steps_of(int len, int cnt, int wl) {
+    const int keys = (kKvBlock * kWaves) >> wl;
+    return cnt == 0 ? 0 : (len + keys - 1) >> (kKeysLog - wl);
 }
 // The list's steps in equal shares: the first `extra` workgroups have one more than `share`. group_of: whose share step s is in.
 __host__ __device__ __forceinline__ int share_start(const CachedAttnArgs& a, int w) {
@@ -197,9 +199,11 @@ struct QueryRow {
 };
 // row r of those that share key/value head hk's keys: tokens, then the group's heads; for the prefix the batch first
 __device__ __forceinline__ QueryRow query_row(const CachedAttnArgs& a, int r, int b, int hk, bool prefix) {
-    const int g = r % a.G, bt = r / a.G;
-    if (prefix) return {bt / a.T, bt % a.T, hk * a.G + g};
-    return {b, bt, hk * a.G + g};
+    // (divisions by numbers that are mostly 1)
+    const int bt = a.G == 1 ? r : r / a.G, g = r - bt * a.G;
+    if (!prefix) return {b, bt, hk * a.G + g};
+    const int of = a.T == 1 ? bt : bt / a.T;
+    return {of, bt - of * a.T, hk * a.G + g};
 }
 
 // One workgroup's stretch of keys for one (head, batch row, tile), or of the prefix for one (head, tile).
@@ -207,7 +211,7 @@ struct Work {
     int hk, b, tile;
     int k0, k1;      // keys
     int slot, len, cnt;  // cnt: the batch row's query tokens
-    int wq;
+    int wl;          // log2 of the waves that take query tiles
     int part;        // where the partial result goes, or -1: the result is written
     bool prefix;
 };
@@ -255,8 +259,8 @@ struct Stretch {
         lane = tid & 63;
         wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int n = lane & 15, g = lane >> 4;
-        const int qw = wave % w.wq, kw = wave / w.wq;
-        step = kKvBlock * kWaves / w.wq;
+        const int qw = wave & ((1 << w.wl) - 1), kw = wave >> w.wl;
+        step = (kKvBlock * kWaves) >> w.wl;
         k1 = w.k1;
         const KvView& c = w.prefix ? a.pre : a.own;
         rsrc = __builtin_amdgcn_make_buffer_rsrc(c.block<kFormat>(w.slot, w.hk, 0), 0, c.blocks * kv_block_bytes(kFormat), kBufferDword3);
@@ -269,7 +273,7 @@ struct Stretch {
             load_v(st[i], kb + i * step);
         }
         const int nrows = (w.prefix ? a.B : 1) * a.T * a.G;
-        const int row0 = w.tile * 16 * w.wq;
+        const int row0 = w.tile * 16 << w.wl;
         const int r = row0 + qw * 16 + n;
         const bool have = r < nrows;
         const QueryRow qr = query_row(a, have ? r : row0, w.b, w.hk, w.prefix);
@@ -438,18 +442,18 @@ struct Stretch {
 // The waves' results meet: a thread sums four values of a row over the key waves, scaled to their common maximum.
 template <bool kF32>
 __device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRows& rows, const Work& w, const Shared& sh) {
-    const int wk = kWaves / w.wq, row0 = w.tile * 16 * w.wq, nrows = (w.prefix ? a.B : 1) * a.T * a.G;
-    for (int it = thread_here(); it < w.wq * 16 * (kD / 4); it += kThreads) {
+    const int wk = kWaves >> w.wl, row0 = w.tile * 16 << w.wl, nrows = (w.prefix ? a.B : 1) * a.T * a.G;
+    for (int it = thread_here(); it < (16 * (kD / 4)) << w.wl; it += kThreads) {
         const int d = (it & 31) * 4, rt = it >> 5;  // (row within the workgroup's tiles)
         const int tq = rt >> 4, rn = rt & 15;
         if (row0 + rt >= nrows) continue;
         float mx = kNegInf;
-        for (int k = 0; k < wk; ++k) mx = fmaxf(mx, sh.ml[k * w.wq + tq][2][rn]);
+        for (int k = 0; k < wk; ++k) mx = fmaxf(mx, sh.ml[(k << w.wl) + tq][2][rn]);
         const float base = mx == kNegInf ? 0.0f : mx;
         float l = 0.0f;
         floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int k = 0; k < wk; ++k) {
-            const int from = k * w.wq + tq;
+            const int from = (k << w.wl) + tq;
             const float f = __builtin_amdgcn_exp2f(sh.ml[from][0][rn] - base);
             l += f * sh.ml[from][1][rn];
             v += f * *reinterpret_cast<const floatx4*>(&sh.o[from][rn][d]);
@@ -479,36 +483,55 @@ template <int kFormat, bool kF32, bool kOnce>
 __global__ __launch_bounds__(kThreads, 2) void cached_attn_kernel(CachedAttnArgs a, AttnRows rows) {
     __shared__ __align__(16) Shared sh;
     __shared__ AttnRows rl;
-    // the batch rows into LDS: one trip to the arguments' memory in place of one for each dependent use
-    for (int i = threadIdx.x; i < a.B; i += kThreads) {
-        rl.len[i] = rows.len[i];
-        rl.cum[i] = rows.cum[i];
-        rl.slot[i] = rows.slot[i];
-        rl.cnt[i] = rows.cnt[i];
-    }
+    // All arguments in one trip to their memory, in place of one for each dependent use: the batch rows into LDS (all of
+    // them, so no length is waited for), the rest into scalar registers or at least the scalar cache.
+    static_assert(kThreads == kMaxRaggedBatch, "one batch row a thread");
+    rl.len[threadIdx.x] = rows.len[threadIdx.x];
+    rl.cum[threadIdx.x] = rows.cum[threadIdx.x];
+    rl.slot[threadIdx.x] = rows.slot[threadIdx.x];
+    rl.cnt[threadIdx.x] = rows.cnt[threadIdx.x];
+    asm volatile("" ::"s"(a.own.data), "s"(a.q), "s"(a.part_o), "s"(a.T), "s"(a.parts), "s"(a.share), "s"(a.pre_groups));
     __syncthreads();
     int id = blockIdx.x;
     Work w;
     w.prefix = id < a.pre_groups;
-    w.wq = w.prefix ? a.pre_wq : a.own_wq;
-    const int keys = kKvBlock * kWaves / w.wq;
-    int s = 0, end = 0;
+    w.wl = w.prefix ? a.pre_wl : a.own_wl;
+    const int keys_log = kKeysLog - w.wl;
+    int s = 0, end = 0, steps = 0, off = 0, count = 0;
+    // the batch row's entries
+    const auto load_row = [&]() {
+        w.len = __builtin_amdgcn_readfirstlane(rl.len[w.b]);
+        w.cnt = __builtin_amdgcn_readfirstlane(rl.cnt[w.b]);
+        w.slot = __builtin_amdgcn_readfirstlane(rl.slot[w.b]);
+        steps = steps_of(w.len, w.cnt, w.wl);
+    };
+    const auto set_keys = [&]() {
+        w.k0 = off << keys_log;
+        w.k1 = min(w.len, (off + count) << keys_log);
+        if (a.causal && a.T > 1) {  // nothing past the tile's newest query
+            const int r = ((w.tile + 1) * 16 << w.wl) - 1, t = min(a.T - 1, a.G == 1 ? r : r / a.G);
+            w.k1 = min(w.k1, max(0, w.len - w.cnt + t + 1));
+        }
+    };
     if (w.prefix) {
         // tiles of one chunk beside each other on one XCD (workgroups go to the eight XCDs in turn), which reads it once
-        const int chunks = a.pre_groups / a.pre_tiles, full = chunks / 8 * 8 * a.pre_tiles;
-        int item;
-        if (id < full) {
-            const int oct = id / (8 * a.pre_tiles), rem = id % (8 * a.pre_tiles);
-            w.tile = rem >> 3;
-            item = oct * 8 + (rem & 7);
-        } else {
-            const int left = chunks % 8;
-            w.tile = (id - full) / left;
-            item = chunks / 8 * 8 + (id - full) % left;
+        int item = id;
+        w.tile = 0;
+        if (a.pre_tiles > 1) {
+            const int chunks = a.pre_groups / a.pre_tiles, full = chunks / 8 * 8 * a.pre_tiles;
+            if (id < full) {
+                const int oct = id / (8 * a.pre_tiles), rem = id - oct * 8 * a.pre_tiles;
+                w.tile = rem >> 3;
+                item = oct * 8 + (rem & 7);
+            } else {
+                const int left = chunks % 8;
+                w.tile = (id - full) / left;
+                item = chunks / 8 * 8 + (id - full) % left;
+            }
         }
-        w.hk = item % a.pre.heads;
-        w.b = 0;
         w.part = item / a.pre.heads;
+        w.hk = item - w.part * a.pre.heads;
+        w.b = 0;
         w.k0 = w.part * a.pre_chunk;
         w.k1 = min(a.pre_len, w.k0 + a.pre_chunk);
         w.slot = a.pre_slot;
@@ -520,23 +543,17 @@ __global__ __launch_bounds__(kThreads, 2) void cached_attn_kernel(CachedAttnArgs
         const int full = a.own_groups / 8 * 8;
         if (id < full) id = (id & 7) * (a.own_groups / 8) + (id >> 3);
         if (a.aligned) {
-            w.tile = id % a.own_tiles;
-            w.b = id / a.own_tiles % a.B;
-            w.hk = id / a.own_tiles / a.B;
+            const int hb = a.own_tiles == 1 ? id : id / a.own_tiles;
+            w.tile = id - hb * a.own_tiles;
+            w.hk = hb / a.B;
+            w.b = hb - w.hk * a.B;
             w.part = a.pre_parts > 0 ? a.pre_parts : -1;
+            load_row();
+            if (steps == 0 && a.pre_parts > 0) return;  // (only the prefix's parts are joined)
+            count = steps;
         } else {
             s = share_start(a, id);
             end = share_start(a, id + 1);
-        }
-    }
-    // fills w with the next stretch of the list's share
-    const auto next = [&]() {
-        int off = 0, count;
-        if (a.aligned) {
-            w.len = __builtin_amdgcn_readfirstlane(rl.len[w.b]);
-            w.cnt = __builtin_amdgcn_readfirstlane(rl.cnt[w.b]);
-            count = steps_of(w.len, w.cnt, w.wq);
-        } else {
             w.hk = s / a.head_steps;
             const int in_head = s - w.hk * a.head_steps;
             // the last batch row that begins at or before this step (rows without steps begin where the next one does)
@@ -547,9 +564,7 @@ __global__ __launch_bounds__(kThreads, 2) void cached_attn_kernel(CachedAttnArgs
                 if (i * 64 < a.B) below += __popcll(__ballot(at < a.B && rl.cum[at] <= in_head));
             }
             w.b = __builtin_amdgcn_readfirstlane(below) - 1;
-            w.len = __builtin_amdgcn_readfirstlane(rl.len[w.b]);
-            w.cnt = __builtin_amdgcn_readfirstlane(rl.cnt[w.b]);
-            const int steps = steps_of(w.len, w.cnt, w.wq);
+            load_row();
             const int in_row = in_head - __builtin_amdgcn_readfirstlane(rl.cum[w.b]);
             w.tile = in_row / steps;
             off = in_row - w.tile * steps;
@@ -557,15 +572,26 @@ __global__ __launch_bounds__(kThreads, 2) void cached_attn_kernel(CachedAttnArgs
             w.part = a.pre_parts == 0 && count == steps ? -1 : a.pre_parts + id - group_of(a, s - off);
             s += count;
         }
-        w.slot = __builtin_amdgcn_readfirstlane(rl.slot[w.b]);
-        w.k0 = off * keys;
-        w.k1 = min(w.len, (off + count) * keys);
-        if (a.causal) {  // nothing past the tile's newest query
-            const int t = min(a.T - 1, ((w.tile + 1) * 16 * w.wq - 1) / a.G);
-            w.k1 = min(w.k1, max(0, w.len - w.cnt + t + 1));
+        set_keys();
+    }
+    // the share's next triple, whole or as much of it as is left: tile, batch row, head
+    const auto next = [&]() {
+        if (++w.tile == a.own_tiles) {
+            w.tile = 0;
+            do {
+                if (++w.b == a.B) {
+                    w.b = 0;
+                    ++w.hk;
+                }
+                load_row();
+            } while (steps == 0);
         }
+        off = 0;
+        count = min(steps, end - s);
+        w.part = a.pre_parts == 0 && count == steps ? -1 : a.pre_parts;  // (its first part)
+        s += count;
+        set_keys();
     };
-    if (!w.prefix) next();
     Stretch<kFormat, kF32, kOnce> st;
     st.begin(a, w);
     for (;;) {
@@ -602,10 +628,10 @@ __global__ __launch_bounds__(kJoinThreads) void cached_attn_join_kernel(CachedAt
     const int b = bt / a.T, t = bt % a.T;
     int parts = 0;
     if (t < rows.cnt[b]) {
-        const int steps = steps_of(rows.len[b], rows.cnt[b], a.own_wq);
+        const int steps = steps_of(rows.len[b], rows.cnt[b], a.own_wl);
         int own = steps > 0;
         if (own && !a.aligned) {
-            const int first = hq / a.G * a.head_steps + rows.cum[b] + (t * a.G + hq % a.G) / (16 * a.own_wq) * steps;
+            const int first = hq / a.G * a.head_steps + rows.cum[b] + ((t * a.G + hq % a.G) >> (4 + a.own_wl)) * steps;
             own = group_of(a, first + steps - 1) - group_of(a, first) + 1;
         }
         if (own == 1 && a.pre_parts == 0) return;  // (written already)
@@ -655,38 +681,40 @@ __global__ __launch_bounds__(kJoinThreads) void cached_attn_join_kernel(CachedAt
 constexpr int kCus = 256;
 constexpr int kWholeSteps = 4;     // up to so many steps (of 256 keys for one query tile) a triple's keys are not cut
 
-// waves that take query tiles: as many as there are tiles of 16 rows
-int query_waves(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : kWaves == 4 || rows <= 64 ? 4 : 8; }
+// log2 of the waves that take query tiles: as many as there are tiles of 16 rows
+int query_waves_log(int64_t rows) { return rows <= 16 ? 0 : rows <= 32 ? 1 : 2; }
 
 // How a call is cut; fills rows' cum and the arguments that follow from the sizes. Returns the workspace's bytes.
 int64_t make_plan(CachedAttnArgs& a, AttnRows& rows, bool* join) {
     constexpr int kResident = 2 * kCus;
     const int heads = a.own.heads;
     const int64_t own_rows = static_cast<int64_t>(a.T) * a.G, all_rows = own_rows * a.B;
-    a.own_wq = query_waves(own_rows);
-    a.own_tiles = static_cast<int>((own_rows + 16 * a.own_wq - 1) / (16 * a.own_wq));
+    a.own_wl = query_waves_log(own_rows);
+    a.own_tiles = static_cast<int>((own_rows + (16 << a.own_wl) - 1) >> (4 + a.own_wl));
     int longest = 0, shortest = kMaxCacheTokens;
     int64_t cum = 0;
     for (int b = 0; b < a.B; ++b) {
         rows.cum[b] = static_cast<int>(cum);
-        const int n = steps_of(rows.len[b], rows.cnt[b], a.own_wq);
+        const int n = steps_of(rows.len[b], rows.cnt[b], a.own_wl);
         cum += static_cast<int64_t>(n) * a.own_tiles;
         longest = std::max(longest, n);
         shortest = std::min(shortest, n);
     }
     const int64_t all = cum * heads, triples = static_cast<int64_t>(heads) * a.B * a.own_tiles;
 
-    a.pre_wq = a.pre_tiles = 1;
-    a.pre_chunk = a.pre_parts = a.pre_groups = 0;
+    a.pre_tiles = 1;
+    a.pre_wl = a.pre_chunk = a.pre_parts = a.pre_groups = 0;
     if (a.pre_len > 0) {
-        // as many of the workgroups as the prefix has of the waves' work
-        a.pre_wq = query_waves(all_rows);
-        a.pre_tiles = static_cast<int>((all_rows + 16 * a.pre_wq - 1) / (16 * a.pre_wq));
-        const int unit = kKvBlock * kWaves / a.pre_wq;
+        // as many of the workgroups as the prefix has of the waves' work (beginning and ending a triple costs about two steps)
+        a.pre_wl = query_waves_log(all_rows);
+        a.pre_tiles = static_cast<int>((all_rows + (16 << a.pre_wl) - 1) >> (4 + a.pre_wl));
+        const int unit = (kKvBlock * kWaves) >> a.pre_wl;
         const int64_t steps = (a.pre_len + unit - 1) / unit, per_chunk = static_cast<int64_t>(a.pre_tiles) * heads;
-        const int64_t groups = std::max<int64_t>(kResident * (steps * per_chunk) / (steps * per_chunk + all), 1);
-        // but at least four steps each: a workgroup's start and end cost about as much
-        const int64_t chunks = std::max<int64_t>(1, groups / per_chunk), each = std::max<int64_t>(4, (steps + chunks - 1) / chunks);
+        const int64_t own_work = all + 2 * std::min(all, triples);
+        const int64_t groups = std::max<int64_t>(kResident * (steps * per_chunk) / (steps * per_chunk + own_work), 1);
+        // but at least four steps each, eight where four waves' rows are left as partial results: these weigh as much as the keys
+        const int64_t chunks = std::max<int64_t>(1, groups / per_chunk);
+        const int64_t each = std::max<int64_t>(a.pre_wl == 2 ? 8 : 4, (steps + chunks - 1) / chunks);
         a.pre_chunk = static_cast<int>(std::min(each, steps) * unit);
         a.pre_parts = (a.pre_len + a.pre_chunk - 1) / a.pre_chunk;
         a.pre_groups = static_cast<int>(a.pre_parts * per_chunk);
@@ -714,7 +742,7 @@ int launch(const CachedAttnArgs& a, const AttnRows& rows, bool join, int format,
     const int64_t groups = static_cast<int64_t>(a.own_groups) + a.pre_groups;
     if (groups > 0x7fffff) return set_error(DT_ERR_UNSUPPORTED, "the call needs %lld workgroups", (long long)groups);
     const bool f32 = dtype != DT_BF16;
-    const bool once = a.own_wq == 1 && a.own_tiles == 1;
+    const bool once = a.own_wl == 0 && a.own_tiles == 1;
     if (groups > 0) {
         const dim3 g(static_cast<unsigned>(groups)), t(kThreads);
 #define DT_GO(F)                                                                                        \
@@ -788,7 +816,7 @@ int dt_cached_attn_workspace(const dt_kv_cache* cache, int B, int T, int H, int 
     clear_error();
     if (!bytes) return set_error(DT_ERR_INVALID_ARG, "bytes is NULL");
     CachedAttnArgs a{};
-    AttnRows rows;
+    AttnRows rows{};
     bool join = false;
     DT_TRY(check_call(cache, B, T, H, D, slots, counts, prefix, prefix_slot, dtype, &a, &rows));
     *bytes = make_plan(a, rows, &join);
@@ -804,7 +832,7 @@ int dt_cached_attn_fwd(dt_kv_cache* cache, const void* q, void* o, float* m, flo
     if (!(scale > 0.0f) || !std::isfinite(scale)) return set_error(DT_ERR_INVALID_ARG, "scale %g must be finite and > 0", scale);
     if (causal != 0 && causal != 1) return set_error(DT_ERR_INVALID_ARG, "causal must be 0 or 1");
     CachedAttnArgs a{};
-    AttnRows rows;
+    AttnRows rows{};
     DT_TRY(check_call(cache, B, T, H, D, slots, counts, prefix, prefix_slot, dtype, &a, &rows));
     const size_t esz = dtype == DT_BF16 ? 2 : 4;
     const int64_t dm = static_cast<int64_t>(H) * kD;
