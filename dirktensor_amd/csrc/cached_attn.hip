@@ -62,7 +62,7 @@ constexpr int stages(int format, bool f32) { return format == DT_KV_BF16 || f32 
 // The batch rows, by value in the kernel's arguments.
 struct AttnRows {
     int32_t len[kMaxRaggedBatch];       // tokens held
-    int32_t cum[kMaxRaggedBatch];       // steps of one head before this row's, all query tiles
+    int32_t cum[kMaxRaggedBatch];       // places of one head in the list before this row's, all query tiles
     uint16_t slot[kMaxRaggedBatch];
     uint16_t cnt[kMaxRaggedBatch];      // query tokens
 };
@@ -82,9 +82,10 @@ struct CachedAttnArgs {
     int parts;       // partial results a row at most
     // own keys, in steps of 32 keys a key wave; own_wl: log2 of the waves that take query tiles
     int own_wl, own_tiles;
-    int head_steps;     // steps of one head: all batch rows and tiles
     int own_groups;     // workgroups
     int aligned;        // one (head, batch row, tile) each; otherwise shares of the list:
+    int lead;           // places that a triple has in the list before those of its steps, for what beginning it costs
+    int head_places;    // of one head: all batch rows and tiles
     int share, extra;
     // prefix
     int pre_slot, pre_len, pre_wl, pre_tiles, pre_chunk;  // pre_chunk: keys a workgroup
@@ -96,7 +97,7 @@ __host__ __device__ __forceinline__ int steps_of(int len, int cnt, int wl) {
     const int keys = (kKvBlock * kWaves) >> wl;
     return cnt == 0 ? 0 : (len + keys - 1) >> (kKeysLog - wl);
 }
-// The list's steps in equal shares: the first `extra` workgroups have one more than `share`. group_of: whose share step s is in.
+// The list's places in equal shares: the first `extra` workgroups have one more than `share`. group_of: whose share place s is in.
 __host__ __device__ __forceinline__ int share_start(const CachedAttnArgs& a, int w) {
     return w * a.share + (w < a.extra ? w : a.extra);
 }
@@ -554,9 +555,9 @@ __global__ __launch_bounds__(kThreads, 2) void cached_attn_kernel(CachedAttnArgs
         } else {
             s = share_start(a, id);
             end = share_start(a, id + 1);
-            w.hk = s / a.head_steps;
-            const int in_head = s - w.hk * a.head_steps;
-            // the last batch row that begins at or before this step (rows without steps begin where the next one does)
+            w.hk = s / a.head_places;
+            const int in_head = s - w.hk * a.head_places;
+            // the last batch row that begins at or before this place (rows without steps begin where the next one does)
             int below = 0;
 #pragma unroll
             for (int i = 0; i < kMaxRaggedBatch / 64; ++i) {
@@ -566,8 +567,13 @@ __global__ __launch_bounds__(kThreads, 2) void cached_attn_kernel(CachedAttnArgs
             w.b = __builtin_amdgcn_readfirstlane(below) - 1;
             load_row();
             const int in_row = in_head - __builtin_amdgcn_readfirstlane(rl.cum[w.b]);
-            w.tile = in_row / steps;
-            off = in_row - w.tile * steps;
+            w.tile = in_row / (steps + a.lead);
+            off = in_row - w.tile * (steps + a.lead) - a.lead;
+            if (off < 0) {
+                s -= off;
+                off = 0;
+            }
+            if (s >= end) return;  // (no step in this share)
             count = min(steps - off, end - s);
             w.part = a.pre_parts == 0 && count == steps ? -1 : a.pre_parts + id - group_of(a, s - off);
             s += count;
@@ -587,6 +593,7 @@ __global__ __launch_bounds__(kThreads, 2) void cached_attn_kernel(CachedAttnArgs
             } while (steps == 0);
         }
         off = 0;
+        s += a.lead;
         count = min(steps, end - s);
         w.part = a.pre_parts == 0 && count == steps ? -1 : a.pre_parts;  // (its first part)
         s += count;
@@ -597,7 +604,7 @@ __global__ __launch_bounds__(kThreads, 2) void cached_attn_kernel(CachedAttnArgs
     for (;;) {
         st.attend(a.scale, sh);
         const Work done = w;
-        const bool more = s < end;
+        const bool more = s + a.lead < end;
         if (more) {  // the next stretch's first loads are under way while this one is put together
             next();
             st.begin(a, w);
@@ -631,7 +638,7 @@ __global__ __launch_bounds__(kJoinThreads) void cached_attn_join_kernel(CachedAt
         const int steps = steps_of(rows.len[b], rows.cnt[b], a.own_wl);
         int own = steps > 0;
         if (own && !a.aligned) {
-            const int first = hq / a.G * a.head_steps + rows.cum[b] + ((t * a.G + hq % a.G) >> (4 + a.own_wl)) * steps;
+            const int first = hq / a.G * a.head_places + rows.cum[b] + ((t * a.G + hq % a.G) >> (4 + a.own_wl)) * (steps + a.lead) + a.lead;
             own = group_of(a, first + steps - 1) - group_of(a, first) + 1;
         }
         if (own == 1 && a.pre_parts == 0) return;  // (written already)
@@ -679,6 +686,7 @@ __global__ __launch_bounds__(kJoinThreads) void cached_attn_join_kernel(CachedAt
 }
 
 constexpr int kCus = 256;
+constexpr int kLead = 2;           // steps that beginning and ending a triple costs
 constexpr int kWholeSteps = 4;     // up to so many steps (of 256 keys for one query tile) a triple's keys are not cut
 
 // log2 of the waves that take query tiles: as many as there are tiles of 16 rows
@@ -692,15 +700,15 @@ int64_t make_plan(CachedAttnArgs& a, AttnRows& rows, bool* join) {
     a.own_wl = query_waves_log(own_rows);
     a.own_tiles = static_cast<int>((own_rows + (16 << a.own_wl) - 1) >> (4 + a.own_wl));
     int longest = 0, shortest = kMaxCacheTokens;
-    int64_t cum = 0;
+    int64_t steps = 0, rows_held = 0;
     for (int b = 0; b < a.B; ++b) {
-        rows.cum[b] = static_cast<int>(cum);
         const int n = steps_of(rows.len[b], rows.cnt[b], a.own_wl);
-        cum += static_cast<int64_t>(n) * a.own_tiles;
+        steps += n;
+        rows_held += n > 0;
         longest = std::max(longest, n);
         shortest = std::min(shortest, n);
     }
-    const int64_t all = cum * heads, triples = static_cast<int64_t>(heads) * a.B * a.own_tiles;
+    const int64_t all = steps * a.own_tiles * heads, triples = static_cast<int64_t>(heads) * a.B * a.own_tiles;
 
     a.pre_tiles = 1;
     a.pre_wl = a.pre_chunk = a.pre_parts = a.pre_groups = 0;
@@ -709,29 +717,39 @@ int64_t make_plan(CachedAttnArgs& a, AttnRows& rows, bool* join) {
         a.pre_wl = query_waves_log(all_rows);
         a.pre_tiles = static_cast<int>((all_rows + (16 << a.pre_wl) - 1) >> (4 + a.pre_wl));
         const int unit = (kKvBlock * kWaves) >> a.pre_wl;
-        const int64_t steps = (a.pre_len + unit - 1) / unit, per_chunk = static_cast<int64_t>(a.pre_tiles) * heads;
-        const int64_t own_work = all + 2 * std::min(all, triples);
-        const int64_t groups = std::max<int64_t>(kResident * (steps * per_chunk) / (steps * per_chunk + own_work), 1);
+        const int64_t pre_steps = (a.pre_len + unit - 1) / unit, per_chunk = static_cast<int64_t>(a.pre_tiles) * heads;
+        const int64_t own_work = all + kLead * rows_held * a.own_tiles * heads;
+        const int64_t groups = std::max<int64_t>(kResident * (pre_steps * per_chunk) / (pre_steps * per_chunk + own_work), 1);
         // but at least four steps each, eight where four waves' rows are left as partial results: these weigh as much as the keys
         const int64_t chunks = std::max<int64_t>(1, groups / per_chunk);
-        const int64_t each = std::max<int64_t>(a.pre_wl == 2 ? 8 : 4, (steps + chunks - 1) / chunks);
-        a.pre_chunk = static_cast<int>(std::min(each, steps) * unit);
+        const int64_t each = std::max<int64_t>(a.pre_wl == 2 ? 8 : 4, (pre_steps + chunks - 1) / chunks);
+        a.pre_chunk = static_cast<int>(std::min(each, pre_steps) * unit);
         a.pre_parts = (a.pre_len + a.pre_chunk - 1) / a.pre_chunk;
         a.pre_groups = static_cast<int>(a.pre_parts * per_chunk);
     }
 
     const int64_t slots = std::max<int64_t>(kResident - a.pre_groups, kResident / 4);
-    // (an empty list has no shares; one past 2^30 steps, thousands of query tiles over the longest cache, has triples enough)
-    a.aligned = all == 0 || all > (1 << 30) || (longest <= kWholeSteps && (a.pre_groups == 0 || triples <= slots));
-    a.head_steps = a.aligned ? 0 : static_cast<int>(cum);
-    a.own_groups = static_cast<int>(a.aligned ? triples : std::min<int64_t>(all, slots));
+    // (an empty list has no shares; one past 2^28 steps, thousands of query tiles over the longest cache, has triples enough)
+    a.aligned = all == 0 || all > (1 << 28) || (longest <= kWholeSteps && (a.pre_groups == 0 || triples <= slots));
     int own_parts = 1;
     bool whole = true;  // every triple's keys in one workgroup
+    a.own_groups = static_cast<int>(triples);
     if (!a.aligned) {
-        a.share = static_cast<int>(all / a.own_groups);
-        a.extra = static_cast<int>(all % a.own_groups);
+        // beginning a triple is counted where workgroups have several; one that is cut is begun twice, which no count would mend
+        a.lead = rows_held * a.own_tiles * heads > slots ? kLead : 0;
+        int64_t cum = 0;
+        for (int b = 0; b < a.B; ++b) {
+            rows.cum[b] = static_cast<int>(cum);
+            const int n = steps_of(rows.len[b], rows.cnt[b], a.own_wl);
+            if (n > 0) cum += static_cast<int64_t>(n + a.lead) * a.own_tiles;
+        }
+        a.head_places = static_cast<int>(cum);
+        const int64_t places = cum * heads;
+        a.own_groups = static_cast<int>(std::min<int64_t>(all, slots));
+        a.share = static_cast<int>(places / a.own_groups);
+        a.extra = static_cast<int>(places % a.own_groups);
         own_parts = std::min(longest, (longest - 1) / a.share + 2);
-        whole = shortest == longest && a.extra == 0 && a.share % longest == 0;
+        whole = shortest == longest && a.extra == 0 && a.share % (longest + a.lead) == 0;
     }
     a.parts = own_parts + a.pre_parts;
     *join = !(whole && a.pre_parts == 0);
