@@ -30,6 +30,8 @@ def _per_row(x, B: int, name: str):
     """A per-row argument as B int32 values in host memory and their address (None: NULL)."""
     if x is None:
         return None, None
+    if type(x) is np.ndarray and x.dtype == np.int32 and x.shape == (B,) and x.flags.c_contiguous:
+        return x, x.ctypes.data
     a = np.asarray(x.cpu() if _is_torch(x) else x)
     if a.dtype.kind not in "iu" or a.shape != (B,):
         raise ValueError(f"{name} must be {B} whole numbers, got {a.dtype} of shape {a.shape}")
@@ -73,6 +75,7 @@ class KVCache:
         C.call("dt_kv_cache_create", self.ctx.handle, self.slots, self.capacity, self.n_heads, C.HEAD_DIM,
                _FORMATS[format], ctypes.byref(h))
         self.handle = h
+        self._device = torch.device("cuda", self.ctx.device) if torch is not None else None
 
     def close(self) -> None:
         if getattr(self, "handle", None):
@@ -115,7 +118,7 @@ class KVCache:
         """Writes the rows of K and V [B, T, n_heads, 128] (both fp32 or both bf16; torch device tensors, views of a
         projection's output among them, or numpy arrays) behind what the B slots hold: slots[b], distinct, or 0 .. B-1.
         With ``counts`` batch row b appends its first counts[b] tokens. Raises DTError where a slot has no room."""
-        if tuple(K.shape) != tuple(V.shape) or len(K.shape) != 4 or tuple(K.shape[2:]) != (self.n_heads, C.HEAD_DIM):
+        if K.shape != V.shape or len(K.shape) != 4 or tuple(K.shape[2:]) != (self.n_heads, C.HEAD_DIM):
             raise ValueError(f"K and V must share a shape [B, T, {self.n_heads}, {C.HEAD_DIM}], got {tuple(K.shape)}, "
                              f"{tuple(V.shape)}")
         if _is_torch(K) != _is_torch(V) or K.dtype != V.dtype:
@@ -151,8 +154,8 @@ class KVCache:
             C.call("dt_kv_cache_read", self._live(), K.ctypes.data, V.ctypes.data, B, T, s_p, st_p, dtype,
                    C.DT_MEM_HOST, None)
             return K, V
-        K, V = (torch.empty(shape, dtype=torch.bfloat16 if dtype == C.DT_BF16 else torch.float32,
-                            device=torch.device("cuda", self.ctx.device)) for _ in range(2))
+        K = torch.empty(shape, dtype=torch.bfloat16 if dtype == C.DT_BF16 else torch.float32, device=self._device)
+        V = torch.empty_like(K)
         C.call("dt_kv_cache_read", self._live(), K.data_ptr(), V.data_ptr(), B, T, s_p, st_p, dtype, C.DT_MEM_DEVICE,
                _stream_of(K))
         return K, V
@@ -173,7 +176,7 @@ def cached_attention(Q, cache: KVCache, scale: float, causal: bool = True, *, sl
     """
     if len(Q.shape) != 4:
         raise ValueError(f"expected [B, T, H, {C.HEAD_DIM}] queries, got {tuple(Q.shape)}")
-    B, T, H, D = (int(n) for n in Q.shape)
+    B, T, H, D = Q.shape
     dtype = _mode_of(Q, None)
     s, s_p = _per_row(slots, B, "slots")
     n, n_p = _per_row(counts, B, "counts")
@@ -185,10 +188,10 @@ def cached_attention(Q, cache: KVCache, scale: float, causal: bool = True, *, sl
         C.call("dt_cached_attn_workspace", cache._live(), B, T, H, D, s_p, n_p, pre, int(prefix_slot), dtype,
                ctypes.byref(nbytes))
         # a workspace of the call's own: torch's allocator keeps it for this stream, or for the graph being captured
-        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=Q.device) if nbytes.value else None
+        ws = Q.new_empty(nbytes.value, dtype=torch.uint8) if nbytes.value else None
         O = Q.new_empty((B, T, H, D))
         m = Q.new_empty((B, T, H), dtype=torch.float32)
-        l = Q.new_empty((B, T, H), dtype=torch.float32)
+        l = torch.empty_like(m)
         C.call("dt_cached_attn_fwd", cache._live(), Q.data_ptr(), O.data_ptr(), m.data_ptr(), l.data_ptr(), B, T, H, D,
                ldq, float(scale), int(bool(causal)), s_p, n_p, pre, int(prefix_slot),
                ws.data_ptr() if ws is not None else None, nbytes.value, dtype, C.DT_MEM_DEVICE, _stream_of(Q))

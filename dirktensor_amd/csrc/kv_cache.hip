@@ -1,12 +1,13 @@
 // The key/value cache: rows are quantised as they are written and read back as the values they stand for.
 // Layout and formats: kv_cache.h.
 //
-// Both kernels are bound by HBM: a written row costs its 512 (fp32) or 256 (bf16) bytes in and 132 (8 bits) or 260
+// Bound by HBM where there is much to move: a written row costs its 512 (fp32) or 256 (bf16) bytes in and 132 (8 bits) or 260
 // out, for K and V each. A workgroup takes the 32 keys of one block of one (batch row, head), eight threads to a key,
 // 16 values a thread: the row's largest magnitude is then three lane exchanges away, K's values leave the
 // registers as one 16-byte store a thread, and V's block, whose order in memory is the attention's, is put
-// together in LDS and written whole. A block that the call covers only in part (a decode step's one key) keeps the
-// other keys' bytes: its V values go out as single bytes from the registers.
+// together in LDS and written whole. A block that the call covers only in part keeps the other keys' bytes: its V values go
+// out as single bytes from the registers. Few tokens a sequence (a decode step's one) go another way, as a block would
+// leave most threads idle: a wave takes one row of K or of V, two values a lane (kv_append_rows_kernel).
 
 #include "kv_cache.h"
 
@@ -19,6 +20,7 @@ namespace {
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256;
 constexpr uint32_t kInfBits = 0x7f800000u;
@@ -37,18 +39,25 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-// 16 values of a row, 16-byte aligned
+// 16 values of a row, 16-byte aligned; returns their largest magnitude as bits: these order like the numbers, an infinity
+// above every number and a NaN above that
 template <bool kBf16>
-__device__ __forceinline__ void load16(const void* p, int64_t at, float (&x)[16]) {
+__device__ __forceinline__ uint32_t load16(const void* p, int64_t at, float (&x)[16]) {
+    uint32_t amax = 0;
     if constexpr (kBf16) {
         const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
+        u16x2 most = {0, 0};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const uint4 w = s[i];
             const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[8 * i + 2 * j] = bf16_lo(u[j]), x[8 * i + 2 * j + 1] = bf16_hi(u[j]);
+            for (int j = 0; j < 4; ++j) {
+                x[8 * i + 2 * j] = bf16_lo(u[j]), x[8 * i + 2 * j + 1] = bf16_hi(u[j]);
+                most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, u[j] & 0x7fff7fffu));
+            }
         }
+        amax = static_cast<uint32_t>(max(most[0], most[1])) << 16;
     } else {
         const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
 #pragma unroll
@@ -56,7 +65,10 @@ __device__ __forceinline__ void load16(const void* p, int64_t at, float (&x)[16]
             const float4 w = s[i];
             x[4 * i] = w.x, x[4 * i + 1] = w.y, x[4 * i + 2] = w.z, x[4 * i + 3] = w.w;
         }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) amax = max(amax, __float_as_uint(x[i]) & 0x7fffffffu);
     }
+    return amax;
 }
 
 template <bool kBf16>
@@ -74,24 +86,12 @@ __device__ __forceinline__ void store16(void* p, int64_t at, const float (&x)[16
     }
 }
 
-// The nearest whole number to x / s (the exact quotient, ties to even) within +-127. x * (1/s) is within a few
-// units in the last place of the quotient, so its nearest whole number is off by one at most, and only where the
-// quotient lies next to a half: there the remainder x - q s decides. It is a multiple of the smaller unit in the last
-// place of x and s (of x only where |q| <= 1) and no larger than s, so the fma gives it exactly.
-__device__ __forceinline__ float quant_int8(float x, float s, float inv) {
-    // (a quotient past 128 belongs to a scale that lost bits below 2^-126: it is clamped before the remainder is taken)
-    float q = fminf(fmaxf(rintf(x * inv), -128.0f), 128.0f);
-    const float r = __builtin_fmaf(-q, s, x);
-    const float twice = 2.0f * fabsf(r);
-    const bool odd = (static_cast<int>(q) & 1) != 0;
-    if (twice > s || (twice == s && odd)) q += copysignf(1.0f, r);
-    return fminf(fmaxf(q, -127.0f), 127.0f);
-}
-
-// A thread's 16 of a row's 128 values, quantised; amax_bits: the row's largest |x| as bits. Returns the scale.
-template <int kFormat>
-__device__ __forceinline__ float quantise(const float (&x)[16], uint32_t amax_bits, uint32_t (&out)[kFormat == DT_KV_BF16 ? 8 : 4]) {
-    constexpr int kWords = kFormat == DT_KV_BF16 ? 8 : 4;
+// kN (16, or 2 in the low bits of one word) of a row's 128 values, quantised; amax_bits: the row's largest |x| as bits. Returns
+// the scale.
+constexpr int words_of(int format, int n) { return (n * kv_elem_bytes(format) + 3) / 4; }
+template <int kFormat, int kN>
+__device__ __forceinline__ float quantise(const float (&x)[kN], uint32_t amax_bits, uint32_t (&out)[words_of(kFormat, kN)]) {
+    constexpr int kWords = words_of(kFormat, kN);
     const float amax = __uint_as_float(amax_bits);
     bool finite = amax_bits < kInfBits;
     if constexpr (kFormat == DT_KV_BF16) finite = finite && (pack_bf16x2(amax, 0.0f) & 0x7fffu) < 0x7f80u;
@@ -102,23 +102,42 @@ __device__ __forceinline__ float quantise(const float (&x)[16], uint32_t amax_bi
     }
     if constexpr (kFormat == DT_KV_BF16) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) out[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+        for (int i = 0; i < kWords; ++i) out[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
         return 1.0f;
     } else if constexpr (kFormat == DT_KV_INT8) {
         const float s = amax / 127.0f;
-        // below 2^-120 the reciprocal nears the end of the range: those rows divide
-        const float inv = s >= 0x1p-120f ? 1.0f / s : 0.0f;
+        float y[kN], ss = s;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t w = 0;
+        for (int i = 0; i < kN; ++i) y[i] = x[i];
+        if (__any(s < 0x1p-100f)) {
+            // a scale near the end of the range, whose reciprocal is none, is divided by 2^100 times larger, like the values (which
+            // pass 127 where it lost bits below 2^-126); with a scale of 0 (amax below 2^-143) all values are 0
+            const float by = s >= 0x1p-100f ? 1.0f : s > 0.0f ? 0x1p100f : 0.0f;
+            ss = s > 0.0f ? s * by : 1.0f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float q = 0.0f;
-                if (inv != 0.0f) q = quant_int8(x[4 * i + j], s, inv);
-                else if (s > 0.0f) q = fminf(fmaxf(static_cast<float>(rint(static_cast<double>(x[4 * i + j]) / static_cast<double>(s))), -127.0f), 127.0f);
-                w |= (static_cast<uint32_t>(static_cast<int>(q)) & 0xffu) << (8 * j);
-            }
-            out[i] = w;
+            for (int i = 0; i < kN; ++i) y[i] = __builtin_amdgcn_fmed3f(x[i] * by, -127.0f * ss, 127.0f * ss);
+        }
+        // The nearest whole number to the exact quotient y / s, ties to even. The sum of y * (1/s) with 1.5 2^23 rounds it; it is
+        // off by one at most, and only where the quotient lies next to a half (which values of half the largest do): the remainder
+        // y - q s decides. It is a multiple of the smaller unit in the last place of y and s (of y only where |q| <= 1) and no larger
+        // than s, so the fma gives it exactly. An odd q moves at half a step too: its bound is the number below.
+        constexpr float kMagic = 12582912.0f;
+        const float quick = __builtin_amdgcn_rcpf(ss);
+        const uint32_t half = __float_as_uint(0.5f * ss);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const float t = __builtin_fmaf(y[i], quick, kMagic);
+            const float r = __builtin_fmaf(-(t - kMagic), ss, y[i]);
+            const float bound = __uint_as_float(half - (__float_as_uint(t) & 1u));
+            y[i] = t + (fabsf(r) > bound ? copysignf(1.0f, r) : 0.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {  // (the sum's low byte is the value)
+            const auto low = [&](int j) { return __float_as_uint(y[4 * i + j]); };
+            if constexpr (kN < 4) out[i] = __builtin_amdgcn_perm(low(1), low(0), 0x0c0c0400u);
+            else
+                out[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(low(3), low(2), 0x04000c0cu),
+                                               __builtin_amdgcn_perm(low(1), low(0), 0x0c0c0400u), 0x07060100u);
         }
         return s;
     } else {
@@ -128,13 +147,14 @@ __device__ __forceinline__ float quantise(const float (&x)[16], uint32_t amax_bi
         const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
         // at the top of the range (scale 2^120) 256 would stand for an infinity: 240 is the last value
         const float lim = e >= 120 ? 240.0f : 448.0f;
-        float y[16];
+        float y[kN];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) y[i] = __builtin_amdgcn_fmed3f(x[i] * inv, -lim, lim);
+        for (int i = 0; i < kN; ++i) y[i] = __builtin_amdgcn_fmed3f(x[i] * inv, -lim, lim);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kWords; ++i) {
             int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i], y[4 * i + 1], 0, false);
-            out[i] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2], y[4 * i + 3], w, true);
+            if constexpr (kN >= 4) w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2], y[4 * i + 3], w, true);
+            out[i] = w;
         }
         return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
     }
@@ -194,16 +214,10 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvMoveArgs a, KvRow
     const bool whole = first >= start && first + kKvBlock <= start + cnt;
 
     float x[16] = {}, y[16] = {};
-    if (mine) {
-        load16<kBf16>(a.k, b * a.bsk + t * a.ldk + h * DT_HEAD_DIM + c * 16, x);
-        load16<kBf16>(a.v, b * a.bsv + t * a.ldv + h * DT_HEAD_DIM + c * 16, y);
-    }
-    // magnitudes as bits: they order like the numbers, an infinity above every number and a NaN above that
     uint32_t kmax = 0, vmax = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        kmax = max(kmax, __float_as_uint(x[i]) & 0x7fffffffu);
-        vmax = max(vmax, __float_as_uint(y[i]) & 0x7fffffffu);
+    if (mine) {
+        kmax = load16<kBf16>(a.k, b * a.bsk + t * a.ldk + h * DT_HEAD_DIM + c * 16, x);
+        vmax = load16<kBf16>(a.v, b * a.bsv + t * a.ldv + h * DT_HEAD_DIM + c * 16, y);
     }
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) {
@@ -223,13 +237,16 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvMoveArgs a, KvRow
             *scale_of<kFormat>(block, false, kk) = sk;
             *scale_of<kFormat>(block, true, kk) = sv;
         }
-        uint8_t* to = whole ? vbuf : vd;
+        const auto put = [&](auto* to, auto offset) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int o = whole ? v_lds_offset<kFormat>(c * 16 + i, kk) : v_offset<kFormat>(c * 16 + i, kk);
-            if constexpr (kEs == 2) *reinterpret_cast<uint16_t*>(to + o) = static_cast<uint16_t>(qv[i >> 1] >> (16 * (i & 1)));
-            else to[o] = static_cast<uint8_t>(qv[i >> 2] >> (8 * (i & 3)));
-        }
+            for (int i = 0; i < 16; ++i) {
+                const int o = offset(c * 16 + i, kk);
+                if constexpr (kEs == 2) *reinterpret_cast<uint16_t*>(to + o) = static_cast<uint16_t>(qv[i >> 1] >> (16 * (i & 1)));
+                else to[o] = static_cast<uint8_t>(qv[i >> 2] >> (8 * (i & 3)));
+            }
+        };
+        if (whole) put(vbuf, v_lds_offset<kFormat>);
+        else put(vd, v_offset<kFormat>);
     }
     if (whole) {  // (the same for the whole workgroup)
         __syncthreads();
@@ -237,6 +254,47 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvMoveArgs a, KvRow
         for (int i = 0; i < kEs; ++i) {
             const int o = (i * kThreads + threadIdx.x) * 16;
             *reinterpret_cast<uint4*>(vd + o) = *reinterpret_cast<const uint4*>(vbuf + (o >> 10) * kRunLds + (o & (kKvRun - 1)));
+        }
+    }
+}
+
+// Few tokens a sequence: a wave takes one row of K (even) or V (odd), lane i its values 2 i and 2 i + 1.
+template <int kFormat, bool kBf16>
+__global__ __launch_bounds__(kThreads) void kv_append_rows_kernel(KvMoveArgs a, KvRows rows) {
+    const int lane = threadIdx.x & 63, unit = blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.z, t = blockIdx.y, h = unit >> 1;
+    const bool v = unit & 1;
+    if (h >= a.c.heads || t >= rows.cnt[b]) return;
+    const int pos = rows.len[b] + t, d = 2 * lane;
+    const int64_t at = v ? b * a.bsv + t * a.ldv : b * a.bsk + t * a.ldk;
+    const void* src = v ? a.v : a.k;
+    float x[2];
+    if constexpr (kBf16) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(src) + at + h * DT_HEAD_DIM + d);
+        x[0] = bf16_lo(w), x[1] = bf16_hi(w);
+    } else {
+        const float2 w = *reinterpret_cast<const float2*>(static_cast<const float*>(src) + at + h * DT_HEAD_DIM + d);
+        x[0] = w.x, x[1] = w.y;
+    }
+    uint32_t amax = max(__float_as_uint(x[0]) & 0x7fffffffu, __float_as_uint(x[1]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), o, 64)));
+    uint32_t q[1];
+    const float s = quantise<kFormat, 2>(x, amax, q);
+    const int kk = pos & (kKvBlock - 1);
+    uint8_t* block = a.c.block<kFormat>(rows.slot[b], h, pos / kKvBlock);
+    if (lane == 0) *scale_of<kFormat>(block, v, kk) = s;
+    if (!v) {  // (two neighbours lie in one piece)
+        uint8_t* to = block + k_offset<kFormat>(d, kk);
+        if constexpr (kFormat == DT_KV_BF16) *reinterpret_cast<uint32_t*>(to) = q[0];
+        else *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(q[0]);
+    } else {
+        uint8_t* vd = block + kv_tensor_bytes(kFormat);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint8_t* to = vd + v_offset<kFormat>(d + i, kk);
+            if constexpr (kFormat == DT_KV_BF16) *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(q[0] >> (16 * i));
+            else *to = static_cast<uint8_t>(q[0] >> (8 * i));
         }
     }
 }
@@ -288,26 +346,37 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(KvMoveArgs a, KvRows 
 
 template <bool kAppend>
 int launch_move(const KvMoveArgs& a, const KvRows& rows, int B, int format, int dtype, hipStream_t s) {
-    int blocks = 0;  // of the batch row that touches most
+    int blocks = 0, tokens = 0;  // of the batch row that touches most
     for (int b = 0; b < B; ++b)
-        if (rows.cnt[b] > 0)
+        if (rows.cnt[b] > 0) {
             blocks = std::max(blocks, (rows.len[b] + rows.cnt[b] - 1) / kKvBlock - rows.len[b] / kKvBlock + 1);
+            tokens = std::max(tokens, rows.cnt[b]);
+        }
     if (blocks == 0) return DT_OK;
-    const dim3 grid(blocks, a.c.heads, B), block(kThreads);
+    // up to kFewTokens a wave a row: one token of 64 sequences (16 heads, int8) 6.3 us by blocks, 3.7 by rows, of 256 13.8 and 6.4;
+    // sixteen of eight sequences 4.5 by blocks
+    constexpr int kFewTokens = 8;
+    const bool few = kAppend && tokens <= kFewTokens;
+    const dim3 grid = few ? dim3((2 * a.c.heads + 3) / 4, tokens, B) : dim3(blocks, a.c.heads, B), block(kThreads);
     const bool bf16 = dtype == DT_BF16;
-#define DT_KV_GO(F)                                                                                              \
+#define DT_KV_GO(F, M)                                                                                            \
     do {                                                                                                         \
         if constexpr (kAppend) {                                                                                 \
-            if (bf16) hipLaunchKernelGGL((kv_append_kernel<F, true>), grid, block, 0, s, a, rows);               \
-            else hipLaunchKernelGGL((kv_append_kernel<F, false>), grid, block, 0, s, a, rows);                   \
+            if (few) hipLaunchKernelGGL((kv_append_rows_kernel<F, M>), grid, block, 0, s, a, rows);              \
+            else hipLaunchKernelGGL((kv_append_kernel<F, M>), grid, block, 0, s, a, rows);                       \
         } else {                                                                                                 \
-            if (bf16) hipLaunchKernelGGL((kv_read_kernel<F, true>), grid, block, 0, s, a, rows);                 \
-            else hipLaunchKernelGGL((kv_read_kernel<F, false>), grid, block, 0, s, a, rows);                     \
+            hipLaunchKernelGGL((kv_read_kernel<F, M>), grid, block, 0, s, a, rows);                              \
         }                                                                                                        \
     } while (0)
-    if (format == DT_KV_INT8) DT_KV_GO(DT_KV_INT8);
-    else if (format == DT_KV_FP8) DT_KV_GO(DT_KV_FP8);
-    else DT_KV_GO(DT_KV_BF16);
+#define DT_KV_GO2(F)                                                                                             \
+    do {                                                                                                         \
+        if (bf16) DT_KV_GO(F, true);                                                                             \
+        else DT_KV_GO(F, false);                                                                                 \
+    } while (0)
+    if (format == DT_KV_INT8) DT_KV_GO2(DT_KV_INT8);
+    else if (format == DT_KV_FP8) DT_KV_GO2(DT_KV_FP8);
+    else DT_KV_GO2(DT_KV_BF16);
+#undef DT_KV_GO2
 #undef DT_KV_GO
     DT_HIP_TRY(hipGetLastError());
     return DT_OK;

@@ -109,10 +109,11 @@ def token_logprobs(logits, tokens, *, top_k: int = 0, ignore_index: Optional[int
         nbytes = ctypes.c_int64()
         C.call("dt_token_logprobs_workspace", B, T, V, k, ctypes.byref(nbytes))
         # a workspace of the call's own: torch's allocator keeps it for this stream, or for the graph being captured
-        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=x.device) if nbytes.value else None
-        lp, ent, m, l = (torch.empty(lead, dtype=torch.float32, device=x.device) for _ in range(4))
-        idx = torch.empty((*lead, k), dtype=torch.int32, device=x.device) if k else None
-        top = torch.empty((*lead, k), dtype=torch.float32, device=x.device) if k else None
+        ws = x.new_empty(nbytes.value, dtype=torch.uint8) if nbytes.value else None
+        lp = x.new_empty(lead, dtype=torch.float32)
+        ent, m, l = torch.empty_like(lp), torch.empty_like(lp), torch.empty_like(lp)
+        idx = x.new_empty((*lead, k), dtype=torch.int32) if k else None
+        top = torch.empty_like(idx, dtype=torch.float32) if k else None
         C.call("dt_token_logprobs", ctx.handle, x.data_ptr(), tok_p, B, T, V, ldb, ldt, tok_bytes, ign, k, lp.data_ptr(),
                ent.data_ptr(), m.data_ptr(), l.data_ptr(), idx.data_ptr() if k else None, top.data_ptr() if k else None,
                ws.data_ptr() if ws is not None else None, nbytes.value, dtype, C.DT_MEM_DEVICE, _stream_of(x))
@@ -153,10 +154,10 @@ def token_logprobs_backward(d_logprob, logits, tokens, result: TokenLogprobs, *,
         if _is_torch(t) != _is_torch(logits) or (_is_torch(t) and t.device != logits.device):
             raise ValueError(f"{name} must be where the logits are")
     if _is_torch(logits):
-        p = {k: t.contiguous().float() for k, t in per_row.items()}
+        p = {k: t if t.dtype == torch.float32 and t.is_contiguous() else t.contiguous().float() for k, t in per_row.items()}
         x, (B, T, ldb, ldt) = _rows(logits)
         if out is None:
-            out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+            out = logits.new_empty(logits.shape)
         elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
             raise ValueError("out must have the logits' shape, dtype and device")
         elif out.stride(-1) != 1 and V != 1:
