@@ -40,6 +40,7 @@ constexpr int kList = 1024;          // values that may reach the bound before t
 constexpr uint32_t kOrderNegInf = 0x007fffffu;  // order_of(-inf): the least there is
 constexpr int kBatch = 16;           // values a thread takes at a time
 constexpr int kMinSegment = 2048;    // values of a segment at least
+constexpr int kJoinKeys = 8;         // keys of a row's segments that a thread of the second kernel takes at most
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLog2eLo = 1.92596303e-8f;  // log2 e - kLog2e
 constexpr float kLn2 = 0.693147180559945f;
@@ -135,15 +136,18 @@ __device__ __forceinline__ float take(Stats& st, const float (&v)[kN], int n) {
         st.m = bm;
     }
     const float base = st.m == kNegInf ? 0.0f : st.m;
+    float s = 0.0f, d = 0.0f;  // (the batch's own sums: fewer roundings one after another)
 #pragma unroll
     for (int i = 0; i < kN; ++i)
         if (i < n) {
             const float t = v[i] - base;
             // (log2 e in two parts: the first alone is off by 1.3e-8, the same way for every term)
             const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(t, kLog2e, t * kLog2eLo));
-            st.s += e;
-            st.d += e * fmaxf(t, -1e4f);  // (0 for -inf; a NaN shows in s)
+            s += e;
+            d += e * fmaxf(t, -1e4f);  // (0 for -inf; a NaN shows in s)
         }
+    st.s += s;
+    st.d += d;
     return bm;
 }
 
@@ -183,11 +187,23 @@ __device__ __forceinline__ Stats join_block(Stats st, float (*buf)[3]) {
     return all;
 }
 
+// The row's token: its logit, and whether it is one of the vocabulary's or skipped. (Read first, as one load waits for another.)
+struct Target {
+    float x;
+    bool skipped, known;
+};
+__device__ __forceinline__ Target target_of(const LogprobArgs& a, int64_t row, const void* xrow, bool bf16) {
+    const int64_t y = token_at(a.tok, a.tok64, row);
+    Target t{0.0f, y == a.ignore, y >= 0 && y < a.V};
+    if (t.known) t.x = bf16 ? __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(xrow)[y]) << 16) : static_cast<const float*>(xrow)[y];
+    return t;
+}
+
 struct Finish {
-    float m, l, logl, nan;
+    float m, l, logl;
 };
 // (a row of nothing but -inf has no distribution: NaN)
-__device__ __forceinline__ Finish finish(const LogprobArgs& a, int64_t row, const void* xrow, bool bf16, const Stats& st, bool write) {
+__device__ __forceinline__ Finish finish(const LogprobArgs& a, int64_t row, const Target& t, const Stats& st, bool write) {
     Finish f;
     f.m = st.m;
     f.l = st.m == kNegInf ? __builtin_nanf("") : st.s;
@@ -197,17 +213,7 @@ __device__ __forceinline__ Finish finish(const LogprobArgs& a, int64_t row, cons
     a.m[row] = f.m;
     a.l[row] = f.l;
     if (a.entropy) a.entropy[row] = f.logl - st.d / f.l;
-    const int64_t y = token_at(a.tok, a.tok64, row);
-    float lp = 0.0f;
-    if (y != a.ignore) {
-        if (y < 0 || y >= a.V) lp = __builtin_nanf("");
-        else {
-            const float x = bf16 ? __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(xrow)[y]) << 16)
-                                 : static_cast<const float*>(xrow)[y];
-            lp = (x - f.m) - f.logl;
-        }
-    }
-    a.logprob[row] = lp;
+    a.logprob[row] = t.skipped ? 0.0f : t.known ? (t.x - f.m) - f.logl : __builtin_nanf("");
     return f;
 }
 
@@ -300,6 +306,8 @@ __global__ __launch_bounds__(kThreads) void logprob_rows_kernel(LogprobArgs a) {
     const int first = seg * a.seg_len;
     const R run(xrow + static_cast<int64_t>(first) * R::kEs, min(a.V - first, a.seg_len));
 
+    Target tgt{};
+    if (a.segments == 1) tgt = target_of(a, row, xrow, kBf16);
     Stats st;
     uint32_t bound = 0;
     const int tail = run.tail() + tid;
@@ -345,9 +353,17 @@ __global__ __launch_bounds__(kThreads) void logprob_rows_kernel(LogprobArgs a) {
     const auto cached = [&](int p) { return run.load(p); };
     const auto once = [&](int p) { return run.load_once(p); };
     if constexpr (kTop) {
-        // (runs of a few batches give their bound from all of them)
+        // (runs of a few batches give their bound from all of them; the first batch stays in registers)
         const int part = run.batches <= 4 ? run.batches : (run.batches + 4) / 5;
-        stream(0, part, cached, [&](const float(&v)[kBatch], int n, int) { take(st, v, n); });
+        float v0[kBatch];
+        int n0 = 0;
+        stream(0, min(part, 1), cached, [&](const float(&v)[kBatch], int n, int) {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) v0[i] = v[i];
+            n0 = n;
+            take(st, v, n);
+        });
+        stream(1, part, cached, [&](const float(&v)[kBatch], int n, int) { take(st, v, n); });
         const bool any = tail < run.n || tid < run.pieces;
         const uint32_t mine = any ? order_of(st.m) : 0;
         bound = find_bound(buf, mine, a.k);
@@ -358,7 +374,8 @@ __global__ __launch_bounds__(kThreads) void logprob_rows_kernel(LogprobArgs a) {
         };
         if (any && mine >= bound) {
             if (tail < run.n && order_of(last[0]) >= bound) push(buf, key_of(last[0], first + tail));
-            stream(0, part, cached, look);
+            if (n0 > 0) look(v0, n0, 0);
+            stream(1, part, cached, look);
         }
         const float least = bound <= kOrderNegInf ? kNegInf : key_value(static_cast<uint64_t>(bound) << 32);
         stream(part, run.batches, once, [&](const float(&v)[kBatch], int n, int j) {
@@ -369,7 +386,7 @@ __global__ __launch_bounds__(kThreads) void logprob_rows_kernel(LogprobArgs a) {
     }
     const Stats all = join_block(st, sbuf);
     Finish f{};
-    if (a.segments == 1) f = finish(a, row, xrow, kBf16, all, tid == 0);
+    if (a.segments == 1) f = finish(a, row, tgt, all, tid == 0);
     else if (tid == 0) {
         float* p = a.part + (row * a.segments + seg) * 4;
         p[0] = all.m, p[1] = all.s, p[2] = all.d;
@@ -400,27 +417,32 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
     const int tid = threadIdx.x;
     const int64_t row = blockIdx.x;
     const uint8_t* xrow = static_cast<const uint8_t*>(a.x) + ((row / a.T) * a.ldb + (row % a.T) * a.ldt) * (kBf16 ? 2 : 4);
+    const Target tgt = target_of(a, row, xrow, kBf16);
     Stats st;
     if (tid < a.segments) {  // (at most kThreads of them)
         const float* p = a.part + (row * a.segments + tid) * 4;
         st.m = p[0], st.s = p[1], st.d = p[2];
     }
-    const Stats all = join_block(st, sbuf);
-    const Finish f = finish(a, row, xrow, kBf16, all, tid == 0);
-    if (a.k == 0) return;
     const uint64_t* keys = a.part_key + row * a.segments * a.k;
     const int n = a.segments * a.k;
-    uint64_t mine = 0;
-    for (int i = tid; i < n; i += kThreads) mine = keys[i] > mine ? keys[i] : mine;
+    uint64_t key[kJoinKeys], mine = 0;  // all under way at once
+#pragma unroll
+    for (int i = 0; i < kJoinKeys; ++i) key[i] = i * kThreads + tid < n ? keys[i * kThreads + tid] : 0;
+    const Stats all = join_block(st, sbuf);
+    const Finish f = finish(a, row, tgt, all, tid == 0);
+    if (a.k == 0) return;
+#pragma unroll
+    for (int i = 0; i < kJoinKeys; ++i) mine = key[i] > mine ? key[i] : mine;
     const uint32_t bound = find_bound(buf, static_cast<uint32_t>(mine >> 32), a.k);
     const auto each = [&](auto&& use) {
-        for (int i = tid; i < n; i += kThreads)
-            if (keys[i] != 0) use(keys[i]);
+#pragma unroll
+        for (int i = 0; i < kJoinKeys; ++i)
+            if (key[i] != 0) use(key[i]);
     };
-    each([&](uint64_t key) {
-        if (static_cast<uint32_t>(key >> 32) >= bound) push(buf, key);
+    each([&](uint64_t k) {
+        if (static_cast<uint32_t>(k >> 32) >= bound) push(buf, k);
     });
-    select(buf, a.k, each, [&](int place, uint64_t key) { write_top(a, row, place, key, f); });
+    select(buf, a.k, each, [&](int place, uint64_t k) { write_top(a, row, place, k, f); });
 }
 
 // Segments a row: enough workgroups to fill the CUs several times, none shorter than kMinSegment, their keys a few a thread.
@@ -428,7 +450,7 @@ void cut(int64_t rows, int V, int k, int* segments, int* seg_len) {
     constexpr int64_t kTarget = 2048;
     int64_t s = std::min<int64_t>((kTarget + rows - 1) / rows, (V + kMinSegment - 1) / kMinSegment);
     s = std::min<int64_t>(s, kThreads);
-    if (k > 0) s = std::min<int64_t>(s, 4096 / k);
+    if (k > 0) s = std::min<int64_t>(s, kJoinKeys * kThreads / k);
     s = std::max<int64_t>(s, 1);
     *seg_len = static_cast<int>(((V + s - 1) / s + 7) / 8 * 8);
     *segments = (V + *seg_len - 1) / *seg_len;
@@ -497,18 +519,21 @@ __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(LogprobBwdArgs a)
     else if (y >= first && y < first + n) hit = static_cast<int>(y) - first;
     const float h = a.h ? a.h[row] : 0.0f;
     const float m = a.m[row], logl = logf(a.l[row]);
-    const float ent = a.h ? a.entropy[row] : 0.0f;
-    auto grad = [&](float v, int i) {
-        const float lp = (v - m) - logl;
-        // exp(lp) with what the product with log2 e rounds away (2^-24 of it: 2e-6 of p at lp = -20) put back
-        const float t2 = lp * kLog2e;
-        const float lo = __builtin_fmaf(lp, kLog2eLo, __builtin_fmaf(lp, kLog2e, -t2));
-        const float e = __builtin_amdgcn_exp2f(t2);
-        const float p = lp < -200.0f ? 0.0f : __builtin_fmaf(e, lo * kLn2, e);  // (-inf, and where the remainder would be none)
-        float d = -p * (g + h * (lp + ent));
-        if (p == 0.0f && g == g) d = 0.0f;  // (log p may be -inf)
-        if (i == hit) d += g;
-        return d;
+    // -dx = p (g + h (log p + entropy)); a row without a distribution (its sum is NaN) is NaN throughout
+    const float lead = logl != logl ? logl : a.h ? g + h * a.entropy[row] : g;
+    // log p is cut at -1000, where p is 0 and the bracket must not be an infinity
+    auto grad = [&](float v) {
+        if constexpr (kBf16) {  // (in the log2 domain: an error of 2^-22 of log p does not count beside the result's rounding)
+            const float l2 = fmaxf(__builtin_fmaf(v - m, kLog2e, -logl * kLog2e), -1000.0f);
+            return -__builtin_amdgcn_exp2f(l2) * __builtin_fmaf(h * kLn2, l2, lead);
+        } else {
+            const float lp = fmaxf((v - m) - logl, -1000.0f);
+            // exp(lp) with what the product with log2 e rounds away (2^-24 of it: 2e-6 of p at lp = -20) put back
+            const float t2 = lp * kLog2e;
+            const float lo = __builtin_fmaf(lp, kLog2eLo, __builtin_fmaf(lp, kLog2e, -t2));
+            const float e = __builtin_amdgcn_exp2f(t2);
+            return -__builtin_fmaf(e, lo * kLn2, e) * __builtin_fmaf(h, lp, lead);
+        }
     };
     auto put = [&](int i, float d) {
         if constexpr (kBf16) reinterpret_cast<uint16_t*>(dx)[i] = static_cast<uint16_t>(__builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2){d, 0.0f}, bf16x2)));
@@ -516,16 +541,19 @@ __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(LogprobBwdArgs a)
     };
     const R run(x, n);
     const int tl = run.tail() + tid;
-    if (tl < n) put(tl, grad(run.one(tl), tl));
+    if (tl < n) put(tl, grad(run.one(tl)) + (tl == hit ? g : 0.0f));
 #pragma unroll 4
     for (int p = tid; p < run.pieces; p += kThreads) {
-        const u32x4 w = run.load(p);
-        const int at = p * R::kPiece;
+        const u32x4 w = run.load_once(p);
         float v[R::kPiece];
         R::unpack(w, v);
         u32x4 o;
 #pragma unroll
-        for (int i = 0; i < R::kPiece; ++i) v[i] = grad(v[i], at + i);
+        for (int i = 0; i < R::kPiece; ++i) v[i] = grad(v[i]);
+        if (hit >= 0 && hit / R::kPiece == p) {
+#pragma unroll
+            for (int i = 0; i < R::kPiece; ++i) v[i] += hit % R::kPiece == i ? g : 0.0f;
+        }
         if constexpr (kBf16) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2){v[2 * i], v[2 * i + 1]}, bf16x2));
