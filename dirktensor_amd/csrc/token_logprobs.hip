@@ -498,7 +498,10 @@ struct LogprobBwdArgs {
     int tok64;
     int T, V;
     int segments, seg_len;
+    int far;         // the gradient is too large to be found in a cache by whoever reads it: it is written past them
 };
+
+constexpr int kBwdPieces = 4;  // 16-byte pieces of a thread: few rows then fill the CUs too, and many leave no long tail
 
 // One workgroup a segment of a row; each value is read and written by one thread, so dx may be x.
 template <bool kBf16>
@@ -511,6 +514,12 @@ __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(LogprobBwdArgs a)
     const int64_t b = row / a.T, t = row % a.T;
     const uint8_t* x = static_cast<const uint8_t*>(a.x) + (b * a.ldb + t * a.ldt + first) * R::kEs;
     uint8_t* dx = static_cast<uint8_t*>(a.dx) + (b * a.ldb_out + t * a.ldt_out + first) * R::kEs;
+    const R run(x, n);
+    // all of a thread's values are under way before the row's own numbers, which wait for one another
+    u32x4 w[kBwdPieces];
+#pragma unroll
+    for (int i = 0; i < kBwdPieces; ++i)
+        if (tid + i * kThreads < run.pieces) w[i] = run.load_once(tid + i * kThreads);
     const int64_t y = token_at(a.tok, a.tok64, row);
     float g = a.g[row];
     int hit = -1;
@@ -539,21 +548,21 @@ __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(LogprobBwdArgs a)
         if constexpr (kBf16) reinterpret_cast<uint16_t*>(dx)[i] = static_cast<uint16_t>(__builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2){d, 0.0f}, bf16x2)));
         else reinterpret_cast<float*>(dx)[i] = d;
     };
-    const R run(x, n);
     const int tl = run.tail() + tid;
     if (tl < n) put(tl, grad(run.one(tl)) + (tl == hit ? g : 0.0f));
-#pragma unroll 4
-    for (int p = tid; p < run.pieces; p += kThreads) {
-        const u32x4 w = run.load_once(p);
+#pragma unroll
+    for (int j = 0; j < kBwdPieces; ++j) {
+        const int p = tid + j * kThreads;
+        if (p >= run.pieces) continue;
         float v[R::kPiece];
-        R::unpack(w, v);
-        u32x4 o;
+        R::unpack(w[j], v);
 #pragma unroll
         for (int i = 0; i < R::kPiece; ++i) v[i] = grad(v[i]);
         if (hit >= 0 && hit / R::kPiece == p) {
 #pragma unroll
             for (int i = 0; i < R::kPiece; ++i) v[i] += hit % R::kPiece == i ? g : 0.0f;
         }
+        u32x4 o;
         if constexpr (kBf16) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2){v[2 * i], v[2 * i + 1]}, bf16x2));
@@ -561,13 +570,17 @@ __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(LogprobBwdArgs a)
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] = __float_as_uint(v[i]);
         }
-        *reinterpret_cast<typename R::Piece*>(dx + p * 16) = o;
+        auto* to = reinterpret_cast<typename R::Piece*>(dx + p * 16);
+        if (a.far) __builtin_nontemporal_store(o, to);
+        else *to = o;
     }
 }
 
 int launch_logprobs_bwd(LogprobBwdArgs a, int64_t rows, bool bf16, hipStream_t s) {
-    // segments of 8192 values, so that few rows fill the CUs too and many leave no long tail
-    a.seg_len = 8192;
+    a.seg_len = kBwdPieces * kThreads * (bf16 ? 8 : 4);
+    // (256 MB of cache behind the L2s; 2048 rows of 100352 in fp32 308 us through them, 299 past them, 300 of 50277 in bf16 14.1
+    // and 14.9)
+    a.far = rows * a.V * (bf16 ? 2 : 4) > (256 << 20);
     a.segments = (a.V + a.seg_len - 1) / a.seg_len;
     const int64_t grid = rows * a.segments;
     if (grid > 0x7fffff) return set_error(DT_ERR_UNSUPPORTED, "%lld rows of %d logits need %lld workgroups", (long long)rows, a.V, (long long)grid);
