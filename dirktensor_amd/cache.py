@@ -44,6 +44,8 @@ def _per_row(x, B: int, name: str):
 def _rows_of(x):
     """[B, T, H, 128] as rows of one token stride: the tensor itself where its strides allow that, else a copy."""
     B, T, H, D = x.shape
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x, H * D
     if x.stride(3) == 1 and x.stride(2) == D or (H == 1 and x.stride(3) == 1):
         ld = x.stride(1) if T > 1 else (x.stride(0) if B > 1 else H * D)
         if ((B == 1 or x.stride(0) == T * ld) and ld >= H * D and ld * x.element_size() % 16 == 0

@@ -50,7 +50,7 @@ def _two_strides(shape, strides):
 
 
 def _check_tokens(tokens, lead, like):
-    if tuple(tokens.shape) != tuple(lead):
+    if tokens.shape != lead:
         raise ValueError(f"tokens have shape {tuple(tokens.shape)}, expected {tuple(lead)}")
     if _is_torch(like):
         if not _is_torch(tokens) or tokens.device != like.device:
@@ -58,7 +58,7 @@ def _check_tokens(tokens, lead, like):
         if tokens.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"unsupported token dtype {tokens.dtype}: int32 or int64")
         t = tokens.contiguous()
-        return t, t.data_ptr(), t.element_size()
+        return t, t.data_ptr(), 4 if t.dtype == torch.int32 else 8
     t = np.asarray(tokens.cpu() if _is_torch(tokens) else tokens)
     if t.dtype not in (np.int32, np.int64):
         raise TypeError(f"unsupported token dtype {t.dtype}: int32 or int64")
@@ -82,13 +82,29 @@ def _check_logits(logits, ctx):
 def _rows(logits):
     """The logits' rows as the library takes them: the tensor itself where its leading dimensions have at most two strides
     (a slice [:, :-1] is one), else a copy."""
-    V = int(logits.shape[-1])
-    if logits.stride(-1) == 1 or V == 1:
+    if logits.is_contiguous():
+        V = logits.shape[-1]
+        return logits, (1, logits.numel() // V if V else 0, 0, V)
+    if logits.stride(-1) == 1 or logits.shape[-1] == 1:
         r = _two_strides(logits.shape[:-1], logits.stride()[:-1])
         if r is not None:
             return logits, r
     logits = logits.contiguous()
     return logits, _two_strides(logits.shape[:-1], logits.stride()[:-1])
+
+
+_workspace: dict = {}  # bytes by (B, T, V, top_k): they follow from the sizes alone
+
+
+def _workspace_bytes(B: int, T: int, V: int, k: int) -> int:
+    n = _workspace.get((B, T, V, k))
+    if n is None:
+        out = ctypes.c_int64()
+        C.call("dt_token_logprobs_workspace", B, T, V, k, ctypes.byref(out))
+        if len(_workspace) >= 4096:
+            _workspace.clear()
+        n = _workspace[(B, T, V, k)] = out.value
+    return n
 
 
 def token_logprobs(logits, tokens, *, top_k: int = 0, ignore_index: Optional[int] = None,
@@ -100,23 +116,21 @@ def token_logprobs(logits, tokens, *, top_k: int = 0, ignore_index: Optional[int
     with numpy arrays and gives NaN on the device. Logits of -inf are tokens of probability 0; a row with a NaN or +inf, or with
     nothing but -inf, gives NaN. top_k: 0 to 64."""
     ctx = _check_logits(logits, ctx)
-    lead, V, k = tuple(logits.shape[:-1]), int(logits.shape[-1]), int(top_k)
+    lead, V, k = logits.shape[:-1], logits.shape[-1], int(top_k)
     dtype = _mode_of(logits, None)
     tok, tok_p, tok_bytes = _check_tokens(tokens, lead, logits)
     ign = C.DT_NO_IGNORE if ignore_index is None else int(ignore_index)
     if _is_torch(logits):
         x, (B, T, ldb, ldt) = _rows(logits)
-        nbytes = ctypes.c_int64()
-        C.call("dt_token_logprobs_workspace", B, T, V, k, ctypes.byref(nbytes))
+        nbytes = _workspace_bytes(B, T, V, k)
         # a workspace of the call's own: torch's allocator keeps it for this stream, or for the graph being captured
-        ws = x.new_empty(nbytes.value, dtype=torch.uint8) if nbytes.value else None
-        lp = x.new_empty(lead, dtype=torch.float32)
-        ent, m, l = torch.empty_like(lp), torch.empty_like(lp), torch.empty_like(lp)
+        ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        lp, ent, m, l = x.new_empty((4, *lead), dtype=torch.float32).unbind(0)
         idx = x.new_empty((*lead, k), dtype=torch.int32) if k else None
         top = torch.empty_like(idx, dtype=torch.float32) if k else None
         C.call("dt_token_logprobs", ctx.handle, x.data_ptr(), tok_p, B, T, V, ldb, ldt, tok_bytes, ign, k, lp.data_ptr(),
                ent.data_ptr(), m.data_ptr(), l.data_ptr(), idx.data_ptr() if k else None, top.data_ptr() if k else None,
-               ws.data_ptr() if ws is not None else None, nbytes.value, dtype, C.DT_MEM_DEVICE, _stream_of(x))
+               ws.data_ptr() if ws is not None else None, nbytes, dtype, C.DT_MEM_DEVICE, _stream_of(x))
         return TokenLogprobs(lp, ent, m, l, idx, top, ignore_index)
     x = np.ascontiguousarray(logits)
     rows = int(np.prod(lead, dtype=np.int64))
@@ -135,50 +149,54 @@ def _span(t):
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
+def _out_rows(out, logits, x, B, T, ldb, ldt):
+    """The rows of ``out`` beside those of x (the logits as they are read), split alike: (B, T, ldb, ldt, ldb_out, ldt_out)."""
+    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+        raise ValueError("out must have the logits' shape, dtype and device")
+    if out.stride(-1) != 1 and out.shape[-1] != 1:
+        raise ValueError("out's vocabulary dimension must be contiguous")
+    same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
+    if not same and out.numel():
+        (a0, a1), (b0, b1) = _span(out), _span(x)
+        if a0 < b1 and b0 < a1:
+            raise ValueError("out overlaps the logits without being them")
+    r = _two_strides(out.shape[:-1], out.stride()[:-1])
+    if r is not None and r[:2] == (B, T):
+        return B, T, ldb, ldt, r[2], r[3]
+    if r is not None and B == 1:  # the logits' rows have one stride: they split like out's
+        return r[0], r[1], r[1] * ldt, ldt, r[2], r[3]
+    if r is not None and r[0] == 1:
+        return B, T, ldb, ldt, T * r[3], r[3]
+    raise ValueError("out's leading dimensions must have at most two strides, split like the logits'")
+
+
 def token_logprobs_backward(d_logprob, logits, tokens, result: TokenLogprobs, *, d_entropy=None, out=None,
                             ctx: Optional[Context] = None):
     """The gradient with respect to the logits, in their dtype, of d_logprob [...] and (optionally) d_entropy [...], fp32, for
     the forward's ``result`` on the same logits and tokens. ``out`` (torch): where to write it, a tensor of the logits' shape and
     dtype, or the logits themselves to overwrite them."""
     ctx = _check_logits(logits, ctx)
-    lead, V = tuple(logits.shape[:-1]), int(logits.shape[-1])
+    lead, V = logits.shape[:-1], logits.shape[-1]
     dtype = _mode_of(logits, None)
     tok, tok_p, tok_bytes = _check_tokens(tokens, lead, logits)
     ign = C.DT_NO_IGNORE if result.ignore_index is None else int(result.ignore_index)
+    on_device = _is_torch(logits)
     per_row = dict(d_logprob=d_logprob, softmax_m=result.softmax_m, softmax_l=result.softmax_l, entropy=result.entropy)
     if d_entropy is not None:
         per_row["d_entropy"] = d_entropy
     for name, t in per_row.items():
-        if tuple(t.shape) != lead:
-            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {lead}")
-        if _is_torch(t) != _is_torch(logits) or (_is_torch(t) and t.device != logits.device):
+        if t.shape != lead:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(lead)}")
+        if _is_torch(t) != on_device or (on_device and t.device != logits.device):
             raise ValueError(f"{name} must be where the logits are")
-    if _is_torch(logits):
+    if on_device:
         p = {k: t if t.dtype == torch.float32 and t.is_contiguous() else t.contiguous().float() for k, t in per_row.items()}
         x, (B, T, ldb, ldt) = _rows(logits)
         if out is None:
-            out = logits.new_empty(logits.shape)
-        elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
-            raise ValueError("out must have the logits' shape, dtype and device")
-        elif out.stride(-1) != 1 and V != 1:
-            raise ValueError("out's vocabulary dimension must be contiguous")
-        r = _two_strides(out.shape[:-1], out.stride()[:-1])
-        same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
-        if not same and out.numel():
-            (a0, a1), (b0, b1) = _span(out), _span(x)
-            if a0 < b1 and b0 < a1:
-                raise ValueError("out overlaps the logits without being them")
-        # (both row orders must have the same two strides' extents)
-        if r is None or (r[:2] != (B, T) and not (r[0] == 1 or B == 1)):
-            raise ValueError("out's leading dimensions must have at most two strides, split like the logits'")
-        if r[:2] != (B, T):
-            if B == 1:  # the logits' rows have one stride: they split like out's
-                ldb, B, T = r[1] * ldt, r[0], r[1]
-                bo, to = r[2], r[3]
-            else:
-                bo, to = T * r[3], r[3]
+            out = x.new_empty(logits.shape)
+            bo, to = T * V, V  # (row (b, t) is row b T + t of a dense tensor)
         else:
-            bo, to = r[2], r[3]
+            B, T, ldb, ldt, bo, to = _out_rows(out, logits, x, B, T, ldb, ldt)
         C.call("dt_token_logprobs_bwd", ctx.handle, p["d_logprob"].data_ptr(),
                p["d_entropy"].data_ptr() if d_entropy is not None else None, x.data_ptr(), tok_p, p["softmax_m"].data_ptr(),
                p["softmax_l"].data_ptr(), p["entropy"].data_ptr(), B, T, V, ldb, ldt, tok_bytes, ign, out.data_ptr(), bo, to,
