@@ -122,13 +122,12 @@ struct Stats {
     float m = kNegInf, s = 0.0f, d = 0.0f;  // maximum; sum e; sum e (x - m)
 };
 
-// takes n of the values, and returns their maximum
+// takes the values, and returns their maximum (-inf in the place of a value that is none)
 template <int kN>
-__device__ __forceinline__ float take(Stats& st, const float (&v)[kN], int n) {
+__device__ __forceinline__ float take(Stats& st, const float (&v)[kN]) {
     float bm = kNegInf;
 #pragma unroll
-    for (int i = 0; i < kN; ++i)
-        if (i < n) bm = fmaxf(bm, v[i]);
+    for (int i = 0; i < kN; ++i) bm = fmaxf(bm, v[i]);
     if (bm > st.m) {
         const float f = __builtin_amdgcn_exp2f((st.m - bm) * kLog2e);
         st.d = (st.d + st.s * fmaxf(st.m - bm, -1e4f)) * f;  // (further down f is 0: the sum must not become an infinity)
@@ -138,14 +137,13 @@ __device__ __forceinline__ float take(Stats& st, const float (&v)[kN], int n) {
     const float base = st.m == kNegInf ? 0.0f : st.m;
     float s = 0.0f, d = 0.0f;  // (the batch's own sums: fewer roundings one after another)
 #pragma unroll
-    for (int i = 0; i < kN; ++i)
-        if (i < n) {
-            const float t = v[i] - base;
-            // (log2 e in two parts: the first alone is off by 1.3e-8, the same way for every term)
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(t, kLog2e, t * kLog2eLo));
-            s += e;
-            d += e * fmaxf(t, -1e4f);  // (0 for -inf; a NaN shows in s)
-        }
+    for (int i = 0; i < kN; ++i) {
+        const float t = v[i] - base;
+        // (log2 e in two parts: the first alone is off by 1.3e-8, the same way for every term)
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(t, kLog2e, t * kLog2eLo));
+        s += e;
+        d += e * fmaxf(t, -1e4f);  // (0 for -inf; a NaN shows in s)
+    }
     st.s += s;
     st.d += d;
     return bm;
@@ -314,9 +312,9 @@ __global__ __launch_bounds__(kThreads) void logprob_rows_kernel(LogprobArgs a) {
     float last[1] = {kNegInf};
     if (tail < run.n) {
         last[0] = run.one(tail);
-        take(st, last, 1);
+        take(st, last);
     }
-    // f(batch's values, how many) for batches from .. to - 1, the next one's loads in flight while one is taken
+    // f(batch's values, its number) for batches from .. to - 1, the next one's loads in flight while one is taken
     auto stream = [&](int from, int to, auto load, auto f) {
         const int whole = min(to, run.pieces / (kThreads * R::kPer));
         u32x4 w[R::kPer];
@@ -333,56 +331,59 @@ __global__ __launch_bounds__(kThreads) void logprob_rows_kernel(LogprobArgs a) {
 #pragma unroll
                 for (int i = 0; i < R::kPer; ++i) w[i] = load(((j + 1) * R::kPer + i) * kThreads + tid);
             }
-            f(v, kBatch, j);
+            f(v, j);
         }
-        for (; j < to; ++j) {  // (the run's last batch at most)
+        if (j < to) {  // the run's last batch: -inf where there is no piece
             float v[kBatch];
-            int n = 0;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) v[i] = kNegInf;
 #pragma unroll
             for (int i = 0; i < R::kPer; ++i) {
                 const int p = (j * R::kPer + i) * kThreads + tid;
-                if (p < run.pieces) {
-                    R::unpack(load(p), v + i * R::kPiece);
-                    n = (i + 1) * R::kPiece;
-                }
+                if (p < run.pieces) R::unpack(load(p), v + i * R::kPiece);
             }
-            if (n > 0) f(v, n, j);
+            f(v, j);
         }
     };
-    auto index_of = [&](int j, int i) { return first + ((j * R::kPer + i / R::kPiece) * kThreads + tid) * R::kPiece + i % R::kPiece; };
+    // use(key) for those of a batch's values that are not below `least`. Few are: they are found in the registers and read again
+    // one by one.
+    const auto look = [&](const float(&v)[kBatch], int j, float least, auto&& use) {
+        uint32_t hits = 0;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) hits |= v[i] < least ? 0u : 1u << i;
+        while (hits) {
+            const int i = __ffs(hits) - 1, p = (j * R::kPer + i / R::kPiece) * kThreads + tid, at = p * R::kPiece + i % R::kPiece;
+            hits &= hits - 1;
+            if (p < run.pieces) use(key_of(run.one(at), first + at));
+        }
+    };
     const auto cached = [&](int p) { return run.load(p); };
     const auto once = [&](int p) { return run.load_once(p); };
     if constexpr (kTop) {
         // (runs of a few batches give their bound from all of them; the first batch stays in registers)
         const int part = run.batches <= 4 ? run.batches : (run.batches + 4) / 5;
         float v0[kBatch];
-        int n0 = 0;
-        stream(0, min(part, 1), cached, [&](const float(&v)[kBatch], int n, int) {
+        stream(0, min(part, 1), cached, [&](const float(&v)[kBatch], int) {
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) v0[i] = v[i];
-            n0 = n;
-            take(st, v, n);
+            take(st, v);
         });
-        stream(1, part, cached, [&](const float(&v)[kBatch], int n, int) { take(st, v, n); });
+        stream(1, part, cached, [&](const float(&v)[kBatch], int) { take(st, v); });
         const bool any = tail < run.n || tid < run.pieces;
         const uint32_t mine = any ? order_of(st.m) : 0;
         bound = find_bound(buf, mine, a.k);
-        const auto look = [&](const float(&v)[kBatch], int n, int j) {
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i)
-                if (i < n && order_of(v[i]) >= bound) push(buf, key_of(v[i], index_of(j, i)));
-        };
-        if (any && mine >= bound) {
-            if (tail < run.n && order_of(last[0]) >= bound) push(buf, key_of(last[0], first + tail));
-            if (n0 > 0) look(v0, n0, 0);
-            stream(1, part, cached, look);
-        }
+        const auto list = [&](uint64_t key) { push(buf, key); };
         const float least = bound <= kOrderNegInf ? kNegInf : key_value(static_cast<uint64_t>(bound) << 32);
-        stream(part, run.batches, once, [&](const float(&v)[kBatch], int n, int j) {
-            if (take(st, v, n) >= least) look(v, n, j);
+        if (any && mine >= bound) {
+            if (tail < run.n && !(last[0] < least)) push(buf, key_of(last[0], first + tail));
+            if (part > 0) look(v0, 0, least, list);
+            stream(1, part, cached, [&](const float(&v)[kBatch], int j) { look(v, j, least, list); });
+        }
+        stream(part, run.batches, once, [&](const float(&v)[kBatch], int j) {
+            if (take(st, v) >= least) look(v, j, least, list);
         });
     } else {
-        stream(0, run.batches, once, [&](const float(&v)[kBatch], int n, int) { take(st, v, n); });
+        stream(0, run.batches, once, [&](const float(&v)[kBatch], int) { take(st, v); });
     }
     const Stats all = join_block(st, sbuf);
     Finish f{};
@@ -396,11 +397,7 @@ __global__ __launch_bounds__(kThreads) void logprob_rows_kernel(LogprobArgs a) {
             buf, a.k,
             [&](auto&& use) {
                 if (tail < run.n) use(key_of(last[0], first + tail));
-                stream(0, run.batches, cached, [&](const float(&v)[kBatch], int n, int j) {
-#pragma unroll
-                    for (int i = 0; i < kBatch; ++i)
-                        if (i < n) use(key_of(v[i], index_of(j, i)));
-                });
+                stream(0, run.batches, cached, [&](const float(&v)[kBatch], int j) { look(v, j, kNegInf, use); });
             },
             [&](int place, uint64_t key) {
                 if (a.segments == 1) write_top(a, row, place, key, f);
