@@ -43,10 +43,11 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kWaves = 4;       // of a workgroup
+constexpr int kWavesFew = 8;    // where there are no more triples than CUs, and few keys each
 constexpr int kJoinThreads = 256;
-constexpr int kKeysLog = 7;  // log2 of kKvBlock * kWaves
-static_assert(1 << kKeysLog == kKvBlock * kWaves, "a step's keys");
+constexpr int keys_log(int waves) { return waves == 4 ? 7 : 8; }  // log2 of the keys of a step: a block a wave
+static_assert(1 << keys_log(kWaves) == kKvBlock * kWaves && 1 << keys_log(kWavesFew) == kKvBlock * kWavesFew, "a step's keys");
 constexpr int kD = DT_HEAD_DIM;
 constexpr int kObufRow = kD + 4;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -83,6 +84,7 @@ struct CachedAttnArgs {
     // own keys, in steps of 32 keys a key wave; own_wl: log2 of the waves that take query tiles
     int own_wl, own_tiles;
     int own_groups;     // workgroups
+    int waves;          // of a workgroup
     int aligned;        // one (head, batch row, tile) each; otherwise shares of the list:
     int lead;           // places that a triple has in the list before those of its steps, for what beginning it costs
     int head_places;    // of one head: all batch rows and tiles
@@ -93,9 +95,9 @@ struct CachedAttnArgs {
 };
 
 // steps of a batch row's keys for a query tile (0: there is nothing to see)
-__host__ __device__ __forceinline__ int steps_of(int len, int cnt, int wl) {
-    const int keys = (kKvBlock * kWaves) >> wl;
-    return cnt == 0 ? 0 : (len + keys - 1) >> (kKeysLog - wl);
+__host__ __device__ __forceinline__ int steps_of(int len, int cnt, int waves, int wl) {
+    const int log = keys_log(waves) - wl;
+    return cnt == 0 ? 0 : (len + (1 << log) - 1) >> log;
 }
 // The list's places in equal shares: the first `extra` workgroups have one more than `share`. group_of: whose share place s is in.
 __host__ __device__ __forceinline__ int share_start(const CachedAttnArgs& a, int w) {
@@ -225,14 +227,15 @@ __device__ __forceinline__ int thread_here() {
     return t;
 }
 
+template <int kW>
 struct Shared {
-    float o[kWaves][16][kObufRow];
-    float ml[kWaves][3][16];  // base, sum, true maximum
+    float o[kW][16][kObufRow];
+    float ml[kW][3][16];  // base, sum, true maximum
 };
 
 // A wave's part of a stretch of work: begin puts the loads of its first blocks and of its Q rows under way, attend does the work
 // and leaves the results in LDS, join (of the whole workgroup) puts the waves' results together.
-template <int kFormat, bool kF32, bool kOnce>
+template <int kFormat, bool kF32, bool kOnce, int kW>
 struct Stretch {
     static constexpr int kQS = kF32 ? 3 : 1, kStages = stages(kFormat, kF32);
     Block<kFormat, kOnce> st[kStages];
@@ -261,7 +264,7 @@ struct Stretch {
         wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int n = lane & 15, g = lane >> 4;
         const int qw = wave & ((1 << w.wl) - 1), kw = wave >> w.wl;
-        step = (kKvBlock * kWaves) >> w.wl;
+        step = (kKvBlock * kW) >> w.wl;
         k1 = w.k1;
         const KvView& c = w.prefix ? a.pre : a.own;
         rsrc = __builtin_amdgcn_make_buffer_rsrc(c.block<kFormat>(w.slot, w.hk, 0), 0, c.blocks * kv_block_bytes(kFormat), kBufferDword3);
@@ -329,7 +332,7 @@ struct Stretch {
         }
     }
 
-    __device__ __forceinline__ void attend(float scale, Shared& sh) {
+    __device__ __forceinline__ void attend(float scale, Shared<kW>& sh) {
         const int n = lane & 15, g = lane >> 4;
         bf16x8 qf[kQS][4];
         const float qscale = operand_q(scale * kLog2e, qf);  // (scores in the log2 domain)
@@ -441,10 +444,10 @@ struct Stretch {
 };
 
 // The waves' results meet: a thread sums four values of a row over the key waves, scaled to their common maximum.
-template <bool kF32>
-__device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRows& rows, const Work& w, const Shared& sh) {
-    const int wk = kWaves >> w.wl, row0 = w.tile * 16 << w.wl, nrows = (w.prefix ? a.B : 1) * a.T * a.G;
-    for (int it = thread_here(); it < (16 * (kD / 4)) << w.wl; it += kThreads) {
+template <bool kF32, int kW>
+__device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRows& rows, const Work& w, const Shared<kW>& sh) {
+    const int wk = kW >> w.wl, row0 = w.tile * 16 << w.wl, nrows = (w.prefix ? a.B : 1) * a.T * a.G;
+    for (int it = thread_here(); it < (16 * (kD / 4)) << w.wl; it += 64 * kW) {
         const int d = (it & 31) * 4, rt = it >> 5;  // (row within the workgroup's tiles)
         const int tq = rt >> 4, rn = rt & 15;
         if (row0 + rt >= nrows) continue;
@@ -480,35 +483,37 @@ __device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRo
     }
 }
 
-template <int kFormat, bool kF32, bool kOnce>
-__global__ __launch_bounds__(kThreads, 2) void cached_attn_kernel(CachedAttnArgs a, AttnRows rows) {
-    __shared__ __align__(16) Shared sh;
+template <int kFormat, bool kF32, bool kOnce, int kW>
+__global__ __launch_bounds__(64 * kW, 2) void cached_attn_kernel(CachedAttnArgs a, AttnRows rows) {
+    __shared__ __align__(16) Shared<kW> sh;
     __shared__ AttnRows rl;
     // All arguments in one trip to their memory, in place of one for each dependent use: the batch rows into LDS (all of
     // them, so no length is waited for), the rest into scalar registers or at least the scalar cache.
-    static_assert(kThreads == kMaxRaggedBatch, "one batch row a thread");
-    rl.len[threadIdx.x] = rows.len[threadIdx.x];
-    rl.cum[threadIdx.x] = rows.cum[threadIdx.x];
-    rl.slot[threadIdx.x] = rows.slot[threadIdx.x];
-    rl.cnt[threadIdx.x] = rows.cnt[threadIdx.x];
+    static_assert(64 * kW >= kMaxRaggedBatch, "one batch row a thread");
+    if (threadIdx.x < kMaxRaggedBatch) {
+        rl.len[threadIdx.x] = rows.len[threadIdx.x];
+        rl.cum[threadIdx.x] = rows.cum[threadIdx.x];
+        rl.slot[threadIdx.x] = rows.slot[threadIdx.x];
+        rl.cnt[threadIdx.x] = rows.cnt[threadIdx.x];
+    }
     asm volatile("" ::"s"(a.own.data), "s"(a.q), "s"(a.part_o), "s"(a.T), "s"(a.parts), "s"(a.share), "s"(a.pre_groups));
     __syncthreads();
     int id = blockIdx.x;
     Work w;
     w.prefix = id < a.pre_groups;
     w.wl = w.prefix ? a.pre_wl : a.own_wl;
-    const int keys_log = kKeysLog - w.wl;
+    const int step_log = keys_log(kW) - w.wl;
     int s = 0, end = 0, steps = 0, off = 0, count = 0;
     // the batch row's entries
     const auto load_row = [&]() {
         w.len = __builtin_amdgcn_readfirstlane(rl.len[w.b]);
         w.cnt = __builtin_amdgcn_readfirstlane(rl.cnt[w.b]);
         w.slot = __builtin_amdgcn_readfirstlane(rl.slot[w.b]);
-        steps = steps_of(w.len, w.cnt, w.wl);
+        steps = steps_of(w.len, w.cnt, kW, w.wl);
     };
     const auto set_keys = [&]() {
-        w.k0 = off << keys_log;
-        w.k1 = min(w.len, (off + count) << keys_log);
+        w.k0 = off << step_log;
+        w.k1 = min(w.len, (off + count) << step_log);
         if (a.causal && a.T > 1) {  // nothing past the tile's newest query
             const int r = ((w.tile + 1) * 16 << w.wl) - 1, t = min(a.T - 1, a.G == 1 ? r : r / a.G);
             w.k1 = min(w.k1, max(0, w.len - w.cnt + t + 1));
@@ -599,7 +604,7 @@ __global__ __launch_bounds__(kThreads, 2) void cached_attn_kernel(CachedAttnArgs
         s += count;
         set_keys();
     };
-    Stretch<kFormat, kF32, kOnce> st;
+    Stretch<kFormat, kF32, kOnce, kW> st;
     st.begin(a, w);
     for (;;) {
         st.attend(a.scale, sh);
@@ -610,7 +615,7 @@ __global__ __launch_bounds__(kThreads, 2) void cached_attn_kernel(CachedAttnArgs
             st.begin(a, w);
         }
         __syncthreads();
-        join_waves<kF32>(a, rl, done, sh);
+        join_waves<kF32, kW>(a, rl, done, sh);
         if (!more) return;
         __syncthreads();
     }
@@ -635,7 +640,7 @@ __global__ __launch_bounds__(kJoinThreads) void cached_attn_join_kernel(CachedAt
     const int b = bt / a.T, t = bt % a.T;
     int parts = 0;
     if (t < rows.cnt[b]) {
-        const int steps = steps_of(rows.len[b], rows.cnt[b], a.own_wl);
+        const int steps = steps_of(rows.len[b], rows.cnt[b], kWaves, a.own_wl);
         int own = steps > 0;
         if (own && !a.aligned) {
             const int first = hq / a.G * a.head_places + rows.cum[b] + ((t * a.G + hq % a.G) >> (4 + a.own_wl)) * (steps + a.lead) + a.lead;
@@ -687,7 +692,7 @@ __global__ __launch_bounds__(kJoinThreads) void cached_attn_join_kernel(CachedAt
 
 constexpr int kCus = 256;
 constexpr int kLead = 2;           // steps that beginning and ending a triple costs
-constexpr int kWholeSteps = 4;     // up to so many steps (of 256 keys for one query tile) a triple's keys are not cut
+constexpr int kWholeSteps = 4;     // up to so many steps a triple's keys are not cut
 
 // log2 of the waves that take query tiles: as many as there are tiles of 16 rows
 int query_waves_log(int64_t rows) { return rows <= 16 ? 0 : rows <= 32 ? 1 : 2; }
@@ -695,6 +700,7 @@ int query_waves_log(int64_t rows) { return rows <= 16 ? 0 : rows <= 32 ? 1 : 2; 
 // How a call is cut; fills rows' cum and the arguments that follow from the sizes. Returns the workspace's bytes.
 int64_t make_plan(CachedAttnArgs& a, AttnRows& rows, bool* join) {
     constexpr int kResident = 2 * kCus;
+    a.waves = kWaves;
     const int heads = a.own.heads;
     const int64_t own_rows = static_cast<int64_t>(a.T) * a.G, all_rows = own_rows * a.B;
     a.own_wl = query_waves_log(own_rows);
@@ -702,7 +708,7 @@ int64_t make_plan(CachedAttnArgs& a, AttnRows& rows, bool* join) {
     int longest = 0, shortest = kMaxCacheTokens;
     int64_t steps = 0, rows_held = 0;
     for (int b = 0; b < a.B; ++b) {
-        const int n = steps_of(rows.len[b], rows.cnt[b], a.own_wl);
+        const int n = steps_of(rows.len[b], rows.cnt[b], a.waves, a.own_wl);
         steps += n;
         rows_held += n > 0;
         longest = std::max(longest, n);
@@ -731,6 +737,14 @@ int64_t make_plan(CachedAttnArgs& a, AttnRows& rows, bool* join) {
     const int64_t slots = std::max<int64_t>(kResident - a.pre_groups, kResident / 4);
     // (an empty list has no shares; one past 2^28 steps, thousands of query tiles over the longest cache, has triples enough)
     a.aligned = all == 0 || all > (1 << 28) || (longest <= kWholeSteps && (a.pre_groups == 0 || triples <= slots));
+    // Few triples of up to twice as many keys: eight waves each, and one launch in place of two (16 heads, one sequence of 1024 in
+    // int8: 6.3 and 4.3 us with a join, 10.7 so, and a launch's 3 us less on the host; sixteen 13.8 and 4.0, 13.7 so; up to four
+    // steps four waves do, 512 keys 7.8 us by four, 8.5 by eight).
+    if (a.pre_groups == 0 && a.own_wl == 0 && triples <= kCus && longest > kWholeSteps && longest <= 2 * kWholeSteps) {
+        static_assert(kWavesFew == 2 * kWaves, "steps twice as long");
+        a.waves = kWavesFew;
+        a.aligned = 1;
+    }
     int own_parts = 1;
     bool whole = true;  // every triple's keys in one workgroup
     a.own_groups = static_cast<int>(triples);
@@ -740,7 +754,7 @@ int64_t make_plan(CachedAttnArgs& a, AttnRows& rows, bool* join) {
         int64_t cum = 0;
         for (int b = 0; b < a.B; ++b) {
             rows.cum[b] = static_cast<int>(cum);
-            const int n = steps_of(rows.len[b], rows.cnt[b], a.own_wl);
+            const int n = steps_of(rows.len[b], rows.cnt[b], a.waves, a.own_wl);
             if (n > 0) cum += static_cast<int64_t>(n + a.lead) * a.own_tiles;
         }
         a.head_places = static_cast<int>(cum);
@@ -762,18 +776,21 @@ int launch(const CachedAttnArgs& a, const AttnRows& rows, bool join, int format,
     const bool f32 = dtype != DT_BF16;
     const bool once = a.own_wl == 0 && a.own_tiles == 1;
     if (groups > 0) {
-        const dim3 g(static_cast<unsigned>(groups)), t(kThreads);
-#define DT_GO(F)                                                                                        \
-    do {                                                                                                \
-        if (f32 && once) hipLaunchKernelGGL((cached_attn_kernel<F, true, true>), g, t, 0, s, a, rows);  \
-        else if (f32) hipLaunchKernelGGL((cached_attn_kernel<F, true, false>), g, t, 0, s, a, rows);    \
-        else if (once) hipLaunchKernelGGL((cached_attn_kernel<F, false, true>), g, t, 0, s, a, rows);   \
-        else hipLaunchKernelGGL((cached_attn_kernel<F, false, false>), g, t, 0, s, a, rows);            \
-    } while (0)
-        if (format == DT_KV_INT8) DT_GO(DT_KV_INT8);
-        else if (format == DT_KV_FP8) DT_GO(DT_KV_FP8);
-        else DT_GO(DT_KV_BF16);
-#undef DT_GO
+        const dim3 g(static_cast<unsigned>(groups)), t(64 * a.waves);
+        const auto go = [&](auto format_, auto f32_) {
+            constexpr int F = decltype(format_)::value;
+            constexpr bool M = decltype(f32_)::value;
+            if (a.waves == kWavesFew) hipLaunchKernelGGL((cached_attn_kernel<F, M, true, kWavesFew>), g, t, 0, s, a, rows);
+            else if (once) hipLaunchKernelGGL((cached_attn_kernel<F, M, true, kWaves>), g, t, 0, s, a, rows);
+            else hipLaunchKernelGGL((cached_attn_kernel<F, M, false, kWaves>), g, t, 0, s, a, rows);
+        };
+        const auto go_mode = [&](auto format_) {
+            if (f32) go(format_, std::true_type());
+            else go(format_, std::false_type());
+        };
+        if (format == DT_KV_INT8) go_mode(std::integral_constant<int, DT_KV_INT8>());
+        else if (format == DT_KV_FP8) go_mode(std::integral_constant<int, DT_KV_FP8>());
+        else go_mode(std::integral_constant<int, DT_KV_BF16>());
         DT_HIP_TRY(hipGetLastError());
     }
     if (!join) return DT_OK;
