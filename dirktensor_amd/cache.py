@@ -93,6 +93,8 @@ class KVCache:
     def _live(self):
         if not self.handle:
             raise RuntimeError("the cache is closed")
+        if not self.ctx.handle:
+            raise RuntimeError("the cache's context is closed")
         return self.handle
 
     @property

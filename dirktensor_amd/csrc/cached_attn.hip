@@ -735,8 +735,10 @@ int64_t make_plan(CachedAttnArgs& a, AttnRows& rows, bool* join) {
     }
 
     const int64_t slots = std::max<int64_t>(kResident - a.pre_groups, kResident / 4);
-    // (an empty list has no shares; one past 2^28 steps, thousands of query tiles over the longest cache, has triples enough)
-    a.aligned = all == 0 || all > (1 << 28) || (longest <= kWholeSteps && (a.pre_groups == 0 || triples <= slots));
+    // Triples are not cut where they are short, or so many that the longest does not show in the end: these need no workspace of
+    // their own. (An empty list has no shares; one past 2^28 steps has triples enough.)
+    a.aligned = all == 0 || all > (1 << 28) || (longest <= kWholeSteps && (a.pre_groups == 0 || triples <= slots)) ||
+                4 * static_cast<int64_t>(longest) * slots <= all;
     // Few triples of up to twice as many keys: eight waves each, and one launch in place of two (16 heads, one sequence of 1024 in
     // int8: 6.3 and 4.3 us with a join, 10.7 so, and a launch's 3 us less on the host; sixteen 13.8 and 4.0, 13.7 so; up to four
     // steps four waves do, 512 keys 7.8 us by four, 8.5 by eight).

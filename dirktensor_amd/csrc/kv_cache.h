@@ -78,7 +78,7 @@ struct KvView {
 
 struct dt_kv_cache {
     dt_ctx* ctx = nullptr;
-    int slots = 0, capacity = 0, heads = 0, format = 0;
+    int device = 0, slots = 0, capacity = 0, heads = 0, format = 0;
     int blocks = 0;  // of 32 tokens per (slot, head)
     void* data = nullptr;
     std::vector<int32_t> len;  // tokens held by each slot

@@ -446,6 +446,7 @@ int dt_kv_cache_create(dt_ctx* ctx, int slots, int capacity, int n_heads, int D,
     dt_kv_cache* c = new (std::nothrow) dt_kv_cache;
     if (!c) return set_error(DT_ERR_INVALID_ARG, "out of host memory");
     c->ctx = ctx;
+    c->device = ctx->device;
     c->slots = slots;
     c->capacity = capacity;
     c->heads = n_heads;
@@ -475,7 +476,7 @@ int dt_kv_cache_create(dt_ctx* ctx, int slots, int capacity, int n_heads, int D,
 int dt_kv_cache_destroy(dt_kv_cache* cache) {
     clear_error();
     if (!cache) return DT_OK;
-    DT_TRY(check_device_binding(cache->ctx));
+    DT_HIP_TRY(hipSetDevice(cache->device));
     free_cache(cache);  // (hipFree waits for the device)
     return DT_OK;
 }

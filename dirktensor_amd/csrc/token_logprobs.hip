@@ -598,6 +598,8 @@ int check_logits(int B, int T, int V, int64_t ldb, int64_t ldt, int token_bytes,
     return DT_OK;
 }
 
+bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
 int check_host_tokens(const void* tok, int token_bytes, int64_t rows, int V, int64_t ignore) {
     for (int64_t i = 0; i < rows; ++i) {
         const int64_t y = token_bytes == 8 ? static_cast<const int64_t*>(tok)[i] : static_cast<const int32_t*>(tok)[i];
@@ -652,7 +654,8 @@ int dt_token_logprobs(dt_ctx* ctx, const void* logits, const void* tokens, int B
     const int64_t need = workspace_bytes(rows, V, top_k);
     const size_t es = dtype == DT_BF16 ? 2 : 4;
     if (mem == DT_MEM_DEVICE) {
-        if (reinterpret_cast<uintptr_t>(logits) % es) return set_error(DT_ERR_INVALID_ARG, "logits are not aligned to their type");
+        if (!aligned_to(logits, es) || !aligned_to(tokens, token_bytes))
+            return set_error(DT_ERR_INVALID_ARG, "logits or tokens are not aligned to their type");
         if (!aligned16(ws)) return set_error(DT_ERR_INVALID_ARG, "the workspace must be 16-byte aligned");
         if (need > 0 && (!ws || ws_bytes < need))
             return set_error(DT_ERR_INVALID_ARG, "the workspace has %lld bytes, the call needs %lld", (long long)(ws ? ws_bytes : 0), (long long)need);
@@ -725,8 +728,8 @@ int dt_token_logprobs_bwd(dt_ctx* ctx, const float* d_logprob, const float* d_en
     const int64_t rows = static_cast<int64_t>(B) * T;
     const size_t es = dtype == DT_BF16 ? 2 : 4;
     if (mem == DT_MEM_DEVICE) {
-        if (reinterpret_cast<uintptr_t>(logits) % es || reinterpret_cast<uintptr_t>(d_logits) % es)
-            return set_error(DT_ERR_INVALID_ARG, "logits or d_logits are not aligned to their type");
+        if (!aligned_to(logits, es) || !aligned_to(d_logits, es) || !aligned_to(tokens, token_bytes))
+            return set_error(DT_ERR_INVALID_ARG, "logits, d_logits or tokens are not aligned to their type");
     } else {
         DT_TRY(check_host_tokens(tokens, token_bytes, rows, V, ignore_index));
     }

@@ -378,6 +378,54 @@ def test_long_cache_past_32_bits():
     assert float((r.output.float() - w.output.float()).abs().max()) <= 2 * 2.0 ** -8 * float(w.output.float().abs().max())
 
 
+def test_many_query_tiles():
+    """More (head, sequence, query tile) triples than are cut: a prompt in chunks over a cache, padded, with and without a
+    prefix; compared with one token at a time at sampled places (the reference's loop would take minutes)."""
+    from dirktensor_amd import KVCache, cached_attention
+
+    B, T, H, Hk = 4, 700, 8, 4
+    c, p = KVCache(B, 900, Hk, format="fp8"), KVCache(1, 200, Hk, format="fp8")
+    fill(c, [900, 700, 350, 701], 800)
+    fill(p, [200], 790)
+    q = randn((B, T, H, D), 801, torch.bfloat16)
+    counts = [700, 700, 500, 1]
+    for pre in (None, p):
+        r = cached_attention(q, c, SCALE, counts=counts, prefix=pre)
+        held_at = c.lengths.copy()
+        for b in range(B):
+            for t in (0, 1, 333, 499, 500, 699):
+                if t >= counts[b]:
+                    assert not bool(r.output[b, t].any()) and bool((r.softmax_l[b, t] == 0).all())
+                    continue
+                seen = max(0, int(held_at[b]) - counts[b] + t + 1)
+                if seen == 0 and pre is None:
+                    assert not bool(r.output[b, t].any())
+                    continue
+                one = KVCache(1, 900, Hk, format="fp8")
+                if seen:
+                    k, v = c.read([0], seen, slots=[b], mode="fp32")  # (held values are held again as they are)
+                    one.append(k, v)
+                w = cached_attention(q[b:b + 1, t:t + 1], one, SCALE, prefix=pre)
+                # the same terms in another order, each rounded to bf16 (2^-8 of a term, values of unit size) and the result once
+                assert float((w.output[0, 0].float() - r.output[b, t].float()).abs().max()) <= 0.03
+                assert float((w.softmax_m[0, 0] - r.softmax_m[b, t]).abs().max()) <= 1e-5
+
+
+def test_a_closed_context():
+    from dirktensor_amd import Context, KVCache, cached_attention
+
+    ctx = Context(0)
+    c = KVCache(1, 40, 2, ctx=ctx)
+    x = randn((1, 4, 2, D), 1)
+    c.append(x, x)
+    ctx.close()
+    with pytest.raises(RuntimeError, match="context"):
+        cached_attention(x, c, SCALE)
+    with pytest.raises(RuntimeError, match="context"):
+        c.append(x, x)
+    c.close()
+
+
 def test_refusals():
     from dirktensor_amd import DTError, KVCache, cached_attention
 

@@ -108,6 +108,7 @@ def test_cached_attn_workspace():
     (dict(top_k=3, top_index=None), C.DT_ERR_INVALID_ARG, "top_index"),
     (dict(logits=FAKE + 2), C.DT_ERR_INVALID_ARG, "aligned"),
     (dict(ws=FAKE + 8), C.DT_ERR_INVALID_ARG, "aligned"),
+    (dict(tokens=FAKE + 4, token_bytes=8), C.DT_ERR_INVALID_ARG, "tokens are not aligned"),
     (dict(V=100352, ws=None), C.DT_ERR_INVALID_ARG, "the workspace has 0"),
     (dict(dtype=9), C.DT_ERR_INVALID_ARG, "dtype"),
     (dict(mem=9), C.DT_ERR_INVALID_ARG, "mem"),
@@ -167,3 +168,18 @@ def test_leading_dimensions_as_two_strides():
     assert _two_strides((2, 3, 5), (126, 42, 7)) == (6, 5, 42, 7)
     assert _two_strides((2, 3, 5), (200, 42, 7)) is None
     assert _two_strides((4, 5), (0, 7)) == (4, 5, 0, 7)
+
+
+def test_kernels_use_no_scratch_memory():
+    """Scratch memory would be allocated at a kernel's first launch, at the latest: a captured call cannot have that."""
+    from test_kernel_scratch_cpu import _code_objects, _kernels
+
+    import dirktensor_amd as dt
+
+    if not dt.LIB_PATH.exists():
+        pytest.skip("the library is not built")
+    sizes = {k[".name"]: (k[".private_segment_fixed_size"], bool(k.get(".uses_dynamic_stack")))
+             for elf in _code_objects(dt.LIB_PATH.read_bytes()) for k in _kernels(elf)}
+    mine = {n: s for n, s in sizes.items() if any(x in n for x in ("cached_attn", "kv_append", "kv_read", "logprob"))}
+    assert len(mine) >= 40, sorted(mine)
+    assert {n: s for n, s in mine.items() if s != (0, False)} == {}
