@@ -10,21 +10,27 @@
 // Work decomposition
 //   * Query rows that share a key/value head's keys go together, 16 to a matrix tile: the tokens and the query heads of
 //     its group for a batch row's own keys; for a shared prefix those of the whole batch, so that the prefix is read
-//     once for all of them.
-//   * A workgroup has eight waves: kWq of them (1, 2, 4 or 8, as many as there are tiles) take a tile of 16 query rows each and
-//     the rest is spread over the keys, 32 at a time. Every wave keeps its own running maximum, sum and O; those of one
+//     once for all of them. Where there are more than 16, a wave takes two tiles and widens each held value once for
+//     both (64 queries over a prefix in int8: 377 and 530 TFLOP/s; 256: 324 and 761, in fp8 390 and 1023).
+//   * A workgroup has four waves: as many of them as there are tiles (one or two, up to four in exact mode) take query rows
+//     and the rest is spread over the keys, 32 at a time. Every wave keeps its own running maximum, sum and O; those of one
 //     tile meet in LDS once at the end. No wave waits for another in the loop, and no key passes through LDS: the cache lies
 //     in memory in the order in which the matrix instructions read it (kv_cache.h).
 //   * The keys of all (head, batch row, query tile) triples form one list, cut into as many equal shares as workgroups fit the
 //     CUs (two each), so ragged lengths leave no CU idle; a share may end within a triple and go on in the next. Short
-//     lists are not cut within a triple: a workgroup then has all keys of one, and no second kernel is needed.
-//     The prefix's keys are cut into chunks for workgroups of the same launch.
+//     lists are not cut within a triple: a workgroup, or where there are many a wave, then has all keys of one, and no
+//     second kernel is needed. The prefix's keys are cut into chunks for workgroups of the same launch.
 //   * A workgroup that has all of a triple's keys writes the result itself; otherwise it leaves (m, l, unnormalised O) in the
 //     workspace, and a second kernel joins a row's parts, the prefix's and its own, in a fixed order.
 //
+// Measured at 16 heads, us: one sequence of 1000 in bf16 9.6 (latency: 16 workgroups); 16 sequences of up to 4096 in int8, 167 MB,
+// 27 and 4 for the join (6.2 TB/s); 32 of 8192 in fp8, 1.1 GB, 158 and 4 (6.9 TB/s, what a read of this size reaches); 64 of up to 512
+// behind a prefix of 4096 in int8 26 and 4 (94 MB, and the prefix's widening and products beside it); 12 by 5 tokens behind 2777
+// in fp8 13.5 and 4; 4 of 1500 in exact mode, int8, 11 and 4.
+//
 // Arithmetic: S^T = K Q^T with v_mfma_f32_16x16x32_bf16 on the held values, which bf16 holds exactly (int8 and e4m3
-// alike); the key's scale multiplies the 32-bit score. P times the value's scale is rounded to bf16 (half a step,
-// 2^-9, for each term of the sum) for O^T += V^T P^T; m, l and O stay in 32 bits, l sums the unrounded probabilities.
+// alike); the key's scale multiplies the 32-bit score. P times the value's scale is rounded to bf16 (at most half a step,
+// 2^-8 relative, for each term of the sum) for O^T += V^T P^T; m, l and O stay in 32 bits, l sums the unrounded probabilities.
 // In fp32 mode q (divided by the power of two below its row's largest magnitude) and P are split into three bf16 values
 // each, whose sum is the fp32 value, so every product is exact in the 32-bit accumulation.
 
@@ -44,10 +50,10 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;       // of a workgroup
-constexpr int kWavesFew = 8;    // where there are no more triples than CUs, and few keys each
 constexpr int kJoinThreads = 256;
-constexpr int keys_log(int waves) { return waves == 4 ? 7 : 8; }  // log2 of the keys of a step: a block a wave
-static_assert(1 << keys_log(kWaves) == kKvBlock * kWaves && 1 << keys_log(kWavesFew) == kKvBlock * kWavesFew, "a step's keys");
+constexpr int kWavesLog = 2;
+constexpr int kStepLog = 5 + kWavesLog;  // log2 of the keys of a step: a block a wave
+static_assert(1 << kWavesLog == kWaves && 1 << kStepLog == kKvBlock * kWaves, "logarithms");
 constexpr int kD = DT_HEAD_DIM;
 constexpr int kObufRow = kD + 4;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -58,7 +64,7 @@ constexpr float kSlack = 8.0f;
 constexpr int kBufferDword3 = 0x00020000;  // raw buffer, 32-bit data format (gfx9 family)
 
 // blocks in flight a wave: what 256 registers a lane hold, which leave two workgroups a CU
-constexpr int stages(int format, bool f32) { return format == DT_KV_BF16 || f32 ? 1 : 2; }
+constexpr int stages(int format, bool f32, int qt) { return format == DT_KV_BF16 || f32 || qt > 1 ? 1 : 2; }
 
 // The batch rows, by value in the kernel's arguments.
 struct AttnRows {
@@ -82,21 +88,21 @@ struct CachedAttnArgs {
     float scale;
     int parts;       // partial results a row at most
     // own keys, in steps of 32 keys a key wave; own_wl: log2 of the waves that take query tiles
-    int own_wl, own_tiles;
+    int own_wl, own_qt, own_tiles;  // own_qt: query tiles of such a wave; own_tiles: workgroups for a batch row's query rows
     int own_groups;     // workgroups
-    int waves;          // of a workgroup
-    int aligned;        // one (head, batch row, tile) each; otherwise shares of the list:
+    int aligned;        // one (head, batch row, tile) a workgroup; otherwise shares of the list
+    int apart;          // one a wave
     int lead;           // places that a triple has in the list before those of its steps, for what beginning it costs
     int head_places;    // of one head: all batch rows and tiles
     int share, extra;
     // prefix
-    int pre_slot, pre_len, pre_wl, pre_tiles, pre_chunk;  // pre_chunk: keys a workgroup
+    int pre_slot, pre_len, pre_wl, pre_qt, pre_tiles, pre_chunk;  // pre_chunk: keys a workgroup
     int pre_parts, pre_groups;
 };
 
 // steps of a batch row's keys for a query tile (0: there is nothing to see)
-__host__ __device__ __forceinline__ int steps_of(int len, int cnt, int waves, int wl) {
-    const int log = keys_log(waves) - wl;
+__host__ __device__ __forceinline__ int steps_of(int len, int cnt, int wl) {
+    const int log = kStepLog - wl;
     return cnt == 0 ? 0 : (len + (1 << log) - 1) >> log;
 }
 // The list's places in equal shares: the first `extra` workgroups have one more than `share`. group_of: whose share place s is in.
@@ -215,6 +221,7 @@ struct Work {
     int k0, k1;      // keys
     int slot, len, cnt;  // cnt: the batch row's query tokens
     int wl;          // log2 of the waves that take query tiles
+    int apart;       // whether each wave has a stretch of its own
     int part;        // where the partial result goes, or -1: the result is written
     bool prefix;
 };
@@ -227,23 +234,24 @@ __device__ __forceinline__ int thread_here() {
     return t;
 }
 
-template <int kW>
+template <int kQT>
 struct Shared {
-    float o[kW][16][kObufRow];
-    float ml[kW][3][16];  // base, sum, true maximum
+    float o[kWaves * kQT][16][kObufRow];
+    float ml[kWaves * kQT][3][16];  // base, sum, true maximum
 };
 
 // A wave's part of a stretch of work: begin puts the loads of its first blocks and of its Q rows under way, attend does the work
-// and leaves the results in LDS, join (of the whole workgroup) puts the waves' results together.
-template <int kFormat, bool kF32, bool kOnce, int kW>
+// and leaves the results in LDS, join (of the whole workgroup) puts the waves' results together. kQT: query tiles a wave.
+template <int kFormat, bool kF32, bool kOnce, int kQT>
 struct Stretch {
-    static constexpr int kQS = kF32 ? 3 : 1, kStages = stages(kFormat, kF32);
+    static constexpr int kQS = kF32 ? 3 : 1, kStages = stages(kFormat, kF32, kQT);
     Block<kFormat, kOnce> st[kStages];
-    u32x4 qraw[kF32 ? 8 : 4];
+    static constexpr int kQRegs = kF32 ? 8 : 4;
+    u32x4 qraw[kQT][kQRegs];
     __amdgpu_buffer_rsrc_t rsrc;  // the (slot, head)'s blocks
     int kb, k1, step;             // the next block's first key, the end, the distance of the wave's blocks
     int at, at_step;              // the byte offset of the next block to load, the distance
-    int lane, wave, lim, minlim;
+    int lane, wave, lim[kQT], minlim;
 
     // Loads the wave's next block into st[i], K or V. Past its last block nothing is read: the lanes' offset is then beyond the
     // buffer and zeros arrive. (No load is under a condition: the compiler would count it as not issued, and every wait
@@ -264,7 +272,7 @@ struct Stretch {
         wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int n = lane & 15, g = lane >> 4;
         const int qw = wave & ((1 << w.wl) - 1), kw = wave >> w.wl;
-        step = (kKvBlock * kW) >> w.wl;
+        step = (1 << kStepLog) >> w.wl;
         k1 = w.k1;
         const KvView& c = w.prefix ? a.pre : a.own;
         rsrc = __builtin_amdgcn_make_buffer_rsrc(c.block<kFormat>(w.slot, w.hk, 0), 0, c.blocks * kv_block_bytes(kFormat), kBufferDword3);
@@ -277,33 +285,37 @@ struct Stretch {
             load_v(st[i], kb + i * step);
         }
         const int nrows = (w.prefix ? a.B : 1) * a.T * a.G;
-        const int row0 = w.tile * 16 << w.wl;
-        const int r = row0 + qw * 16 + n;
-        const bool have = r < nrows;
-        const QueryRow qr = query_row(a, have ? r : row0, w.b, w.hk, w.prefix);
-        const int64_t qat = (static_cast<int64_t>(qr.b) * a.T + qr.t) * a.ldq + qr.hq * kD;
+        const int row0 = w.apart ? w.tile * (16 * kQT) : w.tile * (16 * kQT) << w.wl;
+        minlim = w.len;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            if constexpr (kF32) {
-                const u32x4* q = reinterpret_cast<const u32x4*>(static_cast<const float*>(a.q) + qat + k_dim<kFormat>(s, g));
-                qraw[2 * s] = q[0];
-                qraw[2 * s + 1] = q[1];
-            } else {
-                qraw[s] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + qat + k_dim<kFormat>(s, g));
+        for (int x = 0; x < kQT; ++x) {
+            const int r = row0 + ((w.apart ? 0 : qw * kQT) + x) * 16 + n;
+            const bool have = r < nrows;
+            const QueryRow qr = query_row(a, have ? r : row0, w.b, w.hk, w.prefix);
+            const int64_t qat = (static_cast<int64_t>(qr.b) * a.T + qr.t) * a.ldq + qr.hq * kD;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                if constexpr (kF32) {
+                    const u32x4* q = reinterpret_cast<const u32x4*>(static_cast<const float*>(a.q) + qat + k_dim<kFormat>(s, g));
+                    qraw[x][2 * s] = q[0];
+                    qraw[x][2 * s + 1] = q[1];
+                } else {
+                    qraw[x][s] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + qat + k_dim<kFormat>(s, g));
+                }
             }
+            // keys below lim are seen by the lane's query, keys below minlim by all of the wave's
+            lim[x] = w.len;
+            if (have && !w.prefix && a.causal && qr.t < w.cnt) lim[x] = max(0, min(w.len, w.len - w.cnt + qr.t + 1));
+            minlim = min(minlim, lim[x]);
         }
-        // keys below lim are seen by the lane's query, keys below minlim by all of the wave's
-        lim = w.len;
-        if (have && !w.prefix && a.causal && qr.t < w.cnt) lim = max(0, min(w.len, w.len - w.cnt + qr.t + 1));
-        minlim = lim;
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) minlim = min(minlim, __shfl_xor(minlim, o, 64));
     }
 
     // Q as the matrix operand: as it is, or in three parts; returns what the scores are multiplied with
-    __device__ __forceinline__ float operand_q(float scale, bf16x8 (&qf)[kQS][4]) {
+    static __device__ __forceinline__ float operand_q(u32x4 (&qraw)[kQRegs], float scale, bf16x8 (&qf)[kQS][4]) {
 #pragma unroll
-        for (int i = 0; i < (kF32 ? 8 : 4); ++i) asm volatile("" : "+v"(qraw[i]));  // (arrived: no wait for them in the loop)
+        for (int i = 0; i < kQRegs; ++i) asm volatile("" : "+v"(qraw[i]));  // (arrived: no wait for them in the loop)
         if constexpr (!kF32) {
 #pragma unroll
             for (int s = 0; s < 4; ++s) qf[0][s] = __builtin_bit_cast(bf16x8, qraw[s]);
@@ -332,92 +344,112 @@ struct Stretch {
         }
     }
 
-    __device__ __forceinline__ void attend(float scale, Shared<kW>& sh) {
+    __device__ __forceinline__ void attend(float scale, Shared<kQT>& sh) {
         const int n = lane & 15, g = lane >> 4;
-        bf16x8 qf[kQS][4];
-        const float qscale = operand_q(scale * kLog2e, qf);  // (scores in the log2 domain)
+        bf16x8 qf[kQT][kQS][4];
+        float qscale[kQT];
+#pragma unroll
+        for (int x = 0; x < kQT; ++x) qscale[x] = operand_q(qraw[x], scale * kLog2e, qf[x]);  // (scores in the log2 domain)
 
         // p = exp2(score - base): base is at least the true maximum less kSlack, and moves to it only where a score exceeds it by
         // more, so O is seldom rescaled. Each lane keeps the true maximum and the sum of its own keys.
-        floatx4 acc[8];
-        float base = kLowest, top = kNegInf, sum = 0.0f;
+        floatx4 acc[kQT][8];
+        float base[kQT], top[kQT], sum[kQT];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int x = 0; x < kQT; ++x) {
+            base[x] = kLowest;
+            top[x] = kNegInf;
+            sum[x] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[x][i] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+        }
 
         // one block: scores, probabilities, O; its registers are filled again, K's behind the scores and V's behind O, with the
         // block kStages steps on
         auto take = [&](Block<kFormat, kOnce>& blk) {
             const int next = kb + kStages * step;
             blk.settle(blk.k);
-            floatx4 s[2];
-            s[0] = s[1] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+            floatx4 s[kQT][2];
+#pragma unroll
+            for (int x = 0; x < kQT; ++x) s[x][0] = s[x][1] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const bf16x8 kf = blk.operand(blk.k, i);
 #pragma unroll
-                for (int x = kQS - 1; x >= 0; --x) s[i >> 2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[x][i & 3], s[i >> 2], 0, 0, 0);
+                for (int x = 0; x < kQT; ++x)
+#pragma unroll
+                    for (int y = kQS - 1; y >= 0; --y)
+                        s[x][i >> 2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[x][y][i & 3], s[x][i >> 2], 0, 0, 0);
                 keep_order();
             }
-            floatx4 f[2];
+            floatx4 f[kQT][2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) f[t] = blk.ks[t] * qscale;
+            for (int x = 0; x < kQT; ++x)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) f[x][t] = blk.ks[t] * qscale[x];
             keep_order();
             load_k(blk, next);
             keep_order();
             const bool mask = kb + kKvBlock > minlim;  // (the same for the whole wave)
-            const int rest = lim - kb - g * 4;         // the lane's key 16 t + i is seen if it is below
-            float p[8], most = kNegInf;  // (the maximum of the scores themselves: it does not depend on how the keys are cut)
+            bf16x8 pf[kQT][kQS];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = s[i >> 2][i & 3] * f[i >> 2][i & 3];
-            if (mask) {
+            for (int x = 0; x < kQT; ++x) {
+                const int rest = lim[x] - kb - g * 4;  // the lane's key 16 t + i is seen if it is below
+                float p[8], most = kNegInf;  // (the maximum of the scores themselves: it does not depend on how the keys are cut)
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if ((i >> 2) * 16 + (i & 3) >= rest) p[i] = kNegInf;
-            }
+                for (int i = 0; i < 8; ++i) p[i] = s[x][i >> 2][i & 3] * f[x][i >> 2][i & 3];
+                if (mask) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) most = fmaxf(most, p[i]);
-            top = fmaxf(top, most);
-            if (__any(most - base > kSlack)) {
-                const float to = max_groups(fmaxf(most, base));
-                const float by = __builtin_amdgcn_exp2f(base - to);
-                sum *= by;
+                    for (int i = 0; i < 8; ++i)
+                        if ((i >> 2) * 16 + (i & 3) >= rest) p[i] = kNegInf;
+                }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) acc[i] *= by;
-                base = to;
-            }
-            float add = 0.0f;
+                for (int i = 0; i < 8; ++i) most = fmaxf(most, p[i]);
+                top[x] = fmaxf(top[x], most);
+                if (__any(most - base[x] > kSlack)) {
+                    const float to = max_groups(fmaxf(most, base[x]));
+                    const float by = __builtin_amdgcn_exp2f(base[x] - to);
+                    sum[x] *= by;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float e = __builtin_amdgcn_exp2f(p[i] - base);
-                add += e;
-                p[i] = e * blk.vs[i >> 2][i & 3];
-            }
-            sum += add;
-            if (mask) {  // (a masked key's scale may be anything, NaN too)
+                    for (int i = 0; i < 8; ++i) acc[x][i] *= by;
+                    base[x] = to;
+                }
+                float add = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if ((i >> 2) * 16 + (i & 3) >= rest) p[i] = 0.0f;
+                for (int i = 0; i < 8; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(p[i] - base[x]);
+                    add += e;
+                    p[i] = e * blk.vs[i >> 2][i & 3];
+                }
+                sum[x] += add;
+                if (mask) {  // (a masked key's scale may be anything, NaN too)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if ((i >> 2) * 16 + (i & 3) >= rest) p[i] = 0.0f;
+                }
+#pragma unroll
+                for (int y = 0; y < kQS; ++y) {
+                    union { uint32_t u[4]; bf16x8 v; } h;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        h.u[j] = pack2(p[2 * j], p[2 * j + 1]);
+                        if (y + 1 < kQS) {
+                            p[2 * j] -= __uint_as_float(h.u[j] << 16);
+                            p[2 * j + 1] -= __uint_as_float(h.u[j] & 0xffff0000u);
+                        }
+                    }
+                    pf[x][y] = h.v;
+                }
             }
             blk.settle(blk.v);
-            bf16x8 pf[kQS];
-#pragma unroll
-            for (int x = 0; x < kQS; ++x) {
-                union { uint32_t u[4]; bf16x8 v; } h;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    h.u[j] = pack2(p[2 * j], p[2 * j + 1]);
-                    if (x + 1 < kQS) {
-                        p[2 * j] -= __uint_as_float(h.u[j] << 16);
-                        p[2 * j + 1] -= __uint_as_float(h.u[j] & 0xffff0000u);
-                    }
-                }
-                pf[x] = h.v;
-            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const bf16x8 vf = blk.operand(blk.v, i);
 #pragma unroll
-                for (int x = kQS - 1; x >= 0; --x) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[x], acc[i], 0, 0, 0);
+                for (int x = 0; x < kQT; ++x)
+#pragma unroll
+                    for (int y = kQS - 1; y >= 0; --y)
+                        acc[x][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[x][y], acc[x][i], 0, 0, 0);
                 keep_order();
             }
             load_v(blk, next);
@@ -431,33 +463,39 @@ struct Stretch {
         if constexpr (kStages > 1)
             if (kb < k1) take(st[0]);
         // the sum and O relative to base, base, and the true maximum
-        sum = sum_groups(sum);
-        top = max_groups(top);
-        if (g == 0) {
-            sh.ml[wave][0][n] = base;
-            sh.ml[wave][1][n] = sum;
-            sh.ml[wave][2][n] = top;
-        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) *reinterpret_cast<floatx4*>(&sh.o[wave][n][i * 16 + g * 4]) = acc[i];
+        for (int x = 0; x < kQT; ++x) {
+            const int to = wave * kQT + x;
+            sum[x] = sum_groups(sum[x]);
+            top[x] = max_groups(top[x]);
+            if (g == 0) {
+                sh.ml[to][0][n] = base[x];
+                sh.ml[to][1][n] = sum[x];
+                sh.ml[to][2][n] = top[x];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) *reinterpret_cast<floatx4*>(&sh.o[to][n][i * 16 + g * 4]) = acc[x][i];
+        }
     }
 };
 
-// The waves' results meet: a thread sums four values of a row over the key waves, scaled to their common maximum.
-template <bool kF32, int kW>
-__device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRows& rows, const Work& w, const Shared<kW>& sh) {
-    const int wk = kW >> w.wl, row0 = w.tile * 16 << w.wl, nrows = (w.prefix ? a.B : 1) * a.T * a.G;
-    for (int it = thread_here(); it < (16 * (kD / 4)) << w.wl; it += 64 * kW) {
+// The waves' results meet: a thread sums four values of a row over the key waves, scaled to their common maximum. A wave that
+// has a stretch of its own does so for itself.
+template <bool kF32, int kQT>
+__device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRows& rows, const Work& w, const Shared<kQT>& sh) {
+    const int tid = thread_here(), wave = w.apart ? __builtin_amdgcn_readfirstlane(tid >> 6) : 0;
+    const int wk = w.apart ? 1 : kWaves >> w.wl, tiles = w.apart ? kQT : kQT << w.wl, threads = w.apart ? 64 : 64 * kWaves;
+    const int row0 = w.tile * 16 * tiles, nrows = min((w.prefix ? a.B : 1) * a.T * a.G - row0, 16 * tiles);
+    for (int it = w.apart ? tid & 63 : tid; it < nrows * (kD / 4); it += threads) {
         const int d = (it & 31) * 4, rt = it >> 5;  // (row within the workgroup's tiles)
-        const int tq = rt >> 4, rn = rt & 15;
-        if (row0 + rt >= nrows) continue;
+        const int tq = (rt >> 4) + wave * kQT, rn = rt & 15;
         float mx = kNegInf;
-        for (int k = 0; k < wk; ++k) mx = fmaxf(mx, sh.ml[(k << w.wl) + tq][2][rn]);
+        for (int k = 0; k < wk; ++k) mx = fmaxf(mx, sh.ml[k * tiles + tq][2][rn]);
         const float base = mx == kNegInf ? 0.0f : mx;
         float l = 0.0f;
         floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int k = 0; k < wk; ++k) {
-            const int from = (k << w.wl) + tq;
+            const int from = k * tiles + tq;
             const float f = __builtin_amdgcn_exp2f(sh.ml[from][0][rn] - base);
             l += f * sh.ml[from][1][rn];
             v += f * *reinterpret_cast<const floatx4*>(&sh.o[from][rn][d]);
@@ -483,13 +521,17 @@ __device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRo
     }
 }
 
-template <int kFormat, bool kF32, bool kOnce, int kW>
-__global__ __launch_bounds__(64 * kW, 2) void cached_attn_kernel(CachedAttnArgs a, AttnRows rows) {
-    __shared__ __align__(16) Shared<kW> sh;
+// kQT, kPreQT: query tiles a wave for a batch row's own keys and for the prefix's
+template <int kFormat, bool kF32, bool kOnce, int kQT, int kPreQT>
+__global__ __launch_bounds__(64 * kWaves, 2) void cached_attn_kernel(CachedAttnArgs a, AttnRows rows) {
+    __shared__ __align__(16) union {
+        Shared<kQT> own;
+        Shared<kPreQT> pre;
+    } sh;
     __shared__ AttnRows rl;
     // All arguments in one trip to their memory, in place of one for each dependent use: the batch rows into LDS (all of
     // them, so no length is waited for), the rest into scalar registers or at least the scalar cache.
-    static_assert(64 * kW >= kMaxRaggedBatch, "one batch row a thread");
+    static_assert(64 * kWaves >= kMaxRaggedBatch, "one batch row a thread");
     if (threadIdx.x < kMaxRaggedBatch) {
         rl.len[threadIdx.x] = rows.len[threadIdx.x];
         rl.cum[threadIdx.x] = rows.cum[threadIdx.x];
@@ -501,21 +543,22 @@ __global__ __launch_bounds__(64 * kW, 2) void cached_attn_kernel(CachedAttnArgs 
     int id = blockIdx.x;
     Work w;
     w.prefix = id < a.pre_groups;
-    w.wl = w.prefix ? a.pre_wl : a.own_wl;
-    const int step_log = keys_log(kW) - w.wl;
+    w.wl = w.prefix ? a.pre_wl : a.apart ? kWavesLog : a.own_wl;
+    w.apart = !w.prefix && a.apart;
+    const int step_log = kStepLog - w.wl;
     int s = 0, end = 0, steps = 0, off = 0, count = 0;
     // the batch row's entries
     const auto load_row = [&]() {
         w.len = __builtin_amdgcn_readfirstlane(rl.len[w.b]);
         w.cnt = __builtin_amdgcn_readfirstlane(rl.cnt[w.b]);
         w.slot = __builtin_amdgcn_readfirstlane(rl.slot[w.b]);
-        steps = steps_of(w.len, w.cnt, kW, w.wl);
+        steps = steps_of(w.len, w.cnt, w.wl);
     };
     const auto set_keys = [&]() {
         w.k0 = off << step_log;
         w.k1 = min(w.len, (off + count) << step_log);
         if (a.causal && a.T > 1) {  // nothing past the tile's newest query
-            const int r = ((w.tile + 1) * 16 << w.wl) - 1, t = min(a.T - 1, a.G == 1 ? r : r / a.G);
+            const int r = ((w.tile + 1) * (16 * kQT) << (w.apart ? 0 : w.wl)) - 1, t = min(a.T - 1, a.G == 1 ? r : r / a.G);
             w.k1 = min(w.k1, max(0, w.len - w.cnt + t + 1));
         }
     };
@@ -543,11 +586,22 @@ __global__ __launch_bounds__(64 * kW, 2) void cached_attn_kernel(CachedAttnArgs 
         w.slot = a.pre_slot;
         w.len = a.pre_len;
         w.cnt = 0;
-    } else {
+        Stretch<kFormat, kF32, false, kPreQT> st;
+        st.begin(a, w);
+        st.attend(a.scale, sh.pre);
+        __syncthreads();
+        join_waves<kF32, kPreQT>(a, rl, w, sh.pre);
+        return;
+    }
+    {
         id -= a.pre_groups;
         // the list's neighbours on one XCD: they may share keys
         const int full = a.own_groups / 8 * 8;
         if (id < full) id = (id & 7) * (a.own_groups / 8) + (id >> 3);
+        if (a.apart) {
+            id = id * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+            if (id >= a.own.heads * a.B * a.own_tiles) return;
+        }
         if (a.aligned) {
             const int hb = a.own_tiles == 1 ? id : id / a.own_tiles;
             w.tile = id - hb * a.own_tiles;
@@ -604,18 +658,24 @@ __global__ __launch_bounds__(64 * kW, 2) void cached_attn_kernel(CachedAttnArgs 
         s += count;
         set_keys();
     };
-    Stretch<kFormat, kF32, kOnce, kW> st;
+    Stretch<kFormat, kF32, kOnce, kQT> st;
     st.begin(a, w);
     for (;;) {
-        st.attend(a.scale, sh);
+        st.attend(a.scale, sh.own);
         const Work done = w;
+        if (w.apart) {  // (in its own part of LDS: a wave's accesses of it are in order)
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            join_waves<kF32, kQT>(a, rl, w, sh.own);
+            return;
+        }
         const bool more = s + a.lead < end;
         if (more) {  // the next stretch's first loads are under way while this one is put together
             next();
             st.begin(a, w);
         }
         __syncthreads();
-        join_waves<kF32, kW>(a, rl, done, sh);
+        join_waves<kF32, kQT>(a, rl, done, sh.own);
         if (!more) return;
         __syncthreads();
     }
@@ -640,10 +700,10 @@ __global__ __launch_bounds__(kJoinThreads) void cached_attn_join_kernel(CachedAt
     const int b = bt / a.T, t = bt % a.T;
     int parts = 0;
     if (t < rows.cnt[b]) {
-        const int steps = steps_of(rows.len[b], rows.cnt[b], kWaves, a.own_wl);
+        const int steps = steps_of(rows.len[b], rows.cnt[b], a.own_wl);
         int own = steps > 0;
         if (own && !a.aligned) {
-            const int first = hq / a.G * a.head_places + rows.cum[b] + ((t * a.G + hq % a.G) >> (4 + a.own_wl)) * (steps + a.lead) + a.lead;
+            const int first = hq / a.G * a.head_places + rows.cum[b] + ((t * a.G + hq % a.G) / (16 * a.own_qt << a.own_wl)) * (steps + a.lead) + a.lead;
             own = group_of(a, first + steps - 1) - group_of(a, first) + 1;
         }
         if (own == 1 && a.pre_parts == 0) return;  // (written already)
@@ -692,23 +752,26 @@ __global__ __launch_bounds__(kJoinThreads) void cached_attn_join_kernel(CachedAt
 
 constexpr int kCus = 256;
 constexpr int kLead = 2;           // steps that beginning and ending a triple costs
-constexpr int kWholeSteps = 4;     // up to so many steps a triple's keys are not cut
+constexpr int kApartSteps = 4;     // up to so many a triple may be one wave's
 
-// log2 of the waves that take query tiles: as many as there are tiles of 16 rows
-int query_waves_log(int64_t rows) { return rows <= 16 ? 0 : rows <= 32 ? 1 : 2; }
+// Query tiles a wave, and log2 of the waves that take some: as many as there are tiles of 16 rows. Two tiles a wave where there
+// are as many, so a held value is widened once for both (the exact mode has no registers for that).
+int query_tiles(int64_t rows, bool f32) { return rows > 16 && !f32 ? 2 : 1; }
+int query_waves_log(int64_t rows, int qt) { return rows <= 16 * qt ? 0 : rows <= 32 * qt || qt == 2 ? 1 : 2; }
 
 // How a call is cut; fills rows' cum and the arguments that follow from the sizes. Returns the workspace's bytes.
-int64_t make_plan(CachedAttnArgs& a, AttnRows& rows, bool* join) {
+int64_t make_plan(CachedAttnArgs& a, AttnRows& rows, int format, bool f32, bool* join) {
     constexpr int kResident = 2 * kCus;
-    a.waves = kWaves;
     const int heads = a.own.heads;
     const int64_t own_rows = static_cast<int64_t>(a.T) * a.G, all_rows = own_rows * a.B;
-    a.own_wl = query_waves_log(own_rows);
-    a.own_tiles = static_cast<int>((own_rows + (16 << a.own_wl) - 1) >> (4 + a.own_wl));
+    a.own_qt = query_tiles(own_rows, f32);
+    a.own_wl = query_waves_log(own_rows, a.own_qt);
+    const int own_take = 16 * a.own_qt << a.own_wl;
+    a.own_tiles = static_cast<int>((own_rows + own_take - 1) / own_take);
     int longest = 0, shortest = kMaxCacheTokens;
     int64_t steps = 0, rows_held = 0;
     for (int b = 0; b < a.B; ++b) {
-        const int n = steps_of(rows.len[b], rows.cnt[b], a.waves, a.own_wl);
+        const int n = steps_of(rows.len[b], rows.cnt[b], a.own_wl);
         steps += n;
         rows_held += n > 0;
         longest = std::max(longest, n);
@@ -716,47 +779,52 @@ int64_t make_plan(CachedAttnArgs& a, AttnRows& rows, bool* join) {
     }
     const int64_t all = steps * a.own_tiles * heads, triples = static_cast<int64_t>(heads) * a.B * a.own_tiles;
 
-    a.pre_tiles = 1;
+    // Many short triples: one a wave, whose latencies then overlap. At 16 heads in int8, one a workgroup and one a wave, us: 1024 of 1
+    // key 11.3 and 5.4, of 256 keys 17.3 and 12.1, of 512 26.2 and 23.3; 4096 of 256 61 and 45, of 1024 166 and 168; 512 of 256
+    // 9.1 and 11.0. In bf16, of twice the bytes, 4096 of 256 behind a prefix of 2048 are as fast either way, of 512 174 and 184.
+    a.apart = own_rows <= 16 * a.own_qt && triples >= kResident + (a.pre_len == 0) &&
+              longest <= (format == DT_KV_BF16 ? kApartSteps / 2 : kApartSteps) &&
+              static_cast<int64_t>(longest) * kResident <= 2 * triples;
+    a.pre_tiles = a.pre_qt = 1;
     a.pre_wl = a.pre_chunk = a.pre_parts = a.pre_groups = 0;
     if (a.pre_len > 0) {
-        // as many of the workgroups as the prefix has of the waves' work (beginning and ending a triple costs about two steps)
-        a.pre_wl = query_waves_log(all_rows);
-        a.pre_tiles = static_cast<int>((all_rows + (16 << a.pre_wl) - 1) >> (4 + a.pre_wl));
+        // as many of the workgroups as the prefix has of the waves' work (beginning and ending a triple costs about two steps; half of
+        // both where each wave has one of its own)
+        a.pre_qt = query_tiles(all_rows, f32);
+        a.pre_wl = query_waves_log(all_rows, a.pre_qt);
+        const int take = 16 * a.pre_qt << a.pre_wl;
+        a.pre_tiles = static_cast<int>((all_rows + take - 1) / take);
         const int unit = (kKvBlock * kWaves) >> a.pre_wl;
         const int64_t pre_steps = (a.pre_len + unit - 1) / unit, per_chunk = static_cast<int64_t>(a.pre_tiles) * heads;
-        const int64_t own_work = all + kLead * rows_held * a.own_tiles * heads;
+        const int64_t own_work = (all + kLead * rows_held * a.own_tiles * heads) >> a.apart;
         const int64_t groups = std::max<int64_t>(kResident * (pre_steps * per_chunk) / (pre_steps * per_chunk + own_work), 1);
-        // but at least four steps each, eight where four waves' rows are left as partial results: these weigh as much as the keys
+        // but at least four steps each, 256 keys where those leave 64 rows of partial results: these weigh as much as the keys
         const int64_t chunks = std::max<int64_t>(1, groups / per_chunk);
-        const int64_t each = std::max<int64_t>(a.pre_wl == 2 ? 8 : 4, (pre_steps + chunks - 1) / chunks);
+        const int64_t each = std::max<int64_t>(take == 64 ? 256 / unit : 4, (pre_steps + chunks - 1) / chunks);
         a.pre_chunk = static_cast<int>(std::min(each, pre_steps) * unit);
         a.pre_parts = (a.pre_len + a.pre_chunk - 1) / a.pre_chunk;
         a.pre_groups = static_cast<int>(a.pre_parts * per_chunk);
     }
 
     const int64_t slots = std::max<int64_t>(kResident - a.pre_groups, kResident / 4);
-    // Triples are not cut where they are short, or so many that the longest does not show in the end: these need no workspace of
-    // their own. (An empty list has no shares; one past 2^28 steps has triples enough.)
-    a.aligned = all == 0 || all > (1 << 28) || (longest <= kWholeSteps && (a.pre_groups == 0 || triples <= slots)) ||
-                4 * static_cast<int64_t>(longest) * slots <= all;
-    // Few triples of up to twice as many keys: eight waves each, and one launch in place of two (16 heads, one sequence of 1024 in
-    // int8: 6.3 and 4.3 us with a join, 10.7 so, and a launch's 3 us less on the host; sixteen 13.8 and 4.0, 13.7 so; up to four
-    // steps four waves do, 512 keys 7.8 us by four, 8.5 by eight).
-    if (a.pre_groups == 0 && a.own_wl == 0 && triples <= kCus && longest > kWholeSteps && longest <= 2 * kWholeSteps) {
-        static_assert(kWavesFew == 2 * kWaves, "steps twice as long");
-        a.waves = kWavesFew;
-        a.aligned = 1;
-    }
+    // Triples are not cut where they are short, or so many that the longest does not show in the end: a workgroup's result is then
+    // the last where there is no prefix, and no second launch is needed (3 us of the host's time). 16 heads in int8, whole and
+    // cut, us: one sequence of 600 8.5 and 9.0, of 1024 10.6 and 8.9, of 1500 13.6 and 9.3; 8 of 1500 14.7 and 14.5; 16 of 2048
+    // 23.9 and 27.1, 128 of up to 2048 88 and 92. Behind a prefix of 2048 one of 600 11.3 and 11.0, of 1024 13.5 and 11.0; 8 of
+    // 1024 14.7 and 17.7; 16 of up to 2048 22 and 23, of 2048 35 and 31.
+    // (An empty list has no shares; one past 2^28 steps has triples enough.)
+    const int whole_steps = a.pre_len == 0 ? (triples < kCus ? 8 : 16) : (triples < kCus / 2 ? 4 : 8);
+    a.aligned = a.apart || all == 0 || all > (1 << 28) || longest <= whole_steps || 4 * static_cast<int64_t>(longest) * slots <= all;
     int own_parts = 1;
     bool whole = true;  // every triple's keys in one workgroup
-    a.own_groups = static_cast<int>(triples);
+    a.own_groups = static_cast<int>(a.apart ? (triples + kWaves - 1) / kWaves : triples);
     if (!a.aligned) {
         // beginning a triple is counted where workgroups have several; one that is cut is begun twice, which no count would mend
         a.lead = rows_held * a.own_tiles * heads > slots ? kLead : 0;
         int64_t cum = 0;
         for (int b = 0; b < a.B; ++b) {
             rows.cum[b] = static_cast<int>(cum);
-            const int n = steps_of(rows.len[b], rows.cnt[b], a.waves, a.own_wl);
+            const int n = steps_of(rows.len[b], rows.cnt[b], a.own_wl);
             if (n > 0) cum += static_cast<int64_t>(n + a.lead) * a.own_tiles;
         }
         a.head_places = static_cast<int>(cum);
@@ -778,13 +846,27 @@ int launch(const CachedAttnArgs& a, const AttnRows& rows, bool join, int format,
     const bool f32 = dtype != DT_BF16;
     const bool once = a.own_wl == 0 && a.own_tiles == 1;
     if (groups > 0) {
-        const dim3 g(static_cast<unsigned>(groups)), t(64 * a.waves);
+        const dim3 g(static_cast<unsigned>(groups)), t(64 * kWaves);
         const auto go = [&](auto format_, auto f32_) {
             constexpr int F = decltype(format_)::value;
             constexpr bool M = decltype(f32_)::value;
-            if (a.waves == kWavesFew) hipLaunchKernelGGL((cached_attn_kernel<F, M, true, kWavesFew>), g, t, 0, s, a, rows);
-            else if (once) hipLaunchKernelGGL((cached_attn_kernel<F, M, true, kWaves>), g, t, 0, s, a, rows);
-            else hipLaunchKernelGGL((cached_attn_kernel<F, M, false, kWaves>), g, t, 0, s, a, rows);
+            const auto go_as = [&](auto once_, auto qt_, auto pre_qt_) {
+                hipLaunchKernelGGL((cached_attn_kernel<F, M, decltype(once_)::value, decltype(qt_)::value, decltype(pre_qt_)::value>), g, t,
+                                   0, s, a, rows);
+            };
+            constexpr std::integral_constant<int, 1> one;
+            constexpr std::integral_constant<int, 2> two;
+            constexpr std::true_type yes;
+            constexpr std::false_type no;
+            if constexpr (M) {
+                if (once) go_as(yes, one, one);
+                else go_as(no, one, one);
+            } else {  // (more than one tile: two a wave)
+                if (a.own_qt == 2 && once) go_as(yes, two, two);
+                else if (a.own_qt == 2) go_as(no, two, two);
+                else if (a.pre_qt == 2) go_as(yes, one, two);
+                else go_as(yes, one, one);
+            }
         };
         const auto go_mode = [&](auto format_) {
             if (f32) go(format_, std::true_type());
@@ -856,7 +938,7 @@ int dt_cached_attn_workspace(const dt_kv_cache* cache, int B, int T, int H, int 
     AttnRows rows{};
     bool join = false;
     DT_TRY(check_call(cache, B, T, H, D, slots, counts, prefix, prefix_slot, dtype, &a, &rows));
-    *bytes = make_plan(a, rows, &join);
+    *bytes = make_plan(a, rows, cache->format, dtype != DT_BF16, &join);
     return DT_OK;
 }
 
@@ -877,7 +959,7 @@ int dt_cached_attn_fwd(dt_kv_cache* cache, const void* q, void* o, float* m, flo
     if (mem == DT_MEM_DEVICE && (!aligned16(q) || !aligned16(o) || !aligned16(ws) || ldq * esz % 16))
         return set_error(DT_ERR_INVALID_ARG, "device q/o/workspace and q's row stride must be 16-byte aligned");
     bool join = false;
-    const int64_t need = make_plan(a, rows, &join);
+    const int64_t need = make_plan(a, rows, cache->format, dtype != DT_BF16, &join);
     if (mem == DT_MEM_DEVICE && need > 0 && (!ws || ws_bytes < need))
         return set_error(DT_ERR_INVALID_ARG, "the workspace has %lld bytes, the call needs %lld", (long long)(ws ? ws_bytes : 0), (long long)need);
     dt_ctx* ctx = cache->ctx;

@@ -378,6 +378,29 @@ def test_long_cache_past_32_bits():
     assert float((r.output.float() - w.output.float()).abs().max()) <= 2 * 2.0 ** -8 * float(w.output.float().abs().max())
 
 
+@pytest.mark.parametrize("fmt,tdt", [("int8", torch.bfloat16), ("int8", torch.float32), ("fp8", torch.float32), ("bf16", torch.bfloat16)])
+@pytest.mark.parametrize("B,T,H,Hk,longest,P", [(64, 1, 16, 16, 500, 0), (64, 1, 16, 16, 100, 300), (33, 3, 16, 16, 120, 0),
+                                                (130, 5, 16, 4, 128, 77), (256, 1, 3, 3, 2300, 0), (256, 1, 3, 3, 1200, 200)])
+def test_more_sequences_and_heads_than_workgroups(fmt, tdt, B, T, H, Hk, longest, P):
+    """One (head, sequence) a wave, and shares of a list in which workgroups have several, up to the largest batch."""
+    from dirktensor_amd import KVCache
+
+    print(f"more than workgroups {fmt} {tdt} B={B} T={T} H={H} Hk={Hk} longest={longest} P={P}", flush=True)
+    rng = np.random.default_rng(longest)
+    lens = [int(n) for n in rng.integers(0, longest + 1, size=B)]
+    lens[:4] = [longest, 0, 1, 32]
+    counts = [int(n) for n in rng.integers(0, T + 1, size=B)]
+    counts[:4] = [T, T, T, T]
+    c = KVCache(B, longest, Hk, format=fmt)
+    k, v = randn((B, longest, Hk, D), 900), randn((B, longest, Hk, D), 901)
+    c.append(k, v, counts=lens)
+    p = None
+    if P:
+        p = KVCache(1, P, Hk, format=fmt)
+        fill(p, [P], 902)
+    run(randn((B, T, H, D), 903, tdt), c, counts=counts, prefix=p)
+
+
 def test_many_query_tiles():
     """More (head, sequence, query tile) triples than are cut: a prompt in chunks over a cache, padded, with and without a
     prefix; compared with one token at a time at sampled places (the reference's loop would take minutes)."""
