@@ -963,7 +963,8 @@ int dt_cached_attn_fwd(dt_kv_cache* cache, const void* q, void* o, float* m, flo
     if (mem == DT_MEM_DEVICE && need > 0 && (!ws || ws_bytes < need))
         return set_error(DT_ERR_INVALID_ARG, "the workspace has %lld bytes, the call needs %lld", (long long)(ws ? ws_bytes : 0), (long long)need);
     dt_ctx* ctx = cache->ctx;
-    DT_TRY(check_device_binding(ctx));
+    DeviceScope scope;
+    DT_TRY(scope.enter(cache->device));
     hipStream_t s = static_cast<hipStream_t>(stream);
     a.q = q;
     a.o = o;

@@ -234,6 +234,19 @@ bool aligned16(const void* p);
 // dt_flash_attn_bwd_noalloc (noalloc.hip)
 int noalloc_setup(int device);
 int check_device_binding(dt_ctx* ctx);
+// Makes a context's device the current one for a call, and the caller's again when it ends.
+struct DeviceScope {
+    int before = -1, mine = -1;
+    int enter(int device) {
+        DT_HIP_TRY(hipGetDevice(&before));
+        mine = device;
+        if (before != mine) DT_HIP_TRY(hipSetDevice(mine));
+        return DT_OK;
+    }
+    ~DeviceScope() {
+        if (before >= 0 && before != mine) (void)hipSetDevice(before);
+    }
+};
 // after the stream has been synchronised: DT_ERR_HIP (and clears the word) when a fused QKV wait gave up
 int qkv_status_check(dt_ctx* ctx);
 

@@ -442,7 +442,8 @@ int dt_kv_cache_create(dt_ctx* ctx, int slots, int capacity, int n_heads, int D,
     if (format != DT_KV_INT8 && format != DT_KV_FP8 && format != DT_KV_BF16)
         return set_error(DT_ERR_INVALID_ARG, "unknown cache format %d", format);
     if (!ctx) return set_error(DT_ERR_INVALID_ARG, "ctx is NULL");
-    DT_TRY(check_device_binding(ctx));
+    DeviceScope scope;
+    DT_TRY(scope.enter(ctx->device));
     dt_kv_cache* c = new (std::nothrow) dt_kv_cache;
     if (!c) return set_error(DT_ERR_INVALID_ARG, "out of host memory");
     c->ctx = ctx;
@@ -476,7 +477,8 @@ int dt_kv_cache_create(dt_ctx* ctx, int slots, int capacity, int n_heads, int D,
 int dt_kv_cache_destroy(dt_kv_cache* cache) {
     clear_error();
     if (!cache) return DT_OK;
-    DT_HIP_TRY(hipSetDevice(cache->device));
+    DeviceScope scope;
+    DT_TRY(scope.enter(cache->device));
     free_cache(cache);  // (hipFree waits for the device)
     return DT_OK;
 }
@@ -532,7 +534,8 @@ int dt_kv_cache_append(dt_kv_cache* cache, const void* k, const void* v, int B, 
             return set_error(DT_ERR_INVALID_ARG, "slot %d holds %d of %d tokens: %d more do not fit", rows.slot[b],
                              rows.len[b], cache->capacity, rows.cnt[b]);
     }
-    DT_TRY(check_device_binding(cache->ctx));
+    DeviceScope scope;
+    DT_TRY(scope.enter(cache->device));
     hipStream_t s = static_cast<hipStream_t>(stream);
     KvMoveArgs a{cache->view(), const_cast<void*>(k), const_cast<void*>(v), ldk, ldv, T * ldk, T * ldv};
     if (mem == DT_MEM_HOST) {
@@ -570,7 +573,8 @@ int dt_kv_cache_read(dt_kv_cache* cache, void* k, void* v, int B, int T, const i
         if (rows.len[b] < 0 || rows.len[b] > held || T > held - rows.len[b])
             return set_error(DT_ERR_INVALID_ARG, "%d tokens from %d on: slot %d holds %d", T, rows.len[b], rows.slot[b], held);
     }
-    DT_TRY(check_device_binding(cache->ctx));
+    DeviceScope scope;
+    DT_TRY(scope.enter(cache->device));
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int64_t dm = static_cast<int64_t>(cache->heads) * DT_HEAD_DIM;
     KvMoveArgs a{cache->view(), k, v, dm, dm, T * dm, T * dm};

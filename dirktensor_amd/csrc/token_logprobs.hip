@@ -663,7 +663,8 @@ int dt_token_logprobs(dt_ctx* ctx, const void* logits, const void* tokens, int B
         DT_TRY(check_host_tokens(tokens, token_bytes, rows, V, ignore_index));
     }
     if (!ctx) return set_error(DT_ERR_INVALID_ARG, "ctx is NULL");
-    DT_TRY(check_device_binding(ctx));
+    DeviceScope scope;
+    DT_TRY(scope.enter(ctx->device));
     hipStream_t s = static_cast<hipStream_t>(stream);
     LogprobArgs a{};
     a.x = logits;
@@ -723,7 +724,10 @@ int dt_token_logprobs_bwd(dt_ctx* ctx, const float* d_logprob, const float* d_en
         return set_error(DT_ERR_INVALID_ARG, "d_logprob, logits, tokens, m, l and d_logits must be non-NULL");
     if (d_entropy && !entropy) return set_error(DT_ERR_INVALID_ARG, "entropy must be non-NULL with d_entropy");
     DT_TRY(check_logits(B, T, V, ldb, ldt, token_bytes, dtype, mem));
-    if ((T > 1 && ldt_out < V) || (B > 1 && ldb_out < (T - 1) * ldt_out + V) || ldb_out < 0 || ldt_out < 0)
+    // (either dimension's rows may lie between the other's)
+    const bool by_b = (T == 1 || ldt_out >= V) && (B == 1 || ldb_out >= (T - 1) * ldt_out + V);
+    const bool by_t = (B == 1 || ldb_out >= V) && (T == 1 || ldt_out >= (B - 1) * ldb_out + V);
+    if (!(by_b || by_t) || ldb_out < 0 || ldt_out < 0)
         return set_error(DT_ERR_INVALID_ARG, "rows of d_logits %lld and %lld apart overlap", (long long)ldb_out, (long long)ldt_out);
     const int64_t rows = static_cast<int64_t>(B) * T;
     const size_t es = dtype == DT_BF16 ? 2 : 4;
@@ -734,7 +738,8 @@ int dt_token_logprobs_bwd(dt_ctx* ctx, const float* d_logprob, const float* d_en
         DT_TRY(check_host_tokens(tokens, token_bytes, rows, V, ignore_index));
     }
     if (!ctx) return set_error(DT_ERR_INVALID_ARG, "ctx is NULL");
-    DT_TRY(check_device_binding(ctx));
+    DeviceScope scope;
+    DT_TRY(scope.enter(ctx->device));
     hipStream_t s = static_cast<hipStream_t>(stream);
     LogprobBwdArgs a{};
     a.x = logits;

@@ -256,6 +256,10 @@ def test_next_token_views_and_outputs(tdt):
     # other orders of the leading dimensions, one row, a vocabulary that is not contiguous
     p = dense.transpose(0, 1)
     assert torch.equal(token_logprobs(p, y.transpose(0, 1)).logprob, r.logprob.transpose(0, 1))
+    p2 = p.clone(memory_format=torch.preserve_format)
+    assert p2.stride() == p.stride()
+    got = token_logprobs_backward(g.T, p2, y.T, token_logprobs(p2, y.T), d_entropy=h.T, out=p2)
+    assert got is p2 and torch.equal(got, want.transpose(0, 1))
     one = token_logprobs(dense[0, 0], y[0, 0], top_k=2)
     assert one.logprob.shape == () and torch.equal(one.top_index, r.top_index[0, 0, :2])
     q = dense.transpose(1, 2).contiguous().transpose(1, 2)
