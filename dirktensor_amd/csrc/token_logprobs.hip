@@ -18,6 +18,11 @@
 // (value, index) pairs, so no two are equal, ties go to the lower index and the order of the collection does not matter. Where more values
 // reach the bound than the list holds (rows of many equal values) they are selected one after another in passes over the
 // row. A row cut into segments leaves (m, l, sum, k keys) of each in the workspace and a second kernel joins them.
+//
+// Measured: 2048 rows of 100352 in fp32, 822 MB, with 5 alternatives 134 us (6.1 TB/s; reads past the caches reach 7.0, the rest is
+// the workgroups' beginning and end, each of which does a row), 16 rows with 20 alternatives 10 us (49 segments of 8 KB each:
+// the chain from the first load to the sorted keys) and 5.7 for the join. The gradient of the 2048 rows, 1.64 GB moved, 300 us (5.5 TB/s,
+// a large copy 5.2), of 300 rows of 50277 in bf16, 60 MB, 13.6 us (4.4 TB/s).
 
 #include "dt_internal.h"
 
