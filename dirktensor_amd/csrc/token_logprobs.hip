@@ -127,6 +127,21 @@ struct Stats {
     float m = kNegInf, s = 0.0f, d = 0.0f;  // maximum; sum e; sum e (x - m)
 };
 
+// v[i] without memory (as masks: a choice between two elements would put the array there), four at a time for few registers
+__device__ __forceinline__ float pick(const float (&v)[kBatch], int i) {
+    const auto either = [](uint32_t m, uint32_t a, uint32_t b) { return (a & m) | (b & ~m); };
+    const uint32_t odd = 0u - (i & 1), upper = 0u - (i >> 1 & 1);
+    uint32_t r = 0;
+#pragma unroll
+    for (int q = 0; q < kBatch / 4; ++q) {
+        const auto u = [&](int j) { return __float_as_uint(v[4 * q + j]); };
+        const uint32_t four = either(upper, either(odd, u(3), u(2)), either(odd, u(1), u(0)));
+        r = i >> 2 == q ? four : r;
+        asm volatile("" : "+v"(r));
+    }
+    return __uint_as_float(r);
+}
+
 // takes the values, and returns their maximum (-inf in the place of a value that is none)
 template <int kN>
 __device__ __forceinline__ float take(Stats& st, const float (&v)[kN]) {
@@ -298,7 +313,7 @@ __device__ __forceinline__ void write_top(const LogprobArgs& a, int64_t row, int
 }
 
 template <bool kBf16, bool kTop>
-__global__ __launch_bounds__(kThreads) void logprob_rows_kernel(LogprobArgs a) {
+__global__ __launch_bounds__(kThreads, 8) void logprob_rows_kernel(LogprobArgs a) {
     __shared__ float sbuf[kWaves][3];
     __shared__ SelectBuf buf;
     using R = Run<kBf16>;
@@ -350,8 +365,8 @@ __global__ __launch_bounds__(kThreads) void logprob_rows_kernel(LogprobArgs a) {
             f(v, j);
         }
     };
-    // use(key) for those of a batch's values that are not below `least`. Few are: they are found in the registers and read again
-    // one by one.
+    // use(key) for those of a batch's values that are not below `least`. Few are: a mask finds them, and each is taken from the
+    // registers (read again, it would wait for the next batch's loads, which are under way).
     const auto look = [&](const float(&v)[kBatch], int j, float least, auto&& use) {
         uint32_t hits = 0;
 #pragma unroll
@@ -359,7 +374,7 @@ __global__ __launch_bounds__(kThreads) void logprob_rows_kernel(LogprobArgs a) {
         while (hits) {
             const int i = __ffs(hits) - 1, p = (j * R::kPer + i / R::kPiece) * kThreads + tid, at = p * R::kPiece + i % R::kPiece;
             hits &= hits - 1;
-            if (p < run.pieces) use(key_of(run.one(at), first + at));
+            if (p < run.pieces) use(key_of(pick(v, i), first + at));
         }
     };
     const auto cached = [&](int p) { return run.load(p); };
