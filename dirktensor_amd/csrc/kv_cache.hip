@@ -10,7 +10,8 @@
 // leave most threads idle: a wave takes one row of K or of V, two values a lane (kv_append_rows_kernel).
 //
 // Measured at 16 heads: 2 x 4096 tokens of bf16 into fp8 and back, 102 MB each way, 22.6 and 20.5 us (4.5 and 5.0 TB/s; a large copy
-// 5.2), 17.6 and 19.8 with the rows in the caches (loads past these take 22.6 either way, stores past them 34). One token of eight sequences in int8 3.3 us, and read back 3.4, which is what a launch takes.
+// 5.2), 17.6 and 19.8 with the rows in the caches (loads past these take 22.6 either way, stores past them 34). One token of eight
+// sequences in int8 3.3 us, and read back 3.4, which is what a launch takes.
 
 #include "kv_cache.h"
 

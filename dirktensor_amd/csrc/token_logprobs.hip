@@ -19,8 +19,8 @@
 // reach the bound than the list holds (rows of many equal values) they are selected one after another in passes over the
 // row. A row cut into segments leaves (m, l, sum, k keys) of each in the workspace and a second kernel joins them.
 //
-// Measured: 2048 rows of 100352 in fp32, 822 MB, with 5 alternatives 134 us (6.1 TB/s; reads past the caches reach 7.0, the rest is
-// the workgroups' beginning and end, each of which does a row), 16 rows with 20 alternatives 10 us (49 segments of 8 KB each:
+// Measured: 2048 rows of 100352 in fp32, 822 MB, with 5 alternatives 130 us, without 121 (6.3 and 6.8 TB/s; reads past the
+// caches reach 7.0), with 64 163, 16 rows with 20 alternatives 10 us (49 segments of 8 KB each:
 // the chain from the first load to the sorted keys) and 5.7 for the join. The gradient of the 2048 rows, 1.64 GB moved, 300 us (5.5 TB/s,
 // a large copy 5.2), of 300 rows of 50277 in bf16, 60 MB, 13.6 us (4.4 TB/s).
 
@@ -462,10 +462,11 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
     select(buf, a.k, each, [&](int place, uint64_t k) { write_top(a, row, place, k, f); });
 }
 
-// Segments a row: enough workgroups to fill the CUs several times, none shorter than kMinSegment, their keys a few a thread.
+// Segments a row: about as many workgroups as the CUs hold at once, none shorter than kMinSegment, their keys a few a thread. (To the
+// nearest: 2047 rows of 100352 in fp32 121 us whole, 127 in two segments and their join; 1400 87 and 89, 1100 in two 74.)
 void cut(int64_t rows, int V, int k, int* segments, int* seg_len) {
     constexpr int64_t kTarget = 2048;
-    int64_t s = std::min<int64_t>((kTarget + rows - 1) / rows, (V + kMinSegment - 1) / kMinSegment);
+    int64_t s = std::min<int64_t>((kTarget + rows / 2) / rows, (V + kMinSegment - 1) / kMinSegment);
     s = std::min<int64_t>(s, kThreads);
     if (k > 0) s = std::min<int64_t>(s, kJoinKeys * kThreads / k);
     s = std::max<int64_t>(s, 1);
