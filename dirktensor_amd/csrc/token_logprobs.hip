@@ -16,11 +16,13 @@
 // (from L2), and the rest of the row is compared with the bound as it streams by, one comparison for 16 values; what reaches
 // it (about 5 k values) is collected in LDS, and each takes the place that the number of larger ones gives it. Keys are
 // (value, index) pairs, so no two are equal, ties go to the lower index and the order of the collection does not matter. Where more values
-// reach the bound than the list holds (rows of many equal values) they are selected one after another in passes over the
+// reach the bound than the list holds (rows that rise, or begin with masked values) the maxima of the whole row give another and the
+// row is read once more; where that leaves too many as well (equal values) the k-th key is found digit by digit in passes over the
 // row. A row cut into segments leaves (m, l, sum, k keys) of each in the workspace and a second kernel joins them.
 //
 // Measured: 2048 rows of 100352 in fp32, 822 MB, with 5 alternatives 130 us, without 121 (6.3 and 6.8 TB/s; reads past the
-// caches reach 7.0), with 64 163, 16 rows with 20 alternatives 10 us (49 segments of 8 KB each:
+// caches reach 7.0), with 64 163; rows whose first quarter is masked 259, with fifty tokens left 139, of equal values 2140 (they were
+// 1460, 1470 and 1440 for 5 and ten times as long for 64 alternatives when these were selected one after another). 16 rows with 20 alternatives 10 us (49 segments of 8 KB each:
 // the chain from the first load to the sorted keys) and 5.7 for the join. The gradient of the 2048 rows, 1.64 GB moved, 300 us (5.5 TB/s,
 // a large copy 5.2), of 300 rows of 50277 in bf16, 60 MB, 13.6 us (4.4 TB/s).
 
@@ -50,6 +52,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLog2eLo = 1.92596303e-8f;  // log2 e - kLog2e
 constexpr float kLn2 = 0.693147180559945f;
 constexpr float kNegInf = -__builtin_huge_valf();
+constexpr float kLowest = -3.402823466e38f;
 
 struct LogprobArgs {
     const void* x;
@@ -236,11 +239,11 @@ __device__ __forceinline__ Finish finish(const LogprobArgs& a, int64_t row, cons
 }
 
 struct SelectBuf {
-    uint32_t top[kThreads];
+    uint32_t top[kThreads];  // of the threads (find_bound), or how many have a digit (select)
     uint64_t list[kList];
-    uint64_t best[kWaves];
     int count;
 };
+static_assert(kThreads == 256, "a thread a digit");
 
 // A bound that the k-th largest of the threads' `mine` (order_of their maximum; 0: none) reaches, to 20 bits, the same for all;
 // empties the list. Each wave finds it for itself, bit by bit, from four of the 256 a lane.
@@ -263,48 +266,94 @@ __device__ __forceinline__ uint32_t find_bound(SelectBuf& b, uint32_t mine, int 
     return bound;
 }
 
-__device__ __forceinline__ void push(SelectBuf& b, uint64_t key) {
-    if (*static_cast<volatile int*>(&b.count) >= kList + kThreads) return;  // (the list has long run over)
+// whether the list has run over
+__device__ __forceinline__ bool push(SelectBuf& b, uint64_t key) {
+    if (*static_cast<volatile int*>(&b.count) >= kList + kThreads) return true;  // (long ago)
     const int at = atomicAdd(&b.count, 1);
     if (at < kList) b.list[at] = key;
+    return at >= kList;
+}
+
+// The digit of the `least`-th largest key, given how many keys have each and how many lie `above` them all, which grows by those of
+// larger digits; n: how many have it. The same for all waves: each finds it for itself, four digits a lane.
+__device__ __forceinline__ int find_digit(const SelectBuf& b, int least, int& above, int& n) {
+    const int lane = threadIdx.x & 63;
+    int h[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += h[i] = static_cast<int>(b.top[lane * 4 + i]);
+    int to = sum;  // of the lane's digits and larger
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int more = __shfl_down(to, o, 64);
+        if (lane + o < 64) to += more;
+    }
+    const uint64_t reach = __ballot(above + to >= least);
+    const int at = 63 - __clzll(static_cast<long long>(reach | 1));  // (the last lane that does)
+    int d = 3, over = above + to - sum;
+#pragma unroll
+    for (int i = 3; i > 0; --i)
+        if (d == i && over + h[i] < least) {
+            over += h[i];
+            --d;
+        }
+    n = __shfl(d == 3 ? h[3] : d == 2 ? h[2] : d == 1 ? h[1] : h[0], at, 64);
+    above = __shfl(over, at, 64);
+    return at * 4 + __shfl(d, at, 64);
 }
 
 // The k largest of the collected keys, in order, through out(place, key); places past the last get key 0. Where the list ran
-// over, the k largest of all: each(f) calls f(key) for every value of the thread.
+// over, the k largest of all: each(f) calls f(key) for every key of the thread. The `least`-th key's digits are then found from the
+// first on, a pass over the keys each, until the list holds what reaches them; no two keys are equal, so it does in the end. A list
+// that holds fewer than the `least` that there are lacks only keys of -inf: these are the largest of those by their index.
 template <class Each, class Out>
-__device__ __forceinline__ void select(SelectBuf& b, int k, Each each, Out out) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+__device__ __forceinline__ void select(SelectBuf& b, int k, int least, Each each, Out out) {
+    const int tid = threadIdx.x;
     __syncthreads();
-    const int c = b.count;
-    if (c <= kList) {
-        for (int i = tid; i < c; i += kThreads) {
-            const uint64_t key = b.list[i];
-            int larger = 0;
-#pragma unroll 8
-            for (int j = 0; j < c; ++j) larger += b.list[j] > key;
-            if (larger < k) out(larger, key);
+    if (b.count > kList || b.count < least) {
+        const bool few = b.count < least;
+        uint64_t digits = few ? static_cast<uint64_t>(kOrderNegInf) << 32 : 0, mask = few ? ~uint64_t(0) << 32 : 0;
+        int above = few ? b.count : 0;
+        for (int at = few ? 24 : 56; at >= 0; at -= 8) {
+            if (at == 24) {  // (an index has 24 bits)
+                digits |= 0xffull << 24;
+                mask |= 0xffull << 24;
+                continue;
+            }
+            __syncthreads();
+            b.top[tid] = 0;
+            __syncthreads();
+            each([&](uint64_t key) {
+                if ((key & mask) != digits) return;
+                // (often all are alike: one addition then)
+                const uint32_t d = static_cast<uint32_t>(key >> at) & 255, first = __builtin_amdgcn_readfirstlane(d);
+                const uint64_t alike = __ballot(d == first);
+                if (d != first) atomicAdd(&b.top[d], 1u);
+                else if ((tid & 63) == __ffsll(static_cast<unsigned long long>(alike)) - 1) atomicAdd(&b.top[d], static_cast<uint32_t>(__popcll(alike)));
+            });
+            __syncthreads();
+            int n;
+            const int d = find_digit(b, least, above, n);
+            digits |= static_cast<uint64_t>(d) << at;
+            mask |= 0xffull << at;
+            if (above + n <= kList) break;
         }
-        for (int i = c + tid; i < k; i += kThreads) out(i, 0);
-        return;
-    }
-    uint64_t last = ~uint64_t(0);
-    for (int r = 0; r < k; ++r) {  // the largest key below the last
-        uint64_t top = 0;
+        __syncthreads();
+        if (tid == 0) b.count = 0;
+        __syncthreads();
         each([&](uint64_t key) {
-            if (key < last && key > top) top = key;
+            if ((key & mask) >= digits) push(b, key);
         });
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint64_t other = __shfl_xor(static_cast<unsigned long long>(top), o, 64);
-            top = other > top ? other : top;
-        }
         __syncthreads();
-        if (lane == 0) b.best[wave] = top;
-        __syncthreads();
-        last = b.best[0];
-        for (int w = 1; w < kWaves; ++w) last = b.best[w] > last ? b.best[w] : last;
-        if (tid == 0) out(r, last);
     }
+    const int c = b.count;
+    for (int i = tid; i < c; i += kThreads) {
+        const uint64_t key = b.list[i];
+        int larger = 0;
+#pragma unroll 8
+        for (int j = 0; j < c; ++j) larger += b.list[j] > key;
+        if (larger < k) out(larger, key);
+    }
+    for (int i = c + tid; i < k; i += kThreads) out(i, 0);
 }
 
 __device__ __forceinline__ void write_top(const LogprobArgs& a, int64_t row, int place, uint64_t key, const Finish& f) {
@@ -365,12 +414,15 @@ __global__ __launch_bounds__(kThreads, 8) void logprob_rows_kernel(LogprobArgs a
             f(v, j);
         }
     };
-    // use(key) for those of a batch's values that are not below `least`. Few are: a mask finds them, and each is taken from the
+    // use(key) for those of a batch's values that reach `least`, or all. Few do: a mask finds them, and each is taken from the
     // registers (read again, it would wait for the next batch's loads, which are under way).
-    const auto look = [&](const float(&v)[kBatch], int j, float least, auto&& use) {
-        uint32_t hits = 0;
+    const auto look = [&](const float(&v)[kBatch], int j, bool all, float least, auto&& use) {
+        uint32_t hits = (1u << kBatch) - 1;
+        if (!all) {
+            hits = 0;
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) hits |= v[i] < least ? 0u : 1u << i;
+            for (int i = 0; i < kBatch; ++i) hits |= v[i] >= least ? 1u << i : 0u;
+        }
         while (hits) {
             const int i = __ffs(hits) - 1, p = (j * R::kPer + i / R::kPiece) * kThreads + tid, at = p * R::kPiece + i % R::kPiece;
             hits &= hits - 1;
@@ -389,19 +441,30 @@ __global__ __launch_bounds__(kThreads, 8) void logprob_rows_kernel(LogprobArgs a
             take(st, v);
         });
         stream(1, part, cached, [&](const float(&v)[kBatch], int) { take(st, v); });
-        const bool any = tail < run.n || tid < run.pieces;
+        const bool any = tail < run.n || tid < run.pieces, whole = run.n <= kList;
         const uint32_t mine = any ? order_of(st.m) : 0;
         bound = find_bound(buf, mine, a.k);
-        const auto list = [&](uint64_t key) { push(buf, key); };
-        const float least = bound <= kOrderNegInf ? kNegInf : key_value(static_cast<uint64_t>(bound) << 32);
-        if (any && mine >= bound) {
-            if (tail < run.n && !(last[0] < least)) push(buf, key_of(last[0], first + tail));
-            if (part > 0) look(v0, 0, least, list);
-            stream(1, part, cached, [&](const float(&v)[kBatch], int j) { look(v, j, least, list); });
+        // (values of -inf are listed only where the list holds the whole run: else they would fill it)
+        float least = bound <= kOrderNegInf ? kLowest : key_value(static_cast<uint64_t>(bound) << 32);
+        const auto list = [&](uint64_t key) {
+            if (push(buf, key)) least = -kNegInf;  // (the list is of no use any more)
+        };
+        if (whole || (any && mine >= bound)) {
+            if (tail < run.n && (whole || last[0] >= least)) push(buf, key_of(last[0], first + tail));
+            if (part > 0) look(v0, 0, whole, least, list);
+            stream(1, part, cached, [&](const float(&v)[kBatch], int j) { look(v, j, whole, least, list); });
         }
         stream(part, run.batches, once, [&](const float(&v)[kBatch], int j) {
-            if (take(st, v) >= least) look(v, j, least, list);
+            if (take(st, v) >= least || whole) look(v, j, whole, least, list);
         });
+        // Too many: the threads' maxima of the whole run give a better bound.
+        __syncthreads();
+        if (buf.count > kList) {
+            bound = find_bound(buf, any ? order_of(st.m) : 0, a.k);
+            least = bound <= kOrderNegInf ? kLowest : key_value(static_cast<uint64_t>(bound) << 32);
+            if (tail < run.n && last[0] >= least) push(buf, key_of(last[0], first + tail));
+            stream(0, run.batches, cached, [&](const float(&v)[kBatch], int j) { look(v, j, false, least, list); });
+        }
     } else {
         stream(0, run.batches, once, [&](const float(&v)[kBatch], int) { take(st, v); });
     }
@@ -414,10 +477,10 @@ __global__ __launch_bounds__(kThreads, 8) void logprob_rows_kernel(LogprobArgs a
     }
     if constexpr (kTop) {
         select(
-            buf, a.k,
+            buf, a.k, min(a.k, run.n),
             [&](auto&& use) {
                 if (tail < run.n) use(key_of(last[0], first + tail));
-                stream(0, run.batches, cached, [&](const float(&v)[kBatch], int j) { look(v, j, kNegInf, use); });
+                stream(0, run.batches, cached, [&](const float(&v)[kBatch], int j) { look(v, j, true, kNegInf, use); });
             },
             [&](int place, uint64_t key) {
                 if (a.segments == 1) write_top(a, row, place, key, f);
@@ -459,7 +522,7 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
     each([&](uint64_t k) {
         if (static_cast<uint32_t>(k >> 32) >= bound) push(buf, k);
     });
-    select(buf, a.k, each, [&](int place, uint64_t k) { write_top(a, row, place, k, f); });
+    select(buf, a.k, a.k, each, [&](int place, uint64_t k) { write_top(a, row, place, k, f); });
 }
 
 // Segments a row: about as many workgroups as the CUs hold at once, none shorter than kMinSegment, their keys a few a thread. (To the

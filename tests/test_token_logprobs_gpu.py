@@ -157,6 +157,29 @@ def test_more_values_at_the_bound_than_the_list_holds():
 
 
 @pytest.mark.parametrize("tdt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 2049])
+@pytest.mark.parametrize("kind", ["first_masked", "few_left", "rising_first_masked", "ties_first_masked", "equal_last"])
+@pytest.mark.parametrize("V,k", [(40007, 64), (40007, 5), (1021, 64), (1030, 64), (2900, 33)])
+def test_alternatives_behind_masked_values(tdt, rows, kind, V, k):
+    """Rows that begin with masked values, or have fewer than k others: the bound of the row's beginning lets all values through."""
+    from dirktensor_amd import token_logprobs
+
+    print(f"{kind}, {rows} rows of {V} {tdt}", flush=True)
+    i = torch.arange(V, device="cuda")
+    x = logits_of(1, V, 11, torch.float32)[0]
+    lowest = torch.full_like(x, float("-inf"))
+    x = {"first_masked": torch.where(i < V // 2, lowest, x),
+         "few_left": torch.where((i * 7919 % V) % 1000 == 3, x, lowest),
+         "rising_first_masked": torch.where(i < V // 4, lowest, i * (40.0 / V)),
+         "ties_first_masked": torch.where(i < V // 3, lowest, (i % 5).float()),
+         "equal_last": torch.where(i < V - 1500, lowest, torch.ones_like(x))}[kind]
+    x = x.to(tdt)[None].expand(rows, V)
+    tok = torch.full((rows,), int(x[0].argmax()), dtype=torch.int32, device="cuda")
+    r = token_logprobs(x, tok, top_k=k)
+    check(r, x, tok, k)
+
+
+@pytest.mark.parametrize("tdt", [torch.float32, torch.bfloat16])
 def test_masked_and_degenerate_rows(tdt):
     """-inf and the type's lowest value in most places, rows with one token left, without any, with NaN and +inf."""
     from dirktensor_amd import token_logprobs, token_logprobs_backward
