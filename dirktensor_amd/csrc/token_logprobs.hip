@@ -21,10 +21,10 @@
 // row. A row cut into segments leaves (m, l, sum, k keys) of each in the workspace and a second kernel joins them.
 //
 // Measured: 2048 rows of 100352 in fp32, 822 MB, with 5 alternatives 130 us, without 121 (6.3 and 6.8 TB/s; reads past the
-// caches reach 7.0), with 64 163; rows whose first quarter is masked 259, with fifty tokens left 139, of equal values 2140 (they were
-// 1460, 1470 and 1440 for 5 and ten times as long for 64 alternatives when these were selected one after another). 16 rows with 20 alternatives 10 us (49 segments of 8 KB each:
-// the chain from the first load to the sorted keys) and 5.7 for the join. The gradient of the 2048 rows, 1.64 GB moved, 300 us (5.5 TB/s,
-// a large copy 5.2), of 300 rows of 50277 in bf16, 60 MB, 13.6 us (4.4 TB/s).
+// caches reach 7.0), with 64 163. Rows whose first quarter is masked 259, with fifty tokens left 139, of equal values 2140 (selected one
+// after another 5 alternatives took 1460, 1470 and 1440, 64 ten times as long). 16 rows with 20 alternatives 10 us (49 segments of 8 KB
+// each: the chain from the first load to the sorted keys) and 5.7 for the join. The gradient of the 2048 rows, 1.64 GB moved, 300 us
+// (5.5 TB/s, a large copy 5.2), of 300 rows of 50277 in bf16, 60 MB, 13.6 us (4.4 TB/s).
 
 #include "dt_internal.h"
 
