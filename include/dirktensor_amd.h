@@ -390,9 +390,9 @@ int dt_ce_loss(dt_ctx* ctx, const float* logits, const int32_t* tokens, int B, i
  * places, and a query that sees it gets NaN. Rows of zeros are held exactly.
  * The lengths of the slots are host state of the handle: the calls below read and advance them when they are made,
  * whether or not their stream has run. A captured graph repeats the positions that held at its capture, and does not
- * advance them. Calls on one cache must be ordered, like those on a context (dt_ctx); attention calls that only
- * read a cache (as their own or as prefix) may run at the same time, each with a workspace of its own. Destroy a cache
- * before its context.
+ * advance them. Calls on one cache must be ordered, like those on a context (dt_ctx); attention calls on device memory,
+ * which only read a cache (as their own or as prefix), may run at the same time, each with a workspace of its own.
+ * Destroy a cache before its context.
  */
 #define DT_KV_INT8 0
 #define DT_KV_FP8 1
@@ -434,7 +434,7 @@ int dt_kv_cache_read(dt_kv_cache* cache, void* k, void* v, int B, int T, const i
  *             once for the whole batch.
  *   ws      : a device workspace of at least dt_cached_attn_workspace bytes for the same arguments (0: none is needed),
  *             16-byte aligned, not shared with a call that may run at the same time. Ignored with DT_MEM_HOST.
- * 1 <= B <= 256, 1 <= T <= 8192. Deterministic: the same call gives the same bits.
+ * 1 <= B <= 256, 1 <= T <= 8192, B*T*H <= 8388607. Deterministic: the same call gives the same bits.
  */
 int dt_cached_attn_workspace(const dt_kv_cache* cache, int B, int T, int H, int D, const int32_t* slots,
                              const int32_t* counts, const dt_kv_cache* prefix, int prefix_slot, int dtype,

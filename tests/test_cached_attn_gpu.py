@@ -434,6 +434,51 @@ def test_many_query_tiles():
                 assert float((w.softmax_m[0, 0] - r.softmax_m[b, t]).abs().max()) <= 1e-5
 
 
+def test_a_workspace_that_is_too_small_is_refused():
+    import ctypes
+
+    from dirktensor_amd import KVCache, _capi as C
+
+    B, H = 2, 4
+    c = KVCache(400, 3000, H)  # (more slots than a call has rows)
+    fill(c, [3000, 2999], 950, slots=[399, 300])
+    q = randn((B, 1, H, D), 951, torch.bfloat16)
+    r = run(q, c, slots=[399, 300])
+    slots = np.array([399, 300], np.int32)
+    need = ctypes.c_int64()
+    args = (None, None, 0, C.DT_BF16)
+    C.call("dt_cached_attn_workspace", c.handle, B, 1, H, D, slots.ctypes.data, *args, ctypes.byref(need))
+    assert need.value > 0
+    ws = torch.full((need.value + 256,), 77, dtype=torch.uint8, device="cuda")
+    o = torch.zeros_like(q)
+
+    def call(at, n):
+        return C.lib().dt_cached_attn_fwd(c.handle, q.data_ptr(), o.data_ptr(), None, None, B, 1, H, D, H * D, SCALE, 1,
+                                          slots.ctypes.data, None, None, 0, at, n, C.DT_BF16, C.DT_MEM_DEVICE, None)
+
+    for at, n, msg in ((None, need.value, "the workspace has 0"), (ws.data_ptr(), need.value - 1, "the workspace has"),
+                       (ws.data_ptr() + 8, need.value, "aligned")):
+        assert call(at, n) == C.DT_ERR_INVALID_ARG and msg in C.lib().dt_last_error().decode()
+    assert not bool(o.any())
+    assert call(ws.data_ptr(), need.value) == C.DT_OK
+    torch.cuda.synchronize()
+    assert torch.equal(o, r.output) and bool((ws[need.value:] == 77).all())
+
+
+def test_more_rows_than_a_call_takes():
+    from dirktensor_amd import DTError, KVCache, cached_attention
+
+    c = KVCache(300, 4, 1)
+    x = randn((256, 2, 1, D), 960)
+    c.append(x, x)
+    run(x[:, -1:], c)
+    with pytest.raises(DTError, match="B=257"):
+        cached_attention(randn((257, 1, 1, D), 961), c, SCALE)
+    with pytest.raises(DTError, match="B=257"):
+        c.append(randn((257, 1, 1, D), 962), randn((257, 1, 1, D), 963))
+    assert c.lengths.tolist() == [2] * 256 + [0] * 44
+
+
 def test_a_closed_context():
     from dirktensor_amd import Context, KVCache, cached_attention
 
