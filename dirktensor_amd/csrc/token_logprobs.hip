@@ -11,10 +11,10 @@
 //
 // Forward: a workgroup of 256 threads streams a row (or, where there are few rows, a segment of one) with 16-byte loads;
 // a thread keeps its own running maximum, sum and weighted sum, so the loop has no exchange between lanes, and the statistics
-// meet once at the end. The alternatives cost no second pass: after the first fifth of the row the k-th largest of the
-// threads' maxima is a bound that at least k values reach. The threads whose maximum reaches it look at their share of that fifth again
-// (from L2), and the rest of the row is compared with the bound as it streams by, one comparison for 16 values; what reaches
-// it (about 5 k values) is collected in LDS, and each takes the place that the number of larger ones gives it. Keys are
+// meet once at the end. The alternatives cost no second pass: after the first fifth of the row (more for many) the k-th largest
+// of the threads' maxima is a bound that at least k values reach. The threads whose maximum reaches it look at their share of that part
+// again (from the caches), and the rest of the row is compared with the bound as it streams by, one comparison for 16 values; what reaches
+// it (about 5 k values at most) is collected in LDS, and each takes the place that the number of larger ones gives it. Keys are
 // (value, index) pairs, so no two are equal, ties go to the lower index and the order of the collection does not matter. Where more values
 // reach the bound than the list holds (rows that rise, or begin with masked values) the maxima of the whole row give another and the
 // row is read once more; where that leaves too many as well (equal values) the k-th key is found digit by digit in passes over the
@@ -22,8 +22,8 @@
 //
 // Measured: 2048 rows of 100352 in fp32, 822 MB, with 5 alternatives 130 us, without 121 (6.3 and 6.8 TB/s; reads past the
 // caches reach 7.0), with 64 163. Rows whose first quarter is masked 259, with fifty tokens left 139, of equal values 2140 (selected one
-// after another 5 alternatives took 1460, 1470 and 1440, 64 ten times as long). 16 rows with 20 alternatives 10 us (49 segments of 8 KB
-// each: the chain from the first load to the sorted keys) and 5.7 for the join. The gradient of the 2048 rows, 1.64 GB moved, 300 us
+// after another 5 alternatives took 1460, 1470 and 1440, 64 ten times as long). 16 rows with 20 alternatives 13.2 us, both launches
+// (25 segments of 16 KB each: the chains from the first load to the sorted keys). The gradient of the 2048 rows, 1.64 GB moved, 300 us
 // (5.5 TB/s, a large copy 5.2), of 300 rows of 50277 in bf16, 60 MB, 13.6 us (4.4 TB/s).
 
 #include "dt_internal.h"
@@ -45,8 +45,9 @@ constexpr int kThreads = 256, kWaves = 4;
 constexpr int kMaxTop = 64;
 constexpr int kList = 1024;          // values that may reach the bound before the selection goes one by one
 constexpr uint32_t kOrderNegInf = 0x007fffffu;  // order_of(-inf): the least there is
+constexpr int kBoundBytes = 96 << 10;  // of a run that gives the bound, where more than a fifth of it does
 constexpr int kBatch = 16;           // values a thread takes at a time
-constexpr int kMinSegment = 2048;    // values of a segment at least
+constexpr int kMinSegment = 4096;    // values of a segment at least
 constexpr int kJoinKeys = 8;         // keys of a row's segments that a thread of the second kernel takes at most
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLog2eLo = 1.92596303e-8f;  // log2 e - kLog2e
@@ -432,8 +433,13 @@ __global__ __launch_bounds__(kThreads, 8) void logprob_rows_kernel(LogprobArgs a
     const auto cached = [&](int p) { return run.load(p); };
     const auto once = [&](int p) { return run.load_once(p); };
     if constexpr (kTop) {
-        // (runs of a few batches give their bound from all of them; the first batch stays in registers)
-        const int part = run.batches <= 4 ? run.batches : (run.batches + 4) / 5;
+        // How much of the run gives the bound: more of it leaves fewer values to list, but is looked at twice, which the caches must
+        // hold. From one to two (fp32) or three (bf16) fifths, us: 2048 rows of 100352 in bf16, 64 alternatives, 123 and 105, of 32000 in
+        // fp32 67 and 63; past kBoundBytes 159 and 188 (100352 in fp32, three fifths). Runs of a few batches give it from all of them;
+        // the first batch stays in registers.
+        const int fifths = kBf16 ? (a.k > 32 ? 3 : a.k > 8 ? 2 : 1) : (a.k > 32 ? 2 : 1);
+        const int fifth = (run.batches + 4) / 5, most = kBoundBytes / (kThreads * kBatch * R::kEs);
+        const int part = run.batches <= 4 ? run.batches : max(fifth, min((run.batches * fifths + 4) / 5, most));
         float v0[kBatch];
         stream(0, min(part, 1), cached, [&](const float(&v)[kBatch], int) {
 #pragma unroll
@@ -525,11 +531,15 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LogprobArgs a) {
     select(buf, a.k, a.k, each, [&](int place, uint64_t k) { write_top(a, row, place, k, f); });
 }
 
-// Segments a row: about as many workgroups as the CUs hold at once, none shorter than kMinSegment, their keys a few a thread. (To the
-// nearest: 2047 rows of 100352 in fp32 121 us whole, 127 in two segments and their join; 1400 87 and 89, 1100 in two 74.)
+// Segments a row: about four workgroups a CU, none shorter than kMinSegment, or twice that where there are as many workgroups or many
+// keys, which each segment leaves k of; their keys a few a thread. fp32 rows of 100352, us: 1000 of them, 20 alternatives, in one
+// segment 72, two 80; 300 in three 35, in seven 40; 16 in segments of 4096 13.2, of 2048 15.1, of 8192 14.3, with 64 alternatives 24, 26
+// and 17.
 void cut(int64_t rows, int V, int k, int* segments, int* seg_len) {
-    constexpr int64_t kTarget = 2048;
-    int64_t s = std::min<int64_t>((kTarget + rows / 2) / rows, (V + kMinSegment - 1) / kMinSegment);
+    constexpr int64_t kTarget = 1024, kCus = 256;
+    const bool longer = k > 32 || rows * ((V + kMinSegment - 1) / kMinSegment) >= 4 * kCus;
+    const int least = longer ? 2 * kMinSegment : kMinSegment;
+    int64_t s = std::min<int64_t>((kTarget + rows / 2) / rows, (V + least - 1) / least);
     s = std::min<int64_t>(s, kThreads);
     if (k > 0) s = std::min<int64_t>(s, kJoinKeys * kThreads / k);
     s = std::max<int64_t>(s, 1);
