@@ -66,13 +66,16 @@ constexpr int kBufferDword3 = 0x00020000;  // raw buffer, 32-bit data format (gf
 // blocks in flight a wave: what 256 registers a lane hold, which leave two workgroups a CU
 constexpr int stages(int format, bool f32, int qt) { return format == DT_KV_BF16 || f32 || qt > 1 ? 1 : 2; }
 
-// The batch rows, by value in the kernel's arguments.
-struct AttnRows {
-    int32_t len[kMaxRaggedBatch];       // tokens held
-    int32_t cum[kMaxRaggedBatch];       // places of one head in the list before this row's, all query tiles
-    uint16_t slot[kMaxRaggedBatch];
-    uint16_t cnt[kMaxRaggedBatch];      // query tokens
+// The batch rows, by value in the kernel's arguments (kN places, 32 where these are enough: eager calls at 16 heads in int8, one
+// sequence of 1000 10.8 us with 256 and 10.4 with 32, 8 of 200 behind 2000 14.6 and 13.7).
+template <int kN>
+struct AttnRowsOf {
+    int32_t len[kN];       // tokens held
+    int32_t cum[kN];       // places of one head in the list before this row's, all query tiles
+    uint16_t slot[kN];
+    uint16_t cnt[kN];      // query tokens
 };
+using AttnRows = AttnRowsOf<kMaxRaggedBatch>;
 
 struct CachedAttnArgs {
     KvView own, pre;
@@ -481,8 +484,8 @@ struct Stretch {
 
 // The waves' results meet: a thread sums four values of a row over the key waves, scaled to their common maximum. A wave that
 // has a stretch of its own does so for itself.
-template <bool kF32, int kQT>
-__device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRows& rows, const Work& w, const Shared<kQT>& sh) {
+template <bool kF32, int kQT, int kRows>
+__device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRowsOf<kRows>& rows, const Work& w, const Shared<kQT>& sh) {
     const int tid = thread_here(), wave = w.apart ? __builtin_amdgcn_readfirstlane(tid >> 6) : 0;
     const int wk = w.apart ? 1 : kWaves >> w.wl, tiles = w.apart ? kQT : kQT << w.wl, threads = w.apart ? 64 : 64 * kWaves;
     const int row0 = w.tile * 16 * tiles, nrows = min((w.prefix ? a.B : 1) * a.T * a.G - row0, 16 * tiles);
@@ -522,17 +525,17 @@ __device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRo
 }
 
 // kQT, kPreQT: query tiles a wave for a batch row's own keys and for the prefix's
-template <int kFormat, bool kF32, bool kOnce, int kQT, int kPreQT>
-__global__ __launch_bounds__(64 * kWaves, 2) void cached_attn_kernel(CachedAttnArgs a, AttnRows rows) {
+template <int kFormat, bool kF32, bool kOnce, int kQT, int kPreQT, int kRows>
+__global__ __launch_bounds__(64 * kWaves, 2) void cached_attn_kernel(CachedAttnArgs a, AttnRowsOf<kRows> rows) {
     __shared__ __align__(16) union {
         Shared<kQT> own;
         Shared<kPreQT> pre;
     } sh;
-    __shared__ AttnRows rl;
+    __shared__ AttnRowsOf<kRows> rl;
     // All arguments in one trip to their memory, in place of one for each dependent use: the batch rows into LDS (all of
     // them, so no length is waited for), the rest into scalar registers or at least the scalar cache.
-    static_assert(64 * kWaves >= kMaxRaggedBatch, "one batch row a thread");
-    if (threadIdx.x < kMaxRaggedBatch) {
+    static_assert(64 * kWaves >= kRows, "one batch row a thread");
+    if (threadIdx.x < kRows) {
         rl.len[threadIdx.x] = rows.len[threadIdx.x];
         rl.cum[threadIdx.x] = rows.cum[threadIdx.x];
         rl.slot[threadIdx.x] = rows.slot[threadIdx.x];
@@ -590,7 +593,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cached_attn_kernel(CachedAttnA
         st.begin(a, w);
         st.attend(a.scale, sh.pre);
         __syncthreads();
-        join_waves<kF32, kPreQT>(a, rl, w, sh.pre);
+        join_waves<kF32, kPreQT, kRows>(a, rl, w, sh.pre);
         return;
     }
     {
@@ -619,7 +622,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cached_attn_kernel(CachedAttnA
             // the last batch row that begins at or before this place (rows without steps begin where the next one does)
             int below = 0;
 #pragma unroll
-            for (int i = 0; i < kMaxRaggedBatch / 64; ++i) {
+            for (int i = 0; i < (kRows + 63) / 64; ++i) {
                 const int at = i * 64 + (threadIdx.x & 63);
                 if (i * 64 < a.B) below += __popcll(__ballot(at < a.B && rl.cum[at] <= in_head));
             }
@@ -666,7 +669,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cached_attn_kernel(CachedAttnA
         if (w.apart) {  // (in its own part of LDS: a wave's accesses of it are in order)
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            join_waves<kF32, kQT>(a, rl, w, sh.own);
+            join_waves<kF32, kQT, kRows>(a, rl, w, sh.own);
             return;
         }
         const bool more = s + a.lead < end;
@@ -675,15 +678,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cached_attn_kernel(CachedAttnA
             st.begin(a, w);
         }
         __syncthreads();
-        join_waves<kF32, kQT>(a, rl, done, sh.own);
+        join_waves<kF32, kQT, kRows>(a, rl, done, sh.own);
         if (!more) return;
         __syncthreads();
     }
 }
 
 // Joins a row's partial results: one workgroup a row, 32 threads across the 128 values, eight runs of parts.
-template <bool kF32>
-__global__ __launch_bounds__(kJoinThreads) void cached_attn_join_kernel(CachedAttnArgs a, AttnRows rows) {
+template <bool kF32, int kRows>
+__global__ __launch_bounds__(kJoinThreads) void cached_attn_join_kernel(CachedAttnArgs a, AttnRowsOf<kRows> rows) {
     __shared__ float red[kJoinThreads / 64];
     __shared__ float lred[8];
     __shared__ __align__(16) float obuf[8][kD];
@@ -840,7 +843,8 @@ int64_t make_plan(CachedAttnArgs& a, AttnRows& rows, int format, bool f32, bool*
     return *join ? all_rows * heads * a.parts * (kD + 2) * static_cast<int64_t>(sizeof(float)) : 0;
 }
 
-int launch(const CachedAttnArgs& a, const AttnRows& rows, bool join, int format, int dtype, hipStream_t s) {
+template <int kRows>
+int launch_rows(const CachedAttnArgs& a, const AttnRowsOf<kRows>& rows, bool join, int format, int dtype, hipStream_t s) {
     const int64_t groups = static_cast<int64_t>(a.own_groups) + a.pre_groups;
     if (groups > 0x7fffff) return set_error(DT_ERR_UNSUPPORTED, "the call needs %lld workgroups", (long long)groups);
     const bool f32 = dtype != DT_BF16;
@@ -851,8 +855,8 @@ int launch(const CachedAttnArgs& a, const AttnRows& rows, bool join, int format,
             constexpr int F = decltype(format_)::value;
             constexpr bool M = decltype(f32_)::value;
             const auto go_as = [&](auto once_, auto qt_, auto pre_qt_) {
-                hipLaunchKernelGGL((cached_attn_kernel<F, M, decltype(once_)::value, decltype(qt_)::value, decltype(pre_qt_)::value>), g, t,
-                                   0, s, a, rows);
+                hipLaunchKernelGGL((cached_attn_kernel<F, M, decltype(once_)::value, decltype(qt_)::value, decltype(pre_qt_)::value, kRows>),
+                                   g, t, 0, s, a, rows);
             };
             constexpr std::integral_constant<int, 1> one;
             constexpr std::integral_constant<int, 2> two;
@@ -879,10 +883,20 @@ int launch(const CachedAttnArgs& a, const AttnRows& rows, bool join, int format,
     }
     if (!join) return DT_OK;
     const dim3 g(static_cast<unsigned>(static_cast<int64_t>(a.B) * a.T * a.H)), t(kJoinThreads);
-    if (f32) hipLaunchKernelGGL((cached_attn_join_kernel<true>), g, t, 0, s, a, rows);
-    else hipLaunchKernelGGL((cached_attn_join_kernel<false>), g, t, 0, s, a, rows);
+    if (f32) hipLaunchKernelGGL((cached_attn_join_kernel<true, kRows>), g, t, 0, s, a, rows);
+    else hipLaunchKernelGGL((cached_attn_join_kernel<false, kRows>), g, t, 0, s, a, rows);
     DT_HIP_TRY(hipGetLastError());
     return DT_OK;
+}
+
+int launch(const CachedAttnArgs& a, const AttnRows& rows, bool join, int format, int dtype, hipStream_t s) {
+    if (a.B > kFewRows) return launch_rows(a, rows, join, format, dtype, s);
+    AttnRowsOf<kFewRows> few;
+    std::copy_n(rows.len, kFewRows, few.len);
+    std::copy_n(rows.cum, kFewRows, few.cum);
+    std::copy_n(rows.slot, kFewRows, few.slot);
+    std::copy_n(rows.cnt, kFewRows, few.cnt);
+    return launch_rows(a, few, join, format, dtype, s);
 }
 
 // what dt_cached_attn_fwd and its workspace query check alike; fills rows

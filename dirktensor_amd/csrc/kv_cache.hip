@@ -203,8 +203,8 @@ __device__ __forceinline__ float* scale_of(uint8_t* block, bool v, int kk) {
     return reinterpret_cast<float*>(block + kv_scale_at(kFormat)) + (v ? kKvBlock : 0) + kk;
 }
 
-template <int kFormat, bool kBf16>
-__global__ __launch_bounds__(kThreads) void kv_append_kernel(KvMoveArgs a, KvRows rows) {
+template <int kFormat, bool kBf16, int kRows>
+__global__ __launch_bounds__(kThreads) void kv_append_kernel(KvMoveArgs a, KvRowsOf<kRows> rows) {
     constexpr int kEs = kv_elem_bytes(kFormat), kWords = 4 * kEs, kTensor = kv_tensor_bytes(kFormat);
     __shared__ __align__(16) uint8_t vbuf[kTensor / kKvRun * kRunLds];
     const int b = blockIdx.z, h = blockIdx.y;
@@ -263,8 +263,8 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvMoveArgs a, KvRow
 }
 
 // Few tokens a sequence: a wave takes one row of K (even) or V (odd), lane i its values 2 i and 2 i + 1.
-template <int kFormat, bool kBf16>
-__global__ __launch_bounds__(kThreads) void kv_append_rows_kernel(KvMoveArgs a, KvRows rows) {
+template <int kFormat, bool kBf16, int kRows>
+__global__ __launch_bounds__(kThreads) void kv_append_rows_kernel(KvMoveArgs a, KvRowsOf<kRows> rows) {
     const int lane = threadIdx.x & 63, unit = blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = blockIdx.z, t = blockIdx.y, h = unit >> 1;
     const bool v = unit & 1;
@@ -303,8 +303,8 @@ __global__ __launch_bounds__(kThreads) void kv_append_rows_kernel(KvMoveArgs a, 
     }
 }
 
-template <int kFormat, bool kBf16>
-__global__ __launch_bounds__(kThreads) void kv_read_kernel(KvMoveArgs a, KvRows rows) {
+template <int kFormat, bool kBf16, int kRows>
+__global__ __launch_bounds__(kThreads) void kv_read_kernel(KvMoveArgs a, KvRowsOf<kRows> rows) {
     constexpr int kEs = kv_elem_bytes(kFormat), kWords = 4 * kEs, kTensor = kv_tensor_bytes(kFormat);
     __shared__ __align__(16) uint8_t vbuf[kTensor / kKvRun * kRunLds];
     const int b = blockIdx.z, h = blockIdx.y;
@@ -348,8 +348,8 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(KvMoveArgs a, KvRows 
     }
 }
 
-template <bool kAppend>
-int launch_move(const KvMoveArgs& a, const KvRows& rows, int B, int format, int dtype, hipStream_t s) {
+template <bool kAppend, int kRows>
+int launch_rows(const KvMoveArgs& a, const KvRowsOf<kRows>& rows, int B, int format, int dtype, hipStream_t s) {
     int blocks = 0, tokens = 0;  // of the batch row that touches most
     for (int b = 0; b < B; ++b)
         if (rows.cnt[b] > 0) {
@@ -366,10 +366,10 @@ int launch_move(const KvMoveArgs& a, const KvRows& rows, int B, int format, int 
 #define DT_KV_GO(F, M)                                                                                            \
     do {                                                                                                         \
         if constexpr (kAppend) {                                                                                 \
-            if (few) hipLaunchKernelGGL((kv_append_rows_kernel<F, M>), grid, block, 0, s, a, rows);              \
-            else hipLaunchKernelGGL((kv_append_kernel<F, M>), grid, block, 0, s, a, rows);                       \
+            if (few) hipLaunchKernelGGL((kv_append_rows_kernel<F, M, kRows>), grid, block, 0, s, a, rows);              \
+            else hipLaunchKernelGGL((kv_append_kernel<F, M, kRows>), grid, block, 0, s, a, rows);                       \
         } else {                                                                                                 \
-            hipLaunchKernelGGL((kv_read_kernel<F, M>), grid, block, 0, s, a, rows);                              \
+            hipLaunchKernelGGL((kv_read_kernel<F, M, kRows>), grid, block, 0, s, a, rows);                              \
         }                                                                                                        \
     } while (0)
 #define DT_KV_GO2(F)                                                                                             \
@@ -384,6 +384,16 @@ int launch_move(const KvMoveArgs& a, const KvRows& rows, int B, int format, int 
 #undef DT_KV_GO
     DT_HIP_TRY(hipGetLastError());
     return DT_OK;
+}
+
+template <bool kAppend>
+int launch_move(const KvMoveArgs& a, const KvRows& rows, int B, int format, int dtype, hipStream_t s) {
+    if (B > kFewRows) return launch_rows<kAppend>(a, rows, B, format, dtype, s);
+    KvRowsOf<kFewRows> few;
+    std::copy_n(rows.slot, kFewRows, few.slot);
+    std::copy_n(rows.len, kFewRows, few.len);
+    std::copy_n(rows.cnt, kFewRows, few.cnt);
+    return launch_rows<kAppend>(a, few, B, format, dtype, s);
 }
 
 void free_cache(dt_kv_cache* c) {
@@ -529,7 +539,7 @@ int dt_kv_cache_append(dt_kv_cache* cache, const void* k, const void* v, int B, 
     const int64_t dm = static_cast<int64_t>(cache->heads) * DT_HEAD_DIM;
     if (ldk < dm || ldv < dm)
         return set_error(DT_ERR_INVALID_ARG, "row strides %lld, %lld are below %lld", (long long)ldk, (long long)ldv, (long long)dm);
-    KvRows rows;
+    KvRows rows{};
     DT_TRY(kv_check_slots(cache, B, slots, true, &rows));
     DT_TRY(kv_check_counts(B, T, counts, &rows));
     for (int b = 0; b < B; ++b) {
@@ -568,7 +578,7 @@ int dt_kv_cache_read(dt_kv_cache* cache, void* k, void* v, int B, int T, const i
     if (mem == DT_MEM_DEVICE && (!aligned16(k) || !aligned16(v)))
         return set_error(DT_ERR_INVALID_ARG, "device k/v must be 16-byte aligned");
     if (!cache) return set_error(DT_ERR_INVALID_ARG, "cache is NULL");
-    KvRows rows;
+    KvRows rows{};
     DT_TRY(kv_check_slots(cache, B, slots, false, &rows));
     for (int b = 0; b < B; ++b) {
         rows.len[b] = starts ? starts[b] : 0;
