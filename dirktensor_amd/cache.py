@@ -21,6 +21,7 @@ from typing import Optional
 import numpy as np
 
 from . import _capi as C
+from ._workspace import kept_workspace, new_workspace
 from .attention import Context, FlashAttentionResult, _is_torch, _mode_of, _stream_of, default_context, torch
 
 _FORMATS = {"int8": C.DT_KV_INT8, "fp8": C.DT_KV_FP8, "bf16": C.DT_KV_BF16}
@@ -188,17 +189,24 @@ def cached_attention(Q, cache: KVCache, scale: float, causal: bool = True, *, sl
     if _is_torch(Q):
         cache._check_device(Q)
         Q, ldq = _rows_of(Q)
-        nbytes = ctypes.c_int64()
-        C.call("dt_cached_attn_workspace", cache._live(), B, T, H, D, s_p, n_p, pre, int(prefix_slot), dtype,
-               ctypes.byref(nbytes))
-        # a workspace of the call's own: torch's allocator keeps it for this stream, or for the graph being captured
-        ws = Q.new_empty(nbytes.value, dtype=torch.uint8) if nbytes.value else None
+        stream = _stream_of(Q)
         O = Q.new_empty((B, T, H, D))
         m = Q.new_empty((B, T, H), dtype=torch.float32)
         l = torch.empty_like(m)
-        C.call("dt_cached_attn_fwd", cache._live(), Q.data_ptr(), O.data_ptr(), m.data_ptr(), l.data_ptr(), B, T, H, D,
-               ldq, float(scale), int(bool(causal)), s_p, n_p, pre, int(prefix_slot),
-               ws.data_ptr() if ws is not None else None, nbytes.value, dtype, C.DT_MEM_DEVICE, _stream_of(Q))
+        handle, q_p, o_p, m_p, l_p = cache._live(), Q.data_ptr(), O.data_ptr(), m.data_ptr(), l.data_ptr()
+
+        def attend(ws_p, nbytes):
+            return C.lib().dt_cached_attn_fwd(handle, q_p, o_p, m_p, l_p, B, T, H, D, ldq, float(scale), int(bool(causal)),
+                                              s_p, n_p, pre, int(prefix_slot), ws_p, nbytes, dtype, C.DT_MEM_DEVICE, stream)
+
+        kept = kept_workspace(cache.ctx.device, stream)
+        if kept is not None and attend(kept[0], kept[1]) == C.DT_OK:
+            return FlashAttentionResult(O, m, l)
+        # none yet, too small, or another error, which is found again
+        need = ctypes.c_int64()
+        C.call("dt_cached_attn_workspace", handle, B, T, H, D, s_p, n_p, pre, int(prefix_slot), dtype, ctypes.byref(need))
+        ws = new_workspace(Q, cache.ctx.device, stream, need.value) if kept is None or need.value > kept[1] else kept
+        C.check(attend(ws[0], ws[1]))
         return FlashAttentionResult(O, m, l)
     Qh = np.ascontiguousarray(Q)
     O = np.empty_like(Qh)

@@ -15,6 +15,7 @@ from typing import Optional
 import numpy as np
 
 from . import _capi as C
+from ._workspace import kept_workspace, new_workspace
 from .attention import Context, _is_torch, _mode_of, _stream_of, default_context, torch
 
 
@@ -93,17 +94,17 @@ def _rows(logits):
     return logits, _two_strides(logits.shape[:-1], logits.stride()[:-1])
 
 
-_workspace: dict = {}  # bytes by (B, T, V, top_k): they follow from the sizes alone
+_needs: dict = {}  # bytes by (B, T, V, top_k): they follow from the sizes alone
 
 
 def _workspace_bytes(B: int, T: int, V: int, k: int) -> int:
-    n = _workspace.get((B, T, V, k))
+    n = _needs.get((B, T, V, k))
     if n is None:
         out = ctypes.c_int64()
         C.call("dt_token_logprobs_workspace", B, T, V, k, ctypes.byref(out))
-        if len(_workspace) >= 4096:
-            _workspace.clear()
-        n = _workspace[(B, T, V, k)] = out.value
+        if len(_needs) >= 4096:
+            _needs.clear()
+        n = _needs[(B, T, V, k)] = out.value
     return n
 
 
@@ -123,14 +124,18 @@ def token_logprobs(logits, tokens, *, top_k: int = 0, ignore_index: Optional[int
     if _is_torch(logits):
         x, (B, T, ldb, ldt) = _rows(logits)
         nbytes = _workspace_bytes(B, T, V, k)
-        # a workspace of the call's own: torch's allocator keeps it for this stream, or for the graph being captured
-        ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        stream = _stream_of(x)
+        ws = (None, 0)
+        if nbytes:
+            ws = kept_workspace(ctx.device, stream)
+            if ws is None or ws[1] < nbytes:
+                ws = new_workspace(x, ctx.device, stream, nbytes)
         lp, ent, m, l = x.new_empty((4, *lead), dtype=torch.float32).unbind(0)
         idx = x.new_empty((*lead, k), dtype=torch.int32) if k else None
         top = torch.empty_like(idx, dtype=torch.float32) if k else None
         C.call("dt_token_logprobs", ctx.handle, x.data_ptr(), tok_p, B, T, V, ldb, ldt, tok_bytes, ign, k, lp.data_ptr(),
                ent.data_ptr(), m.data_ptr(), l.data_ptr(), idx.data_ptr() if k else None, top.data_ptr() if k else None,
-               ws.data_ptr() if ws is not None else None, nbytes, dtype, C.DT_MEM_DEVICE, _stream_of(x))
+               ws[0], ws[1], dtype, C.DT_MEM_DEVICE, stream)
         return TokenLogprobs(lp, ent, m, l, idx, top, ignore_index)
     x = np.ascontiguousarray(logits)
     rows = int(np.prod(lead, dtype=np.int64))

@@ -107,3 +107,80 @@ def test_answers_to_one_prompt(fmt):
     attn.check(cached_attention(q, own, scale, prefix=shared), attn.reference(q, own, True, range(N), [S] * N, shared, 0, scale), torch.float32)
     for o, y0 in zip(again, logits[S // 2:]):
         assert torch.equal(o.view(N, H * D) @ w, y0)
+
+
+def test_threads_streams_and_graphs_beside_each_other():
+    """Attention and scores that need workspaces, from several threads on one stream, on streams of their own, and replayed from
+    graphs beside them: each gets its own result."""
+    import threading
+
+    from dirktensor_amd import KVCache, cached_attention, token_logprobs
+
+    B, H, L, V = 3, 4, 3000, 50021
+    c = KVCache(B, L, H)
+    c.append(randn((B, L, H, D), 30), randn((B, L, H, D), 31))
+    qs = [randn((B, 1, H, D), 32 + i) for i in range(4)]
+    xs = [randn((2 + i, V), 40 + i, 3.0) for i in range(4)]
+    toks = [torch.arange(len(x), device="cuda") for x in xs]
+    call = lambda i: (cached_attention(qs[i], c, 0.09).output, token_logprobs(xs[i], toks[i], top_k=9))
+    want = [call(i) for i in range(4)]
+    torch.cuda.synchronize()
+
+    def same(got, i):
+        assert torch.equal(got[0], want[i][0]) and torch.equal(got[1].top_index, want[i][1].top_index)
+        assert torch.equal(got[1].logprob, want[i][1].logprob) and torch.equal(got[1].top_logprob, want[i][1].top_logprob)
+
+    side = torch.cuda.Stream()
+    graphs = []
+    for i in (0, 1):  # (captured on one stream: they may not share a workspace with each other or with eager calls there)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            r = call(i)
+        graphs.append((g, r))
+    replayers = [torch.cuda.Stream() for _ in graphs]
+    got, errors = [[] for _ in range(4)], []
+
+    def work(i, stream):
+        try:
+            with torch.cuda.stream(stream):
+                for _ in range(40):
+                    got[i].append(call(i))
+        except Exception as e:  # (shown below)
+            errors.append(e)
+
+    streams = [torch.cuda.default_stream()] * 2 + [side, torch.cuda.Stream()]
+    threads = [threading.Thread(target=work, args=(i, streams[i])) for i in range(4)]
+    for t in threads:
+        t.start()
+    for _ in range(10):
+        for (g, _), s in zip(graphs, replayers):
+            with torch.cuda.stream(s):
+                g.replay()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for i in range(4):
+        assert len(got[i]) == 40
+        for r in got[i]:
+            same(r, i)
+    for i, (_, r) in enumerate(graphs):
+        same(r, i)
+
+
+def test_workspaces_grow_with_the_call():
+    from dirktensor_amd import KVCache, cached_attention
+
+    c = KVCache(64, 6000, 8)
+    x = randn((64, 6000, 8, D), 60).bfloat16()
+    c.append(x, x)
+    torch.cuda.synchronize()  # (calls on one cache are ordered by their caller)
+    stream = torch.cuda.Stream()  # (nothing kept for it yet)
+    with torch.cuda.stream(stream):
+        for B, T in ((1, 1), (16, 2), (64, 1), (2, 1), (5, 40), (64, 9)):
+            q = randn((B, T, 32, D), 61).bfloat16()
+            r, again = cached_attention(q, c, 0.09), cached_attention(q, c, 0.09)
+            assert torch.equal(r.output, again.output) and bool(torch.isfinite(r.output.float()).all())
+            for b in (0, B - 1):
+                attn.check(type(r)(r.output[b:b + 1], r.softmax_m[b:b + 1], r.softmax_l[b:b + 1]),
+                           attn.reference(q[b:b + 1], c, True, [b], [T], None, 0, 0.09), torch.bfloat16)
