@@ -27,19 +27,27 @@ from .attention import Context, FlashAttentionResult, _is_torch, _mode_of, _stre
 _FORMATS = {"int8": C.DT_KV_INT8, "fp8": C.DT_KV_FP8, "bf16": C.DT_KV_BF16}
 
 
+def _address(a: np.ndarray) -> int:
+    """Where a contiguous array's values lie (``a.ctypes`` builds an object for that)."""
+    try:
+        return ctypes.addressof(ctypes.c_char.from_buffer(a))
+    except (TypeError, ValueError):  # read-only or empty
+        return a.ctypes.data
+
+
 def _per_row(x, B: int, name: str):
     """A per-row argument as B int32 values in host memory and their address (None: NULL)."""
     if x is None:
         return None, None
     if type(x) is np.ndarray and x.dtype == np.int32 and x.shape == (B,) and x.flags.c_contiguous:
-        return x, x.ctypes.data
+        return x, _address(x)
     a = np.asarray(x.cpu() if _is_torch(x) else x)
     if a.dtype.kind not in "iu" or a.shape != (B,):
         raise ValueError(f"{name} must be {B} whole numbers, got {a.dtype} of shape {a.shape}")
     if a.size and (a.max() > 0x7FFFFFFF or a.min() < -0x80000000):
         raise ValueError(f"{name} holds a number beyond 32 bits")
     a = np.ascontiguousarray(a, dtype=np.int32)
-    return a, a.ctypes.data
+    return a, _address(a)
 
 
 def _rows_of(x):
