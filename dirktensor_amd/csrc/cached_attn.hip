@@ -801,9 +801,11 @@ int64_t make_plan(CachedAttnArgs& a, AttnRows& rows, int format, bool f32, bool*
         const int64_t pre_steps = (a.pre_len + unit - 1) / unit, per_chunk = static_cast<int64_t>(a.pre_tiles) * heads;
         const int64_t own_work = (all + kLead * rows_held * a.own_tiles * heads) >> a.apart;
         const int64_t groups = std::max<int64_t>(kResident * (pre_steps * per_chunk) / (pre_steps * per_chunk + own_work), 1);
-        // but at least four steps each, 256 keys where those leave 64 rows of partial results: these weigh as much as the keys
+        // but at least three steps each, 192 keys where those leave 64 rows of partial results: these weigh as much as the keys (16 heads
+        // in fp8, us for two, three and four: 12 x 5 tokens behind 2777 16.0, 15.9 and 16.3, 8 tokens behind 1000 8.7, 8.9 and 9.5; in
+        // exact mode, int8, 12 x 5 behind 2777 23.5, 19.9 and 21.3)
         const int64_t chunks = std::max<int64_t>(1, groups / per_chunk);
-        const int64_t each = std::max<int64_t>(take == 64 ? 256 / unit : 4, (pre_steps + chunks - 1) / chunks);
+        const int64_t each = std::max<int64_t>(take == 64 ? 192 / unit : 3, (pre_steps + chunks - 1) / chunks);
         a.pre_chunk = static_cast<int>(std::min(each, pre_steps) * unit);
         a.pre_parts = (a.pre_len + a.pre_chunk - 1) / a.pre_chunk;
         a.pre_groups = static_cast<int>(a.pre_parts * per_chunk);
