@@ -470,7 +470,8 @@ int dt_token_logprobs(dt_ctx* ctx, const void* logits, const void* tokens, int B
 /*
  * Its gradient: d_logprob [B, T] and d_entropy [B, T] (or NULL: 0) fp32 -> d_logits, B x T rows in dtype at b*ldb_out +
  * t*ldt_out, rows not overlapping: g (1[j = token] - p_j) - h p_j (log p_j + entropy). m, l and (with d_entropy) entropy are
- * the forward's. d_logits may be logits themselves (the same address and strides). The alternatives have no gradient.
+ * the forward's. d_logits may be logits themselves (the same address and strides). The alternatives have no gradient. A p_j below
+ * fp32's normal numbers (2^-126) counts as 0.
  */
 int dt_token_logprobs_bwd(dt_ctx* ctx, const float* d_logprob, const float* d_entropy, const void* logits,
                           const void* tokens, const float* m, const float* l, const float* entropy, int B, int T, int V,
