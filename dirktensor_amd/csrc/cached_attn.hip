@@ -61,6 +61,13 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kSlack = 8.0f;
+// O before its division by l exceeds the values by up to 2^kSlack times the number of keys, and so fp32's range where the values lie
+// near its end. A wave whose O reaches kLimit (or has left the range) does its stretch once more with V's scales times kLower: O is
+// then at most 2^8 (a probability) 2^128 (a value) 2^21 (keys) 2^-32 = 2^125, and such results meet others, times kLower too. What
+// that loses are values below 2^-70, in a wave that has others above 2^70. (The check and the way back cost 0.4 us of the
+// 11 of one sequence of 1000 in bf16 and 0.8 of the 14 of 4 of 1500 in exact mode; 32 of 8192 in fp8 take no longer.)
+constexpr float kLimit = 0x1p100f;
+constexpr float kLower = 0x1p-32f, kRaise = 0x1p32f;
 constexpr int kBufferDword3 = 0x00020000;  // raw buffer, 32-bit data format (gfx9 family)
 
 // blocks in flight a wave: what 256 registers a lane hold, which leave two workgroups a CU
@@ -84,7 +91,7 @@ struct CachedAttnArgs {
     float* m;  // nullable
     float* l;  // nullable
     float* part_o;   // [row][parts][kD]
-    float* part_ml;  // [row][parts][2]
+    float* part_ml;  // [row][parts][2]: the maximum; l, negative where O is times kLower
     int64_t ldq;     // token stride of q, elements
     int B, T, H, G;  // G: query heads a key/value head
     int causal;
@@ -240,7 +247,7 @@ __device__ __forceinline__ int thread_here() {
 template <int kQT>
 struct Shared {
     float o[kWaves * kQT][16][kObufRow];
-    float ml[kWaves * kQT][3][16];  // base, sum, true maximum
+    float ml[kWaves * kQT][3][16];  // base, sum (negative where O is times kLower), true maximum
 };
 
 // A wave's part of a stretch of work: begin puts the loads of its first blocks and of its Q rows under way, attend does the work
@@ -252,7 +259,7 @@ struct Stretch {
     static constexpr int kQRegs = kF32 ? 8 : 4;
     u32x4 qraw[kQT][kQRegs];
     __amdgpu_buffer_rsrc_t rsrc;  // the (slot, head)'s blocks
-    int kb, k1, step;             // the next block's first key, the end, the distance of the wave's blocks
+    int k0, kb, k1, step;         // the first block's first key, the next one's, the end, the distance of the wave's blocks
     int at, at_step;              // the byte offset of the next block to load, the distance
     int lane, wave, lim[kQT], minlim;
 
@@ -269,6 +276,16 @@ struct Stretch {
         at += at_step;
     }
 
+    __device__ __forceinline__ void load_first() {
+        kb = k0;
+        at = kb / kKvBlock * kv_block_bytes(kFormat);
+#pragma unroll
+        for (int i = 0; i < kStages; ++i) {
+            load_k(st[i], kb + i * step);
+            load_v(st[i], kb + i * step);
+        }
+    }
+
     __device__ __forceinline__ void begin(const CachedAttnArgs& a, const Work& w) {
         const int tid = thread_here();
         lane = tid & 63;
@@ -279,14 +296,9 @@ struct Stretch {
         k1 = w.k1;
         const KvView& c = w.prefix ? a.pre : a.own;
         rsrc = __builtin_amdgcn_make_buffer_rsrc(c.block<kFormat>(w.slot, w.hk, 0), 0, c.blocks * kv_block_bytes(kFormat), kBufferDword3);
-        kb = w.k0 + kw * kKvBlock;
-        at = kb / kKvBlock * kv_block_bytes(kFormat);
+        k0 = w.k0 + kw * kKvBlock;
         at_step = step / kKvBlock * kv_block_bytes(kFormat);
-#pragma unroll
-        for (int i = 0; i < kStages; ++i) {
-            load_k(st[i], kb + i * step);
-            load_v(st[i], kb + i * step);
-        }
+        load_first();
         const int nrows = (w.prefix ? a.B : 1) * a.T * a.G;
         const int row0 = w.apart ? w.tile * (16 * kQT) : w.tile * (16 * kQT) << w.wl;
         minlim = w.len;
@@ -358,14 +370,7 @@ struct Stretch {
         // more, so O is seldom rescaled. Each lane keeps the true maximum and the sum of its own keys.
         floatx4 acc[kQT][8];
         float base[kQT], top[kQT], sum[kQT];
-#pragma unroll
-        for (int x = 0; x < kQT; ++x) {
-            base[x] = kLowest;
-            top[x] = kNegInf;
-            sum[x] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) acc[x][i] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
-        }
+        bool lowered = false;  // (the same for the whole wave)
 
         // one block: scores, probabilities, O; its registers are filled again, K's behind the scores and V's behind O, with the
         // block kStages steps on
@@ -395,6 +400,7 @@ struct Stretch {
             keep_order();
             const bool mask = kb + kKvBlock > minlim;  // (the same for the whole wave)
             bf16x8 pf[kQT][kQS];
+            if (__builtin_expect(lowered, 0)) blk.vs[0] *= kLower, blk.vs[1] *= kLower;
 #pragma unroll
             for (int x = 0; x < kQT; ++x) {
                 const int rest = lim[x] - kb - g * 4;  // the lane's key 16 t + i is seen if it is below
@@ -458,22 +464,45 @@ struct Stretch {
             load_v(blk, next);
             kb += step;
         };
-        // (a way out of the middle of the loop would cost it the same)
-        while (kb + (kStages - 1) * step < k1) {
-            take(st[0]);
-            if constexpr (kStages > 1) take(st[1]);
+        for (;;) {
+#pragma unroll
+            for (int x = 0; x < kQT; ++x) {
+                base[x] = kLowest;
+                top[x] = kNegInf;
+                sum[x] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[x][i] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+            }
+            // (a way out of the middle of the loop would cost it the same)
+            while (kb + (kStages - 1) * step < k1) {
+                take(st[0]);
+                if constexpr (kStages > 1) take(st[1]);
+            }
+            if constexpr (kStages > 1)
+                if (kb < k1) take(st[0]);
+            bool over = false;
+#pragma unroll
+            for (int x = 0; x < kQT; ++x) {
+                sum[x] = sum_groups(sum[x]);
+                uint32_t most = 0;  // (as bits: NaN, which an infinite term leaves, lies above all)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) most = max(most, __float_as_uint(acc[x][i][j]) & 0x7fffffffu);
+                over |= most >= __float_as_uint(kLimit) && sum[x] == sum[x];  // (NaN scores stay NaN)
+            }
+            if (__builtin_expect(lowered || !__any(over), 1)) break;
+            lowered = true;
+            load_first();
         }
-        if constexpr (kStages > 1)
-            if (kb < k1) take(st[0]);
         // the sum and O relative to base, base, and the true maximum
 #pragma unroll
         for (int x = 0; x < kQT; ++x) {
             const int to = wave * kQT + x;
-            sum[x] = sum_groups(sum[x]);
             top[x] = max_groups(top[x]);
             if (g == 0) {
                 sh.ml[to][0][n] = base[x];
-                sh.ml[to][1][n] = sum[x];
+                sh.ml[to][1][n] = lowered ? -sum[x] : sum[x];
                 sh.ml[to][2][n] = top[x];
             }
 #pragma unroll
@@ -497,11 +526,22 @@ __device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRo
         const float base = mx == kNegInf ? 0.0f : mx;
         float l = 0.0f;
         floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t signs = 0;
         for (int k = 0; k < wk; ++k) {
             const int from = k * tiles + tq;
-            const float f = __builtin_amdgcn_exp2f(sh.ml[from][0][rn] - base);
-            l += f * sh.ml[from][1][rn];
+            const float f = __builtin_amdgcn_exp2f(sh.ml[from][0][rn] - base), sum = sh.ml[from][1][rn];
+            signs |= __float_as_uint(sum);
+            l += f * fabsf(sum);
             v += f * *reinterpret_cast<const floatx4*>(&sh.o[from][rn][d]);
+        }
+        const bool lowered = signs >> 31;
+        if (__builtin_expect(lowered, 0)) {
+            v = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+            for (int k = 0; k < wk; ++k) {
+                const int from = k * tiles + tq;
+                const float f = __builtin_amdgcn_exp2f(sh.ml[from][0][rn] - base) * (sh.ml[from][1][rn] < 0.0f ? 1.0f : kLower);
+                v += f * *reinterpret_cast<const floatx4*>(&sh.o[from][rn][d]);
+            }
         }
         const QueryRow to = query_row(a, row0 + rt, w.b, w.hk, w.prefix);
         const int64_t row = (static_cast<int64_t>(to.b) * a.T + to.t) * a.H + to.hq;
@@ -509,6 +549,7 @@ __device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRo
             const bool nan = l != l;  // (a maximum passes NaN scores over: they show in the sum)
             const bool empty = to.t >= rows.cnt[to.b] || (mx == kNegInf && !nan);
             v = empty ? (floatx4){0.0f, 0.0f, 0.0f, 0.0f} : v * (1.0f / l);
+            if (lowered) v *= kRaise;
             const int64_t at = row * kD + d;
             if constexpr (kF32) *reinterpret_cast<floatx4*>(static_cast<float*>(a.o) + at) = v;
             else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
@@ -519,7 +560,7 @@ __device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRo
         } else {
             const int64_t part = row * a.parts + w.part;
             *reinterpret_cast<floatx4*>(a.part_o + part * kD + d) = v;
-            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(mx, l);
+            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(mx, lowered ? -l : l);
         }
     }
 }
@@ -722,28 +763,46 @@ __global__ __launch_bounds__(kJoinThreads) void cached_attn_join_kernel(CachedAt
     const float base = mx == kNegInf ? 0.0f : mx;
     floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     float l = 0.0f;
+    uint32_t signs = 0;
 #pragma unroll 4
     for (int p = run; p < parts; p += 8) {
         const float2 s = *reinterpret_cast<const float2*>(pml + 2 * p);
         const floatx4 v = p == run ? v0 : *reinterpret_cast<const floatx4*>(po + static_cast<int64_t>(p) * kD + d);
         const float f = __builtin_amdgcn_exp2f(s.x - base);
-        l += f * s.y;
+        signs |= __float_as_uint(s.y);
+        l += f * fabsf(s.y);
         acc += f * v;
     }
+    if (__builtin_expect(signs >> 31, 0)) {  // (a run's parts with O times kLower: then all of the run)
+        acc = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int p = run; p < parts; p += 8) {
+            const float2 s = *reinterpret_cast<const float2*>(pml + 2 * p);
+            const float f = __builtin_amdgcn_exp2f(s.x - base) * (s.y < 0.0f ? 1.0f : kLower);
+            acc += f * *reinterpret_cast<const floatx4*>(po + static_cast<int64_t>(p) * kD + d);
+        }
+    }
     *reinterpret_cast<floatx4*>(&obuf[run][d]) = acc;
-    if ((threadIdx.x & 31) == 0) lred[run] = l;
+    if ((threadIdx.x & 31) == 0) lred[run] = signs >> 31 ? -l : l;
     __syncthreads();
     if (threadIdx.x >= 32) return;
     l = 0.0f;
     acc = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+    signs = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        l += lred[i];
+        signs |= __float_as_uint(lred[i]);
+        l += fabsf(lred[i]);
         acc += *reinterpret_cast<const floatx4*>(&obuf[i][d]);
+    }
+    const bool lowered = signs >> 31;
+    if (__builtin_expect(lowered, 0)) {
+        acc = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < 8; ++i) acc += (lred[i] < 0.0f ? 1.0f : kLower) * *reinterpret_cast<const floatx4*>(&obuf[i][d]);
     }
     const bool nan = l != l;  // (a maximum passes NaN scores over: they show in the sum)
     const bool empty = mx == kNegInf && !nan;
     acc = empty ? (floatx4){0.0f, 0.0f, 0.0f, 0.0f} : acc * (1.0f / l);
+    if (lowered) acc *= kRaise;
     const int64_t at = row * kD + d;
     if constexpr (kF32) *reinterpret_cast<floatx4*>(static_cast<float*>(a.o) + at) = acc;
     else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = make_uint2(pack2(acc[0], acc[1]), pack2(acc[2], acc[3]));
