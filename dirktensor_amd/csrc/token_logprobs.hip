@@ -73,6 +73,9 @@ struct LogprobArgs {
     uint64_t* part_key;   // [rows][segments][k], sorted
 };
 
+// whether a token is skipped: a token that has DT_NO_IGNORE's bits is none of the vocabulary's, not one to ignore
+__host__ __device__ __forceinline__ bool is_skipped(int64_t y, int64_t ignore) { return y == ignore && ignore != DT_NO_IGNORE; }
+
 __device__ __forceinline__ int64_t token_at(const void* tok, int tok64, int64_t row) {
     return tok64 ? static_cast<const int64_t*>(tok)[row] : static_cast<const int32_t*>(tok)[row];
 }
@@ -216,7 +219,7 @@ struct Target {
 };
 __device__ __forceinline__ Target target_of(const LogprobArgs& a, int64_t row, const void* xrow, bool bf16) {
     const int64_t y = token_at(a.tok, a.tok64, row);
-    Target t{0.0f, y == a.ignore, y >= 0 && y < a.V};
+    Target t{0.0f, is_skipped(y, a.ignore), y >= 0 && y < a.V};
     if (t.known) t.x = bf16 ? __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(xrow)[y]) << 16) : static_cast<const float*>(xrow)[y];
     return t;
 }
@@ -614,7 +617,7 @@ __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(LogprobBwdArgs a)
     const int64_t y = token_at(a.tok, a.tok64, row);
     float g = a.g[row];
     int hit = -1;
-    if (y == a.ignore) g = 0.0f;
+    if (is_skipped(y, a.ignore)) g = 0.0f;
     else if (y < 0 || y >= a.V) g = __builtin_nanf("");
     else if (y >= first && y < first + n) hit = static_cast<int>(y) - first;
     const float h = a.h ? a.h[row] : 0.0f;
@@ -697,7 +700,7 @@ bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p)
 int check_host_tokens(const void* tok, int token_bytes, int64_t rows, int V, int64_t ignore) {
     for (int64_t i = 0; i < rows; ++i) {
         const int64_t y = token_bytes == 8 ? static_cast<const int64_t*>(tok)[i] : static_cast<const int32_t*>(tok)[i];
-        if (y != ignore && (y < 0 || y >= V))
+        if (!is_skipped(y, ignore) && (y < 0 || y >= V))
             return set_error(DT_ERR_INVALID_ARG, "token %lld of row %lld outside [0, %d)", (long long)y, (long long)i, V);
     }
     return DT_OK;

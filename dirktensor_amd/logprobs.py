@@ -67,6 +67,15 @@ def _check_tokens(tokens, lead, like):
     return t, t.ctypes.data, t.itemsize
 
 
+def _ignore_of(ignore_index) -> int:
+    if ignore_index is None:
+        return C.DT_NO_IGNORE
+    i = int(ignore_index)
+    if not C.DT_NO_IGNORE < i < 2**63:
+        raise ValueError(f"ignore_index={i} is no token index of 64 bits, or the least one, which stands for none")
+    return i
+
+
 def _check_logits(logits, ctx):
     if len(logits.shape) < 1:
         raise ValueError("logits need a vocabulary dimension")
@@ -120,7 +129,7 @@ def token_logprobs(logits, tokens, *, top_k: int = 0, ignore_index: Optional[int
     lead, V, k = logits.shape[:-1], logits.shape[-1], int(top_k)
     dtype = _mode_of(logits, None)
     tok, tok_p, tok_bytes = _check_tokens(tokens, lead, logits)
-    ign = C.DT_NO_IGNORE if ignore_index is None else int(ignore_index)
+    ign = _ignore_of(ignore_index)
     if _is_torch(logits):
         x, (B, T, ldb, ldt) = _rows(logits)
         nbytes = _workspace_bytes(B, T, V, k)
@@ -184,7 +193,7 @@ def token_logprobs_backward(d_logprob, logits, tokens, result: TokenLogprobs, *,
     lead, V = logits.shape[:-1], logits.shape[-1]
     dtype = _mode_of(logits, None)
     tok, tok_p, tok_bytes = _check_tokens(tokens, lead, logits)
-    ign = C.DT_NO_IGNORE if result.ignore_index is None else int(result.ignore_index)
+    ign = _ignore_of(result.ignore_index)
     on_device = _is_torch(logits)
     per_row = dict(d_logprob=d_logprob, softmax_m=result.softmax_m, softmax_l=result.softmax_l, entropy=result.entropy)
     if d_entropy is not None:
