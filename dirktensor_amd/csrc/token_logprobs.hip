@@ -592,6 +592,7 @@ struct LogprobBwdArgs {
     int tok64;
     int T, V;
     int segments, seg_len;
+    int64_t row0;    // the launch's first row
     int far;         // the gradient is too large to be found in a cache by whoever reads it: it is written past them
 };
 
@@ -602,8 +603,9 @@ template <bool kBf16>
 __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(LogprobBwdArgs a) {
     using R = Run<kBf16>;
     const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x / a.segments;
-    const int first = static_cast<int>(blockIdx.x - row * a.segments) * a.seg_len;
+    const int in_launch = blockIdx.x / a.segments;
+    const int64_t row = a.row0 + in_launch;
+    const int first = static_cast<int>(blockIdx.x - in_launch * a.segments) * a.seg_len;
     const int n = min(a.V - first, a.seg_len);
     const int64_t b = row / a.T, t = row % a.T;
     const uint8_t* x = static_cast<const uint8_t*>(a.x) + (b * a.ldb + t * a.ldt + first) * R::kEs;
@@ -676,11 +678,14 @@ int launch_logprobs_bwd(LogprobBwdArgs a, int64_t rows, bool bf16, hipStream_t s
     // and 14.9)
     a.far = rows * a.V * (bf16 ? 2 : 4) > (256 << 20);
     a.segments = (a.V + a.seg_len - 1) / a.seg_len;
-    const int64_t grid = rows * a.segments;
-    if (grid > 0x7fffff) return set_error(DT_ERR_UNSUPPORTED, "%lld rows of %d logits need %lld workgroups", (long long)rows, a.V, (long long)grid);
-    if (bf16) hipLaunchKernelGGL((logprob_bwd_kernel<true>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, s, a);
-    else hipLaunchKernelGGL((logprob_bwd_kernel<false>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, s, a);
-    DT_HIP_TRY(hipGetLastError());
+    // (a launch has fewer than 2^32 threads; one takes 335000 rows of 100352 in fp32, 135 GB)
+    const int64_t most = 0x7fffff / a.segments;
+    for (a.row0 = 0; a.row0 < rows; a.row0 += most) {
+        const dim3 grid(static_cast<unsigned>(std::min(most, rows - a.row0) * a.segments));
+        if (bf16) hipLaunchKernelGGL((logprob_bwd_kernel<true>), grid, dim3(kThreads), 0, s, a);
+        else hipLaunchKernelGGL((logprob_bwd_kernel<false>), grid, dim3(kThreads), 0, s, a);
+        DT_HIP_TRY(hipGetLastError());
+    }
     return DT_OK;
 }
 
