@@ -2,7 +2,8 @@
 
 Work on one stream runs in order, and a thread enqueues one call's kernels before the next one's, so calls that share a
 workspace here do not overlap. A call that is captured into a graph gets one of its own from the graph's memory (None
-here), as its replays may run beside anything."""
+here), as its replays may run beside anything. So does a call on a stream that is not torch's: such a stream's address may be
+another's later, while the last kernels of the first still run."""
 
 from __future__ import annotations
 
@@ -33,6 +34,13 @@ def _shared(device: int) -> bool:
     return not _capturing() and _current() == device
 
 
+def _lasting(device: int) -> bool:
+    """Whether the device's current stream is the default one or of torch's pool, which are never destroyed. (The id of a stream
+    from elsewhere, torch.cuda.ExternalStream, is its address.)"""
+    s = torch.cuda.current_stream(device)
+    return s.cuda_stream == 0 or s.stream_id != s.cuda_stream
+
+
 def kept_workspace(device: int, stream: int):
     """The thread's workspace for the stream as (address, bytes, tensor); None if there is none yet, or a call must not use it."""
     return _kept.by_stream.get((device, stream)) if _shared(device) else None
@@ -40,8 +48,9 @@ def kept_workspace(device: int, stream: int):
 
 def new_workspace(like, device: int, stream: int, nbytes: int):
     """A workspace of at least ``nbytes`` for a call on ``stream``, the current one: (address, bytes, the tensor to hold until
-    the call was made). It is kept for the thread's next calls unless it is large or the call is being captured."""
-    if nbytes > _KEEP or not _shared(device):
+    the call was made). It is kept for the thread's next calls unless it is large, the call is being captured or the stream may be
+    destroyed."""
+    if nbytes > _KEEP or not _shared(device) or not _lasting(device):
         ws = like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         return (ws.data_ptr() if ws is not None else None), nbytes, ws
     n = max(_LEAST, 1 << (nbytes - 1).bit_length()) if nbytes else _LEAST
