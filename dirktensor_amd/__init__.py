@@ -17,6 +17,7 @@ from .attention import (  # noqa: F401
 from .cache import KVCache, cached_attention  # noqa: F401
 from .logprobs import TokenLogprobs, token_logprobs, token_logprobs_backward  # noqa: F401
 from .model import OlmoModel, ce_loss  # noqa: F401
+from ._workspace import release_workspaces  # noqa: F401
 from ._capi import DTError, LIB_PATH  # noqa: F401
 
 __all__ = [
@@ -34,6 +35,7 @@ __all__ = [
     "flash_attention_backward",
     "flash_attention_forward",
     "qk_norm_rope",
+    "release_workspaces",
     "token_logprobs",
     "token_logprobs_backward",
 ]

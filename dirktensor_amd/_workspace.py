@@ -8,6 +8,7 @@ another's later, while the last kernels of the first still run."""
 from __future__ import annotations
 
 import threading
+import weakref
 
 from .attention import torch
 
@@ -17,11 +18,23 @@ _current = getattr(getattr(torch, "_C", None), "_cuda_getDevice", None)
 
 _KEEP = 64 << 20   # larger ones live as long as their call
 _LEAST = 1 << 20
+_STREAMS = 8       # a thread keeps workspaces for so many, the newest
+
+
+class _Streams(dict):
+    __slots__ = ("__weakref__",)
+    __eq__, __hash__ = object.__eq__, object.__hash__
+
+
+_threads = weakref.WeakSet()  # every living thread's
+_threads_lock = threading.Lock()
 
 
 class _Kept(threading.local):
     def __init__(self):
-        self.by_stream = {}
+        self.by_stream = _Streams()
+        with _threads_lock:
+            _threads.add(self.by_stream)
 
 
 _kept = _Kept()
@@ -55,5 +68,21 @@ def new_workspace(like, device: int, stream: int, nbytes: int):
         return (ws.data_ptr() if ws is not None else None), nbytes, ws
     n = max(_LEAST, 1 << (nbytes - 1).bit_length()) if nbytes else _LEAST
     ws = like.new_empty(n, dtype=torch.uint8)
-    _kept.by_stream[(device, stream)] = k = (ws.data_ptr(), n, ws)
+    mine = _kept.by_stream
+    mine.pop((device, stream), None)
+    while len(mine) >= _STREAMS:  # (its memory goes to its stream's next allocations, which run behind the calls that used it)
+        try:
+            mine.pop(next(iter(mine)), None)
+        except (StopIteration, RuntimeError):  # another thread released them
+            break
+    mine[(device, stream)] = k = (ws.data_ptr(), n, ws)
     return k
+
+
+def release_workspaces() -> None:
+    """Gives back to torch's allocator what all threads keep for their next calls (up to 64 MiB a thread and stream, for at most
+    eight streams a thread); those allocate again. Calls under way are not disturbed."""
+    with _threads_lock:
+        every = list(_threads)
+    for s in every:
+        s.clear()

@@ -69,3 +69,47 @@ def test_streams_from_elsewhere_keep_none(kept, calls):
     with torch.cuda.stream(torch.cuda.ExternalStream(pool.cuda_stream)):
         n = len(kept)
         assert calls() and len(kept) == n
+
+
+def test_a_thread_keeps_them_for_few_streams(kept, calls):
+    streams = {}
+    for _ in range(40):
+        s = torch.cuda.Stream()
+        streams[s.cuda_stream] = s
+        with torch.cuda.stream(s):
+            assert calls()
+        assert len(kept) <= 8 and (0, s.cuda_stream) in kept
+    assert len(streams) > 8
+
+
+def test_they_are_given_back(kept, calls):
+    import threading
+
+    import dirktensor_amd as dt
+
+    def held():
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        return torch.cuda.memory_allocated()
+
+    dt.release_workspaces()
+    before = held()
+    done, go, ok = threading.Event(), threading.Event(), []
+
+    def work():
+        ok.append(calls())
+        done.set()
+        go.wait(60)
+        ok.append(calls())
+
+    t = threading.Thread(target=work)
+    t.start()
+    done.wait(60)
+    assert calls() and held() >= before + 2 * (1 << 20)  # this thread's and the other's
+    dt.release_workspaces()
+    assert held() == before
+    go.set()
+    t.join()
+    assert ok == [True, True] and calls()
+    dt.release_workspaces()
+    assert held() == before
