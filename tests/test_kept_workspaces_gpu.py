@@ -83,11 +83,13 @@ def test_a_thread_keeps_them_for_few_streams(kept, calls):
 
 
 def test_they_are_given_back(kept, calls):
+    import gc
     import threading
 
     import dirktensor_amd as dt
 
     def held():
+        gc.collect()  # (what earlier tests left in cycles)
         torch.cuda.synchronize()
         torch.cuda.empty_cache()
         return torch.cuda.memory_allocated()
