@@ -208,9 +208,13 @@ def cached_attention(Q, cache: KVCache, scale: float, causal: bool = True, *, sl
                                               s_p, n_p, pre, int(prefix_slot), ws_p, nbytes, dtype, C.DT_MEM_DEVICE, stream)
 
         kept = kept_workspace(cache.ctx.device, stream)
-        if kept is not None and attend(kept[0], kept[1]) == C.DT_OK:
-            return FlashAttentionResult(O, m, l)
-        # none yet, too small, or another error, which is found again
+        if kept is not None:
+            rc = attend(kept[0], kept[1])
+            if rc == C.DT_OK:
+                return FlashAttentionResult(O, m, l)
+            if rc != C.DT_ERR_INVALID_ARG:
+                C.check(rc)
+        # none yet, too small, or another argument that is refused, again then
         need = ctypes.c_int64()
         C.call("dt_cached_attn_workspace", handle, B, T, H, D, s_p, n_p, pre, int(prefix_slot), dtype, ctypes.byref(need))
         ws = new_workspace(Q, cache.ctx.device, stream, need.value) if kept is None or need.value > kept[1] else kept
