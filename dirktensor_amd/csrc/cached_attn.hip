@@ -31,7 +31,7 @@
 // Arithmetic: S^T = K Q^T with v_mfma_f32_16x16x32_bf16 on the held values, which bf16 holds exactly (int8 and e4m3
 // alike); the key's scale multiplies the 32-bit score. P times the value's scale is rounded to bf16 (at most half a step,
 // 2^-8 relative, for each term of the sum) for O^T += V^T P^T; m, l and O stay in 32 bits, l sums the unrounded probabilities.
-// In fp32 mode q (divided by the power of two below its row's largest magnitude) and P are split into three bf16 values
+// In fp32 mode q (divided by 2^9 times the power of two below its row's largest magnitude) and P are split into three bf16 values
 // each, whose sum is the fp32 value, so every product is exact in the 32-bit accumulation.
 
 #include "kv_cache.h"
@@ -343,9 +343,11 @@ struct Stretch {
                 for (int j = 0; j < 4; ++j) top = max(top, qraw[s][j] & 0x7f800000u);
             top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, 64)));
             top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, 64)));
-            // exponents from 2^-126 to 2^126 have a reciprocal; rows beyond (and with infinities, NaN) stay as they are
+            // exponents from 2^-126 to 2^126 have a reciprocal; rows beyond (and with infinities, NaN) stay as they are. Divided by 2^9
+            // times their power of two the values are below 2^-8, and 128 products with keys of any size stay in range.
             const bool norm = top >= 0x00800000u && top <= 0x7e800000u;
-            const float inv = norm ? __uint_as_float(0x7f000000u - top) : 1.0f;
+            const uint32_t by = min(top + (9u << 23), 0x7e800000u);
+            const float inv = norm ? __uint_as_float(0x7f000000u - by) : 1.0f;
 #pragma unroll
             for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -355,7 +357,7 @@ struct Stretch {
                     qf[1][s][j] = static_cast<__bf16>(m);
                     qf[2][s][j] = static_cast<__bf16>(v - h - m);
                 }
-            return norm ? scale * __uint_as_float(top) : scale;
+            return norm ? scale * __uint_as_float(by) : scale;
         }
     }
 

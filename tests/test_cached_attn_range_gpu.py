@@ -139,3 +139,19 @@ def test_ordinary_sequences_beside_large_ones(tdt):
     c.append(attn.randn((B, L, H, D), 53), v)
     p.append(attn.randn((1, P, H, D), 54), attn.randn((1, P, H, D), 55))
     assert numbers(attn.run(attn.randn((B, 2, H, D), 56, tdt), c, prefix=p))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("qsize,ksize", [(1e-34, 3e37), (1e-36, 2.5e38), (1e-30, 1e30), (1e30, 1e-30), (1.0, 1.0)])
+def test_large_keys_and_small_queries_in_fp32(fmt, qsize, ksize):
+    """Scores of ordinary size from keys near the end of the range: no sum on the way to them may pass it."""
+    from dirktensor_amd import KVCache
+
+    L, H, T = 300, 2, 3
+    c = KVCache(1, L, H, format=fmt)
+    c.append(values((1, L, H, D), 61, ksize), attn.randn((1, L, H, D), 62))
+    assert numbers(attn.run(attn.randn((1, T, H, D), 63, scale=qsize), c))
+    # the same sign everywhere: the largest sums that such values have
+    c.truncate([0])
+    c.append(values((1, L, H, D), 64, ksize).abs(), attn.randn((1, L, H, D), 65))
+    assert numbers(attn.run(attn.randn((1, T, H, D), 66, scale=qsize).abs(), c))
