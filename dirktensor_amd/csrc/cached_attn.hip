@@ -23,10 +23,10 @@
 //   * A workgroup that has all of a triple's keys writes the result itself; otherwise it leaves (m, l, unnormalised O) in the
 //     workspace, and a second kernel joins a row's parts, the prefix's and its own, in a fixed order.
 //
-// Measured at 16 heads, us: one sequence of 1000 in bf16 9.6 (latency: 16 workgroups); 16 sequences of up to 4096 in int8, 167 MB,
-// 27 and 4 for the join (6.2 TB/s); 32 of 8192 in fp8, 1.1 GB, 158 and 4 (6.9 TB/s, what a read of this size reaches); 64 of up to 512
-// behind a prefix of 4096 in int8 26 and 4 (94 MB, and the prefix's widening and products beside it); 12 by 5 tokens behind 2777
-// in fp8 13.5 and 4; 4 of 1500 in exact mode, int8, 11 and 4.
+// Measured at 16 heads, us: one sequence of 1000 in bf16 9.7 (latency: 16 workgroups); 16 sequences of up to 4096 in int8, 167 MB,
+// 28 and 4.4 for the join (6.0 TB/s); 32 of 8192 in fp8, 1.1 GB, 161 without a join (6.9 TB/s, what a read of this size reaches); 64 of
+// up to 512 behind a prefix of 4096 in int8 26.7 and 4.4 (94 MB, and the prefix's widening and products beside it); 12 by 5 tokens
+// behind 2777 in fp8 13.7 and 4; 4 of 1500 in exact mode, int8, 12 and 4.
 //
 // Arithmetic: S^T = K Q^T with v_mfma_f32_16x16x32_bf16 on the held values, which bf16 holds exactly (int8 and e4m3
 // alike); the key's scale multiplies the 32-bit score. P times the value's scale is rounded to bf16 (at most half a step,
@@ -64,13 +64,15 @@ constexpr float kSlack = 8.0f;
 // O before its division by l exceeds the values by up to 2^kSlack times the number of keys, and so fp32's range where the values lie
 // near its end. A wave whose O reaches kLimit (or has left the range) does its stretch once more with V's scales times kLower: O is
 // then at most 2^8 (a probability) 2^128 (a value) 2^21 (keys) 2^-32 = 2^125, and such results meet others, times kLower too. What
-// that loses are values below 2^-70, in a wave that has others above 2^70. (The check and the way back cost 0.4 us of the
-// 11 of one sequence of 1000 in bf16 and 0.8 of the 14 of 4 of 1500 in exact mode; 32 of 8192 in fp8 take no longer.)
+// that loses are values below 2^-70, in a wave that has others above 2^70. (The check and the way back cost 0.3 us of the 11 of one
+// sequence of 1000 in bf16, 0.4 of the 14 of 4 of 1500 in exact mode and 2 of the 86 of 700 tokens behind 2000 in fp8; 32 of 8192 in fp8
+// take no longer.)
 constexpr float kLimit = 0x1p100f;
 constexpr float kLower = 0x1p-32f, kRaise = 0x1p32f;
 constexpr int kBufferDword3 = 0x00020000;  // raw buffer, 32-bit data format (gfx9 family)
 
-// blocks in flight a wave: what 256 registers a lane hold, which leave two workgroups a CU
+// blocks in flight a wave: what 256 registers a lane hold, which leave two workgroups a CU. Two of 8 bits with one query tile take 212;
+// two of bf16, in exact mode or with two tiles would spill 8, 19 and 79.
 constexpr int stages(int format, bool f32, int qt) { return format == DT_KV_BF16 || f32 || qt > 1 ? 1 : 2; }
 
 // The batch rows, by value in the kernel's arguments (kN places, 32 where these are enough: eager calls at 16 heads in int8, one
@@ -247,7 +249,8 @@ __device__ __forceinline__ int thread_here() {
 template <int kQT>
 struct Shared {
     float o[kWaves * kQT][16][kObufRow];
-    float ml[kWaves * kQT][3][16];  // base, sum (negative where O is times kLower), true maximum
+    float ml[kWaves * kQT][3][16];  // base, sum, true maximum
+    int lowered[kWaves];            // whether the wave's O is times kLower
 };
 
 // A wave's part of a stretch of work: begin puts the loads of its first blocks and of its Q rows under way, attend does the work
@@ -496,15 +499,17 @@ struct Stretch {
             if (__builtin_expect(lowered || !__any(over), 1)) break;
             lowered = true;
             load_first();
+            __builtin_amdgcn_s_waitcnt(0);  // (else the loop's waits would be for the order in which these loads are issued, too)
         }
         // the sum and O relative to base, base, and the true maximum
+        if (lane == 0) sh.lowered[wave] = lowered;
 #pragma unroll
         for (int x = 0; x < kQT; ++x) {
             const int to = wave * kQT + x;
             top[x] = max_groups(top[x]);
             if (g == 0) {
                 sh.ml[to][0][n] = base[x];
-                sh.ml[to][1][n] = lowered ? -sum[x] : sum[x];
+                sh.ml[to][1][n] = sum[x];
                 sh.ml[to][2][n] = top[x];
             }
 #pragma unroll
@@ -514,9 +519,9 @@ struct Stretch {
 };
 
 // The waves' results meet: a thread sums four values of a row over the key waves, scaled to their common maximum. A wave that
-// has a stretch of its own does so for itself.
-template <bool kF32, int kQT, int kRows>
-__device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRowsOf<kRows>& rows, const Work& w, const Shared<kQT>& sh) {
+// has a stretch of its own does so for itself. kLowered: O of some wave is times kLower, so all of them are taken so.
+template <bool kLowered, bool kF32, int kQT, int kRows>
+__device__ __forceinline__ void join_waves_as(const CachedAttnArgs& a, const AttnRowsOf<kRows>& rows, const Work& w, const Shared<kQT>& sh) {
     const int tid = thread_here(), wave = w.apart ? __builtin_amdgcn_readfirstlane(tid >> 6) : 0;
     const int wk = w.apart ? 1 : kWaves >> w.wl, tiles = w.apart ? kQT : kQT << w.wl, threads = w.apart ? 64 : 64 * kWaves;
     const int row0 = w.tile * 16 * tiles, nrows = min((w.prefix ? a.B : 1) * a.T * a.G - row0, 16 * tiles);
@@ -528,22 +533,12 @@ __device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRo
         const float base = mx == kNegInf ? 0.0f : mx;
         float l = 0.0f;
         floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-        uint32_t signs = 0;
         for (int k = 0; k < wk; ++k) {
             const int from = k * tiles + tq;
-            const float f = __builtin_amdgcn_exp2f(sh.ml[from][0][rn] - base), sum = sh.ml[from][1][rn];
-            signs |= __float_as_uint(sum);
-            l += f * fabsf(sum);
+            float f = __builtin_amdgcn_exp2f(sh.ml[from][0][rn] - base);
+            l += f * sh.ml[from][1][rn];
+            if (kLowered && !sh.lowered[from / kQT]) f *= kLower;
             v += f * *reinterpret_cast<const floatx4*>(&sh.o[from][rn][d]);
-        }
-        const bool lowered = signs >> 31;
-        if (__builtin_expect(lowered, 0)) {
-            v = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
-            for (int k = 0; k < wk; ++k) {
-                const int from = k * tiles + tq;
-                const float f = __builtin_amdgcn_exp2f(sh.ml[from][0][rn] - base) * (sh.ml[from][1][rn] < 0.0f ? 1.0f : kLower);
-                v += f * *reinterpret_cast<const floatx4*>(&sh.o[from][rn][d]);
-            }
         }
         const QueryRow to = query_row(a, row0 + rt, w.b, w.hk, w.prefix);
         const int64_t row = (static_cast<int64_t>(to.b) * a.T + to.t) * a.H + to.hq;
@@ -551,7 +546,7 @@ __device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRo
             const bool nan = l != l;  // (a maximum passes NaN scores over: they show in the sum)
             const bool empty = to.t >= rows.cnt[to.b] || (mx == kNegInf && !nan);
             v = empty ? (floatx4){0.0f, 0.0f, 0.0f, 0.0f} : v * (1.0f / l);
-            if (lowered) v *= kRaise;
+            if (kLowered) v *= kRaise;
             const int64_t at = row * kD + d;
             if constexpr (kF32) *reinterpret_cast<floatx4*>(static_cast<float*>(a.o) + at) = v;
             else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
@@ -562,9 +557,18 @@ __device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRo
         } else {
             const int64_t part = row * a.parts + w.part;
             *reinterpret_cast<floatx4*>(a.part_o + part * kD + d) = v;
-            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(mx, lowered ? -l : l);
+            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(mx, kLowered ? -l : l);
         }
     }
+}
+template <bool kF32, int kQT, int kRows>
+__device__ __forceinline__ void join_waves(const CachedAttnArgs& a, const AttnRowsOf<kRows>& rows, const Work& w, const Shared<kQT>& sh) {
+    int lowered = 0;
+    if (w.apart) lowered = sh.lowered[threadIdx.x >> 6];
+    else
+        for (int i = 0; i < kWaves; ++i) lowered |= sh.lowered[i];
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(lowered), 0)) join_waves_as<true, kF32>(a, rows, w, sh);
+    else join_waves_as<false, kF32>(a, rows, w, sh);
 }
 
 // kQT, kPreQT: query tiles a wave for a batch row's own keys and for the prefix's
