@@ -11,7 +11,8 @@
 //   * Query rows that share a key/value head's keys go together, 16 to a matrix tile: the tokens and the query heads of
 //     its group for a batch row's own keys; for a shared prefix those of the whole batch, so that the prefix is read
 //     once for all of them. Where there are more than 16, a wave takes two tiles and widens each held value once for
-//     both (64 queries over a prefix in int8: 377 and 530 TFLOP/s; 256: 324 and 761, in fp8 390 and 1023).
+//     both (64 queries over a prefix in int8: 377 and 530 TFLOP/s; 256: 324 and 761, in fp8 390 and 1023; whole calls at 16 heads over
+//     131072 keys reach 452 and 613 in int8, 549 and 768 in fp8).
 //   * A workgroup has four waves: as many of them as there are tiles (one or two, up to four in exact mode) take query rows
 //     and the rest is spread over the keys, 32 at a time. Every wave keeps its own running maximum, sum and O; those of one
 //     tile meet in LDS once at the end. No wave waits for another in the loop, and no key passes through LDS: the cache lies
@@ -23,10 +24,10 @@
 //   * A workgroup that has all of a triple's keys writes the result itself; otherwise it leaves (m, l, unnormalised O) in the
 //     workspace, and a second kernel joins a row's parts, the prefix's and its own, in a fixed order.
 //
-// Measured at 16 heads, us: one sequence of 1000 in bf16 9.7 (latency: 16 workgroups); 16 sequences of up to 4096 in int8, 167 MB,
+// Measured at 16 heads, us: one sequence of 1000 in bf16 9.8 (latency: 16 workgroups); 16 sequences of up to 4096 in int8, 167 MB,
 // 28 and 4.4 for the join (6.0 TB/s); 32 of 8192 in fp8, 1.1 GB, 161 without a join (6.9 TB/s, what a read of this size reaches); 64 of
-// up to 512 behind a prefix of 4096 in int8 26.7 and 4.4 (94 MB, and the prefix's widening and products beside it); 12 by 5 tokens
-// behind 2777 in fp8 13.7 and 4; 4 of 1500 in exact mode, int8, 12 and 4.
+// up to 512 behind a prefix of 4096 in int8 27 and 4.4 (94 MB, and the prefix's widening and products beside it); 12 by 5 tokens
+// behind 2777 in fp8 13 and 4; 4 of 1500 in exact mode, int8, 12 and 4.
 //
 // Arithmetic: S^T = K Q^T with v_mfma_f32_16x16x32_bf16 on the held values, which bf16 holds exactly (int8 and e4m3
 // alike); the key's scale multiplies the 32-bit score. P times the value's scale is rounded to bf16 (at most half a step,

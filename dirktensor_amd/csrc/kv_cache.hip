@@ -9,9 +9,10 @@
 // out as single bytes from the registers. Few tokens a sequence (a decode step's one) go another way, as a block would
 // leave most threads idle: a wave takes one row of K or of V, two values a lane (kv_append_rows_kernel).
 //
-// Measured at 16 heads: 2 x 4096 tokens of bf16 into fp8 and back, 102 MB each way, 22.6 and 20.5 us (4.5 and 5.0 TB/s; a large copy
-// 5.2), 17.6 and 19.8 with the rows in the caches (loads past these take 22.6 either way, stores past them 34). One token of eight
-// sequences in int8 3.3 us, and read back 3.4, which is what a launch takes.
+// Measured at 16 heads: 2 x 4096 tokens of bf16 into fp8 and back, 102 MB moved each time, 22.6 and 20.5 us (4.5 and 5.0 TB/s; a
+// copy of 67 MB each way 4.9 through the caches, 5.5 past them), 17.6 and 19.8 with the rows in the caches (loads past these take
+// 22.6 either way, stores past them 34). One token of eight sequences in int8 3.3 us, and read back 3.4, which is what a launch
+// takes.
 
 #include "kv_cache.h"
 

@@ -24,7 +24,8 @@
 // caches reach 7.0), with 64 163. Rows whose first quarter is masked 259, with fifty tokens left 139, of equal values 2140 (selected one
 // after another 5 alternatives took 1460, 1470 and 1440, 64 ten times as long). 16 rows with 20 alternatives 13.2 us, both launches
 // (25 segments of 16 KB each: the chains from the first load to the sorted keys). The gradient of the 2048 rows, 1.64 GB moved, 300 us
-// (5.5 TB/s, a large copy 5.2), of 300 rows of 50277 in bf16, 60 MB, 13.6 us (4.4 TB/s).
+// (5.5 TB/s; a copy of as much 5.7 through the caches, 6.3 past them), of 300 rows of 50277 in bf16, 60 MB, 13.6 us (4.4 TB/s; a copy
+// 4.1 and 5.3).
 
 #include "dt_internal.h"
 

@@ -435,6 +435,9 @@ int dt_kv_cache_read(dt_kv_cache* cache, void* k, void* v, int B, int T, const i
  *   ws      : a device workspace of at least dt_cached_attn_workspace bytes for the same arguments (0: none is needed),
  *             16-byte aligned, not shared with a call that may run at the same time. Ignored with DT_MEM_HOST.
  * 1 <= B <= 256, 1 <= T <= 8192, B*T*H <= 8388607. Deterministic: the same call gives the same bits.
+ * Values may be as large as a cache holds. Scores are held in 32 bits in the log2 domain: one of 2.3e38 or more is infinite and gives
+ * NaN, a row whose scores all lie at -2.3e38 or below is the empty row. With DT_BF16 the sums of q times what is held (up to 127 or 448
+ * in 8 bits) must be in range too; DT_FP32_EXACT scales q first.
  */
 int dt_cached_attn_workspace(const dt_kv_cache* cache, int B, int T, int H, int D, const int32_t* slots,
                              const int32_t* counts, const dt_kv_cache* prefix, int prefix_slot, int dtype,
