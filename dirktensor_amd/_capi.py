@@ -31,6 +31,13 @@ DT_KV_INT8 = 0
 DT_KV_FP8 = 1
 DT_KV_BF16 = 2
 
+DT_ROTARY_HALF = 0
+DT_ROTARY_INTERLEAVED = 1
+DT_ROTARY_UNSCALED = 0
+DT_ROTARY_LINEAR = 1
+DT_ROTARY_THETA = 2
+DT_ROTARY_RAMP = 3
+
 DT_OPT_QKV_FUSED = 1
 DT_QKV_GEMM = 0
 DT_QKV_FUSED = 1
@@ -53,6 +60,14 @@ _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _fp = ctypes.POINTER(ctypes.c_float)
 _i32p = ctypes.POINTER(ctypes.c_int32)
+_dbl = ctypes.c_double
+
+
+class DTRotary(ctypes.Structure):
+    """dt_rotary"""
+
+    _fields_ = [("dims", ctypes.c_int32), ("layout", ctypes.c_int32), ("magnitude", _dbl), ("frequency", _dbl * (HEAD_DIM // 2))]
+
 
 # name -> (restype, argtypes); must match include/dirktensor_amd.h
 SIGNATURES = {
@@ -103,6 +118,16 @@ SIGNATURES = {
                           + [_i64, _c_int, _c_int, _vp]),
     "dt_token_logprobs_bwd": (_c_int, [_vp] * 8 + [_c_int, _c_int, _c_int, _i64, _i64, _c_int, _i64, _vp, _i64, _i64, _c_int,
                                                    _c_int, _vp]),
+    "dt_rotary_init": (_c_int, [_vp, _c_int, _c_int, _dbl, _c_int] + [_dbl] * 5),
+    "dt_rotary_fwd": (_c_int, [_vp] * 5 + [_c_int] * 5 + [_i64] * 4 + [_vp, _c_int, _vp, _vp, _c_int, _c_int, _c_int, _vp]),
+    "dt_head_norm_rotary_fwd": (_c_int, [_vp] * 7 + [_c_int] * 5 + [_i64] * 4 + [_vp, _c_int, _vp, _vp, ctypes.c_float, _c_int,
+                                                                                 _c_int, _vp]),
+    "dt_head_norm_rotary_bwd_workspace": (_c_int, [_c_int] * 4 + [_vp]),
+    "dt_head_norm_rotary_bwd": (_c_int, [_vp] * 11 + [_c_int] * 5 + [_i64] * 6 + [_vp, _c_int, _vp, _vp, ctypes.c_float, _vp, _i64,
+                                                                                  _c_int, _c_int, _vp]),
+    "dt_verify_drafts_workspace": (_c_int, [_c_int] * 4 + [_dbl, _vp]),
+    "dt_verify_drafts": (_c_int, [_vp] * 5 + [_c_int] * 3 + [_i64] * 4 + [_c_int, _vp, _dbl, _vp, _vp, _vp, _vp, _i64,
+                                                                          _c_int, _c_int, _vp]),
     "dt_ce_loss": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _c_int, _vp]),
 }
 

@@ -1,0 +1,614 @@
+// Rotation of queries and keys to their positions, with or without each head's RMSNorm in the same pass, and the gradients.
+//
+// A pair (a, b) of a head's values, of those that turn (the first `dims` of 128: d and d + dims/2, or 2i and 2i + 1), at
+// position p goes to
+//   a' = mag (a cos t - b sin t),   b' = mag (b cos t + a sin t),   t = p f_i
+// and the rest of the head stays. With the norm, y = x inv w with inv = 1 / sqrt(mean x^2 + eps) over the head is what turns.
+// Gradients: g = the rotation's transpose (angle -t) of the output's gradient; with the norm, n = x inv,
+//   dx = inv (w g - n mean(w g n)),   dw = sum over tokens and heads of g n.
+//
+// All of it is bound by HBM (each value is read and written once), where it is not bound by the launch.
+//
+// A wave takes eight heads of one token, eight lanes a head, 16 values a lane: both values of each pair lie in one lane, and
+// a head's sums are three lane exchanges away. The angles need no table: lane i works out pair i's angle for the token, in 64
+// bits down to a fraction of a quarter turn, and the lanes read the pairs that they need from LDS; so positions are bounded by
+// nothing but their type, and nothing is fetched for them.
+
+#include "dt_internal.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+namespace dt {
+namespace {
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kPairs = DT_HEAD_DIM / 2;
+constexpr int kGroupHeads = 8;  // heads of a wave
+constexpr int kFewRows = 32;
+constexpr int kMaxHeads = 1024;
+constexpr int kCus = 256;
+
+// kRows: places for the batch rows' first positions, by value
+template <int kRows>
+struct RotaryArgs {
+    const void* in[2];    // q, k rows (of the backward: the outputs' gradients)
+    const void* x[2];     // backward with norm: the forward's inputs
+    void* out[2];
+    const float* w[2];    // norm weights [128]
+    float* dw[2];         // their gradients
+    float* partial;       // [blocks][128] column sums, q's blocks first
+    int64_t ld_in[2], ld_x[2], ld_out[2];
+    const void* positions;  // [tokens], or NULL: start[b] + t
+    int pos_bytes;
+    int has_starts;       // start is set (otherwise there may be more rows than places)
+    int tokens, T;
+    int heads[2];
+    int octets;           // dims / 16
+    int blocks[2];        // backward: workgroups of q, of k
+    float mag, sign, eps;
+    double turns[kPairs];  // a position's step of each pair, in whole turns
+    int32_t start[kRows];
+};
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2){lo, hi}, bf16x2));
+}
+
+// 8 values, 16-byte aligned
+template <bool kBf16>
+__device__ __forceinline__ void load8(const void* p, int64_t at, float* x) {
+    if constexpr (kBf16) {
+        const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(u[i] << 16);
+            x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        }
+    } else {
+        const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float4 w = s[i];
+            x[4 * i] = w.x, x[4 * i + 1] = w.y, x[4 * i + 2] = w.z, x[4 * i + 3] = w.w;
+        }
+    }
+}
+template <bool kBf16>
+__device__ __forceinline__ void store8(void* p, int64_t at, const float* x) {
+    if constexpr (kBf16) {
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at) =
+            make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
+    } else {
+        float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
+        d[0] = make_float4(x[0], x[1], x[2], x[3]);
+        d[1] = make_float4(x[4], x[5], x[6], x[7]);
+    }
+}
+
+// The 16 values of a lane: two runs of 8, at `a` and `b` of the head. Lane j < octets has pairs 8j .. 8j + 7; the lanes behind
+// have values that do not turn.
+template <bool kInter>
+struct Place {
+    int a, b;
+    bool turns;
+    __device__ __forceinline__ Place(int lane, int octets) {
+        const int j = lane & 7;
+        turns = j < octets;
+        a = kInter || !turns ? 16 * j : 8 * j;
+        b = kInter || !turns ? a + 8 : a + 8 * octets;
+    }
+};
+
+// cos and sin (times mag) of a token's pairs into the wave's part of LDS
+template <int kRows>
+__device__ __forceinline__ void angles(const RotaryArgs<kRows>& a, int token, int lane, float2* cs) {
+    if (lane < 8 * a.octets) {
+        double p;
+        if (a.positions)
+            p = a.pos_bytes == 4 ? static_cast<const int32_t*>(a.positions)[token]
+                                 : static_cast<double>(static_cast<const int64_t*>(a.positions)[token]);
+        else {
+            const int b = token / a.T;
+            p = static_cast<double>(a.has_starts ? a.start[b] : 0) + (token - b * a.T);
+        }
+        double t = p * a.turns[lane];
+        t = 4.0 * (t - rint(t));       // quarter turns, in [-2, 2]
+        const double q = rint(t);
+        float s, c;
+        sincospif(0.5f * static_cast<float>(t - q), &s, &c);  // (of at most an eighth of a turn)
+        const int quarter = static_cast<int>(q);
+        if (quarter & 1) {
+            const float u = s;
+            s = c, c = -u;
+        }
+        if (quarter & 2) s = -s, c = -c;
+        cs[lane] = make_float2(a.mag * c, a.mag * a.sign * s);
+    }
+    // (the wave's own part: its accesses are in order)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <bool kInter>
+__device__ __forceinline__ void turn(float (&x)[16], const float2* cs) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        constexpr int kStep = kInter ? 2 : 1, kNext = kInter ? 1 : 8;
+        float& u = x[kStep * i];
+        float& v = x[kStep * i + kNext];
+        const float p = u, r = v;
+        const float2 f = cs[i];
+        u = p * f.x - r * f.y;
+        v = r * f.x + p * f.y;
+    }
+}
+
+// over the eight lanes of a head
+__device__ __forceinline__ float sum_head(float x) {
+    x += __shfl_xor(x, 1, 64);
+    x += __shfl_xor(x, 2, 64);
+    return x + __shfl_xor(x, 4, 64);
+}
+
+// 1 / sqrt(mean x^2 + eps) of the head
+__device__ __forceinline__ float inverse_rms(const float (&x)[16], float eps) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) ss += x[i] * x[i];
+    ss = sum_head(ss);
+    float inv = 1.0f / sqrtf(ss * (1.0f / DT_HEAD_DIM) + eps);
+    if (__any(ss == __builtin_huge_valf())) {  // squares past fp32's range: once more, of values 2^-70 times as large
+        float s2 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s2 += (x[i] * 0x1p-70f) * (x[i] * 0x1p-70f);
+        s2 = sum_head(s2);
+        if (ss == __builtin_huge_valf()) inv = 0x1p-70f / sqrtf(s2 * (1.0f / DT_HEAD_DIM));
+    }
+    return inv;
+}
+
+template <bool kBf16, bool kNorm, bool kInter, int kRows>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs<kRows> a, int groups, int items) {
+    __shared__ float2 cs[kWaves][kPairs];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int item = blockIdx.x * kWaves + wave;
+    if (item >= items) return;
+    const int token = item / groups;
+    // q's heads, then k's
+    int head = (item - token * groups) * kGroupHeads + (lane >> 3);
+    const bool second = head >= a.heads[0];
+    if (second) head -= a.heads[0];
+    const bool have = !second || head < a.heads[1];
+    const Place<kInter> at(lane, a.octets);
+    const void* in = second ? a.in[1] : a.in[0];
+    const int64_t from = token * (second ? a.ld_in[1] : a.ld_in[0]) + head * DT_HEAD_DIM;
+    float x[16];
+    if (have) {
+        load8<kBf16>(in, from + at.a, x);
+        load8<kBf16>(in, from + at.b, x + 8);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+    }
+    float w[16];
+    if constexpr (kNorm) {
+        load8<false>(second && have ? a.w[1] : a.w[0], at.a, w);
+        load8<false>(second && have ? a.w[1] : a.w[0], at.b, w + 8);
+    }
+    angles(a, token, lane, cs[wave]);
+    if constexpr (kNorm) {
+        const float inv = inverse_rms(x, a.eps);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = x[i] * inv * w[i];
+    }
+    if (at.turns) turn<kInter>(x, cs[wave] + 8 * (lane & 7));
+    if (have) {
+        void* out = second ? a.out[1] : a.out[0];
+        const int64_t to = token * (second ? a.ld_out[1] : a.ld_out[0]) + head * DT_HEAD_DIM;
+        store8<kBf16>(out, to + at.a, x);
+        store8<kBf16>(out, to + at.b, x + 8);
+    }
+}
+
+// The norm's backward: workgroups of q (the first blocks[0]) or of k; their waves take groups of eight heads in turn, and each
+// workgroup leaves the column sums of g n.
+template <bool kBf16, bool kInter, int kRows>
+__global__ __launch_bounds__(kThreads) void head_norm_rotary_bwd_kernel(RotaryArgs<kRows> a) {
+    __shared__ float2 cs[kWaves][kPairs];
+    __shared__ float sums[kWaves][DT_HEAD_DIM];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int which = static_cast<int>(blockIdx.x) >= a.blocks[0];
+    const int block = blockIdx.x - (which ? a.blocks[0] : 0);
+    const int heads = a.heads[which], groups = (heads + kGroupHeads - 1) / kGroupHeads;
+    const int items = a.tokens * groups;
+    const Place<kInter> at(lane, a.octets);
+    float w[16], dw[16];
+    load8<false>(a.w[which], at.a, w);
+    load8<false>(a.w[which], at.b, w + 8);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dw[i] = 0.0f;
+    for (int item = block * kWaves + wave; item < items; item += a.blocks[which] * kWaves) {
+        const int token = item / groups, head = (item - token * groups) * kGroupHeads + (lane >> 3);
+        const bool have = head < heads;
+        float g[16], x[16];
+        if (have) {
+            const int64_t gi = token * a.ld_in[which] + head * DT_HEAD_DIM, xi = token * a.ld_x[which] + head * DT_HEAD_DIM;
+            load8<kBf16>(a.in[which], gi + at.a, g);
+            load8<kBf16>(a.in[which], gi + at.b, g + 8);
+            load8<kBf16>(a.x[which], xi + at.a, x);
+            load8<kBf16>(a.x[which], xi + at.b, x + 8);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) g[i] = x[i] = 0.0f;
+        }
+        angles(a, token, lane, cs[wave]);
+        if (at.turns) turn<kInter>(g, cs[wave] + 8 * (lane & 7));
+        const float inv = inverse_rms(x, a.eps);
+        float dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            x[i] *= inv;
+            dw[i] += g[i] * x[i];
+            g[i] *= w[i];
+            dot += g[i] * x[i];
+        }
+        dot = sum_head(dot) * (1.0f / DT_HEAD_DIM);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) g[i] = inv * (g[i] - x[i] * dot);
+        if (have) {
+            const int64_t to = token * a.ld_out[which] + head * DT_HEAD_DIM;
+            store8<kBf16>(a.out[which], to + at.a, g);
+            store8<kBf16>(a.out[which], to + at.b, g + 8);
+        }
+    }
+    // the eight heads of a wave, then the waves
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        dw[i] += __shfl_xor(dw[i], 8, 64);
+        dw[i] += __shfl_xor(dw[i], 16, 64);
+        dw[i] += __shfl_xor(dw[i], 32, 64);
+    }
+    if (lane < 8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            sums[wave][at.a + i] = dw[i];
+            sums[wave][at.b + i] = dw[8 + i];
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < DT_HEAD_DIM) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) s += sums[i][threadIdx.x];
+        a.partial[static_cast<int64_t>(blockIdx.x) * DT_HEAD_DIM + threadIdx.x] = s;
+    }
+}
+
+// The workgroups' column sums, added in a fixed order: 16 columns of q or k a workgroup, 16 runs of rows.
+constexpr int kSumCols = 16;
+__global__ __launch_bounds__(kThreads) void head_norm_dw_kernel(const float* partial, int q_blocks, int k_blocks, float* dq, float* dk) {
+    __shared__ float red[kThreads / kSumCols][kSumCols + 1];
+    const int which = blockIdx.y, rows = which ? k_blocks : q_blocks;
+    const float* p = partial + (which ? static_cast<int64_t>(q_blocks) * DT_HEAD_DIM : 0);
+    const int c = threadIdx.x % kSumCols, r = threadIdx.x / kSumCols, col = blockIdx.x * kSumCols + c;
+    float s = 0.0f;
+#pragma unroll 8
+    for (int i = r; i < rows; i += kThreads / kSumCols) s += p[static_cast<int64_t>(i) * DT_HEAD_DIM + col];
+    red[r][c] = s;
+    __syncthreads();
+    if (r == 0) {
+        s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kThreads / kSumCols; ++i) s += red[i][c];
+        (which ? dk : dq)[col] = s;
+    }
+}
+
+struct Call {
+    const void *q, *k, *xq, *xk;
+    void *oq, *ok;
+    const float *wq, *wk;
+    float *dwq, *dwk;
+    int B, T, H, Hk, D;
+    int64_t ldq, ldk, ldxq, ldxk, ldoq, ldok;
+    const void* positions;
+    int pos_bytes;
+    const int32_t* starts;
+    const dt_rotary* rot;
+    float eps;
+    int dtype, mem;
+    bool norm, backward;
+};
+
+bool good_rotary(const dt_rotary* r) {
+    if (r->dims < 16 || r->dims > DT_HEAD_DIM || r->dims % 16) return false;
+    if (r->layout != DT_ROTARY_HALF && r->layout != DT_ROTARY_INTERLEAVED) return false;
+    if (!std::isfinite(r->magnitude) || !(r->magnitude > 0.0)) return false;
+    for (int i = 0; i < r->dims / 2; ++i)
+        if (!std::isfinite(r->frequency[i])) return false;
+    return true;
+}
+
+int check_call(const dt_ctx* ctx, const Call& c) {
+    if (c.B < 1 || c.T < 1 || c.H < 1 || c.Hk < 0)
+        return set_error(DT_ERR_INVALID_ARG, "B=%d, T=%d, H=%d must be >= 1, Hk=%d >= 0", c.B, c.T, c.H, c.Hk);
+    if (!c.q || !c.oq) return set_error(DT_ERR_INVALID_ARG, "q and its output must be non-NULL");
+    if (!c.rot) return set_error(DT_ERR_INVALID_ARG, "rotary is NULL");
+    if (!good_rotary(c.rot))
+        return set_error(DT_ERR_INVALID_ARG, "the rotary needs dims of 16, 32 .. %d, a known layout, a magnitude above 0 and finite frequencies", DT_HEAD_DIM);
+    if (c.D != DT_HEAD_DIM) return set_error(DT_ERR_UNSUPPORTED, "head_dim D=%d, kernels are built for D=%d", c.D, DT_HEAD_DIM);
+    if (c.H + static_cast<int64_t>(c.Hk) > kMaxHeads) return set_error(DT_ERR_UNSUPPORTED, "%d and %d heads are more than %d", c.H, c.Hk, kMaxHeads);
+    if (c.Hk > 0 && (!c.k || !c.ok)) return set_error(DT_ERR_INVALID_ARG, "k and its output must be non-NULL with Hk=%d", c.Hk);
+    // (indices of groups of heads stay within 31 bits)
+    if (static_cast<int64_t>(c.B) * c.T * ((c.H + 7) / 8 + (c.Hk + 7) / 8) > 0x7fffffff / 2)
+        return set_error(DT_ERR_UNSUPPORTED, "B*T = %lld tokens", (long long)c.B * c.T);
+    if (c.dtype != DT_FP32_EXACT && c.dtype != DT_BF16) return set_error(DT_ERR_INVALID_ARG, "unknown dtype %d", c.dtype);
+    if (c.mem != DT_MEM_DEVICE && c.mem != DT_MEM_HOST) return set_error(DT_ERR_INVALID_ARG, "unknown mem %d", c.mem);
+    if (c.positions && c.starts) return set_error(DT_ERR_INVALID_ARG, "positions and starts exclude each other");
+    if (c.positions && c.pos_bytes != 4 && c.pos_bytes != 8)
+        return set_error(DT_ERR_INVALID_ARG, "pos_bytes=%d must be 4 or 8", c.pos_bytes);
+    if (c.starts && c.B > kMaxRaggedBatch) return set_error(DT_ERR_UNSUPPORTED, "B=%d > %d rows with starts", c.B, kMaxRaggedBatch);
+    if (c.norm && (!c.wq || (c.Hk > 0 && !c.wk))) return set_error(DT_ERR_INVALID_ARG, "norm weights must be non-NULL");
+    if (c.norm && (!(c.eps >= 1e-30f) || !std::isfinite(c.eps))) return set_error(DT_ERR_INVALID_ARG, "eps %g must be at least 1e-30", c.eps);
+    if (c.norm && c.backward && (!c.xq || !c.dwq || (c.Hk > 0 && (!c.xk || !c.dwk))))
+        return set_error(DT_ERR_INVALID_ARG, "the forward's inputs and the weights' gradients must be non-NULL");
+    const int64_t dq = static_cast<int64_t>(c.H) * DT_HEAD_DIM, dk = static_cast<int64_t>(c.Hk) * DT_HEAD_DIM;
+    const bool xs = c.norm && c.backward;
+    if (c.ldq < dq || c.ldoq < dq || (xs && c.ldxq < dq) || (c.Hk > 0 && (c.ldk < dk || c.ldok < dk || (xs && c.ldxk < dk))))
+        return set_error(DT_ERR_INVALID_ARG, "row strides are below the heads' %lld or %lld values", (long long)dq, (long long)dk);
+    if (c.mem == DT_MEM_DEVICE) {
+        const int64_t per = c.dtype == DT_BF16 ? 8 : 4;
+        bool bad = !aligned16(c.q) || !aligned16(c.oq) || c.ldq % per || c.ldoq % per;
+        if (c.Hk > 0) bad = bad || !aligned16(c.k) || !aligned16(c.ok) || c.ldk % per || c.ldok % per;
+        if (xs) bad = bad || !aligned16(c.xq) || c.ldxq % per || (c.Hk > 0 && (!aligned16(c.xk) || c.ldxk % per));
+        if (c.norm) bad = bad || !aligned16(c.wq) || (c.Hk > 0 && !aligned16(c.wk));
+        if (bad) return set_error(DT_ERR_INVALID_ARG, "device rows, their strides and norm weights must be 16-byte aligned");
+        if (c.positions && reinterpret_cast<uintptr_t>(c.positions) % c.pos_bytes)
+            return set_error(DT_ERR_INVALID_ARG, "positions are not aligned to their size");
+    }
+    if (!ctx) return set_error(DT_ERR_INVALID_ARG, "ctx is NULL");
+    return DT_OK;
+}
+
+// workgroups of the norm's backward for `heads` heads: two a CU at most, so the sums that they leave stay few
+int bwd_blocks(int64_t tokens, int heads) {
+    const int64_t items = tokens * ((heads + kGroupHeads - 1) / kGroupHeads);
+    return static_cast<int>(std::min<int64_t>((items + kWaves - 1) / kWaves, 2 * kCus));
+}
+
+template <int kRows>
+int launch_rows(const Call& c, void* ws, hipStream_t s) {
+    RotaryArgs<kRows> a{};
+    a.in[0] = c.q, a.in[1] = c.k;
+    a.x[0] = c.xq, a.x[1] = c.xk;
+    a.out[0] = c.oq, a.out[1] = c.ok;
+    a.w[0] = c.wq, a.w[1] = c.wk;
+    a.ld_in[0] = c.ldq, a.ld_in[1] = c.ldk;
+    a.ld_x[0] = c.ldxq, a.ld_x[1] = c.ldxk;
+    a.ld_out[0] = c.ldoq, a.ld_out[1] = c.ldok;
+    a.positions = c.positions;
+    a.pos_bytes = c.pos_bytes;
+    a.tokens = c.B * c.T;
+    a.T = c.T;
+    a.has_starts = c.starts != nullptr;
+    a.heads[0] = c.H, a.heads[1] = c.Hk;
+    a.octets = c.rot->dims / 16;
+    a.mag = static_cast<float>(c.rot->magnitude);
+    a.sign = c.backward ? -1.0f : 1.0f;
+    a.eps = c.eps;
+    for (int i = 0; i < c.rot->dims / 2; ++i) a.turns[i] = c.rot->frequency[i] / 6.283185307179586476925;
+    if (c.starts) std::copy_n(c.starts, c.B, a.start);
+    const bool bf16 = c.dtype == DT_BF16, inter = c.rot->layout == DT_ROTARY_INTERLEAVED;
+    if (c.norm && c.backward) {
+        a.blocks[0] = bwd_blocks(a.tokens, c.H);
+        a.blocks[1] = c.Hk > 0 ? bwd_blocks(a.tokens, c.Hk) : 0;
+        a.partial = static_cast<float*>(ws);
+        const dim3 grid(a.blocks[0] + a.blocks[1]), block(kThreads);
+#define DT_GO(M, I) hipLaunchKernelGGL((head_norm_rotary_bwd_kernel<M, I, kRows>), grid, block, 0, s, a)
+        if (bf16) {
+            if (inter) DT_GO(true, true);
+            else DT_GO(true, false);
+        } else {
+            if (inter) DT_GO(false, true);
+            else DT_GO(false, false);
+        }
+#undef DT_GO
+        DT_HIP_TRY(hipGetLastError());
+        hipLaunchKernelGGL(head_norm_dw_kernel, dim3(DT_HEAD_DIM / kSumCols, c.Hk > 0 ? 2 : 1), block, 0, s, a.partial, a.blocks[0],
+                           a.blocks[1], c.dwq, c.dwk);
+        DT_HIP_TRY(hipGetLastError());
+        return DT_OK;
+    }
+    const int groups = (c.H + c.Hk + kGroupHeads - 1) / kGroupHeads, items = a.tokens * groups;
+    const dim3 grid((items + kWaves - 1) / kWaves), block(kThreads);
+#define DT_GO(M, N, I) hipLaunchKernelGGL((rotary_kernel<M, N, I, kRows>), grid, block, 0, s, a, groups, items)
+#define DT_GO2(M, N)                \
+    do {                            \
+        if (inter) DT_GO(M, N, true); \
+        else DT_GO(M, N, false);    \
+    } while (0)
+    if (bf16) {
+        if (c.norm) DT_GO2(true, true);
+        else DT_GO2(true, false);
+    } else {
+        if (c.norm) DT_GO2(false, true);
+        else DT_GO2(false, false);
+    }
+#undef DT_GO2
+#undef DT_GO
+    DT_HIP_TRY(hipGetLastError());
+    return DT_OK;
+}
+
+int launch(const Call& c, void* ws, hipStream_t s) {
+    return c.starts && c.B > kFewRows ? launch_rows<kMaxRaggedBatch>(c, ws, s) : launch_rows<kFewRows>(c, ws, s);
+}
+
+int64_t workspace_bytes(const Call& c) {
+    if (!c.norm || !c.backward) return 0;
+    const int64_t tokens = static_cast<int64_t>(c.B) * c.T;
+    return (bwd_blocks(tokens, c.H) + (c.Hk > 0 ? bwd_blocks(tokens, c.Hk) : 0)) * static_cast<int64_t>(DT_HEAD_DIM * sizeof(float));
+}
+
+int run(dt_ctx* ctx, const Call& call, void* ws, int64_t ws_bytes, void* stream) {
+    DT_TRY(check_call(ctx, call));
+    Call c = call;
+    const int64_t need = workspace_bytes(c);
+    if (c.mem == DT_MEM_DEVICE && need > 0 && (!ws || ws_bytes < need || !aligned16(ws)))
+        return set_error(DT_ERR_INVALID_ARG, "the workspace has %lld bytes (16-byte aligned), the call needs %lld", (long long)(ws ? ws_bytes : 0), (long long)need);
+    DeviceScope scope;
+    DT_TRY(scope.enter(ctx->device));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (c.mem == DT_MEM_DEVICE) return launch(c, ws, s);
+
+    // host memory: staged through the context's buffers, synchronous
+    const size_t esz = c.dtype == DT_BF16 ? 2 : 4, tok = static_cast<size_t>(c.B) * c.T;
+    const bool xs = c.norm && c.backward;
+    const size_t wbytes = DT_HEAD_DIM * sizeof(float);
+    DT_TRY(ctx->stage[6].ensure(4 * wbytes));
+    char* wbuf = static_cast<char*>(ctx->stage[6].ptr);
+    for (int i = 0; i < (c.Hk > 0 ? 2 : 1); ++i) {
+        const size_t row = static_cast<size_t>(i ? c.Hk : c.H) * DT_HEAD_DIM * esz;
+        const void*& in = i ? c.k : c.q;
+        const void*& x = i ? c.xk : c.xq;
+        int64_t &ld = i ? c.ldk : c.ldq, &ldx = i ? c.ldxk : c.ldxq;
+        DT_TRY(ctx->stage[i].ensure(tok * row));
+        DT_HIP_TRY(hipMemcpy2DAsync(ctx->stage[i].ptr, row, in, ld * esz, row, tok, hipMemcpyHostToDevice, s));
+        if (xs) {
+            DT_TRY(ctx->stage[2 + i].ensure(tok * row));
+            DT_HIP_TRY(hipMemcpy2DAsync(ctx->stage[2 + i].ptr, row, x, ldx * esz, row, tok, hipMemcpyHostToDevice, s));
+            x = ctx->stage[2 + i].ptr;
+            ldx = row / esz;
+        }
+        if (c.norm) {
+            const float*& w = i ? c.wk : c.wq;
+            DT_HIP_TRY(hipMemcpyAsync(wbuf + i * wbytes, w, wbytes, hipMemcpyHostToDevice, s));
+            w = reinterpret_cast<const float*>(wbuf + i * wbytes);
+        }
+        // (a row's values are read before it is written, by the same lanes)
+        in = ctx->stage[i].ptr;
+        ld = row / esz;
+        (i ? c.ok : c.oq) = ctx->stage[i].ptr;
+        (i ? c.ldok : c.ldoq) = row / esz;
+    }
+    c.dwq = reinterpret_cast<float*>(wbuf + 2 * wbytes);
+    c.dwk = reinterpret_cast<float*>(wbuf + 3 * wbytes);
+    if (c.positions) {
+        DT_TRY(ctx->stage[4].ensure(tok * c.pos_bytes));
+        DT_HIP_TRY(hipMemcpyAsync(ctx->stage[4].ptr, c.positions, tok * c.pos_bytes, hipMemcpyHostToDevice, s));
+        c.positions = ctx->stage[4].ptr;
+    }
+    if (need > 0) DT_TRY(ctx->stage[5].ensure(need));
+    DT_TRY(launch(c, ctx->stage[5].ptr, s));
+    for (int i = 0; i < (c.Hk > 0 ? 2 : 1); ++i) {
+        const size_t row = static_cast<size_t>(i ? c.Hk : c.H) * DT_HEAD_DIM * esz;
+        DT_HIP_TRY(hipMemcpy2DAsync(i ? call.ok : call.oq, (i ? call.ldok : call.ldoq) * esz, ctx->stage[i].ptr, row, row, tok,
+                                    hipMemcpyDeviceToHost, s));
+        if (xs) DT_HIP_TRY(hipMemcpyAsync(i ? call.dwk : call.dwq, i ? c.dwk : c.dwq, wbytes, hipMemcpyDeviceToHost, s));
+    }
+    DT_HIP_TRY(hipStreamSynchronize(s));
+    return DT_OK;
+}
+
+}  // namespace
+}  // namespace dt
+
+using namespace dt;
+
+extern "C" {
+
+int dt_rotary_init(dt_rotary* rot, int dims, int layout, double theta, int scaling, double factor, double original_length, double low,
+                   double high, double magnitude) {
+    clear_error();
+    if (!rot) return set_error(DT_ERR_INVALID_ARG, "rotary is NULL");
+    if (dims < 16 || dims > DT_HEAD_DIM || dims % 16)
+        return set_error(DT_ERR_INVALID_ARG, "dims=%d must be a multiple of 16, at most %d", dims, DT_HEAD_DIM);
+    if (layout != DT_ROTARY_HALF && layout != DT_ROTARY_INTERLEAVED) return set_error(DT_ERR_INVALID_ARG, "unknown layout %d", layout);
+    if (!std::isfinite(theta) || !(theta > 1.0)) return set_error(DT_ERR_INVALID_ARG, "theta %g must be finite and above 1", theta);
+    if (scaling < DT_ROTARY_UNSCALED || scaling > DT_ROTARY_RAMP) return set_error(DT_ERR_INVALID_ARG, "unknown scaling %d", scaling);
+    if (scaling != DT_ROTARY_UNSCALED && (!std::isfinite(factor) || !(factor >= 1.0)))
+        return set_error(DT_ERR_INVALID_ARG, "factor %g must be finite and at least 1", factor);
+    if (scaling == DT_ROTARY_RAMP &&
+        (!std::isfinite(original_length) || !(original_length > 0.0) || !std::isfinite(low) || !std::isfinite(high) || !(low < high)))
+        return set_error(DT_ERR_INVALID_ARG, "a ramp needs an original length above 0 and low < high, got %g, %g, %g", original_length, low, high);
+    if (!std::isfinite(magnitude) || !(magnitude > 0.0)) return set_error(DT_ERR_INVALID_ARG, "magnitude %g must be finite and above 0", magnitude);
+    if (scaling == DT_ROTARY_THETA) theta *= std::pow(factor, static_cast<double>(dims) / (dims - 2));
+    if (!std::isfinite(theta)) return set_error(DT_ERR_INVALID_ARG, "theta times the factor's power is past the range");
+    *rot = {};
+    rot->dims = dims;
+    rot->layout = layout;
+    rot->magnitude = magnitude;
+    for (int i = 0; i < dims / 2; ++i) {
+        double f = std::pow(theta, -2.0 * i / dims);
+        if (scaling == DT_ROTARY_LINEAR) f /= factor;
+        if (scaling == DT_ROTARY_RAMP) {
+            const double turns = f * original_length / 6.283185307179586476925;
+            const double keep = std::min(1.0, std::max(0.0, (turns - low) / (high - low)));
+            f *= keep + (1.0 - keep) / factor;
+        }
+        rot->frequency[i] = f;
+    }
+    return DT_OK;
+}
+
+int dt_rotary_fwd(dt_ctx* ctx, const void* q, const void* k, void* q_out, void* k_out, int B, int T, int H, int Hk, int D, int64_t ldq,
+                  int64_t ldk, int64_t ldq_out, int64_t ldk_out, const void* positions, int pos_bytes, const int32_t* starts,
+                  const dt_rotary* rotary, int backward, int dtype, int mem, void* stream) {
+    clear_error();
+    if (backward != 0 && backward != 1) return set_error(DT_ERR_INVALID_ARG, "backward must be 0 or 1");
+    Call c{};
+    c.q = q, c.k = k, c.oq = q_out, c.ok = k_out;
+    c.B = B, c.T = T, c.H = H, c.Hk = Hk, c.D = D;
+    c.ldq = ldq, c.ldk = ldk, c.ldoq = ldq_out, c.ldok = ldk_out;
+    c.positions = positions, c.pos_bytes = pos_bytes, c.starts = starts, c.rot = rotary;
+    c.dtype = dtype, c.mem = mem, c.backward = backward;
+    return run(ctx, c, nullptr, 0, stream);
+}
+
+int dt_head_norm_rotary_fwd(dt_ctx* ctx, const void* q, const void* k, const float* q_weight, const float* k_weight, void* q_out,
+                            void* k_out, int B, int T, int H, int Hk, int D, int64_t ldq, int64_t ldk, int64_t ldq_out,
+                            int64_t ldk_out, const void* positions, int pos_bytes, const int32_t* starts, const dt_rotary* rotary,
+                            float eps, int dtype, int mem, void* stream) {
+    clear_error();
+    Call c{};
+    c.q = q, c.k = k, c.oq = q_out, c.ok = k_out, c.wq = q_weight, c.wk = k_weight;
+    c.B = B, c.T = T, c.H = H, c.Hk = Hk, c.D = D;
+    c.ldq = ldq, c.ldk = ldk, c.ldoq = ldq_out, c.ldok = ldk_out;
+    c.positions = positions, c.pos_bytes = pos_bytes, c.starts = starts, c.rot = rotary;
+    c.eps = eps, c.dtype = dtype, c.mem = mem, c.norm = true;
+    return run(ctx, c, nullptr, 0, stream);
+}
+
+int dt_head_norm_rotary_bwd_workspace(int B, int T, int H, int Hk, int64_t* bytes) {
+    clear_error();
+    if (!bytes) return set_error(DT_ERR_INVALID_ARG, "bytes is NULL");
+    if (B < 1 || T < 1 || H < 1 || Hk < 0) return set_error(DT_ERR_INVALID_ARG, "B=%d, T=%d, H=%d must be >= 1, Hk=%d >= 0", B, T, H, Hk);
+    Call c{};
+    c.B = B, c.T = T, c.H = H, c.Hk = Hk, c.norm = c.backward = true;
+    *bytes = workspace_bytes(c);
+    return DT_OK;
+}
+
+int dt_head_norm_rotary_bwd(dt_ctx* ctx, const void* d_q_out, const void* d_k_out, const void* q, const void* k, const float* q_weight,
+                            const float* k_weight, void* d_q, void* d_k, float* d_q_weight, float* d_k_weight, int B, int T, int H,
+                            int Hk, int D, int64_t ld_dq_out, int64_t ld_dk_out, int64_t ldq, int64_t ldk, int64_t ld_dq,
+                            int64_t ld_dk, const void* positions, int pos_bytes, const int32_t* starts, const dt_rotary* rotary,
+                            float eps, void* ws, int64_t ws_bytes, int dtype, int mem, void* stream) {
+    clear_error();
+    Call c{};
+    c.q = d_q_out, c.k = d_k_out, c.xq = q, c.xk = k, c.oq = d_q, c.ok = d_k;
+    c.wq = q_weight, c.wk = k_weight, c.dwq = d_q_weight, c.dwk = d_k_weight;
+    c.B = B, c.T = T, c.H = H, c.Hk = Hk, c.D = D;
+    c.ldq = ld_dq_out, c.ldk = ld_dk_out, c.ldxq = ldq, c.ldxk = ldk, c.ldoq = ld_dq, c.ldok = ld_dk;
+    c.positions = positions, c.pos_bytes = pos_bytes, c.starts = starts, c.rot = rotary;
+    c.eps = eps, c.dtype = dtype, c.mem = mem, c.norm = c.backward = true;
+    return run(ctx, c, ws, ws_bytes, stream);
+}
+
+}  // extern "C"

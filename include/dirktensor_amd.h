@@ -481,6 +481,97 @@ int dt_token_logprobs_bwd(dt_ctx* ctx, const float* d_logprob, const float* d_en
                           int64_t ldb, int64_t ldt, int token_bytes, int64_t ignore_index, void* d_logits,
                           int64_t ldb_out, int64_t ldt_out, int dtype, int mem, void* stream);
 
+/*
+ * Rotary positions (the rotation of apply_rope, OlmoAttention.cpp:111-146, at any positions, of part of the head, in either
+ * layout of the pairs, scaled for contexts beyond the trained one): a pair (a, b) at position p goes to
+ *   magnitude * (a cos t - b sin t),  magnitude * (b cos t + a sin t),  t = p * frequency[i],
+ * and the values of the head from `dims` on stay. The angles are worked out in 64 bits where they are used: no table bounds the
+ * positions, which may be negative.
+ * dt_rotary is filled by dt_rotary_init, or by the caller:
+ *   dims       values that turn, from the head's first on: 16, 32 .. 128
+ *   layout     DT_ROTARY_HALF: pairs (d, d + dims/2); DT_ROTARY_INTERLEAVED: pairs (2i, 2i + 1)
+ *   frequency  radians a position of pair i < dims/2
+ * dt_rotary_init: frequency[i] = theta^(-2i/dims), scaled by `factor` >= 1:
+ *   DT_ROTARY_LINEAR  divided by the factor (positions are brought closer)
+ *   DT_ROTARY_THETA   theta times factor^(dims / (dims - 2)): the last pair is divided by the factor, the first stays
+ *   DT_ROTARY_RAMP    by the turns that a pair makes over original_length: at `high` and more it stays, at `low` and fewer it is
+ *                     divided by the factor, between them a share of both, linear in the turns
+ */
+#define DT_ROTARY_HALF 0
+#define DT_ROTARY_INTERLEAVED 1
+#define DT_ROTARY_UNSCALED 0
+#define DT_ROTARY_LINEAR 1
+#define DT_ROTARY_THETA 2
+#define DT_ROTARY_RAMP 3
+typedef struct dt_rotary {
+    int32_t dims, layout;
+    double magnitude;
+    double frequency[DT_HEAD_DIM / 2];
+} dt_rotary;
+int dt_rotary_init(dt_rotary* rotary, int dims, int layout, double theta, int scaling, double factor, double original_length,
+                   double low, double high, double magnitude);
+/*
+ * Rotates B x T tokens' queries (H heads) and keys (Hk heads; 0: none, k and k_out are ignored).
+ *   q, k, q_out, k_out : tokens of heads*128 values in dtype, ld* elements apart; an output may be its input (same address and
+ *                        stride), and must not overlap it otherwise
+ *   positions : [B, T] whole numbers of pos_bytes (4 or 8), in the same memory as q, or NULL: token (b, t) is at starts[b] + t
+ *   starts    : B host values (B <= 256 then), or NULL: 0
+ *   rotary    : host memory, read during the call
+ *   backward  : 1: the transpose, which takes the outputs' gradients to the inputs'
+ */
+int dt_rotary_fwd(dt_ctx* ctx, const void* q, const void* k, void* q_out, void* k_out, int B, int T, int H, int Hk, int D,
+                  int64_t ldq, int64_t ldk, int64_t ldq_out, int64_t ldk_out, const void* positions, int pos_bytes,
+                  const int32_t* starts, const dt_rotary* rotary, int backward, int dtype, int mem, void* stream);
+/*
+ * RMSNorm of each head and the rotation in one pass (beside dt_qk_norm_rope_fwd, whose norm spans all heads):
+ * x / sqrt(mean x^2 + eps) * weight over the head's 128 values, then as dt_rotary_fwd. q_weight, k_weight: [128] fp32,
+ * eps >= 1e-30. Rounded to dtype once.
+ */
+int dt_head_norm_rotary_fwd(dt_ctx* ctx, const void* q, const void* k, const float* q_weight, const float* k_weight, void* q_out,
+                            void* k_out, int B, int T, int H, int Hk, int D, int64_t ldq, int64_t ldk, int64_t ldq_out,
+                            int64_t ldk_out, const void* positions, int pos_bytes, const int32_t* starts, const dt_rotary* rotary,
+                            float eps, int dtype, int mem, void* stream);
+/*
+ * Its gradients: d_q_out, d_k_out (of the outputs) and the forward's q, k -> d_q, d_k in dtype (which may be the outputs'
+ * gradients or the inputs themselves, the same address and stride) and d_q_weight, d_k_weight [128] fp32 (overwritten).
+ * ws: a device workspace of at least dt_head_norm_rotary_bwd_workspace bytes, 16-byte aligned, not shared with a call that may run
+ * at the same time; ignored with DT_MEM_HOST. Deterministic.
+ */
+int dt_head_norm_rotary_bwd_workspace(int B, int T, int H, int Hk, int64_t* bytes);
+int dt_head_norm_rotary_bwd(dt_ctx* ctx, const void* d_q_out, const void* d_k_out, const void* q, const void* k,
+                            const float* q_weight, const float* k_weight, void* d_q, void* d_k, float* d_q_weight,
+                            float* d_k_weight, int B, int T, int H, int Hk, int D, int64_t ld_dq_out, int64_t ld_dk_out,
+                            int64_t ldq, int64_t ldk, int64_t ld_dq, int64_t ld_dk, const void* positions, int pos_bytes,
+                            const int32_t* starts, const dt_rotary* rotary, float eps, void* ws, int64_t ws_bytes, int dtype,
+                            int mem, void* stream);
+
+/*
+ * Verification of drafted tokens against the model's probabilities, from given random numbers (no reference counterpart).
+ *   logits       : B x (K + 1) rows of V (<= 2^24) logits in dtype, row (b, i) at element b*ldb + i*ldt: row i gives the token
+ *                  behind the first i drafts
+ *   drafts       : [B, K] tokens of token_bytes (4 or 8) each, K in 0 .. 64; with K = 0 a token is drawn
+ *   uniforms     : [B, K + 1] fp32 in [0, 1): K for the drafts, one for the token that follows (NULL allowed at temperature 0)
+ *   draft_logits : B x K rows (b*ldb_draft + i*ldt_draft) of the logits that the drafts were drawn from at the same temperature, or
+ *                  NULL: drafts that nothing was drawn for (probability 1)
+ *   counts       : how many drafts each batch row has (host, 0 .. K), or NULL for all K
+ * With p = softmax(logits / temperature), q = softmax(draft_logits / temperature): draft i is accepted, if those before it were,
+ * while uniform_i * q_i(draft_i) < p_i(draft_i). One token more is drawn with the last uniform: from max(p - q, 0) of the first row
+ * whose draft was refused (from p where that leaves nothing), or from p of the row behind the last draft: the first token with
+ * which the sum of the weights exceeds uniform * their total. At temperature 0 a draft is accepted while it is the largest logit
+ * (the first of equals), and that token follows. Probabilities are held in 64 bits.
+ *   accepted [B] int32 : how many drafts were accepted, n
+ *   tokens [B, K + 1] int32 : the accepted drafts, the token that follows, then -1
+ *   logprob [B, K + 1] fp32 : their log p (at temperature 0 that of temperature 1), then 0
+ * Logits of -inf have probability 0. A row with a NaN or +inf, or with nothing but -inf, refuses its draft and gives token -1 with log
+ * probability NaN. A draft outside [0, V) is refused with DT_MEM_HOST (DT_ERR_INVALID_ARG); on the device it has probability 0.
+ * 1 <= B <= 256. ws as for dt_token_logprobs. Deterministic.
+ */
+int dt_verify_drafts_workspace(int B, int K, int V, int has_draft_logits, double temperature, int64_t* bytes);
+int dt_verify_drafts(dt_ctx* ctx, const void* logits, const void* drafts, const float* uniforms, const void* draft_logits, int B,
+                     int K, int V, int64_t ldb, int64_t ldt, int64_t ldb_draft, int64_t ldt_draft, int token_bytes,
+                     const int32_t* counts, double temperature, int32_t* accepted, int32_t* tokens, float* logprob, void* ws,
+                     int64_t ws_bytes, int dtype, int mem, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
