@@ -30,6 +30,7 @@ DT_NO_IGNORE = -(2**63)
 DT_KV_INT8 = 0
 DT_KV_FP8 = 1
 DT_KV_BF16 = 2
+DT_KV_FP4 = 4
 
 DT_ROTARY_HALF = 0
 DT_ROTARY_INTERLEAVED = 1

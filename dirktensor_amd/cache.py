@@ -1,7 +1,7 @@
 """A quantised key/value cache and the attention that reads it, on the HIP path: every call goes to
 libdirktensor_amd.so; nothing here computes.
 
-    KVCache(slots, capacity, n_heads, format="int8" | "fp8" | "bf16")
+    KVCache(slots, capacity, n_heads, format="int8" | "fp8" | "bf16" | "fp4")
         append(K, V)              quantises rows as they are written behind what the slots hold
         read(starts, count)       the rows as the values they stand for
         truncate(lengths)         shortens slots (0: free for another sequence)
@@ -24,7 +24,7 @@ from . import _capi as C
 from ._workspace import kept_workspace, new_workspace
 from .attention import Context, FlashAttentionResult, _is_torch, _mode_of, _stream_of, default_context, torch
 
-_FORMATS = {"int8": C.DT_KV_INT8, "fp8": C.DT_KV_FP8, "bf16": C.DT_KV_BF16}
+_FORMATS = {"int8": C.DT_KV_INT8, "fp8": C.DT_KV_FP8, "bf16": C.DT_KV_BF16, "fp4": C.DT_KV_FP4}
 
 
 def _address(a: np.ndarray) -> int:
@@ -68,7 +68,8 @@ def _rows_of(x):
 
 class KVCache:
     """Keys and values of ``slots`` sequences of at most ``capacity`` tokens, ``n_heads`` heads of 128 values each,
-    held in ``format``: "int8" (one scale a token and head), "fp8" (e4m3, scaled by a power of two) or "bf16".
+    held in ``format``: "int8" (one scale a token and head), "fp8" (e4m3, scaled by a power of two), "bf16" or
+    "fp4" (e2m1, each 32 values scaled by a power of two; half the bytes of the 8-bit formats).
 
     A row with an infinity or a NaN reads back as NaN and gives NaN to the queries that see it. The lengths live on the
     host and move when a call is made; calls on one cache must be ordered on their streams, except calls that only

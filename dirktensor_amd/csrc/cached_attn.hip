@@ -171,13 +171,26 @@ __device__ __forceinline__ bf16x8 widen(uint32_t a, uint32_t b) {
     return r.v;
 }
 
+// 8 held values of 4 bits times their scale, a power of two (an infinity, which no scale is, gives NaN)
+__device__ __forceinline__ bf16x8 widen4(uint32_t w, float scale) {
+    union { uint32_t u[4]; bf16x8 v; } r;
+    r.u[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0));
+    r.u[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1));
+    r.u[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2));
+    r.u[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3));
+    return r.v;
+}
+
 // A block as loaded: 16-byte pieces of K (two tiles of 16 keys) and V (eight tiles of 16 values), and the scales of the lane's
 // keys. kOnce: no other wave reads these keys, so they pass the caches by.
 template <int kFormat, bool kOnce>
 struct Block {
-    static constexpr int kPieces = kFormat == DT_KV_BF16 ? 8 : 4;
+    static constexpr int kPieces = kv_elem_bits(kFormat) / 2;
     u32x4 k[kPieces], v[kPieces];
     floatx4 ks[2], vs[2];
+    // fp4: of K the scale of the lane's key and group of values, as a float's exponent; of V the four scales of each of the lane's keys
+    uint32_t k4[2];
+    u32x4 v4[2];
     // 16 bytes at `at` + the lane's offset of the block that begins at `from` (the immediate offset holds 12 bits)
     template <bool kNt>
     static __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off, int from, int at) {
@@ -187,14 +200,22 @@ struct Block {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) k[i] = load16<kOnce>(r, off, from, i * kKvRun);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) ks[t] = __builtin_bit_cast(floatx4, load16<false>(r, scale_off, from, kv_scale_at(kFormat) + t * 64));
+        for (int t = 0; t < 2; ++t) {
+            if constexpr (kFormat == DT_KV_FP4)
+                k4[t] = __builtin_amdgcn_raw_buffer_load_b8(r, scale_off + t * 64, from + kv_scale_at(kFormat), 0);
+            else
+                ks[t] = __builtin_bit_cast(floatx4, load16<false>(r, scale_off, from, kv_scale_at(kFormat) + t * 64));
+        }
     }
     __device__ __forceinline__ void load_v(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t scale_off, int from) {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) v[i] = load16<kOnce>(r, off, from, kv_tensor_bytes(kFormat) + i * kKvRun);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-            vs[t] = __builtin_bit_cast(floatx4, load16<false>(r, scale_off, from, kv_scale_at(kFormat) + 128 + t * 64));
+        for (int t = 0; t < 2; ++t) {
+            const u32x4 w = load16<false>(r, scale_off, from, kv_scale_at(kFormat) + 128 + t * 64);
+            if constexpr (kFormat == DT_KV_FP4) v4[t] = w;
+            else vs[t] = __builtin_bit_cast(floatx4, w);
+        }
     }
     // the pieces as values of their own: else the compiler carries them through the loop widened, in twice or four times the
     // registers
@@ -202,7 +223,15 @@ struct Block {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) asm volatile("" : "+v"(w[i]));
     }
-    // operand i of 8: K tile i / 4, step i % 4; V tile i
+    // operand i of 8: K tile i / 4, step i % 4; V tile i. fp4: K times its scale
+    __device__ __forceinline__ bf16x8 operand_k(int i) {
+        if constexpr (kFormat == DT_KV_FP4) return widen4(k[i >> 2][i & 3], __uint_as_float(k4[i >> 2] << 23));
+        else return operand(k, i);
+    }
+    __device__ __forceinline__ bf16x8 operand_v(int i) {
+        if constexpr (kFormat == DT_KV_FP4) return widen4(v[i >> 2][i & 3], 1.0f);
+        else return operand(v, i);
+    }
     static __device__ __forceinline__ bf16x8 operand(const u32x4 (&w)[kPieces], int i) {
         if constexpr (kFormat == DT_KV_BF16) return __builtin_bit_cast(bf16x8, w[i]);
         else return widen<kFormat>(w[i >> 1][(i & 1) * 2], w[i >> 1][(i & 1) * 2 + 1]);
@@ -213,6 +242,7 @@ struct Block {
 template <int kFormat>
 __device__ __forceinline__ int k_dim(int s, int g) {
     if constexpr (kFormat == DT_KV_BF16) return s * 32 + g * 8;
+    if constexpr (kFormat == DT_KV_FP4) return g * 32 + s * 8;
     return (s >> 1) * 64 + g * 16 + (s & 1) * 8;
 }
 
@@ -259,6 +289,7 @@ struct Shared {
 template <int kFormat, bool kF32, bool kOnce, int kQT>
 struct Stretch {
     static constexpr int kQS = kF32 ? 3 : 1, kStages = stages(kFormat, kF32, kQT);
+    static constexpr bool kFp4 = kFormat == DT_KV_FP4;
     Block<kFormat, kOnce> st[kStages];
     static constexpr int kQRegs = kF32 ? 8 : 4;
     u32x4 qraw[kQT][kQRegs];
@@ -272,7 +303,8 @@ struct Stretch {
     // for a block would be one for all loads.)
     __device__ __forceinline__ void load_k(Block<kFormat, kOnce>& b, int key) {
         const uint32_t beyond = key < k1 ? 0u : 0x80000000u;
-        b.load_k(rsrc, lane * 16 + beyond, (lane >> 4) * 16 + beyond, at);
+        // (fp4: the byte of the lane's key and group of values)
+        b.load_k(rsrc, lane * 16 + beyond, (kFormat == DT_KV_FP4 ? (lane & 15) * 4 + (lane >> 4) : (lane >> 4) * 16) + beyond, at);
     }
     __device__ __forceinline__ void load_v(Block<kFormat, kOnce>& b, int key) {
         const uint32_t beyond = key < k1 ? 0u : 0x80000000u;
@@ -365,6 +397,28 @@ struct Stretch {
         }
     }
 
+    // probabilities times V's scales as the matrix operand: rounded to bf16, or in three parts
+    static __device__ __forceinline__ void operand_p(float (&p)[8], bf16x8 (&pf)[kQS]) {
+#pragma unroll
+        for (int y = 0; y < kQS; ++y) {
+            union { uint32_t u[4]; bf16x8 v; } h;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                h.u[j] = pack2(p[2 * j], p[2 * j + 1]);
+                if (y + 1 < kQS) {
+                    p[2 * j] -= __uint_as_float(h.u[j] << 16);
+                    p[2 * j + 1] -= __uint_as_float(h.u[j] & 0xffff0000u);
+                }
+            }
+            pf[y] = h.v;
+        }
+    }
+
+    // byte i of a key's scales
+    static __device__ __forceinline__ float scale4(uint32_t w, int i) {
+        return __uint_as_float((i < 3 ? w << (23 - 8 * i) : w >> 1) & 0x7f800000u);
+    }
+
     __device__ __forceinline__ void attend(float scale, Shared<kQT>& sh) {
         const int n = lane & 15, g = lane >> 4;
         bf16x8 qf[kQT][kQS][4];
@@ -388,7 +442,7 @@ struct Stretch {
             for (int x = 0; x < kQT; ++x) s[x][0] = s[x][1] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const bf16x8 kf = blk.operand(blk.k, i);
+                const bf16x8 kf = blk.operand_k(i);
 #pragma unroll
                 for (int x = 0; x < kQT; ++x)
 #pragma unroll
@@ -400,13 +454,18 @@ struct Stretch {
 #pragma unroll
             for (int x = 0; x < kQT; ++x)
 #pragma unroll
-                for (int t = 0; t < 2; ++t) f[x][t] = blk.ks[t] * qscale[x];
+                for (int t = 0; t < 2; ++t) {
+                    if constexpr (kFormat == DT_KV_FP4) f[x][t] = (floatx4){qscale[x], qscale[x], qscale[x], qscale[x]};
+                    else f[x][t] = blk.ks[t] * qscale[x];
+                }
             keep_order();
             load_k(blk, next);
             keep_order();
             const bool mask = kb + kKvBlock > minlim;  // (the same for the whole wave)
             bf16x8 pf[kQT][kQS];
-            if (__builtin_expect(lowered, 0)) blk.vs[0] *= kLower, blk.vs[1] *= kLower;
+            float pe[kFp4 ? kQT : 1][8];  // fp4: the probabilities, as V's scales are one for each 32 values
+            if constexpr (!kFp4)
+                if (__builtin_expect(lowered, 0)) blk.vs[0] *= kLower, blk.vs[1] *= kLower;
 #pragma unroll
             for (int x = 0; x < kQT; ++x) {
                 const int rest = lim[x] - kb - g * 4;  // the lane's key 16 t + i is seen if it is below
@@ -434,32 +493,44 @@ struct Stretch {
                 for (int i = 0; i < 8; ++i) {
                     const float e = __builtin_amdgcn_exp2f(p[i] - base[x]);
                     add += e;
-                    p[i] = e * blk.vs[i >> 2][i & 3];
+                    if constexpr (kFp4) pe[x][i] = e;
+                    else p[i] = e * blk.vs[i >> 2][i & 3];
                 }
                 sum[x] += add;
+                if constexpr (kFp4) {
+                    if (__builtin_expect(lowered, 0))
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) pe[x][i] *= kLower;
+                    continue;
+                }
                 if (mask) {  // (a masked key's scale may be anything, NaN too)
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         if ((i >> 2) * 16 + (i & 3) >= rest) p[i] = 0.0f;
                 }
-#pragma unroll
-                for (int y = 0; y < kQS; ++y) {
-                    union { uint32_t u[4]; bf16x8 v; } h;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        h.u[j] = pack2(p[2 * j], p[2 * j + 1]);
-                        if (y + 1 < kQS) {
-                            p[2 * j] -= __uint_as_float(h.u[j] << 16);
-                            p[2 * j + 1] -= __uint_as_float(h.u[j] & 0xffff0000u);
-                        }
-                    }
-                    pf[x][y] = h.v;
-                }
+                operand_p(p, pf[x]);
             }
             blk.settle(blk.v);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const bf16x8 vf = blk.operand(blk.v, i);
+                if constexpr (kFp4) {
+                    if ((i & 1) == 0) {  // the next 32 values: P times their scales
+#pragma unroll
+                        for (int x = 0; x < kQT; ++x) {
+                            float p[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) p[j] = pe[x][j] * scale4(blk.v4[j >> 2][j & 3], i >> 1);
+                            if (mask) {  // (a masked key's scale may be anything, NaN too)
+                                const int rest = lim[x] - kb - g * 4;
+#pragma unroll
+                                for (int j = 0; j < 8; ++j)
+                                    if ((j >> 2) * 16 + (j & 3) >= rest) p[j] = 0.0f;
+                            }
+                            operand_p(p, pf[x]);
+                        }
+                    }
+                }
+                const bf16x8 vf = blk.operand_v(i);
 #pragma unroll
                 for (int x = 0; x < kQT; ++x)
 #pragma unroll
@@ -946,6 +1017,7 @@ int launch_rows(const CachedAttnArgs& a, const AttnRowsOf<kRows>& rows, bool joi
         };
         if (format == DT_KV_INT8) go_mode(std::integral_constant<int, DT_KV_INT8>());
         else if (format == DT_KV_FP8) go_mode(std::integral_constant<int, DT_KV_FP8>());
+        else if (format == DT_KV_FP4) go_mode(std::integral_constant<int, DT_KV_FP4>());
         else go_mode(std::integral_constant<int, DT_KV_BF16>());
         DT_HIP_TRY(hipGetLastError());
     }

@@ -8,8 +8,11 @@
 //         e4m3, ties to even: a power of two leaves the division exact, and e4m3's relative step does not gain from
 //         a finer scale; where the value would stand for more than fp32's range, the largest that does not
 //   bf16  value = x as bf16, scale 1
+//   fp4   four scales, one for each 32 values: the smallest power of two (at least 2^-120) with amax / scale <= 6, as its
+//         exponent + 127 in a byte each of the row's 32 bits; value = x / scale as e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6), ties to
+//         even; where it would stand for more than fp32's range, the largest that does not
 // A row that holds an infinity or a NaN (in bf16 also one that rounding makes infinite) has value 0 and scale
-// NaN: it reads back as NaN, and no held value is ever infinite or NaN. A masked key may then go through the
+// NaN (fp4: bytes of 255): it reads back as NaN, and no held value is ever infinite or NaN. A masked key may then go through the
 // matrix instructions with probability 0 (0 times a held value is 0).
 //
 // Per (slot, head), keys in blocks of 32 (the k extent of one v_mfma_f32_16x16x32_bf16), a block's K, V and scales behind
@@ -40,31 +43,37 @@ struct KvRowsOf {
 };
 using KvRows = KvRowsOf<kMaxRaggedBatch>;
 
-__host__ __device__ constexpr int kv_elem_bytes(int format) { return format == DT_KV_BF16 ? 2 : 1; }
+__host__ __device__ constexpr int kv_elem_bits(int format) { return format == DT_KV_BF16 ? 16 : format == DT_KV_FP4 ? 4 : 8; }
+__host__ __device__ constexpr int kv_elem_bytes(int format) { return kv_elem_bits(format) / 8; }  // (of formats that have whole ones)
 
 constexpr int kKvRun = 1024;  // bytes of a wave's load
-__host__ __device__ constexpr int kv_tensor_bytes(int format) { return kKvBlock * DT_HEAD_DIM * kv_elem_bytes(format); }
+constexpr int kKvGroup = 32;  // fp4: values of a scale
+constexpr uint32_t kKvNoScale = 255;  // fp4: the scale of a row that is none
+__host__ __device__ constexpr int kv_tensor_bytes(int format) { return kKvBlock * DT_HEAD_DIM * kv_elem_bits(format) / 8; }
 __host__ __device__ constexpr int kv_scale_at(int format) { return 2 * kv_tensor_bytes(format); }  // K's; V's behind
 __host__ __device__ constexpr int kv_block_bytes(int format) { return kv_scale_at(format) + 2 * kKvBlock * 4; }
 
 // Byte offset of value d (0..127) of key kk (0..31) in a block's K. The A operand of the 16x16x32 product takes 16 keys
 // (lane & 15) and 32 values d, 8 a lane group g = lane >> 4; which those are may be chosen freely as long as Q's fragment has the
-// same order. A 16-byte piece has 16 (8 bits) or 8 (bf16) consecutive ones: two steps, or one.
+// same order. A 16-byte piece has 16 (8 bits) or 8 (bf16) consecutive ones: two steps, or one. In fp4
+// it has 32, all four steps of the lane group, which share a scale; the offset is that of the byte, an even d in its low half.
 template <int kFormat>
 __host__ __device__ __forceinline__ int k_offset(int d, int kk) {
     const int tile = kk >> 4, m = kk & 15;
     if constexpr (kFormat == DT_KV_BF16) return tile * 4096 + (d >> 5) * kKvRun + ((d >> 3 & 3) * 16 + m) * 16 + (d & 7) * 2;
+    if constexpr (kFormat == DT_KV_FP4) return tile * kKvRun + ((d >> 5) * 16 + m) * 16 + ((d & 31) >> 1);
     return tile * 2048 + (d >> 6) * kKvRun + ((d >> 4 & 3) * 16 + m) * 16 + (d & 15);
 }
 
 // Byte offset of value d of key kk in a block's V. The operand takes 16 values d (lane & 15) and 32 keys, 8 a lane group.
 // P comes out of S^T's accumulators, where group g holds keys 4g..4g+3 of each 16-key tile: so slots 0..3 are those of the
-// first tile, 4..7 those of the second.
+// first tile, 4..7 those of the second. In fp4 two neighbouring keys share a byte, the even one in its low half.
 template <int kFormat>
 __host__ __device__ __forceinline__ int v_offset(int d, int kk) {
     const int g = (kk & 15) >> 2, j = (kk >> 4) * 4 + (kk & 3);
     const int mt = d >> 4, lane = g * 16 + (d & 15);
     if constexpr (kFormat == DT_KV_BF16) return mt * kKvRun + lane * 16 + j * 2;
+    if constexpr (kFormat == DT_KV_FP4) return (mt >> 2) * kKvRun + lane * 16 + (mt & 3) * 4 + (j >> 1);
     return (mt >> 1) * kKvRun + lane * 16 + (mt & 1) * 8 + j;
 }
 

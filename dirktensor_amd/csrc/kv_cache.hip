@@ -91,6 +91,40 @@ __device__ __forceinline__ void store16(void* p, int64_t at, const float (&x)[16
     }
 }
 
+// A group's values in 4 bits, its scale's byte; amax_bits: the group's largest |x| as bits, finite: whether the row is.
+template <int kN>
+__device__ __forceinline__ uint32_t quantise4(const float (&x)[kN], uint32_t amax_bits, bool finite, uint32_t (&out)[(kN + 7) / 8]) {
+    // amax = 1.f 2^a: the scale's exponent is a - 2, one more where 1.f > 1.5 (6 = 1.5 2^2)
+    int e = static_cast<int>(amax_bits >> 23) - 127 - 2 + ((amax_bits & 0x7fffffu) > 0x400000u ? 1 : 0);
+    e = !finite || e < -120 ? -120 : e;
+    const float inv = finite ? __uint_as_float(static_cast<uint32_t>(127 - e) << 23) : 0.0f;
+    // at the top of the range (scale 2^126) 4 would stand for an infinity: 3 is the last value
+    const float lim = e >= 126 ? 3.0f : 6.0f;
+    float y[kN];
+#pragma unroll
+    for (int i = 0; i < kN; ++i) y[i] = finite ? __builtin_amdgcn_fmed3f(x[i] * inv, -lim, lim) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < (kN + 7) / 8; ++i) {
+        uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, y[8 * i], y[8 * i + 1], 1.0f, 0);
+        if constexpr (kN >= 8) {
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[8 * i + 2], y[8 * i + 3], 1.0f, 1);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[8 * i + 4], y[8 * i + 5], 1.0f, 2);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[8 * i + 6], y[8 * i + 7], 1.0f, 3);
+        }
+        out[i] = w;
+    }
+    return finite ? static_cast<uint32_t>(127 + e) : kKvNoScale;
+}
+
+// 8 values of 4 bits times the scale of a byte
+__device__ __forceinline__ void dequantise4(uint32_t w, uint32_t scale, float* x) {
+    const float s = __uint_as_float(scale == kKvNoScale ? 0x7fc00000u : scale << 23);
+    const floatx2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1),
+                          __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[2 * i] = v[i][0] * s, x[2 * i + 1] = v[i][1] * s;
+}
+
 // kN (16, or 2 in the low bits of one word) of a row's 128 values, quantised; amax_bits: the row's largest |x| as bits. Returns
 // the scale.
 constexpr int words_of(int format, int n) { return (n * kv_elem_bytes(format) + 3) / 4; }
@@ -304,6 +338,174 @@ __global__ __launch_bounds__(kThreads) void kv_append_rows_kernel(KvMoveArgs a, 
     }
 }
 
+// The same of a block in 4 bits. Two neighbouring keys share V's bytes: where the call has both, their threads (eight lanes apart)
+// exchange their values and each writes half of the 16 bytes; a key whose neighbour is not the call's keeps that one's halves.
+template <bool kBf16, int kRows>
+__global__ __launch_bounds__(kThreads) void kv_append_fp4_kernel(KvMoveArgs a, KvRowsOf<kRows> rows) {
+    constexpr int kTensor = kv_tensor_bytes(DT_KV_FP4);
+    __shared__ __align__(16) uint8_t vbuf[kTensor / kKvRun * kRunLds];
+    const int b = blockIdx.z, h = blockIdx.y;
+    const int start = rows.len[b], cnt = rows.cnt[b];
+    const int blk = start / kKvBlock + static_cast<int>(blockIdx.x);
+    const int first = blk * kKvBlock;
+    if (first >= start + cnt) return;  // (whole workgroups)
+    const int kk = threadIdx.x >> 3, c = threadIdx.x & 7;
+    const int t = first + kk - start;
+    const auto ours = [&](int key) { return first + key >= start && first + key < start + cnt; };
+    const bool mine = ours(kk), both = mine && ours(kk ^ 1);
+    const bool whole = first >= start && first + kKvBlock <= start + cnt;
+
+    float x[16] = {}, y[16] = {};
+    uint32_t kmax = 0, vmax = 0;
+    if (mine) {
+        kmax = load16<kBf16>(a.k, b * a.bsk + t * a.ldk + h * DT_HEAD_DIM + c * 16, x);
+        vmax = load16<kBf16>(a.v, b * a.bsv + t * a.ldv + h * DT_HEAD_DIM + c * 16, y);
+    }
+    const auto other = [](uint32_t v, int o) { return static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), o, 64)); };
+    kmax = max(kmax, other(kmax, 1));  // (of the group)
+    vmax = max(vmax, other(vmax, 1));
+    uint32_t krow = max(kmax, other(kmax, 2)), vrow = max(vmax, other(vmax, 2));
+    krow = max(krow, other(krow, 4));
+    vrow = max(vrow, other(vrow, 4));
+    uint32_t qk[2], qv[2];
+    const uint32_t sk = quantise4(x, kmax, krow < kInfBits, qk), sv = quantise4(y, vmax, vrow < kInfBits, qv);
+    const uint32_t pv[2] = {other(qv[0], 8), other(qv[1], 8)};  // the neighbouring key's
+
+    uint8_t* block = a.c.block<DT_KV_FP4>(rows.slot[b], h, blk);
+    uint8_t* vd = block + kTensor;
+    if (mine) {
+        *reinterpret_cast<uint2*>(block + k_offset<DT_KV_FP4>(c * 16, kk)) = make_uint2(qk[0], qk[1]);
+        if (!(c & 1)) {
+            reinterpret_cast<uint8_t*>(scale_of<DT_KV_FP4>(block, false, kk))[c >> 1] = static_cast<uint8_t>(sk);
+            reinterpret_cast<uint8_t*>(scale_of<DT_KV_FP4>(block, true, kk))[c >> 1] = static_cast<uint8_t>(sv);
+        }
+        const int odd = kk & 1;
+        if (both) {
+            // values 8 odd .. 8 odd + 7 of both keys: the even key's in the low halves
+            const uint32_t even4 = odd ? pv[1] : qv[0], odd4 = odd ? qv[1] : pv[0];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint8_t v = static_cast<uint8_t>((even4 >> (4 * i) & 15) | (odd4 >> (4 * i) & 15) << 4);
+                const int d = c * 16 + odd * 8 + i;
+                if (whole) vbuf[v_lds_offset<DT_KV_FP4>(d, kk)] = v;
+                else vd[v_offset<DT_KV_FP4>(d, kk)] = v;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                uint8_t* to = vd + v_offset<DT_KV_FP4>(c * 16 + i, kk);
+                const uint32_t v = qv[i >> 3] >> (4 * (i & 7)) & 15;
+                *to = static_cast<uint8_t>(odd ? (*to & 15) | v << 4 : (*to & 0xf0) | v);
+            }
+        }
+    }
+    if (whole) {  // (the same for the whole workgroup)
+        __syncthreads();
+        if (threadIdx.x < kTensor / 16) {
+            const int o = threadIdx.x * 16;
+            *reinterpret_cast<uint4*>(vd + o) = *reinterpret_cast<const uint4*>(vbuf + (o >> 10) * kRunLds + (o & (kKvRun - 1)));
+        }
+    }
+}
+
+// Few tokens a sequence: a wave takes a pair of neighbouring keys, of which the call has one or both, of K (even) or V (odd), lane i
+// their values 2 i and 2 i + 1.
+template <bool kBf16, int kRows>
+__global__ __launch_bounds__(kThreads) void kv_append_rows_fp4_kernel(KvMoveArgs a, KvRowsOf<kRows> rows) {
+    const int lane = threadIdx.x & 63, unit = blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.z, h = unit >> 1;
+    const bool v = unit & 1;
+    const int start = rows.len[b], cnt = rows.cnt[b];
+    const int pos = (start & ~1) + 2 * static_cast<int>(blockIdx.y);  // the pair's even key
+    if (h >= a.c.heads || pos >= start + cnt) return;
+    const int d = 2 * lane;
+    const void* src = v ? a.v : a.k;
+    uint8_t* block = a.c.block<DT_KV_FP4>(rows.slot[b], h, pos / kKvBlock);
+    uint32_t q[2];
+    bool have[2];
+    float x[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int t = pos + i - start;
+        have[i] = t >= 0 && t < cnt;
+        x[i][0] = x[i][1] = 0.0f;
+        if (have[i]) {
+            const int64_t at = (v ? b * a.bsv + t * a.ldv : b * a.bsk + t * a.ldk) + h * DT_HEAD_DIM + d;
+            if constexpr (kBf16) {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(src) + at);
+                x[i][0] = bf16_lo(w), x[i][1] = bf16_hi(w);
+            } else {
+                const float2 w = *reinterpret_cast<const float2*>(static_cast<const float*>(src) + at);
+                x[i][0] = w.x, x[i][1] = w.y;
+            }
+        }
+    }
+    const int kk = pos & (kKvBlock - 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        uint32_t amax = max(__float_as_uint(x[i][0]) & 0x7fffffffu, __float_as_uint(x[i][1]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), o, 64)));
+        const bool finite = !__any(amax >= kInfBits);
+        uint32_t w[1];
+        const uint32_t s = quantise4<2>(x[i], amax, finite, w);
+        q[i] = w[0];
+        if (have[i] && (lane & 15) == 0)
+            reinterpret_cast<uint8_t*>(scale_of<DT_KV_FP4>(block, v, kk + i))[lane >> 4] = static_cast<uint8_t>(s);
+    }
+    if (!v) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (have[i]) block[k_offset<DT_KV_FP4>(d, kk + i)] = static_cast<uint8_t>(q[i]);
+    } else {
+        uint8_t* vd = block + kv_tensor_bytes(DT_KV_FP4);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint8_t* to = vd + v_offset<DT_KV_FP4>(d + i, kk);
+            const uint32_t lo = q[0] >> (4 * i) & 15, hi = q[1] >> (4 * i) & 15;
+            const uint32_t old = have[0] && have[1] ? 0 : *to;
+            *to = static_cast<uint8_t>((have[0] ? lo : old & 15) | (have[1] ? hi << 4 : old & 0xf0));
+        }
+    }
+}
+
+template <bool kBf16, int kRows>
+__global__ __launch_bounds__(kThreads) void kv_read_fp4_kernel(KvMoveArgs a, KvRowsOf<kRows> rows) {
+    constexpr int kTensor = kv_tensor_bytes(DT_KV_FP4);
+    __shared__ __align__(16) uint8_t vbuf[kTensor / kKvRun * kRunLds];
+    const int b = blockIdx.z, h = blockIdx.y;
+    const int start = rows.len[b], cnt = rows.cnt[b];
+    const int blk = start / kKvBlock + static_cast<int>(blockIdx.x);
+    const int first = blk * kKvBlock;
+    if (first >= start + cnt) return;
+    const int kk = threadIdx.x >> 3, c = threadIdx.x & 7;
+    const int t = first + kk - start;
+    const bool mine = t >= 0 && t < cnt;
+    uint8_t* block = a.c.block<DT_KV_FP4>(rows.slot[b], h, blk);
+    if (threadIdx.x < kTensor / 16) {
+        const int o = threadIdx.x * 16;
+        *reinterpret_cast<uint4*>(vbuf + (o >> 10) * kRunLds + (o & (kKvRun - 1))) = *reinterpret_cast<const uint4*>(block + kTensor + o);
+    }
+    const auto scale = [&](bool v) { return reinterpret_cast<const uint8_t*>(scale_of<DT_KV_FP4>(block, v, kk))[c >> 1]; };
+    float x[16];
+    if (mine) {
+        const uint2 w = *reinterpret_cast<const uint2*>(block + k_offset<DT_KV_FP4>(c * 16, kk));
+        dequantise4(w.x, scale(false), x);
+        dequantise4(w.y, scale(false), x + 8);
+        store16<kBf16>(a.k, b * a.bsk + t * a.ldk + h * DT_HEAD_DIM + c * 16, x);
+    }
+    __syncthreads();
+    if (mine) {
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            w[i >> 3] |= (static_cast<uint32_t>(vbuf[v_lds_offset<DT_KV_FP4>(c * 16 + i, kk)]) >> (4 * (kk & 1)) & 15) << (4 * (i & 7));
+        dequantise4(w[0], scale(true), x);
+        dequantise4(w[1], scale(true), x + 8);
+        store16<kBf16>(a.v, b * a.bsv + t * a.ldv + h * DT_HEAD_DIM + c * 16, x);
+    }
+}
+
 template <int kFormat, bool kBf16, int kRows>
 __global__ __launch_bounds__(kThreads) void kv_read_kernel(KvMoveArgs a, KvRowsOf<kRows> rows) {
     constexpr int kEs = kv_elem_bytes(kFormat), kWords = 4 * kEs, kTensor = kv_tensor_bytes(kFormat);
@@ -378,7 +580,24 @@ int launch_rows(const KvMoveArgs& a, const KvRowsOf<kRows>& rows, int B, int for
         if (bf16) DT_KV_GO(F, true);                                                                             \
         else DT_KV_GO(F, false);                                                                                 \
     } while (0)
-    if (format == DT_KV_INT8) DT_KV_GO2(DT_KV_INT8);
+    if (format == DT_KV_FP4) {
+        int pairs = 0;  // of neighbouring keys
+        for (int b = 0; b < B; ++b)
+            if (rows.cnt[b] > 0) pairs = std::max(pairs, (rows.len[b] + rows.cnt[b] - 1) / 2 - rows.len[b] / 2 + 1);
+        const dim3 grid4 = few ? dim3(grid.x, pairs, B) : grid;
+#define DT_KV_GO4(M)                                                                                                       \
+    do {                                                                                                                   \
+        if constexpr (kAppend) {                                                                                           \
+            if (few) hipLaunchKernelGGL((kv_append_rows_fp4_kernel<M, kRows>), grid4, block, 0, s, a, rows);               \
+            else hipLaunchKernelGGL((kv_append_fp4_kernel<M, kRows>), grid4, block, 0, s, a, rows);                        \
+        } else {                                                                                                           \
+            hipLaunchKernelGGL((kv_read_fp4_kernel<M, kRows>), grid4, block, 0, s, a, rows);                               \
+        }                                                                                                                  \
+    } while (0)
+        if (bf16) DT_KV_GO4(true);
+        else DT_KV_GO4(false);
+#undef DT_KV_GO4
+    } else if (format == DT_KV_INT8) DT_KV_GO2(DT_KV_INT8);
     else if (format == DT_KV_FP8) DT_KV_GO2(DT_KV_FP8);
     else DT_KV_GO2(DT_KV_BF16);
 #undef DT_KV_GO2
@@ -454,7 +673,7 @@ int dt_kv_cache_create(dt_ctx* ctx, int slots, int capacity, int n_heads, int D,
         return set_error(DT_ERR_INVALID_ARG, "capacity=%d outside [1, %d]", capacity, kMaxCacheTokens);
     if (n_heads < 1 || n_heads > kMaxCacheHeads)
         return set_error(DT_ERR_INVALID_ARG, "n_heads=%d outside [1, %d]", n_heads, kMaxCacheHeads);
-    if (format != DT_KV_INT8 && format != DT_KV_FP8 && format != DT_KV_BF16)
+    if (format != DT_KV_INT8 && format != DT_KV_FP8 && format != DT_KV_BF16 && format != DT_KV_FP4)
         return set_error(DT_ERR_INVALID_ARG, "unknown cache format %d", format);
     if (!ctx) return set_error(DT_ERR_INVALID_ARG, "ctx is NULL");
     DeviceScope scope;

@@ -386,6 +386,9 @@ int dt_ce_loss(dt_ctx* ctx, const float* logits, const int32_t* tokens, int B, i
  *   DT_KV_FP8   scale = the smallest power of two >= 2^-126 with amax / scale <= 448; value = x / scale as OCP
  *               e4m3, ties to even (where that would stand for more than fp32's range, the largest that does not)
  *   DT_KV_BF16  x as bf16
+ *   DT_KV_FP4   in place of the one scale four bytes, a power of two for each 32 values: the smallest >= 2^-120 with amax / scale
+ *               <= 6; value = x / scale as e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6), ties to even (where that would stand for more than
+ *               fp32's range, the largest that does not)
  * A row that holds an infinity or a NaN (DT_KV_BF16: also one whose rounding is infinite) reads back as NaN in all its
  * places, and a query that sees it gets NaN. Rows of zeros are held exactly.
  * The lengths of the slots are host state of the handle: the calls below read and advance them when they are made,
@@ -397,6 +400,7 @@ int dt_ce_loss(dt_ctx* ctx, const float* logits, const int32_t* tokens, int B, i
 #define DT_KV_INT8 0
 #define DT_KV_FP8 1
 #define DT_KV_BF16 2
+#define DT_KV_FP4 4
 typedef struct dt_kv_cache dt_kv_cache;
 int dt_kv_cache_create(dt_ctx* ctx, int slots, int capacity, int n_heads, int D, int format, dt_kv_cache** out);
 int dt_kv_cache_destroy(dt_kv_cache* cache);
