@@ -8,13 +8,18 @@
 //   w = p_{n+1}            where all were accepted.
 // At T = 0 a draft is accepted where it is the largest logit's token (the first of equals), and that token is the one that follows.
 //
-// A token is one side of a border or the other, and there are as many borders as tokens in the vocabulary: sums whose terms are off by
-// 2^-24 would give another token about once in a few hundred calls. So probabilities and sums are held in 64 bits, the terms to 10^-12.
+// A token is one side of a border or the other, and there are as many borders as tokens in the vocabulary: weights that are off by
+// 2^-24 of their probability would give another token about once in a few hundred calls. So the weights and their sums are held in
+// 64 bits, the terms to 10^-12. The rows' sums that decide on drafts (one border each) are of terms in 32 bits, summed in 64; the largest
+// term is exact, so the log probability of a token that is almost certain is, too.
 //
-// Work: every row is read once for its sum (first kernel: a row in segments, as many as fill the CUs), and behind a refused draft the two
-// rows that the weights come from once more, mostly from the caches (second kernel: 2048 values of a batch row a workgroup; each
-// works out from the first kernel's sums which draft was refused). The last workgroup of a batch row to leave its weights' sum finds
-// the segment that the border lies in, and in it the token.
+// Work: every row is read once for its sum (first kernel: a row in segments, as many as fill the CUs), and the one or two rows that the
+// weights come from once more, mostly from the caches (second kernel: each workgroup works out from the first kernel's sums which draft
+// was refused, and its waves take chunks of 1024 values). The weights' difference needs the ratio of both rows' sums, which is known
+// to 2^-24 only: a chunk leaves sum p' and sum q' over the values with p' > ratio q' (p', q': the powers, not divided by their sums),
+// and over all of them; the last workgroup of a batch row to be done has the ratio to 64 bits then, and a value whose sign the first
+// ratio got wrong has a weight below 2^-23 of its probability. Only where the weights' total is itself small (below kSmall) does that
+// count: that workgroup then sums the weights again. Last it finds the chunk that the border lies in, and in it the token.
 
 #include "dt_internal.h"
 
@@ -34,14 +39,15 @@ constexpr int kFewRows = 32;
 constexpr int kMaxDrafts = 64;
 constexpr int kMaxRows = 2 * kMaxDrafts + 1;  // of a batch row
 constexpr int kMaxVocab = 1 << 24;
-constexpr int kOwn = 8;                       // values of a thread in the second kernel
-constexpr int kSegment = kOwn * kThreads;
+constexpr int kChunk = 1024;                  // values that a wave of the second kernel takes at a time: 16 a lane
+constexpr int kWhole = 4096;                  // of a batch of the first kernel, all threads
 constexpr int kMinSegment = 2048;             // values of a segment of the first kernel at least
 constexpr int kFill = 2048;                   // workgroups that the first kernel aims at, eight a CU
+constexpr int kDrawFill = 1024;               // and the second
+constexpr double kSmall = 1e-4;
 constexpr double kLog2e = 1.4426950408889634074;
 constexpr double kLn2 = 0.69314718055994530942;
 constexpr double kFar = -1000.0;              // 2^kFar and below counts as 0
-constexpr double kNear = 500.0;               // a term may be 2^kNear; above it the sum's reference moves
 constexpr float kLowest = -3.402823466e38f;
 
 template <int kRows>
@@ -54,15 +60,16 @@ struct VerifyArgs {
     int32_t* tokens;      // [B, K + 1]
     float* logprob;       // [B, K + 1]
     int32_t* count;       // [B]: workgroups of the second kernel that are done
-    double2* part;        // [B][rows][segments]: one of the logits as reference, and the sum of 2^(c (x - reference))
+    double2* part;        // [B][rows][segments]: the largest logit, and the sum of 2^(c (x - it))
     float2* best;         // [B][K + 1][segments] at T = 0: the largest logit, its index (as bits)
-    double* total;        // [B][own segments]
+    double* sums;         // [B][chunks][4]: sum p' and q' of the values with a weight, of all
     int64_t ldb_x, ldt_x, ldb_y, ldt_y;
     double c;             // log2(e) / T
+    float c_hi, c_lo;     // in two parts, both above 0 (a logit of -inf times either is -inf)
     int K, V, tok_bytes;
     int rows;             // of a batch row: K + 1, and K of the drafts
     int segments, segment;  // of the first kernel, values of one
-    int own_segments;     // of the second
+    int chunks, runs;     // of the second, at most one a thread; a chunk has so many times kChunk values
     uint8_t n[kRows];     // drafts of each batch row
 };
 
@@ -87,6 +94,11 @@ __device__ __forceinline__ double exp2_64(double t) {
 template <bool kBf16>
 constexpr int kPer = kBf16 ? 8 : 4;  // values of a 16-byte piece
 
+template <bool kBf16>
+__device__ __forceinline__ float load_one(const void* row, int at) {
+    if constexpr (kBf16) return __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(row)[at]) << 16);
+    else return static_cast<const float*>(row)[at];
+}
 // the values at..at+15 bytes of a row; with fewer than a whole piece left, one by one (and -inf behind the end)
 template <bool kBf16>
 __device__ __forceinline__ void load_piece(const void* row, int at, int end, float (&x)[kPer<kBf16>]) {
@@ -103,18 +115,14 @@ __device__ __forceinline__ void load_piece(const void* row, int at, int end, flo
         return;
     }
 #pragma unroll
-    for (int i = 0; i < kPer<kBf16>; ++i) {
-        x[i] = -__builtin_huge_valf();
-        if (at + i < end) {
-            if constexpr (kBf16) x[i] = __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(row)[at + i]) << 16);
-            else x[i] = static_cast<const float*>(row)[at + i];
+    for (int i = 0; i < kPer<kBf16>; ++i) x[i] = -__builtin_huge_valf();
+    if (at < end) {  // (all loads at once)
+#pragma unroll
+        for (int i = 0; i < kPer<kBf16>; ++i) {
+            const float v = load_one<kBf16>(row, min(at + i, end - 1));
+            if (at + i < end) x[i] = v;
         }
     }
-}
-template <bool kBf16>
-__device__ __forceinline__ float load_one(const void* row, int at) {
-    if constexpr (kBf16) return __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(row)[at]) << 16);
-    else return static_cast<const float*>(row)[at];
 }
 
 // row r of a batch row: the model's (r <= K) or the drafts'
@@ -124,79 +132,163 @@ __device__ __forceinline__ const void* row_of(const VerifyArgs<kRows>& a, int b,
     return static_cast<const char*>(r <= a.K ? a.x : a.y) + at * (kBf16 ? 2 : 4);
 }
 
-// a sum of 2^(c (x - ref)), joined with another. (Differences of logits are exact in 64 bits, or their smaller one does not count; their
-// products with c are not, which would show in logits of 10^6 and more.)
-__device__ __forceinline__ void join(double c, double& ref, double& sum, double r2, double s2) {
-    const double to = ref > r2 ? ref : r2;
-    sum = sum * exp2_64(c * (ref - to)) + s2 * exp2_64(c * (r2 - to));
-    ref = to;
+// Sums over a wave without LDS: within 16 lanes by data-parallel moves, across by permutes of halves.
+template <int kCtrl, int kRowMask>
+__device__ __forceinline__ double moved(double x) {  // (0 from lanes that are none, in rows that are masked)
+    const uint64_t u = static_cast<uint64_t>(__double_as_longlong(x));
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), kCtrl, kRowMask, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), kCtrl, kRowMask, 0xf, false);
+    return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(hi) << 32 | lo));
+}
+__device__ __forceinline__ double sum16(double x) {
+    x += moved<0xb1, 0xf>(x);   // the neighbour
+    x += moved<0x4e, 0xf>(x);   // the other pair of four
+    x += moved<0x141, 0xf>(x);  // mirrored within 8
+    return x + moved<0x140, 0xf>(x);  // and within 16
+}
+template <bool k32>
+__device__ __forceinline__ double sum_halves(double x) {
+    const uint64_t u = static_cast<uint64_t>(__double_as_longlong(x));
+    const uint32_t l = static_cast<uint32_t>(u), h = static_cast<uint32_t>(u >> 32);
+    const auto lo = k32 ? __builtin_amdgcn_permlane32_swap(l, l, false, false) : __builtin_amdgcn_permlane16_swap(l, l, false, false);
+    const auto hi = k32 ? __builtin_amdgcn_permlane32_swap(h, h, false, false) : __builtin_amdgcn_permlane16_swap(h, h, false, false);
+    const auto join = [](uint32_t a, uint32_t b) { return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(b) << 32 | a)); };
+    return join(lo[0], hi[0]) + join(lo[1], hi[1]);
+}
+__device__ __forceinline__ double sum_wave(double x) { return sum_halves<true>(sum_halves<false>(sum16(x))); }
+// the sums of a lane's and all lower lanes' values
+__device__ __forceinline__ double scan_wave(double x) {
+    x += moved<0x111, 0xf>(x);
+    x += moved<0x112, 0xf>(x);
+    x += moved<0x114, 0xf>(x);
+    x += moved<0x118, 0xf>(x);
+    x += moved<0x142, 0xa>(x);  // the last lane of a row of 16 to the next, of 32 to the other half
+    return x + moved<0x143, 0xc>(x);
 }
 
+// kPieces whole pieces of a thread, and their values
+template <bool kBf16, int kN>
+__device__ __forceinline__ void load_batch(const void* row, int at, u32x4 (&w)[kN]) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+        const int to = at + i * kThreads * kPer<kBf16>;
+        if constexpr (kBf16) w[i] = *reinterpret_cast<const u32x4_at2*>(static_cast<const uint16_t*>(row) + to);
+        else w[i] = *reinterpret_cast<const u32x4_at4*>(static_cast<const float*>(row) + to);
+    }
+}
+template <bool kBf16, int kN>
+__device__ __forceinline__ void open_batch(const u32x4 (&w)[kN], float (&x)[kN][kPer<kBf16>]) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (kBf16) x[i][2 * j] = __uint_as_float(w[i][j] << 16), x[i][2 * j + 1] = __uint_as_float(w[i][j] & 0xffff0000u);
+            else x[i][j] = __uint_as_float(w[i][j]);
+        }
+}
+
+// 2^(c d) in 32 bits, for d <= 0
+template <int kRows>
+__device__ __forceinline__ float power(const VerifyArgs<kRows>& a, float d) {
+    return __builtin_amdgcn_exp2f(fmaf(d, a.c_hi, d * a.c_lo));
+}
 template <bool kBf16, bool kGreedy, int kRows>
 __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs<kRows> a) {
     constexpr int P = kPer<kBf16>;
     constexpr int kPieces = kBf16 ? 2 : 4;  // under way at once
-    __shared__ double2 red[kWaves];
+    __shared__ double red[kWaves];
+    __shared__ float red_top[kWaves];
     __shared__ float2 red_best[kWaves];
     const int b = blockIdx.z, r = blockIdx.y, seg = blockIdx.x, n = a.n[b];
     if (seg == 0 && r == 0 && threadIdx.x == 0) a.count[b] = 0;
     if (r <= a.K ? r > n : r - a.K - 1 >= n) return;
     const void* row = row_of<kBf16>(a, b, r);
     const int from = seg * a.segment, end = min(a.V, from + a.segment);
-    const double c = a.c;
-    double ref = kLowest, sum = 0.0;
-    float top = -__builtin_huge_valf();
-    int top_at = from;
-    for (int at = from + static_cast<int>(threadIdx.x) * P; at < end; at += kPieces * kThreads * P) {
-        float x[kPieces][P];
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) load_piece<kBf16>(row, at + i * kThreads * P, end, x[i]);
-        float most = x[0][0];
+    float top = kLowest, best = -__builtin_huge_valf();
+    double sum = 0.0;
+    int best_at = from;
+    constexpr int kBatch = kPieces * kThreads * P;
+    static_assert(kBatch == kWhole, "segments of whole batches");
+    const auto take = [&](const float (&x)[kPieces][P], int at) {
+        float most = top;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i)
 #pragma unroll
             for (int j = 0; j < P; ++j) {
                 most = fmaxf(most, x[i][j]);
-                if (kGreedy && x[i][j] > top) top = x[i][j], top_at = at + i * kThreads * P + j;
+                if (kGreedy && x[i][j] > best) best = x[i][j], best_at = at + i * kThreads * P + j;
             }
-        if ((most - ref) * c > kNear) {  // (seldom: the first values, and those far above them)
-            sum *= exp2_64((ref - most) * c);
-            ref = most;
-        }
+        sum *= exp2_64((static_cast<double>(top) - most) * a.c);
+        top = most;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i)
 #pragma unroll
-            for (int j = 0; j < P; ++j) sum += exp2_64((x[i][j] - ref) * c);
+            for (int j = 0; j < P; ++j) sum += static_cast<double>(power(a, x[i][j] - top));
+    };
+    // whole batches, two under way (the last ones are loaded twice, from the caches: a load under a condition would make every wait one
+    // for all loads); then what is left
+    int at = from + static_cast<int>(threadIdx.x) * P;
+    const int whole = (end - from) / kBatch;
+    if (whole > 0) {
+        u32x4 w[2][kPieces];
+        const auto load = [&](int i, u32x4 (&to)[kPieces]) { load_batch<kBf16>(row, at + min(i, whole - 1) * kBatch, to); };
+        const auto use = [&](int i, u32x4 (&of)[kPieces]) {
+            float x[kPieces][P];
+            open_batch<kBf16>(of, x);
+            take(x, at + i * kBatch);
+        };
+        load(0, w[0]);
+        load(1, w[1]);
+        int i = 0;
+        for (; i + 1 < whole; i += 2) {
+            use(i, w[0]);
+            load(i + 2, w[0]);
+            use(i + 1, w[1]);
+            load(i + 3, w[1]);
+        }
+        if (i < whole) use(i, w[0]);
+        at += whole * kBatch;
     }
+    if (whole * kBatch < end - from) {
+        float x[kPieces][P];
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) load_piece<kBf16>(row, at + i * kThreads * P, end, x[i]);
+        take(x, at);
+    }
+    // the threads' sums meet: brought to the largest logit of all, each by one factor
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float most = top;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) {
-        join(c, ref, sum, __shfl_xor(ref, o, 64), __shfl_xor(sum, o, 64));
+        most = fmaxf(most, __shfl_xor(most, o, 64));
         if constexpr (kGreedy) {
-            const float t2 = __shfl_xor(top, o, 64);
-            const int a2 = __shfl_xor(top_at, o, 64);
-            if (t2 > top || (t2 == top && a2 < top_at)) top = t2, top_at = a2;
+            const float t2 = __shfl_xor(best, o, 64);
+            const int a2 = __shfl_xor(best_at, o, 64);
+            if (t2 > best || (t2 == best && a2 < best_at)) best = t2, best_at = a2;
         }
     }
-    if ((threadIdx.x & 63) == 0) {
-        red[threadIdx.x >> 6] = make_double2(ref, sum);
-        if constexpr (kGreedy) red_best[threadIdx.x >> 6] = make_float2(top, __int_as_float(top_at));
+    if (lane == 0) {
+        red_top[wave] = most;
+        if constexpr (kGreedy) red_best[wave] = make_float2(best, __int_as_float(best_at));
     }
     __syncthreads();
+    most = fmaxf(fmaxf(red_top[0], red_top[1]), fmaxf(red_top[2], red_top[3]));
+    sum = sum_wave(sum * exp2_64((static_cast<double>(top) - most) * a.c));
+    if (lane == 0) red[wave] = sum;
+    __syncthreads();
     if (threadIdx.x != 0) return;
+    sum = red[0] + red[1] + red[2] + red[3];
+    a.part[(static_cast<int64_t>(b) * a.rows + r) * a.segments + seg] = make_double2(most, sum);
+    if constexpr (kGreedy) {
 #pragma unroll
-    for (int i = 1; i < kWaves; ++i) {
-        join(c, ref, sum, red[i].x, red[i].y);
-        if constexpr (kGreedy) {
+        for (int i = 1; i < kWaves; ++i) {
             const float t2 = red_best[i].x;
             const int a2 = __float_as_int(red_best[i].y);
-            if (t2 > top || (t2 == top && a2 < top_at)) top = t2, top_at = a2;
+            if (t2 > best || (t2 == best && a2 < best_at)) best = t2, best_at = a2;
         }
+        a.best[(static_cast<int64_t>(b) * (a.K + 1) + r) * a.segments + seg] = make_float2(best, __int_as_float(best_at));
     }
-    a.part[(static_cast<int64_t>(b) * a.rows + r) * a.segments + seg] = make_double2(ref, sum);
-    if constexpr (kGreedy) a.best[(static_cast<int64_t>(b) * (a.K + 1) + r) * a.segments + seg] = make_float2(top, __int_as_float(top_at));
 }
-
-__device__ __forceinline__ double log2_p(double c, float x, double2 row) { return fma(x - row.x, c, -row.y); }
 
 template <int kRows>
 __device__ __forceinline__ int draft_of(const VerifyArgs<kRows>& a, int b, int i) {
@@ -209,12 +301,7 @@ __device__ __forceinline__ int draft_of(const VerifyArgs<kRows>& a, int b, int i
 // sums before a thread's own of the workgroup's, in the threads' order, and of all
 __device__ __forceinline__ double scan(double v, double (&red)[kWaves], double* all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    double s = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double before = __shfl_up(s, o, 64);
-        if (lane >= o) s += before;
-    }
+    const double s = scan_wave(v);
     __syncthreads();
     if (lane == 63) red[wave] = s;
     __syncthreads();
@@ -228,226 +315,311 @@ __device__ __forceinline__ double scan(double v, double (&red)[kWaves], double* 
     return base + (s - v);
 }
 
+__device__ __forceinline__ double sum_all(double v, double (&red)[kWaves]) {
+    v = sum_wave(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) s += red[i];
+    return s;
+}
+
+// log2 of a sum, at least 1: the instruction's, once corrected
+__device__ __forceinline__ double log2_64(double s) {
+    const double y = static_cast<double>(__builtin_amdgcn_logf(static_cast<float>(s)));
+    return y + (s * exp2_64(-y) - 1.0) * kLog2e;
+}
+
+// The two rows that the weights come from: p', 0 for a draft that nothing was drawn for, and q', 0 where there is no such row. Their
+// values go by twos through loops that are not unrolled: a kernel that runs once through its code waits for the code, too.
+struct Rows {
+    const void *px, *qx;  // qx: or NULL
+    double p_top, q_top, c;
+    int skip, V;
+    __device__ __forceinline__ void powers(float x, float y, int at, double& p, double& q) const {
+        p = exp2_64((static_cast<double>(x) - p_top) * c);
+        if (at == skip) p = 0.0;
+        q = 0.0;
+        if (qx) q = exp2_64((static_cast<double>(y) - q_top) * c);
+    }
+};
+// 8 values of a row as four pairs of words (bf16: two in a word)
+struct Eight {
+    uint32_t lo[4], hi[4];
+    template <bool kBf16>
+    __device__ __forceinline__ void load(const void* row, int at, int end) {
+        constexpr int P = kPer<kBf16>;
+#pragma unroll
+        for (int i = 0; i < 8 / P; ++i) {
+            float x[P];
+            load_piece<kBf16>(row, at + i * P, end, x);
+#pragma unroll
+            for (int j = 0; j < P / 2; ++j) {
+                lo[i * P / 2 + j] = __float_as_uint(x[2 * j]);
+                hi[i * P / 2 + j] = __float_as_uint(x[2 * j + 1]);
+            }
+        }
+    }
+    __device__ __forceinline__ void next() {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) lo[i] = lo[i + 1], hi[i] = hi[i + 1];
+    }
+};
+
 template <bool kBf16, bool kGreedy, int kRows>
 __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs<kRows> a) {
-    __shared__ double2 lse[kMaxRows];  // each row's reference, and log2 of its sum; NaN of a row that has none
+    __shared__ float tops[kMaxRows];
+    __shared__ double sums[kMaxRows];  // NaN of a row that has none
     __shared__ int best[kMaxDrafts + 1];
-    __shared__ float score[kMaxDrafts + 1];
+    __shared__ float draft_x[kMaxDrafts];
     __shared__ int drafts[kMaxDrafts];
     __shared__ double red[kWaves];
-    __shared__ int sh_accepted, sh_last, sh_at;
-    const int b = blockIdx.y, seg = blockIdx.x, tid = threadIdx.x, n = a.n[b], K = a.K, V = a.V;
+    __shared__ double sh_before;
+    __shared__ int sh_over[kWaves], sh_some[kWaves];
+    __shared__ int sh_accepted, sh_last, sh_token;
+    __shared__ float sh_logit;
+    const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = a.n[b], K = a.K, V = a.V;
 
-    // the rows' sums: 16 lanes a row
+    // the drafts' logits, while the rows' sums are joined: 16 lanes a row
+    int draft = -1;
+    float x = 0.0f, y = 0.0f, u = 0.0f;
+    if (tid < n) {
+        draft = draft_of(a, b, tid);
+        if (!kGreedy) u = a.u[static_cast<int64_t>(b) * (K + 1) + tid];
+        if (draft >= 0 && draft < V) {
+            x = load_one<kBf16>(row_of<kBf16>(a, b, tid), draft);
+            if (a.y) y = load_one<kBf16>(row_of<kBf16>(a, b, K + 1 + tid), draft);
+        }
+    }
+    const double last_u = kGreedy ? 0.0 : a.u[static_cast<int64_t>(b) * (K + 1) + K];
     const int own_rows = n + 1 + (a.y ? n : 0);
     for (int i = tid >> 4; i < own_rows; i += kThreads / 16) {
         const int r = i <= n ? i : K + 1 + (i - n - 1);
         const double2* p = a.part + (static_cast<int64_t>(b) * a.rows + r) * a.segments;
-        double ref = kLowest, sum = 0.0;
-        float top = -__builtin_huge_valf();
-        int top_at = 0;
-        for (int s = tid & 15; s < a.segments; s += 16) {
-            const double2 v = p[s];
-            join(a.c, ref, sum, v.x, v.y);
-            if (kGreedy) {
-                const float2 w = a.best[(static_cast<int64_t>(b) * (K + 1) + r) * a.segments + s];
-                if (w.x > top) top = w.x, top_at = __float_as_int(w.y);
+        // (four of a lane's segments at a time; rows of more are brought from one largest logit to the next)
+        float top = kLowest, most = -__builtin_huge_valf();
+        double sum = 0.0;
+        int most_at = 0;
+        for (int s = tid & 15; s < a.segments; s += 64) {
+            double2 v[4];
+            float to = top;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[j] = s + 16 * j < a.segments ? p[s + 16 * j] : make_double2(kLowest, 0.0);
+                if (kGreedy && s + 16 * j < a.segments) {
+                    const float2 w = a.best[(static_cast<int64_t>(b) * (K + 1) + r) * a.segments + s + 16 * j];
+                    if (w.x > most) most = w.x, most_at = __float_as_int(w.y);
+                }
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to = fmaxf(to, static_cast<float>(v[j].x));
+            sum *= exp2_64((static_cast<double>(top) - to) * a.c);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum += v[j].y * exp2_64((v[j].x - to) * a.c);
+            top = to;
         }
+        float to = top;
 #pragma unroll
         for (int o = 8; o >= 1; o >>= 1) {
-            join(a.c, ref, sum, __shfl_xor(ref, o, 16), __shfl_xor(sum, o, 16));
+            to = fmaxf(to, __shfl_xor(to, o, 16));
             if (kGreedy) {
-                const float t2 = __shfl_xor(top, o, 16);
-                const int a2 = __shfl_xor(top_at, o, 16);
-                if (t2 > top || (t2 == top && a2 < top_at)) top = t2, top_at = a2;
+                const float t2 = __shfl_xor(most, o, 16);
+                const int a2 = __shfl_xor(most_at, o, 16);
+                if (t2 > most || (t2 == most && a2 < most_at)) most = t2, most_at = a2;
             }
         }
+        sum *= exp2_64((static_cast<double>(top) - to) * a.c);
+        sum = sum16(sum);
         if ((tid & 15) == 0) {
-            const double l = sum > 0.0 ? log2(sum) : __builtin_nan("");
-            lse[i <= n ? i : K + 1 + (i - n - 1)] = make_double2(ref, l);
-            if (kGreedy) best[i] = l == l ? top_at : -1;
+            tops[r] = to;
+            sums[r] = sum > 0.0 ? sum : __builtin_nan("");
+            if (kGreedy) best[i] = sum > 0.0 ? most_at : -1;
         }
     }
     __syncthreads();
-    if (tid < 64) {
+    if (wave == 0) {
         bool ok = false;
         if (tid < n) {
-            const int d = draft_of(a, b, tid);
-            float lp = 0.0f;
-            if (d >= 0 && d < V) {
-                const double t = log2_p(a.c, load_one<kBf16>(row_of<kBf16>(a, b, tid), d), lse[tid]);
-                lp = static_cast<float>(t * kLn2);
-                if (kGreedy) ok = d == best[tid];
+            if (draft >= 0 && draft < V) {
+                if (kGreedy) ok = draft == best[tid];
                 else {
-                    double q = 1.0;
-                    if (a.y) q = exp2_64(log2_p(a.c, load_one<kBf16>(row_of<kBf16>(a, b, K + 1 + tid), d), lse[K + 1 + tid]));
-                    ok = a.u[static_cast<int64_t>(b) * (K + 1) + tid] * q < exp2_64(t);
+                    // u q < p, times both sums
+                    const double p = exp2_64((static_cast<double>(x) - tops[tid]) * a.c);
+                    double q = u * sums[tid];
+                    if (a.y) q *= exp2_64((static_cast<double>(y) - tops[K + 1 + tid]) * a.c);
+                    ok = q < (a.y ? p * sums[K + 1 + tid] : p);
                 }
             }
-            drafts[tid] = d;
-            score[tid] = lp;
+            drafts[tid] = draft;
+            draft_x[tid] = x;
         }
         const uint64_t yes = __ballot(ok);
         if (tid == 0) sh_accepted = yes == ~0ull ? 64 : __builtin_ctzll(~yes);
     }
     __syncthreads();
     const int acc = sh_accepted;
-    // results of row b: the accepted drafts, `token` and its log probability, then nothing
-    const auto finish = [&](int token) {
-        for (int i = tid; i <= K; i += kThreads) {
-            const int64_t at = static_cast<int64_t>(b) * (K + 1) + i;
-            if (i < acc) {
-                a.tokens[at] = drafts[i];
-                a.logprob[at] = score[i];
-            } else if (i == acc) {
-                a.tokens[at] = token;
-                a.logprob[at] = token < 0 ? __builtin_nanf("")
-                                          : static_cast<float>(log2_p(a.c, load_one<kBf16>(row_of<kBf16>(a, b, i), token), lse[i]) * kLn2);
-            } else {
-                a.tokens[at] = -1;
-                a.logprob[at] = 0.0f;
-            }
-        }
-        if (tid == 0) a.accepted[b] = acc;
-    };
+    int token = -1;    // the one that follows
+    double sum = sums[acc];
     if constexpr (kGreedy) {
-        finish(best[acc]);
-        return;
-    }
-
-    // the weights of the thread's values, at seg * kSegment + tid * kOwn
-    const void* px = row_of<kBf16>(a, b, acc);
-    const bool refused = acc < n;
-    const int not_this = refused && !a.y ? drafts[acc] : -1;
-    const void* qx = refused && a.y ? row_of<kBf16>(a, b, K + 1 + acc) : nullptr;
-    const double2 lp = lse[acc], lq = lse[qx ? K + 1 + acc : acc];
-    bool plain = false;  // w = p: the difference left nothing
-    const auto weights = [&](int at, double (&w)[kOwn]) {
-        constexpr int P = kPer<kBf16>;
-#pragma unroll
-        for (int i = 0; i < kOwn / P; ++i) {
-            float x[P];
-            load_piece<kBf16>(px, at + i * P, V, x);
-#pragma unroll
-            for (int j = 0; j < P; ++j) w[i * P + j] = exp2_64(log2_p(a.c, x[j], lp));
+        token = best[acc];
+    } else {
+        const bool refused = acc < n;
+        Rows rows{row_of<kBf16>(a, b, acc), refused && a.y ? row_of<kBf16>(a, b, K + 1 + acc) : nullptr, tops[acc], 0.0, a.c,
+                  refused && !a.y ? drafts[acc] : -1, V};
+        double near = 0.0;  // the ratio of the rows' sums, to 32 bits
+        if (rows.qx) {
+            rows.q_top = tops[K + 1 + acc];
+            near = sums[acc] / sums[K + 1 + acc];
         }
-        if (plain) return;
-        if (qx) {
+        double* out = a.sums + static_cast<int64_t>(b) * a.chunks * 4;
+        double h[4], p_sum = 0.0, ratio = 0.0, weight, before, all;
+        int first = blockIdx.x * kWaves + wave, step = gridDim.x * kWaves;
+        for (bool again = false;; again = true) {
+#pragma unroll 1
+            for (int chunk = first; chunk < a.chunks; chunk += step) {
+                double pw = 0.0, qw = 0.0, pa = 0.0, qa = 0.0;
+#pragma unroll 1
+                for (int at = chunk * a.runs * kChunk + lane * 8, end = at + a.runs * kChunk; at < end; at += kChunk) {
+                    Eight x[2], y[2];
 #pragma unroll
-            for (int i = 0; i < kOwn / P; ++i) {
-                float x[P];
-                load_piece<kBf16>(qx, at + i * P, V, x);
+                    for (int i = 0; i < 2; ++i) {
+                        x[i].load<kBf16>(rows.px, at + i * (kChunk / 2), V);
+                        if (rows.qx) y[i].load<kBf16>(rows.qx, at + i * (kChunk / 2), V);
+                    }
+#pragma unroll 1
+                    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int j = 0; j < P; ++j) {
-                    const double d = w[i * P + j] - exp2_64(log2_p(a.c, x[j], lq));
-                    w[i * P + j] = d < 0.0 ? 0.0 : d;  // (NaN stays)
+                        for (int j = 0; j < 4; ++j) {
+                            double p, q;
+                            rows.powers(__uint_as_float(j & 1 ? x[j >> 1].hi[0] : x[j >> 1].lo[0]),
+                                        __uint_as_float(j & 1 ? y[j >> 1].hi[0] : y[j >> 1].lo[0]), at + (j >> 1) * (kChunk / 2) + 2 * i + (j & 1), p, q);
+                            const bool some = p > near * q;
+                            pa += p;
+                            qa += q;
+                            pw += some ? p : 0.0;
+                            qw += some ? q : 0.0;
+                        }
+                        x[0].next(), x[1].next(), y[0].next(), y[1].next();
+                    }
                 }
-            }
-        } else {
+                const double mine[4] = {pw, qw, pa, qa};
+                double to = 0.0;
 #pragma unroll
-            for (int i = 0; i < kOwn; ++i)
-                if (at + i == not_this) w[i] = 0.0;
-        }
-    };
-    const auto own_sum = [&](int at, double (&w)[kOwn]) {
-        double s = 0.0;
-        weights(at, w);
-#pragma unroll
-        for (int i = 0; i < kOwn; ++i) s += w[i];
-        return s;
-    };
-    double w[kOwn], all;
-    scan(own_sum(seg * kSegment + tid * kOwn, w), red, &all);
-    double* totals = a.total + static_cast<int64_t>(b) * a.own_segments;
-    if (tid == 0) {
-        // through to the memory that all XCDs see, and complete before it is counted
-        __hip_atomic_store(totals + seg, all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        sh_last = __hip_atomic_fetch_add(a.count + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.own_segments - 1;
-    }
-    __syncthreads();
-    if (!sh_last) return;
-
-    // the last workgroup: the border's segment, then its token
-    const int each = (a.own_segments + kThreads - 1) / kThreads;
-    const auto total_of = [&](int s) {
-        return s < a.own_segments ? __hip_atomic_load(totals + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
-    };
-    const auto pick = [&]() -> int {
-        double mine = 0.0;
-        for (int i = 0; i < each; ++i) mine += total_of(tid * each + i);
-        double before = scan(mine, red, &all);
-        if (!(all > 0.0)) return all == 0.0 ? -2 : -1;
-        const double bound = a.u[static_cast<int64_t>(b) * (K + 1) + K] * all;
-        // the first whose sum passes the border; where rounding leaves none, the last that has a weight
-        const auto first_over = [&](bool over, bool some, int at) {
-            if (tid == 0) sh_at = 0x7fffffff;
-            __syncthreads();
-            if (over) atomicMin(&sh_at, at);
-            __syncthreads();
-            const int found = sh_at;
-            __syncthreads();
-            if (found != 0x7fffffff) return found;
-            if (tid == 0) sh_at = -1;
-            __syncthreads();
-            if (some) atomicMax(&sh_at, at);
-            __syncthreads();
-            const int last = sh_at;
-            __syncthreads();
-            return last;
-        };
-        int my_at = 0;
-        double my_before = 0.0;
-        {
-            bool over = false, some = false;
-            for (int i = 0; i < each && !over; ++i) {
-                const double t = total_of(tid * each + i);
-                if (t > 0.0) {
-                    some = true;
-                    my_at = tid * each + i;
-                    my_before = before;
-                    over = before + t > bound;
+                for (int i = 0; i < 4; ++i) {
+                    const double s = sum_wave(mine[i]);
+                    if (lane == i) to = s;
                 }
-                before += t;
+                if (lane < 4)  // through to the memory that all XCDs see
+                    __hip_atomic_store(out + chunk * 4 + lane, to, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
-            const int s = first_over(over, some, my_at);
-            if (some && my_at == s) red[0] = my_before;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // and complete before they are counted
             __syncthreads();
-            my_before = red[0];
-            my_at = s;
-        }
-        const int at = my_at * kSegment + tid * kOwn;
-        const double sum = own_sum(at, w);
-        double in_segment;
-        double upto = my_before + scan(sum, red, &in_segment);
-        bool over = false, some = false;
-        int token = 0;
-#pragma unroll
-        for (int i = 0; i < kOwn; ++i) {
-            if (!over && w[i] > 0.0) {
-                some = true;
-                token = at + i;
-                upto += w[i];
-                over = upto > bound;
+            if (!again) {
+                if (tid == 0)
+                    sh_last = __hip_atomic_fetch_add(a.count + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == static_cast<int>(gridDim.x) - 1;
+                __syncthreads();
+                if (!sh_last) return;
             }
+            // the last workgroup: thread i has chunk i
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[i] = tid < a.chunks ? __hip_atomic_load(out + tid * 4 + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+            if (!again) {
+                p_sum = sum_all(h[2], red);
+                if (rows.qx) ratio = p_sum / sum_all(h[3], red);
+            }
+            weight = rows.qx ? h[0] - ratio * h[1] : h[2];
+            if (weight < 0.0) weight = 0.0;  // (NaN stays)
+            before = scan(weight, red, &all);
+            if (again || !rows.qx || !(all < kSmall * p_sum)) break;  // (the same for the whole workgroup)
+            near = ratio;
+            first = wave, step = kWaves;
         }
-        return first_over(over, some, token);
-    };
-    int token = pick();
-    if (token == -2) {  // (the same for the whole workgroup)
-        plain = true;
-        // p's sums, by this workgroup alone
-        for (int s = 0; s < a.own_segments; ++s) {
-            scan(own_sum(s * kSegment + tid * kOwn, w), red, &all);
-            if (tid == 0) __hip_atomic_store(totals + s, all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (all == 0.0 && rows.qx) {  // nothing is left: p itself
+            rows.qx = nullptr;
+            ratio = 0.0;
+            weight = h[2];
+            before = scan(weight, red, &all);
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        token = pick();
-        if (token < 0) token = -1;
+        if (rows.skip < 0) sum = p_sum;
+        if (all > 0.0) {
+            const double bound = last_u * all;
+            // the first thread whose sum passes the border; where rounding leaves none, the last that has a weight (none: -1)
+            bool passed = false;
+            const auto first_over = [&](bool over, bool some) {
+                const uint64_t o = __ballot(over), w = __ballot(some);
+                if (lane == 0) {
+                    sh_over[wave] = o ? wave * 64 + __builtin_ctzll(o) : kThreads;
+                    sh_some[wave] = w ? wave * 64 + 63 - __builtin_clzll(w) : -1;
+                }
+                __syncthreads();
+                const int f = min(min(sh_over[0], sh_over[1]), min(sh_over[2], sh_over[3]));
+                passed = f < kThreads;
+                return passed ? f : max(max(sh_some[0], sh_some[1]), max(sh_some[2], sh_some[3]));
+            };
+            const int chunk = first_over(weight > 0.0 && before + weight > bound, weight > 0.0);
+            if (tid == chunk) sh_before = before;
+            __syncthreads();
+            before = sh_before;
+            if (tid == 0) sh_token = -1;
+            constexpr int kOwn = kChunk / kThreads;  // neighbouring values of a thread
+#pragma unroll 1
+            for (int run = 0; run < a.runs; ++run) {
+                const int at = (chunk * a.runs + run) * kChunk + tid * kOwn;
+                float x[kOwn], y[kOwn];
+                double w[kOwn], mine = 0.0;
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i) {
+                    x[i] = at + i < V ? load_one<kBf16>(rows.px, at + i) : -__builtin_huge_valf();
+                    y[i] = rows.qx && at + i < V ? load_one<kBf16>(rows.qx, at + i) : -__builtin_huge_valf();
+                }
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i) {
+                    double q;
+                    rows.powers(x[i], y[i], at + i, w[i], q);
+                    w[i] = fmax(w[i] - ratio * q, 0.0);
+                    mine += w[i];
+                }
+                double upto = before + scan(mine, red, &all);
+                bool over = false, some = false;
+                int mine_at = 0;
+                float mine_x = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i) {
+                    if (!over && w[i] > 0.0) {
+                        some = true;
+                        mine_at = at + i;
+                        mine_x = x[i];
+                        upto += w[i];
+                        over = upto > bound;
+                    }
+                }
+                const int found = first_over(over, some);
+                if (tid == found) sh_token = mine_at, sh_logit = mine_x;
+                before += all;
+                __syncthreads();
+                if (passed) break;
+            }
+            token = sh_token;
+        }
     }
-    finish(token);
+    // the accepted drafts, the token and their log probabilities, then nothing
+    for (int i = tid; i <= K; i += kThreads) {
+        const int64_t at = static_cast<int64_t>(b) * (K + 1) + i;
+        const int t = i < acc ? drafts[i] : i == acc ? token : -1;
+        float lp = 0.0f;
+        if (i <= acc) {
+            float v = __builtin_nanf("");
+            if (i < acc) v = draft_x[i];
+            else if (t >= 0) v = kGreedy ? load_one<kBf16>(row_of<kBf16>(a, b, i), t) : sh_logit;
+            lp = static_cast<float>(((static_cast<double>(v) - tops[i]) * a.c - log2_64(i < acc ? sums[i] : sum)) * kLn2);
+        }
+        a.tokens[at] = t;
+        a.logprob[at] = lp;
+    }
+    if (tid == 0) a.accepted[b] = acc;
 }
 
 struct Call {
@@ -464,8 +636,8 @@ struct Call {
 };
 
 struct Plan {
-    int rows, segments, segment, own_segments;
-    int64_t part, best, total, bytes;  // offsets
+    int rows, segments, segment, chunks, runs, groups;
+    int64_t part, best, sums, bytes;  // offsets
 };
 Plan make_plan(int B, int K, int V, bool drafts, bool greedy) {
     Plan p{};
@@ -473,13 +645,19 @@ Plan make_plan(int B, int K, int V, bool drafts, bool greedy) {
     const int64_t rows = static_cast<int64_t>(B) * p.rows;
     const int most = (V + kMinSegment - 1) / kMinSegment;
     p.segments = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, (kFill + rows - 1) / rows)));
-    p.segment = ((V + p.segments - 1) / p.segments + 7) / 8 * 8;
+    const int batch = V / p.segments >= kWhole ? kWhole : 8;  // (a part of a batch takes as long as a whole one)
+    p.segment = ((V + p.segments - 1) / p.segments + batch - 1) / batch * batch;
     p.segments = (V + p.segment - 1) / p.segment;
-    p.own_segments = greedy ? 1 : (V + kSegment - 1) / kSegment;
+    p.runs = (V + kChunk * kThreads - 1) / (kChunk * kThreads);
+    p.chunks = greedy ? 0 : (V + kChunk * p.runs - 1) / (kChunk * p.runs);
+    // a chunk a wave, more where there would be many workgroups
+    const int groups = (p.chunks + kWaves - 1) / kWaves;
+    const int each = static_cast<int>((static_cast<int64_t>(groups) * B + kDrawFill - 1) / kDrawFill);
+    p.groups = greedy ? 1 : (groups + each - 1) / each;
     p.part = (static_cast<int64_t>(B) * 4 + 255) / 256 * 256;
     p.best = p.part + rows * p.segments * 16;
-    p.total = p.best + (greedy ? rows * p.segments * 8 : 0);
-    p.bytes = p.total + (greedy ? 0 : static_cast<int64_t>(B) * p.own_segments * 8);
+    p.sums = p.best + (greedy ? rows * p.segments * 8 : 0);
+    p.bytes = p.sums + static_cast<int64_t>(B) * p.chunks * 32;
     return p;
 }
 
@@ -489,8 +667,8 @@ int check_sizes(int B, int K, int V, double temperature) {
     if (K < 0 || K > kMaxDrafts) return set_error(K < 0 ? DT_ERR_INVALID_ARG : DT_ERR_UNSUPPORTED, "K=%d drafts outside [0, %d]", K, kMaxDrafts);
     if (V < 1) return set_error(DT_ERR_INVALID_ARG, "V=%d must be >= 1", V);
     if (V > kMaxVocab) return set_error(DT_ERR_UNSUPPORTED, "V=%d > %d", V, kMaxVocab);
-    if (!std::isfinite(temperature) || !(temperature >= 0.0))
-        return set_error(DT_ERR_INVALID_ARG, "temperature %g must be finite and >= 0", temperature);
+    if (!(temperature == 0.0 || (temperature >= 1e-6 && temperature <= 1e6)))
+        return set_error(DT_ERR_INVALID_ARG, "temperature %g must be 0 or from 1e-6 to 1e6", temperature);
     return DT_OK;
 }
 
@@ -507,13 +685,15 @@ int launch_rows(const Call& c, const Plan& p, void* ws, hipStream_t s) {
     a.count = reinterpret_cast<int32_t*>(w);
     a.part = reinterpret_cast<double2*>(w + p.part);
     a.best = reinterpret_cast<float2*>(w + p.best);
-    a.total = reinterpret_cast<double*>(w + p.total);
+    a.sums = reinterpret_cast<double*>(w + p.sums);
     a.ldb_x = c.ldb_x, a.ldt_x = c.ldt_x, a.ldb_y = c.ldb_y, a.ldt_y = c.ldt_y;
     a.c = greedy ? kLog2e : kLog2e / c.temperature;
+    a.c_hi = std::nextafterf(static_cast<float>(a.c), 0.0f);
+    a.c_lo = static_cast<float>(a.c - static_cast<double>(a.c_hi));
     a.K = c.K, a.V = c.V, a.tok_bytes = c.tok_bytes;
-    a.rows = p.rows, a.segments = p.segments, a.segment = p.segment, a.own_segments = p.own_segments;
+    a.rows = p.rows, a.segments = p.segments, a.segment = p.segment, a.chunks = p.chunks, a.runs = p.runs;
     for (int b = 0; b < c.B; ++b) a.n[b] = static_cast<uint8_t>(c.counts ? c.counts[b] : c.K);
-    const dim3 first(p.segments, p.rows, c.B), second(p.own_segments, c.B), block(kThreads);
+    const dim3 first(p.segments, p.rows, c.B), second(p.groups, c.B), block(kThreads);
 #define DT_GO(M, G)                                                                           \
     do {                                                                                      \
         hipLaunchKernelGGL((verify_rows_kernel<M, G, kRows>), first, block, 0, s, a);         \

@@ -558,11 +558,13 @@ int dt_head_norm_rotary_bwd(dt_ctx* ctx, const void* d_q_out, const void* d_k_ou
  *   draft_logits : B x K rows (b*ldb_draft + i*ldt_draft) of the logits that the drafts were drawn from at the same temperature, or
  *                  NULL: drafts that nothing was drawn for (probability 1)
  *   counts       : how many drafts each batch row has (host, 0 .. K), or NULL for all K
+ *   temperature  : 0, or from 1e-6 to 1e6
  * With p = softmax(logits / temperature), q = softmax(draft_logits / temperature): draft i is accepted, if those before it were,
  * while uniform_i * q_i(draft_i) < p_i(draft_i). One token more is drawn with the last uniform: from max(p - q, 0) of the first row
  * whose draft was refused (from p where that leaves nothing), or from p of the row behind the last draft: the first token with
  * which the sum of the weights exceeds uniform * their total. At temperature 0 a draft is accepted while it is the largest logit
- * (the first of equals), and that token follows. Probabilities are held in 64 bits.
+ * (the first of equals), and that token follows. The
+ * weights that a token is drawn from are held in 64 bits.
  *   accepted [B] int32 : how many drafts were accepted, n
  *   tokens [B, K + 1] int32 : the accepted drafts, the token that follows, then -1
  *   logprob [B, K + 1] fp32 : their log p (at temperature 0 that of temperature 1), then 0

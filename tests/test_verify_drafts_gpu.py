@@ -1,5 +1,7 @@
 """Verified drafts against the definition in 64 bits: tokens and counts are the same, log probabilities are off by their rounding to
-32 bits (2^-24 of them) and what is left of 64.
+32 bits (2^-24 of them), what is left of 64, and the error of the row's sum: its largest term is exact, another 2^t (t <= 0, the
+difference of the logits times log2 e / T) is off by 2^-24 (2 |t| ln 2) for the difference and the product and by 2^-23 for the power:
+the logarithm of the sum by sum p (1.4 |t| + 2) 2^-24 over all but the largest.
 
 A token next to a border: the kernel's powers are off by 1.1e-12, so a row's sum is too, and an exponent x / T log2 e of at most 1500
 by 2^-52 of it, 4e-13: a probability by less than 5e-12 of itself (in the reference by 1e-12). Sums over p and q, which are 1 each,
@@ -47,7 +49,7 @@ def reference(x, drafts, u, y, T, counts=None):
     B, K = drafts.shape
     V = x.shape[2]
     acc, tok = np.zeros(B, np.int64), np.full((B, K + 1), -1)
-    score = np.zeros((B, K + 1))
+    score, slack = np.zeros((B, K + 1)), np.zeros((B, K + 1))
     others = {}  # tokens as right as the one named, with their scores
     for b in range(B):
         n = K if counts is None else int(counts[b])
@@ -89,15 +91,18 @@ def reference(x, drafts, u, y, T, counts=None):
             if taken:
                 token = d
             tok[b, i] = token
+            t = (lp[i].max() - lp[i]) / np.log(2)
+            p = lp[i].exp()
+            slack[b, i] = 2.0 ** -24 * float(torch.where(p > 0, p * (1.4 * t + 2), p).sum() - 2 * p.max())
             score[b, i] = float(lp[i, token]) if token >= 0 else np.nan
             if not taken:
                 break
             acc[b] += 1
-    return acc, tok, score, others
+    return acc, tok, score, slack, others
 
 
 def check(r, ref):
-    acc, tok, score, others = ref
+    acc, tok, score, slack, others = ref
     tok, score = tok.copy(), score.copy()
     for b, n in enumerate(acc):
         got = int(r.tokens[b, n])
@@ -108,7 +113,7 @@ def check(r, ref):
     got = np.asarray(r.logprob.cpu() if torch.is_tensor(r.logprob) else r.logprob).astype(np.float64)
     assert np.array_equal(np.isnan(got), np.isnan(score))
     ok = ~np.isnan(score)
-    assert (np.abs(got - score)[ok] <= 2.0 ** -24 * np.abs(score)[ok] + 1e-10).all()
+    assert (np.abs(got - score)[ok] <= 2.0 ** -24 * np.abs(score)[ok] + slack[ok] + 1e-10).all()
 
 
 @pytest.mark.parametrize("tdt", TYPES)
@@ -119,6 +124,16 @@ def check(r, ref):
 def test_tokens(gpu, tdt, draft, T, B, K, V):
     x, d, u, y = inputs(B, K, V, B + K + V, tdt, draft)
     check(dt().verify_drafts(x, d, u, draft_logits=y, temperature=T), reference(x, d, u, y, T))
+
+
+@pytest.mark.parametrize("draft", [True, False])
+def test_a_large_vocabulary(gpu, draft):
+    """More chunks than threads: a thread's chunk has several runs."""
+    x, d, u, y = inputs(2, 1, 600011, 6, torch.bfloat16, draft)
+    check(dt().verify_drafts(x, d, u, draft_logits=y), reference(x, d, u, y, 1.0))
+    x[:, :, :500000] = float("-inf")
+    u[:] = 1.0 - 2.0 ** -24
+    check(dt().verify_drafts(x, d, u, draft_logits=y), reference(x, d, u, y, 1.0))
 
 
 @pytest.mark.parametrize("draft", [True, False])
