@@ -9,8 +9,9 @@
 //
 // All of it is bound by HBM (each value is read and written once), where it is not bound by the launch.
 //
-// A wave takes eight heads of one token, eight lanes a head, 16 values a lane: both values of each pair lie in one lane, and
-// a head's sums are three lane exchanges away. The angles need no table: lane i works out pair i's angle for the token, in 64
+// A wave takes eight heads of one token, eight lanes a head, 16 values a lane in pieces of 16 bytes: both values of each pair lie in one
+// lane, the eight lanes' pieces beside each other (in fp32 four pieces a lane; four of a lane behind each other took 198 in place of
+// 104 us past the caches), and a head's sums are three lane exchanges away. The angles need no table: lane i works out pair i's angle for the token, in 64
 // bits down to a fraction of a quarter turn, and the lanes read the pairs that they need from LDS; so positions are bounded by
 // nothing but their type, and nothing is fetched for them.
 
@@ -19,19 +20,25 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 namespace dt {
 namespace {
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kPairs = DT_HEAD_DIM / 2;
 constexpr int kGroupHeads = 8;  // heads of a wave
 constexpr int kFewRows = 32;
 constexpr int kMaxHeads = 1024;
+constexpr int kGridRows = 32768;  // batch rows of the grid's second dimension
 constexpr int kCus = 256;
+constexpr int kBwdGroups = 3 * kCus;
+constexpr int64_t kCacheBytes = 256 << 20;
 
 // kRows: places for the batch rows' first positions, by value
 template <int kRows>
@@ -46,10 +53,11 @@ struct RotaryArgs {
     const void* positions;  // [tokens], or NULL: start[b] + t
     int pos_bytes;
     int has_starts;       // start is set (otherwise there may be more rows than places)
-    int tokens, T;
+    int tokens, B, T;
     int heads[2];
     int octets;           // dims / 16
     int blocks[2];        // backward: workgroups of q, of k
+    int parts[2];         // of a token's heads, one wave's each
     float mag, sign, eps;
     double turns[kPairs];  // a position's step of each pair, in whole turns
     int32_t start[kRows];
@@ -59,65 +67,143 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2){lo, hi}, bf16x2));
 }
 
-// 8 values, 16-byte aligned
 template <bool kBf16>
-__device__ __forceinline__ void load8(const void* p, int64_t at, float* x) {
-    if constexpr (kBf16) {
-        const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+constexpr int kPer = kBf16 ? 8 : 4;  // values of a piece
+
+// past the caches: nothing, what is written, or what is read too
+enum Past { kNothing, kWrites, kAll };
+template <bool kBf16, int kPast>
+__device__ __forceinline__ u32x4 load_piece(const void* p, int64_t at) {
+    const u32x4* from = reinterpret_cast<const u32x4*>(static_cast<const char*>(p) + at * (kBf16 ? 2 : 4));
+    if constexpr (kPast == kAll) return __builtin_nontemporal_load(from);
+    else return *from;
+}
+template <bool kBf16>
+__device__ __forceinline__ void open_piece(u32x4 w, float (&x)[kPer<kBf16>]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = __uint_as_float(u[i] << 16);
-            x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-        }
-    } else {
-        const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float4 w = s[i];
-            x[4 * i] = w.x, x[4 * i + 1] = w.y, x[4 * i + 2] = w.z, x[4 * i + 3] = w.w;
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (kBf16) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+            x[i] = __uint_as_float(w[i]);
         }
     }
 }
-template <bool kBf16>
-__device__ __forceinline__ void store8(void* p, int64_t at, const float* x) {
+template <bool kBf16, int kPast>
+__device__ __forceinline__ void store_piece(void* p, int64_t at, const float (&x)[kPer<kBf16>]) {
+    u32x4 w;
+    u32x4* to;
     if constexpr (kBf16) {
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at) =
-            make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
+        w = (u32x4){pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7])};
+        to = reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + at);
     } else {
-        float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
-        d[0] = make_float4(x[0], x[1], x[2], x[3]);
-        d[1] = make_float4(x[4], x[5], x[6], x[7]);
+        w = (u32x4){__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+        to = reinterpret_cast<u32x4*>(static_cast<float*>(p) + at);
     }
+    if constexpr (kPast != kNothing) __builtin_nontemporal_store(w, to);
+    else *to = w;
 }
 
-// The 16 values of a lane: two runs of 8, at `a` and `b` of the head. Lane j < octets has pairs 8j .. 8j + 7; the lanes behind
-// have values that do not turn.
-template <bool kInter>
-struct Place {
-    int a, b;
-    bool turns;
-    __device__ __forceinline__ Place(int lane, int octets) {
-        const int j = lane & 7;
-        turns = j < octets;
-        a = kInter || !turns ? 16 * j : 8 * j;
-        b = kInter || !turns ? a + 8 : a + 8 * octets;
+// A lane's 16 values as pieces, and where they lie in the head. In the half layout two pieces go together, number t and t + dims/2 (in
+// pieces); those that do not turn are taken two by two. In the interleaved layout a piece has whole pairs.
+template <bool kBf16, bool kInter>
+struct Pieces {
+    static constexpr int P = kPer<kBf16>, kN = 16 / P;
+    float x[kN][P];
+
+    static __device__ __forceinline__ int offset(int i, int lane, int octets) {
+        const int t = (lane & 7) + (i >> 1) * 8;
+        if constexpr (kInter) return (t + (i & 1) * (8 * kN / 2)) * P;
+        const int half = octets * (8 / P);
+        return (t < half ? t + (i & 1) * half : 2 * t + (i & 1)) * P;
+    }
+    // as loaded, and as values
+    struct Raw {
+        u32x4 w[kN];
+        template <int kPast>
+        __device__ __forceinline__ void load(const void* p, int64_t head, int lane, int octets) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) w[i] = load_piece<kBf16, kPast>(p, head + offset(i, lane, octets));
+        }
+    };
+    __device__ __forceinline__ void open(const Raw& r) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) open_piece<kBf16>(r.w[i], x[i]);
+    }
+    template <int kPast>
+    __device__ __forceinline__ void load(const void* p, int64_t head, int lane, int octets) {
+        Raw r;
+        r.template load<kPast>(p, head, lane, octets);
+        open(r);
+    }
+    template <int kPast>
+    __device__ __forceinline__ void store(void* p, int64_t head, int lane, int octets) const {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) store_piece<kBf16, kPast>(p, head + offset(i, lane, octets), x[i]);
+    }
+    // the same places of a row of fp32
+    __device__ __forceinline__ void load_row(const float* p, int lane, int octets) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const int at = offset(i, lane, octets);
+#pragma unroll
+            for (int j = 0; j < P; j += 4) {
+                const floatx4 w = *reinterpret_cast<const floatx4*>(p + at + j);
+                x[i][j] = w[0], x[i][j + 1] = w[1], x[i][j + 2] = w[2], x[i][j + 3] = w[3];
+            }
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+#pragma unroll
+            for (int j = 0; j < P; ++j) x[i][j] = 0.0f;
+    }
+    static __device__ __forceinline__ void turn_pair(float& u, float& v, float2 f) {
+        const float p = u, r = v;
+        u = p * f.x - r * f.y;
+        v = r * f.x + p * f.y;
+    }
+    __device__ __forceinline__ void turn(const float2* cs, int lane, int octets) {
+        if constexpr (kInter) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                const int at = offset(i, lane, octets);
+                if (at < 16 * octets) {
+#pragma unroll
+                    for (int j = 0; j < P / 2; ++j) turn_pair(x[i][2 * j], x[i][2 * j + 1], cs[at / 2 + j]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kN; i += 2) {
+                const int at = offset(i, lane, octets);
+                if (at < 8 * octets) {
+#pragma unroll
+                    for (int j = 0; j < P; ++j) turn_pair(x[i][j], x[i + 1][j], cs[at + j]);
+                }
+            }
+        }
     }
 };
 
-// cos and sin (times mag) of a token's pairs into the wave's part of LDS
+// the position of token t of batch row b
 template <int kRows>
-__device__ __forceinline__ void angles(const RotaryArgs<kRows>& a, int token, int lane, float2* cs) {
+__device__ __forceinline__ double position(const RotaryArgs<kRows>& a, int b, int t) {
+    if (a.positions) {
+        const int64_t token = static_cast<int64_t>(b) * a.T + t;
+        return a.pos_bytes == 4 ? static_cast<const int32_t*>(a.positions)[token]
+                                : static_cast<double>(static_cast<const int64_t*>(a.positions)[token]);
+    }
+    return static_cast<double>(a.has_starts ? a.start[b] : 0) + t;
+}
+
+// cos and sin (times mag) of the pairs at a position into the wave's part of LDS
+template <int kRows>
+__device__ __forceinline__ void angles(const RotaryArgs<kRows>& a, double at, int lane, float2* cs) {
     if (lane < 8 * a.octets) {
-        double p;
-        if (a.positions)
-            p = a.pos_bytes == 4 ? static_cast<const int32_t*>(a.positions)[token]
-                                 : static_cast<double>(static_cast<const int64_t*>(a.positions)[token]);
-        else {
-            const int b = token / a.T;
-            p = static_cast<double>(a.has_starts ? a.start[b] : 0) + (token - b * a.T);
-        }
-        double t = p * a.turns[lane];
+        double t = at * a.turns[lane];
         t = 4.0 * (t - rint(t));       // quarter turns, in [-2, 2]
         const double q = rint(t);
         float s, c;
@@ -135,152 +221,157 @@ __device__ __forceinline__ void angles(const RotaryArgs<kRows>& a, int token, in
     __builtin_amdgcn_wave_barrier();
 }
 
-template <bool kInter>
-__device__ __forceinline__ void turn(float (&x)[16], const float2* cs) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        constexpr int kStep = kInter ? 2 : 1, kNext = kInter ? 1 : 8;
-        float& u = x[kStep * i];
-        float& v = x[kStep * i + kNext];
-        const float p = u, r = v;
-        const float2 f = cs[i];
-        u = p * f.x - r * f.y;
-        v = r * f.x + p * f.y;
-    }
+// over the eight lanes of a head: with the neighbour, the other pair of four, and mirrored
+template <int kCtrl>
+__device__ __forceinline__ float moved(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), kCtrl, 0xf, 0xf, true));
 }
-
-// over the eight lanes of a head
 __device__ __forceinline__ float sum_head(float x) {
-    x += __shfl_xor(x, 1, 64);
-    x += __shfl_xor(x, 2, 64);
-    return x + __shfl_xor(x, 4, 64);
+    x += moved<0xb1>(x);
+    x += moved<0x4e>(x);
+    return x + moved<0x141>(x);
+}
+// with the other row of 16 of a half, with the other half
+template <bool k32>
+__device__ __forceinline__ float sum_halves(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto r = k32 ? __builtin_amdgcn_permlane32_swap(u, u, false, false) : __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// 1 / sqrt(x): the instruction's, once corrected
+__device__ __forceinline__ float inverse_root(float x) {
+    const float r = __builtin_amdgcn_rsqf(x);
+    return fmaf(r, fmaf(-0.5f * x * r, r, 0.5f), r);
 }
 
 // 1 / sqrt(mean x^2 + eps) of the head
-__device__ __forceinline__ float inverse_rms(const float (&x)[16], float eps) {
+template <bool kBf16, bool kInter>
+__device__ __forceinline__ float inverse_rms(const Pieces<kBf16, kInter>& v, float eps) {
+    using V = Pieces<kBf16, kInter>;
     float ss = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) ss += x[i] * x[i];
+    for (int i = 0; i < 16; ++i) ss += v.x[i / V::P][i % V::P] * v.x[i / V::P][i % V::P];
     ss = sum_head(ss);
-    float inv = 1.0f / sqrtf(ss * (1.0f / DT_HEAD_DIM) + eps);
+    float inv = inverse_root(fmaf(ss, 1.0f / DT_HEAD_DIM, eps));
     if (__any(ss == __builtin_huge_valf())) {  // squares past fp32's range: once more, of values 2^-70 times as large
         float s2 = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s2 += (x[i] * 0x1p-70f) * (x[i] * 0x1p-70f);
+        for (int i = 0; i < 16; ++i) {
+            const float y = v.x[i / V::P][i % V::P] * 0x1p-70f;
+            s2 += y * y;
+        }
         s2 = sum_head(s2);
-        if (ss == __builtin_huge_valf()) inv = 0x1p-70f / sqrtf(s2 * (1.0f / DT_HEAD_DIM));
+        if (ss == __builtin_huge_valf()) inv = 0x1p-70f * inverse_root(s2 * (1.0f / DT_HEAD_DIM));
     }
     return inv;
 }
 
-template <bool kBf16, bool kNorm, bool kInter, int kRows>
-__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs<kRows> a, int groups, int items) {
+// A workgroup takes a token, its waves the groups of eight heads: q's, then k's.
+template <bool kBf16, bool kNorm, bool kInter, int kPast, int kRows>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs<kRows> a) {
+    using V = Pieces<kBf16, kInter>;
     __shared__ float2 cs[kWaves][kPairs];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int item = blockIdx.x * kWaves + wave;
-    if (item >= items) return;
-    const int token = item / groups;
-    // q's heads, then k's
-    int head = (item - token * groups) * kGroupHeads + (lane >> 3);
-    const bool second = head >= a.heads[0];
-    if (second) head -= a.heads[0];
-    const bool have = !second || head < a.heads[1];
-    const Place<kInter> at(lane, a.octets);
-    const void* in = second ? a.in[1] : a.in[0];
-    const int64_t from = token * (second ? a.ld_in[1] : a.ld_in[0]) + head * DT_HEAD_DIM;
-    float x[16];
-    if (have) {
-        load8<kBf16>(in, from + at.a, x);
-        load8<kBf16>(in, from + at.b, x + 8);
-    } else {
+    const int t = blockIdx.x, b = blockIdx.z * kGridRows + blockIdx.y;
+    if (b >= a.B) return;
+    const int64_t token = static_cast<int64_t>(b) * a.T + t;
+    for (int first = wave * kGroupHeads; first < a.heads[0] + a.heads[1]; first += blockDim.x / 64 * kGroupHeads) {
+        int head = first + (lane >> 3);
+        const bool second = head >= a.heads[0];
+        if (second) head -= a.heads[0];
+        const bool have = !second || head < a.heads[1];
+        V x, w;
+        if (have) x.template load<kPast>(second ? a.in[1] : a.in[0], token * (second ? a.ld_in[1] : a.ld_in[0]) + head * DT_HEAD_DIM, lane, a.octets);
+        else x.zero();
+        if constexpr (kNorm) w.load_row(second && have ? a.w[1] : a.w[0], lane, a.octets);
+        if (first == wave * kGroupHeads) angles(a, position(a, b, t), lane, cs[wave]);
+        if constexpr (kNorm) {
+            const float inv = inverse_rms(x, a.eps);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = 0.0f;
-    }
-    float w[16];
-    if constexpr (kNorm) {
-        load8<false>(second && have ? a.w[1] : a.w[0], at.a, w);
-        load8<false>(second && have ? a.w[1] : a.w[0], at.b, w + 8);
-    }
-    angles(a, token, lane, cs[wave]);
-    if constexpr (kNorm) {
-        const float inv = inverse_rms(x, a.eps);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = x[i] * inv * w[i];
-    }
-    if (at.turns) turn<kInter>(x, cs[wave] + 8 * (lane & 7));
-    if (have) {
-        void* out = second ? a.out[1] : a.out[0];
-        const int64_t to = token * (second ? a.ld_out[1] : a.ld_out[0]) + head * DT_HEAD_DIM;
-        store8<kBf16>(out, to + at.a, x);
-        store8<kBf16>(out, to + at.b, x + 8);
+            for (int i = 0; i < 16; ++i) x.x[i / V::P][i % V::P] = x.x[i / V::P][i % V::P] * inv * w.x[i / V::P][i % V::P];
+        }
+        x.turn(cs[wave], lane, a.octets);
+        if (have)
+            x.template store<kPast>(second ? a.out[1] : a.out[0], token * (second ? a.ld_out[1] : a.ld_out[0]) + head * DT_HEAD_DIM, lane, a.octets);
     }
 }
 
-// The norm's backward: workgroups of q (the first blocks[0]) or of k; their waves take groups of eight heads in turn, and each
-// workgroup leaves the column sums of g n.
-template <bool kBf16, bool kInter, int kRows>
+// The norm's backward: workgroups of q (the first blocks[0]) or of k; their waves take tokens (or, where these are few, their groups of
+// eight heads) in turn, and each workgroup leaves the column sums of g n.
+template <bool kBf16, bool kInter, int kPast, int kRows>
 __global__ __launch_bounds__(kThreads) void head_norm_rotary_bwd_kernel(RotaryArgs<kRows> a) {
+    using V = Pieces<kBf16, kInter>;
     __shared__ float2 cs[kWaves][kPairs];
     __shared__ float sums[kWaves][DT_HEAD_DIM];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int which = static_cast<int>(blockIdx.x) >= a.blocks[0];
     const int block = blockIdx.x - (which ? a.blocks[0] : 0);
-    const int heads = a.heads[which], groups = (heads + kGroupHeads - 1) / kGroupHeads;
-    const int items = a.tokens * groups;
-    const Place<kInter> at(lane, a.octets);
-    float w[16], dw[16];
-    load8<false>(a.w[which], at.a, w);
-    load8<false>(a.w[which], at.b, w + 8);
+    const int heads = a.heads[which], step = a.blocks[which] * kWaves;
+    const int parts = a.parts[which], span = parts > 1 ? kGroupHeads : heads;  // of a token, heads of a part
+    V w, dw;
+    w.load_row(a.w[which], lane, a.octets);
+    dw.zero();
+    // The next eight heads' values are under way while some are worked on. (Lanes without a head read another's, and behind the last
+    // token it is read again: a load under a condition would make the wait for one a wait for all.)
+    typename V::Raw next_g, next_x;
+    const auto fetch = [&](int token, int first) {
+        token = min(token, a.tokens - 1);
+        const int head = min(first + (lane >> 3), heads - 1);
+        next_g.template load<kPast>(a.in[which], token * a.ld_in[which] + head * DT_HEAD_DIM, lane, a.octets);
+        next_x.template load<kPast>(a.x[which], token * a.ld_x[which] + head * DT_HEAD_DIM, lane, a.octets);
+    };
+    // token and part, row and place in the row: divided once
+    const int item = block * kWaves + wave;
+    int token = item / parts, part = item - token * parts, b = token / a.T, t = token - b * a.T;
+    const int step_token = step / parts, step_part = step - step_token * parts;
+    if (token < a.tokens) fetch(token, part * span);
+    while (token < a.tokens) {
+        angles(a, position(a, b, t), lane, cs[wave]);
+        int next_token = token + step_token, next_part = part + step_part;
+        if (next_part >= parts) next_part -= parts, ++next_token;
+        const int end = min(part * span + span, heads);
+        for (int first = part * span; first < end; first += kGroupHeads) {
+            const int head = first + (lane >> 3);
+            const bool have = head < end, more = first + kGroupHeads < end;
+            V g, x;
+            g.open(next_g);
+            x.open(next_x);
+            fetch(more ? token : next_token, more ? first + kGroupHeads : next_part * span);
+            if (!have) g.zero();
+            g.turn(cs[wave], lane, a.octets);
+            const float inv = inverse_rms(x, a.eps);
+            float dot = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) dw[i] = 0.0f;
-    for (int item = block * kWaves + wave; item < items; item += a.blocks[which] * kWaves) {
-        const int token = item / groups, head = (item - token * groups) * kGroupHeads + (lane >> 3);
-        const bool have = head < heads;
-        float g[16], x[16];
-        if (have) {
-            const int64_t gi = token * a.ld_in[which] + head * DT_HEAD_DIM, xi = token * a.ld_x[which] + head * DT_HEAD_DIM;
-            load8<kBf16>(a.in[which], gi + at.a, g);
-            load8<kBf16>(a.in[which], gi + at.b, g + 8);
-            load8<kBf16>(a.x[which], xi + at.a, x);
-            load8<kBf16>(a.x[which], xi + at.b, x + 8);
-        } else {
+            for (int i = 0; i < V::kN; ++i)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) g[i] = x[i] = 0.0f;
+                for (int j = 0; j < V::P; ++j) {
+                    x.x[i][j] *= inv;
+                    dw.x[i][j] += g.x[i][j] * x.x[i][j];
+                    g.x[i][j] *= w.x[i][j];
+                    dot += g.x[i][j] * x.x[i][j];
+                }
+            dot = sum_head(dot) * (1.0f / DT_HEAD_DIM);
+#pragma unroll
+            for (int i = 0; i < V::kN; ++i)
+#pragma unroll
+                for (int j = 0; j < V::P; ++j) g.x[i][j] = inv * (g.x[i][j] - x.x[i][j] * dot);
+            if (have) g.template store<kPast>(a.out[which], token * a.ld_out[which] + head * DT_HEAD_DIM, lane, a.octets);
         }
-        angles(a, token, lane, cs[wave]);
-        if (at.turns) turn<kInter>(g, cs[wave] + 8 * (lane & 7));
-        const float inv = inverse_rms(x, a.eps);
-        float dot = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            x[i] *= inv;
-            dw[i] += g[i] * x[i];
-            g[i] *= w[i];
-            dot += g[i] * x[i];
-        }
-        dot = sum_head(dot) * (1.0f / DT_HEAD_DIM);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) g[i] = inv * (g[i] - x[i] * dot);
-        if (have) {
-            const int64_t to = token * a.ld_out[which] + head * DT_HEAD_DIM;
-            store8<kBf16>(a.out[which], to + at.a, g);
-            store8<kBf16>(a.out[which], to + at.b, g + 8);
-        }
+        t += next_token - token;
+        while (t >= a.T) t -= a.T, ++b;
+        token = next_token;
+        part = next_part;
     }
     // the eight heads of a wave, then the waves
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        dw[i] += __shfl_xor(dw[i], 8, 64);
-        dw[i] += __shfl_xor(dw[i], 16, 64);
-        dw[i] += __shfl_xor(dw[i], 32, 64);
-    }
-    if (lane < 8) {
+    for (int i = 0; i < V::kN; ++i)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            sums[wave][at.a + i] = dw[i];
-            sums[wave][at.b + i] = dw[8 + i];
+        for (int j = 0; j < V::P; ++j) {
+            float s = dw.x[i][j];
+            s += moved<0x128>(s);  // rotated by 8 within 16
+            s = sum_halves<true>(sum_halves<false>(s));
+            if (lane < 8) sums[wave][V::offset(i, lane, a.octets) + j] = s;
         }
-    }
     __syncthreads();
     if (threadIdx.x < DT_HEAD_DIM) {
         float s = 0.0f;
@@ -376,10 +467,14 @@ int check_call(const dt_ctx* ctx, const Call& c) {
     return DT_OK;
 }
 
-// workgroups of the norm's backward for `heads` heads: two a CU at most, so the sums that they leave stay few
-int bwd_blocks(int64_t tokens, int heads) {
-    const int64_t items = tokens * ((heads + kGroupHeads - 1) / kGroupHeads);
-    return static_cast<int>(std::min<int64_t>((items + kWaves - 1) / kWaves, 2 * kCus));
+// Workgroups of the norm's backward for `heads` heads beside `others`: their share of as many as fit the CUs by the groups of eight,
+// as a group that is not full takes as long, so that q's and k's end together and the sums that they leave stay few.
+// parts: a wave has a whole token's heads, whose angles are worked out once then, where that leaves waves enough.
+int bwd_blocks(int64_t tokens, int heads, int others, int* parts) {
+    const int groups = (heads + kGroupHeads - 1) / kGroupHeads, all = groups + (others + kGroupHeads - 1) / kGroupHeads;
+    const int most = std::max(1, kBwdGroups * groups / all);
+    *parts = tokens < static_cast<int64_t>(most) * kWaves ? groups : 1;
+    return static_cast<int>(std::min<int64_t>((tokens * *parts + kWaves - 1) / kWaves, most));
 }
 
 template <int kRows>
@@ -395,6 +490,7 @@ int launch_rows(const Call& c, void* ws, hipStream_t s) {
     a.positions = c.positions;
     a.pos_bytes = c.pos_bytes;
     a.tokens = c.B * c.T;
+    a.B = c.B;
     a.T = c.T;
     a.has_starts = c.starts != nullptr;
     a.heads[0] = c.H, a.heads[1] = c.Hk;
@@ -405,44 +501,45 @@ int launch_rows(const Call& c, void* ws, hipStream_t s) {
     for (int i = 0; i < c.rot->dims / 2; ++i) a.turns[i] = c.rot->frequency[i] / 6.283185307179586476925;
     if (c.starts) std::copy_n(c.starts, c.B, a.start);
     const bool bf16 = c.dtype == DT_BF16, inter = c.rot->layout == DT_ROTARY_INTERLEAVED;
+    const dim3 block(kThreads);
+    // Results that would push much else out of the last-level cache (256 MB) go past it, and so do reads of what cannot all be in it: 537
+    // MB moved in fp32 95 us, 88 with reads past it, too; 268 MB in bf16 with the norm 52 us, 49 with writes past it, 54 with reads as well.
+    const int64_t bytes = static_cast<int64_t>(a.tokens) * (c.H + c.Hk) * DT_HEAD_DIM * (bf16 ? 2 : 4);
+    const int past = bytes * (c.norm && c.backward ? 2 : 1) >= kCacheBytes ? kAll : bytes >= kCacheBytes / 4 ? kWrites : kNothing;
+    constexpr std::true_type yes;
+    constexpr std::false_type no;
+    const auto choose = [&](bool which, auto go) {
+        if (which) go(yes);
+        else go(no);
+    };
+    const int groups = (c.H + c.Hk + kGroupHeads - 1) / kGroupHeads;
+    choose(bf16, [&](auto M) {
+        choose(inter, [&](auto I) {
+            const auto go = [&](auto O) {
+                constexpr bool kM = decltype(M)::value, kI = decltype(I)::value;
+                constexpr int kO = decltype(O)::value;
+                if (c.norm && c.backward) {
+                    a.blocks[0] = bwd_blocks(a.tokens, c.H, c.Hk, &a.parts[0]);
+                    a.blocks[1] = c.Hk > 0 ? bwd_blocks(a.tokens, c.Hk, c.H, &a.parts[1]) : 0;
+                    a.partial = static_cast<float*>(ws);
+                    hipLaunchKernelGGL((head_norm_rotary_bwd_kernel<kM, kI, kO, kRows>), dim3(a.blocks[0] + a.blocks[1]), block, 0, s, a);
+                } else {
+                    const dim3 grid(c.T, std::min(c.B, kGridRows), (c.B + kGridRows - 1) / kGridRows), waves(64 * std::min(groups, kWaves));
+                    if (c.norm) hipLaunchKernelGGL((rotary_kernel<kM, true, kI, kO, kRows>), grid, waves, 0, s, a);
+                    else hipLaunchKernelGGL((rotary_kernel<kM, false, kI, kO, kRows>), grid, waves, 0, s, a);
+                }
+            };
+            if (past == kAll) go(std::integral_constant<int, kAll>());
+            else if (past == kWrites) go(std::integral_constant<int, kWrites>());
+            else go(std::integral_constant<int, kNothing>());
+        });
+    });
+    DT_HIP_TRY(hipGetLastError());
     if (c.norm && c.backward) {
-        a.blocks[0] = bwd_blocks(a.tokens, c.H);
-        a.blocks[1] = c.Hk > 0 ? bwd_blocks(a.tokens, c.Hk) : 0;
-        a.partial = static_cast<float*>(ws);
-        const dim3 grid(a.blocks[0] + a.blocks[1]), block(kThreads);
-#define DT_GO(M, I) hipLaunchKernelGGL((head_norm_rotary_bwd_kernel<M, I, kRows>), grid, block, 0, s, a)
-        if (bf16) {
-            if (inter) DT_GO(true, true);
-            else DT_GO(true, false);
-        } else {
-            if (inter) DT_GO(false, true);
-            else DT_GO(false, false);
-        }
-#undef DT_GO
-        DT_HIP_TRY(hipGetLastError());
         hipLaunchKernelGGL(head_norm_dw_kernel, dim3(DT_HEAD_DIM / kSumCols, c.Hk > 0 ? 2 : 1), block, 0, s, a.partial, a.blocks[0],
                            a.blocks[1], c.dwq, c.dwk);
         DT_HIP_TRY(hipGetLastError());
-        return DT_OK;
     }
-    const int groups = (c.H + c.Hk + kGroupHeads - 1) / kGroupHeads, items = a.tokens * groups;
-    const dim3 grid((items + kWaves - 1) / kWaves), block(kThreads);
-#define DT_GO(M, N, I) hipLaunchKernelGGL((rotary_kernel<M, N, I, kRows>), grid, block, 0, s, a, groups, items)
-#define DT_GO2(M, N)                \
-    do {                            \
-        if (inter) DT_GO(M, N, true); \
-        else DT_GO(M, N, false);    \
-    } while (0)
-    if (bf16) {
-        if (c.norm) DT_GO2(true, true);
-        else DT_GO2(true, false);
-    } else {
-        if (c.norm) DT_GO2(false, true);
-        else DT_GO2(false, false);
-    }
-#undef DT_GO2
-#undef DT_GO
-    DT_HIP_TRY(hipGetLastError());
     return DT_OK;
 }
 
@@ -453,7 +550,9 @@ int launch(const Call& c, void* ws, hipStream_t s) {
 int64_t workspace_bytes(const Call& c) {
     if (!c.norm || !c.backward) return 0;
     const int64_t tokens = static_cast<int64_t>(c.B) * c.T;
-    return (bwd_blocks(tokens, c.H) + (c.Hk > 0 ? bwd_blocks(tokens, c.Hk) : 0)) * static_cast<int64_t>(DT_HEAD_DIM * sizeof(float));
+    int parts;
+    return (bwd_blocks(tokens, c.H, c.Hk, &parts) + (c.Hk > 0 ? bwd_blocks(tokens, c.Hk, c.H, &parts) : 0)) *
+           static_cast<int64_t>(DT_HEAD_DIM * sizeof(float));
 }
 
 int run(dt_ctx* ctx, const Call& call, void* ws, int64_t ws_bytes, void* stream) {

@@ -74,9 +74,10 @@ def verify_drafts(logits, drafts, uniforms, *, draft_logits=None, temperature: f
     the last row's p: what is emitted is distributed as p. At temperature 0 it is the largest logit's token, and drafts that are it
     are accepted. A row with a NaN or +inf, or with nothing but -inf, gives token -1 and log probability NaN."""
     ctx = _check_logits(logits, ctx)
-    if len(logits.shape) != 3 or logits.shape[1] < 1:
-        raise ValueError(f"logits must be [B, K + 1, V], got {tuple(logits.shape)}")
-    B, K, V = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
+    shape = logits.shape
+    if len(shape) != 3 or shape[1] < 1:
+        raise ValueError(f"logits must be [B, K + 1, V], got {tuple(shape)}")
+    B, K, V = shape[0], shape[1] - 1, shape[2]
     dtype, on_device, temperature = _mode_of(logits, None), _is_torch(logits), float(temperature)
     if tuple(drafts.shape) != (B, K):
         raise ValueError(f"drafts have shape {tuple(drafts.shape)}, expected {(B, K)}")
@@ -106,7 +107,7 @@ def verify_drafts(logits, drafts, uniforms, *, draft_logits=None, temperature: f
             ws = new_workspace(x, ctx.device, stream, need)
         accepted = x.new_empty((B,), dtype=torch.int32)
         tokens = x.new_empty((B, K + 1), dtype=torch.int32)
-        logprob = x.new_empty((B, K + 1), dtype=torch.float32)
+        logprob = torch.empty_like(tokens, dtype=torch.float32)
         C.call("dt_verify_drafts", ctx.handle, x.data_ptr(), d.data_ptr() or None, u.data_ptr() if u is not None else None,
                y.data_ptr() if has else None, B, K, V, ldb, ldt, ldb_y, ldt_y, d.element_size(), n_p, temperature,
                accepted.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), ws[0], ws[1], dtype, C.DT_MEM_DEVICE, stream)

@@ -85,15 +85,18 @@ class HeadNormRotaryGradients:
 
 def _check_rows(Q, K, names=("Q", "K")):
     """[B, T, heads, 128] tensors of one kind, dtype and place; K may be None. (B, T, H, Hk)"""
-    if len(Q.shape) != 4 or Q.shape[3] != C.HEAD_DIM:
-        raise ValueError(f"{names[0]} must be [B, T, H, {C.HEAD_DIM}], got {tuple(Q.shape)}")
+    q = Q.shape
+    if len(q) != 4 or q[3] != C.HEAD_DIM:
+        raise ValueError(f"{names[0]} must be [B, T, H, {C.HEAD_DIM}], got {tuple(q)}")
+    B, T, H = q[0], q[1], q[2]
     if K is None:
-        return (*Q.shape[:3], 0)
-    if len(K.shape) != 4 or K.shape[3] != C.HEAD_DIM or K.shape[:2] != Q.shape[:2]:
-        raise ValueError(f"{names[1]} must be [{Q.shape[0]}, {Q.shape[1]}, heads, {C.HEAD_DIM}], got {tuple(K.shape)}")
+        return B, T, H, 0
+    k = K.shape
+    if len(k) != 4 or k[3] != C.HEAD_DIM or k[0] != B or k[1] != T:
+        raise ValueError(f"{names[1]} must be [{B}, {T}, heads, {C.HEAD_DIM}], got {tuple(k)}")
     if _is_torch(Q) != _is_torch(K) or Q.dtype != K.dtype or (_is_torch(Q) and Q.device != K.device):
         raise TypeError(f"{names[0]} and {names[1]} must be of one kind, dtype and device")
-    return (*Q.shape[:3], K.shape[2])
+    return B, T, H, k[2]
 
 
 def _context_of(Q, ctx):
@@ -139,6 +142,10 @@ def _inputs(x, host):
     if host:
         a = np.ascontiguousarray(x)
         return a, a.ctypes.data, a.shape[2] * C.HEAD_DIM
+    if x.is_contiguous():  # (as _rows_of has it)
+        p = x.data_ptr()
+        if p % 16 == 0:
+            return x, p, x.shape[2] * C.HEAD_DIM
     r, ld = _rows_of(x)
     return r, r.data_ptr(), ld
 
@@ -154,8 +161,8 @@ def _outputs(x, rows, host, inplace):
     if host:
         o = np.empty(x.shape, x.dtype)
         return o, o.ctypes.data, o.shape[2] * C.HEAD_DIM
-    o = x.new_empty(x.shape)
-    return o, o.data_ptr(), o.shape[2] * C.HEAD_DIM
+    o = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+    return o, o.data_ptr(), x.shape[2] * C.HEAD_DIM
 
 
 def _weight(w, like, name):
@@ -179,8 +186,8 @@ def _rotate(Q, K, rot, positions, starts, inplace, ctx, backward):
     pos = _positions_of(positions, starts, B, T, Q)
     q, k = _inputs(Q, host), _inputs(K, host)
     oq, ok = _outputs(Q, q, host, inplace), _outputs(K, k, host, inplace)
-    C.call("dt_rotary_fwd", ctx.handle, q[1], k[1], oq[1], ok[1], B, T, H, Hk, C.HEAD_DIM, q[2], k[2], oq[2], ok[2], pos[1], pos[2],
-           pos[3], rot._p, backward, dtype, C.DT_MEM_HOST if host else C.DT_MEM_DEVICE, None if host else _stream_of(Q))
+    C.check(C.lib().dt_rotary_fwd(ctx.handle, q[1], k[1], oq[1], ok[1], B, T, H, Hk, C.HEAD_DIM, q[2], k[2], oq[2], ok[2], pos[1], pos[2],
+           pos[3], rot._p, backward, dtype, C.DT_MEM_HOST if host else C.DT_MEM_DEVICE, None if host else _stream_of(Q)))
     return oq[0], ok[0]
 
 
