@@ -228,10 +228,26 @@ struct Block {
         if constexpr (kFormat == DT_KV_FP4) return widen4(k[i >> 2][i & 3], __uint_as_float(k4[i >> 2] << 23));
         else return operand(k, i);
     }
-    __device__ __forceinline__ bf16x8 operand_v(int i) {
-        if constexpr (kFormat == DT_KV_FP4) return widen4(v[i >> 2][i & 3], 1.0f);
-        else return operand(v, i);
+    // fp4: V tiles 2 i and 2 i + 1 times their scales
+    __device__ __forceinline__ void operands_v(int i, bf16x8 (&to)[2]) {
+        union { uint32_t u[4]; bf16x8 v; } r[2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // (keys 2 j and 2 j + 1 of the lane's)
+            const uint32_t w = v[i >> 1][(i & 1) * 2 + (j >> 1)];
+            const float s0 = scale4(v4[j >> 1][2 * j & 3], i), s1 = scale4(v4[j >> 1][(2 * j + 1) & 3], i);
+            const auto pair = [&](float s, auto at) {
+                return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, decltype(at)::value));
+            };
+            const uint32_t a = j & 1 ? pair(s0, std::integral_constant<int, 2>()) : pair(s0, std::integral_constant<int, 0>());
+            const uint32_t b = j & 1 ? pair(s1, std::integral_constant<int, 3>()) : pair(s1, std::integral_constant<int, 1>());
+            r[0].u[j] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+            r[1].u[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+        }
+        to[0] = r[0].v;
+        to[1] = r[1].v;
     }
+    // byte i of a key's scales
+    static __device__ __forceinline__ float scale4(uint32_t w, int i) { return __uint_as_float((w >> (8 * i) & 0xffu) << 23); }
     static __device__ __forceinline__ bf16x8 operand(const u32x4 (&w)[kPieces], int i) {
         if constexpr (kFormat == DT_KV_BF16) return __builtin_bit_cast(bf16x8, w[i]);
         else return widen<kFormat>(w[i >> 1][(i & 1) * 2], w[i >> 1][(i & 1) * 2 + 1]);
@@ -414,11 +430,6 @@ struct Stretch {
         }
     }
 
-    // byte i of a key's scales
-    static __device__ __forceinline__ float scale4(uint32_t w, int i) {
-        return __uint_as_float((i < 3 ? w << (23 - 8 * i) : w >> 1) & 0x7f800000u);
-    }
-
     __device__ __forceinline__ void attend(float scale, Shared<kQT>& sh) {
         const int n = lane & 15, g = lane >> 4;
         bf16x8 qf[kQT][kQS][4];
@@ -463,9 +474,13 @@ struct Stretch {
             keep_order();
             const bool mask = kb + kKvBlock > minlim;  // (the same for the whole wave)
             bf16x8 pf[kQT][kQS];
-            float pe[kFp4 ? kQT : 1][8];  // fp4: the probabilities, as V's scales are one for each 32 values
-            if constexpr (!kFp4)
+            uint32_t none = 0;  // fp4: whether some key of the lane's has a row of V that is none
+            if constexpr (kFp4) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) none = max(none, blk.v4[i >> 2][i & 3]);
+            } else {
                 if (__builtin_expect(lowered, 0)) blk.vs[0] *= kLower, blk.vs[1] *= kLower;
+            }
 #pragma unroll
             for (int x = 0; x < kQT; ++x) {
                 const int rest = lim[x] - kb - g * 4;  // the lane's key 16 t + i is seen if it is below
@@ -493,15 +508,19 @@ struct Stretch {
                 for (int i = 0; i < 8; ++i) {
                     const float e = __builtin_amdgcn_exp2f(p[i] - base[x]);
                     add += e;
-                    if constexpr (kFp4) pe[x][i] = e;
+                    if constexpr (kFp4) p[i] = e;  // (V's scales go with V)
                     else p[i] = e * blk.vs[i >> 2][i & 3];
                 }
                 sum[x] += add;
                 if constexpr (kFp4) {
                     if (__builtin_expect(lowered, 0))
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) pe[x][i] *= kLower;
-                    continue;
+                        for (int i = 0; i < 8; ++i) p[i] *= kLower;
+                    // such a row's values are 0, and the queries that see it get their NaN here
+                    if (__builtin_expect(__any(none == 0xffffffffu), 0))
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (blk.v4[i >> 2][i & 3] == 0xffffffffu) p[i] = __uint_as_float(0x7fc00000u);
                 }
                 if (mask) {  // (a masked key's scale may be anything, NaN too)
 #pragma unroll
@@ -511,32 +530,29 @@ struct Stretch {
                 operand_p(p, pf[x]);
             }
             blk.settle(blk.v);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if constexpr (kFp4) {
-                    if ((i & 1) == 0) {  // the next 32 values: P times their scales
-#pragma unroll
-                        for (int x = 0; x < kQT; ++x) {
-                            float p[8];
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) p[j] = pe[x][j] * scale4(blk.v4[j >> 2][j & 3], i >> 1);
-                            if (mask) {  // (a masked key's scale may be anything, NaN too)
-                                const int rest = lim[x] - kb - g * 4;
-#pragma unroll
-                                for (int j = 0; j < 8; ++j)
-                                    if ((j >> 2) * 16 + (j & 3) >= rest) p[j] = 0.0f;
-                            }
-                            operand_p(p, pf[x]);
-                        }
-                    }
-                }
-                const bf16x8 vf = blk.operand_v(i);
+            const auto add_v = [&](int i, const bf16x8& vf) {
 #pragma unroll
                 for (int x = 0; x < kQT; ++x)
 #pragma unroll
                     for (int y = kQS - 1; y >= 0; --y)
                         acc[x][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[x][y], acc[x][i], 0, 0, 0);
                 keep_order();
+            };
+            if constexpr (kFp4) {
+                if (__builtin_expect(__any(none == 0xffffffffu), 0))
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (blk.v4[i >> 2][i & 3] == 0xffffffffu) blk.v4[i >> 2][i & 3] = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    bf16x8 vf[2];
+                    blk.operands_v(i, vf);
+                    add_v(2 * i, vf[0]);
+                    add_v(2 * i + 1, vf[1]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) add_v(i, blk.operand(blk.v, i));
             }
             load_v(blk, next);
             kb += step;
@@ -552,11 +568,12 @@ struct Stretch {
             }
             // (a way out of the middle of the loop would cost it the same)
             while (kb + (kStages - 1) * step < k1) {
-                take(st[0]);
-                if constexpr (kStages > 1) take(st[1]);
+#pragma unroll
+                for (int i = 0; i < kStages; ++i) take(st[i]);
             }
-            if constexpr (kStages > 1)
-                if (kb < k1) take(st[0]);
+#pragma unroll
+            for (int i = 0; i + 1 < kStages; ++i)
+                if (kb < k1) take(st[i]);
             bool over = false;
 #pragma unroll
             for (int x = 0; x < kQT; ++x) {

@@ -67,13 +67,14 @@ __host__ __device__ __forceinline__ int k_offset(int d, int kk) {
 
 // Byte offset of value d of key kk in a block's V. The operand takes 16 values d (lane & 15) and 32 keys, 8 a lane group.
 // P comes out of S^T's accumulators, where group g holds keys 4g..4g+3 of each 16-key tile: so slots 0..3 are those of the
-// first tile, 4..7 those of the second. In fp4 two neighbouring keys share a byte, the even one in its low half.
+// first tile, 4..7 those of the second. In fp4 a byte has
+// the values d and d + 16 of a key, which share a scale: one instruction makes bf16 of both.
 template <int kFormat>
 __host__ __device__ __forceinline__ int v_offset(int d, int kk) {
     const int g = (kk & 15) >> 2, j = (kk >> 4) * 4 + (kk & 3);
     const int mt = d >> 4, lane = g * 16 + (d & 15);
     if constexpr (kFormat == DT_KV_BF16) return mt * kKvRun + lane * 16 + j * 2;
-    if constexpr (kFormat == DT_KV_FP4) return (mt >> 2) * kKvRun + lane * 16 + (mt & 3) * 4 + (j >> 1);
+    if constexpr (kFormat == DT_KV_FP4) return (mt >> 2) * kKvRun + lane * 16 + (mt >> 1 & 1) * 8 + j;
     return (mt >> 1) * kKvRun + lane * 16 + (mt & 1) * 8 + j;
 }
 

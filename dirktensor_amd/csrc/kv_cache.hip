@@ -338,8 +338,8 @@ __global__ __launch_bounds__(kThreads) void kv_append_rows_kernel(KvMoveArgs a, 
     }
 }
 
-// The same of a block in 4 bits. Two neighbouring keys share V's bytes: where the call has both, their threads (eight lanes apart)
-// exchange their values and each writes half of the 16 bytes; a key whose neighbour is not the call's keeps that one's halves.
+// The same of a block in 4 bits. A byte of V has values 16 apart, of two neighbouring threads: these exchange theirs, and each writes
+// eight of their sixteen bytes.
 template <bool kBf16, int kRows>
 __global__ __launch_bounds__(kThreads) void kv_append_fp4_kernel(KvMoveArgs a, KvRowsOf<kRows> rows) {
     constexpr int kTensor = kv_tensor_bytes(DT_KV_FP4);
@@ -351,8 +351,7 @@ __global__ __launch_bounds__(kThreads) void kv_append_fp4_kernel(KvMoveArgs a, K
     if (first >= start + cnt) return;  // (whole workgroups)
     const int kk = threadIdx.x >> 3, c = threadIdx.x & 7;
     const int t = first + kk - start;
-    const auto ours = [&](int key) { return first + key >= start && first + key < start + cnt; };
-    const bool mine = ours(kk), both = mine && ours(kk ^ 1);
+    const bool mine = t >= 0 && t < cnt;
     const bool whole = first >= start && first + kKvBlock <= start + cnt;
 
     float x[16] = {}, y[16] = {};
@@ -369,34 +368,25 @@ __global__ __launch_bounds__(kThreads) void kv_append_fp4_kernel(KvMoveArgs a, K
     vrow = max(vrow, other(vrow, 4));
     uint32_t qk[2], qv[2];
     const uint32_t sk = quantise4(x, kmax, krow < kInfBits, qk), sv = quantise4(y, vmax, vrow < kInfBits, qv);
-    const uint32_t pv[2] = {other(qv[0], 8), other(qv[1], 8)};  // the neighbouring key's
+    const uint32_t pv[2] = {other(qv[0], 1), other(qv[1], 1)};
 
     uint8_t* block = a.c.block<DT_KV_FP4>(rows.slot[b], h, blk);
     uint8_t* vd = block + kTensor;
     if (mine) {
         *reinterpret_cast<uint2*>(block + k_offset<DT_KV_FP4>(c * 16, kk)) = make_uint2(qk[0], qk[1]);
-        if (!(c & 1)) {
+        const int odd = c & 1;
+        if (!odd) {
             reinterpret_cast<uint8_t*>(scale_of<DT_KV_FP4>(block, false, kk))[c >> 1] = static_cast<uint8_t>(sk);
             reinterpret_cast<uint8_t*>(scale_of<DT_KV_FP4>(block, true, kk))[c >> 1] = static_cast<uint8_t>(sv);
         }
-        const int odd = kk & 1;
-        if (both) {
-            // values 8 odd .. 8 odd + 7 of both keys: the even key's in the low halves
-            const uint32_t even4 = odd ? pv[1] : qv[0], odd4 = odd ? qv[1] : pv[0];
+        // values 8 odd .. 8 odd + 7 of both, the even thread's in the low halves
+        const uint32_t low = odd ? pv[1] : qv[0], high = odd ? qv[1] : pv[0];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint8_t v = static_cast<uint8_t>((even4 >> (4 * i) & 15) | (odd4 >> (4 * i) & 15) << 4);
-                const int d = c * 16 + odd * 8 + i;
-                if (whole) vbuf[v_lds_offset<DT_KV_FP4>(d, kk)] = v;
-                else vd[v_offset<DT_KV_FP4>(d, kk)] = v;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                uint8_t* to = vd + v_offset<DT_KV_FP4>(c * 16 + i, kk);
-                const uint32_t v = qv[i >> 3] >> (4 * (i & 7)) & 15;
-                *to = static_cast<uint8_t>(odd ? (*to & 15) | v << 4 : (*to & 0xf0) | v);
-            }
+        for (int i = 0; i < 8; ++i) {
+            const uint8_t v = static_cast<uint8_t>((low >> (4 * i) & 15) | (high >> (4 * i) & 15) << 4);
+            const int d = c * 16 + odd * 8 + i;
+            if (whole) vbuf[v_lds_offset<DT_KV_FP4>(d, kk)] = v;
+            else vd[v_offset<DT_KV_FP4>(d, kk)] = v;
         }
     }
     if (whole) {  // (the same for the whole workgroup)
@@ -408,64 +398,39 @@ __global__ __launch_bounds__(kThreads) void kv_append_fp4_kernel(KvMoveArgs a, K
     }
 }
 
-// Few tokens a sequence: a wave takes a pair of neighbouring keys, of which the call has one or both, of K (even) or V (odd), lane i
-// their values 2 i and 2 i + 1.
+// Few tokens a sequence: a wave takes one row, 2 values a lane as above. A byte of V has values of lanes 8 apart.
 template <bool kBf16, int kRows>
 __global__ __launch_bounds__(kThreads) void kv_append_rows_fp4_kernel(KvMoveArgs a, KvRowsOf<kRows> rows) {
     const int lane = threadIdx.x & 63, unit = blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int b = blockIdx.z, h = unit >> 1;
+    const int b = blockIdx.z, t = blockIdx.y, h = unit >> 1;
     const bool v = unit & 1;
-    const int start = rows.len[b], cnt = rows.cnt[b];
-    const int pos = (start & ~1) + 2 * static_cast<int>(blockIdx.y);  // the pair's even key
-    if (h >= a.c.heads || pos >= start + cnt) return;
-    const int d = 2 * lane;
+    if (h >= a.c.heads || t >= rows.cnt[b]) return;
+    const int pos = rows.len[b] + t, d = 2 * lane;
+    const int64_t at = (v ? b * a.bsv + t * a.ldv : b * a.bsk + t * a.ldk) + h * DT_HEAD_DIM + d;
     const void* src = v ? a.v : a.k;
-    uint8_t* block = a.c.block<DT_KV_FP4>(rows.slot[b], h, pos / kKvBlock);
-    uint32_t q[2];
-    bool have[2];
-    float x[2][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int t = pos + i - start;
-        have[i] = t >= 0 && t < cnt;
-        x[i][0] = x[i][1] = 0.0f;
-        if (have[i]) {
-            const int64_t at = (v ? b * a.bsv + t * a.ldv : b * a.bsk + t * a.ldk) + h * DT_HEAD_DIM + d;
-            if constexpr (kBf16) {
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(src) + at);
-                x[i][0] = bf16_lo(w), x[i][1] = bf16_hi(w);
-            } else {
-                const float2 w = *reinterpret_cast<const float2*>(static_cast<const float*>(src) + at);
-                x[i][0] = w.x, x[i][1] = w.y;
-            }
-        }
-    }
-    const int kk = pos & (kKvBlock - 1);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        uint32_t amax = max(__float_as_uint(x[i][0]) & 0x7fffffffu, __float_as_uint(x[i][1]) & 0x7fffffffu);
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), o, 64)));
-        const bool finite = !__any(amax >= kInfBits);
-        uint32_t w[1];
-        const uint32_t s = quantise4<2>(x[i], amax, finite, w);
-        q[i] = w[0];
-        if (have[i] && (lane & 15) == 0)
-            reinterpret_cast<uint8_t*>(scale_of<DT_KV_FP4>(block, v, kk + i))[lane >> 4] = static_cast<uint8_t>(s);
-    }
-    if (!v) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (have[i]) block[k_offset<DT_KV_FP4>(d, kk + i)] = static_cast<uint8_t>(q[i]);
+    float x[2];
+    if constexpr (kBf16) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(src) + at);
+        x[0] = bf16_lo(w), x[1] = bf16_hi(w);
     } else {
-        uint8_t* vd = block + kv_tensor_bytes(DT_KV_FP4);
+        const float2 w = *reinterpret_cast<const float2*>(static_cast<const float*>(src) + at);
+        x[0] = w.x, x[1] = w.y;
+    }
+    uint32_t amax = max(__float_as_uint(x[0]) & 0x7fffffffu, __float_as_uint(x[1]) & 0x7fffffffu);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            uint8_t* to = vd + v_offset<DT_KV_FP4>(d + i, kk);
-            const uint32_t lo = q[0] >> (4 * i) & 15, hi = q[1] >> (4 * i) & 15;
-            const uint32_t old = have[0] && have[1] ? 0 : *to;
-            *to = static_cast<uint8_t>((have[0] ? lo : old & 15) | (have[1] ? hi << 4 : old & 0xf0));
-        }
+    for (int o = 1; o < 16; o <<= 1) amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), o, 64)));
+    uint32_t q[1];
+    const uint32_t s = quantise4<2>(x, amax, !__any(amax >= kInfBits), q);
+    const int kk = pos & (kKvBlock - 1);
+    uint8_t* block = a.c.block<DT_KV_FP4>(rows.slot[b], h, pos / kKvBlock);
+    if ((lane & 15) == 0) reinterpret_cast<uint8_t*>(scale_of<DT_KV_FP4>(block, v, kk))[lane >> 4] = static_cast<uint8_t>(s);
+    if (!v) {
+        block[k_offset<DT_KV_FP4>(d, kk)] = static_cast<uint8_t>(q[0]);
+    } else {
+        const uint32_t p = static_cast<uint32_t>(__shfl_xor(static_cast<int>(q[0]), 8, 64));
+        const int odd = lane >> 3 & 1;  // which of the two this lane has, and which of its two values' bytes it writes
+        const uint32_t low = odd ? p : q[0], high = odd ? q[0] : p;
+        block[kv_tensor_bytes(DT_KV_FP4) + v_offset<DT_KV_FP4>(d + odd, kk)] = static_cast<uint8_t>((low >> (4 * odd) & 15) | (high >> (4 * odd) & 15) << 4);
     }
 }
 
@@ -499,7 +464,7 @@ __global__ __launch_bounds__(kThreads) void kv_read_fp4_kernel(KvMoveArgs a, KvR
         uint32_t w[2] = {0, 0};
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            w[i >> 3] |= (static_cast<uint32_t>(vbuf[v_lds_offset<DT_KV_FP4>(c * 16 + i, kk)]) >> (4 * (kk & 1)) & 15) << (4 * (i & 7));
+            w[i >> 3] |= (static_cast<uint32_t>(vbuf[v_lds_offset<DT_KV_FP4>(c * 16 + i, kk)]) >> (4 * (c & 1)) & 15) << (4 * (i & 7));
         dequantise4(w[0], scale(true), x);
         dequantise4(w[1], scale(true), x + 8);
         store16<kBf16>(a.v, b * a.bsv + t * a.ldv + h * DT_HEAD_DIM + c * 16, x);
@@ -581,17 +546,13 @@ int launch_rows(const KvMoveArgs& a, const KvRowsOf<kRows>& rows, int B, int for
         else DT_KV_GO(F, false);                                                                                 \
     } while (0)
     if (format == DT_KV_FP4) {
-        int pairs = 0;  // of neighbouring keys
-        for (int b = 0; b < B; ++b)
-            if (rows.cnt[b] > 0) pairs = std::max(pairs, (rows.len[b] + rows.cnt[b] - 1) / 2 - rows.len[b] / 2 + 1);
-        const dim3 grid4 = few ? dim3(grid.x, pairs, B) : grid;
 #define DT_KV_GO4(M)                                                                                                       \
     do {                                                                                                                   \
         if constexpr (kAppend) {                                                                                           \
-            if (few) hipLaunchKernelGGL((kv_append_rows_fp4_kernel<M, kRows>), grid4, block, 0, s, a, rows);               \
-            else hipLaunchKernelGGL((kv_append_fp4_kernel<M, kRows>), grid4, block, 0, s, a, rows);                        \
+            if (few) hipLaunchKernelGGL((kv_append_rows_fp4_kernel<M, kRows>), grid, block, 0, s, a, rows);               \
+            else hipLaunchKernelGGL((kv_append_fp4_kernel<M, kRows>), grid, block, 0, s, a, rows);                        \
         } else {                                                                                                           \
-            hipLaunchKernelGGL((kv_read_fp4_kernel<M, kRows>), grid4, block, 0, s, a, rows);                               \
+            hipLaunchKernelGGL((kv_read_fp4_kernel<M, kRows>), grid, block, 0, s, a, rows);                               \
         }                                                                                                                  \
     } while (0)
         if (bf16) DT_KV_GO4(true);
