@@ -97,6 +97,7 @@ struct CachedAttnArgs {
     float* part_ml;  // [row][parts][2]: the maximum; l, negative where O is times kLower
     int64_t ldq;     // token stride of q, elements
     int B, T, H, G;  // G: query heads a key/value head
+    uint64_t by_G, by_T;  // 2^40 / G and / T, rounded up (divided)
     int causal;
     float scale;
     int parts;       // partial results a row at most
@@ -262,15 +263,18 @@ __device__ __forceinline__ int k_dim(int s, int g) {
     return (s >> 1) * 64 + g * 16 + (s & 1) * 8;
 }
 
+__device__ __forceinline__ int divided(int r, uint64_t by) { return static_cast<int>(static_cast<uint32_t>(r) * by >> 40); }
+
 struct QueryRow {
     int b, t, hq;
 };
 // row r of those that share key/value head hk's keys: tokens, then the group's heads; for the prefix the batch first
 __device__ __forceinline__ QueryRow query_row(const CachedAttnArgs& a, int r, int b, int hk, bool prefix) {
-    // (divisions by numbers that are mostly 1)
-    const int bt = a.G == 1 ? r : r / a.G, g = r - bt * a.G;
+    // (divisions by numbers that are mostly 1; r < 2^23, G <= 2^10 and T <= 2^13, so r times what the reciprocal is too large by, less
+    // than G or T, stays below 2^40)
+    const int bt = a.G == 1 ? r : divided(r, a.by_G), g = r - bt * a.G;
     if (!prefix) return {b, bt, hk * a.G + g};
-    const int of = a.T == 1 ? bt : bt / a.T;
+    const int of = a.T == 1 ? bt : divided(bt, a.by_T);
     return {of, bt - of * a.T, hk * a.G + g};
 }
 
@@ -1091,6 +1095,8 @@ int check_call(const dt_kv_cache* cache, int B, int T, int H, int D, const int32
     a->T = T;
     a->H = H;
     a->G = H / cache->heads;
+    a->by_G = ((1ull << 40) + a->G - 1) / a->G;
+    a->by_T = ((1ull << 40) + T - 1) / T;
     return DT_OK;
 }
 
