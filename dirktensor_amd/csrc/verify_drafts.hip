@@ -15,11 +15,12 @@
 //
 // Work: every row is read once for its sum (first kernel: a row in segments, as many as fill the CUs), and the one or two rows that the
 // weights come from once more, mostly from the caches (second kernel: each workgroup works out from the first kernel's sums which draft
-// was refused, and its waves take chunks of 1024 values). The weights' difference needs the ratio of both rows' sums, which is known
-// to 2^-24 only: a chunk leaves sum p' and sum q' over the values with p' > ratio q' (p', q': the powers, not divided by their sums),
-// and over all of them; the last workgroup of a batch row to be done has the ratio to 64 bits then, and a value whose sign the first
-// ratio got wrong has a weight below 2^-23 of its probability. Only where the weights' total is itself small (below kSmall) does that
-// count: that workgroup then sums the weights again. Last it finds the chunk that the border lies in, and in it the token.
+// was refused, and its waves take chunks of 512 values). The weights' difference needs the ratio of both rows' sums, which is known
+// to 2^-24 only: a chunk leaves sum (p' - ratio q') and sum q' over the values where that is above 0 (p', q': the powers, not divided
+// by their sums), and sum p' and sum q' over all; the last workgroup of a batch row to be done has the ratio to 64 bits then and
+// corrects the chunks' weights by it. A value whose sign the first ratio got wrong has a weight below 2^-23 of its probability; only
+// where the weights' total is itself small (below kSmall) does that count: that workgroup then sums the weights again. Last it finds
+// the chunk that the border lies in, and in it the token.
 
 #include "dt_internal.h"
 
@@ -39,7 +40,7 @@ constexpr int kFewRows = 32;
 constexpr int kMaxDrafts = 64;
 constexpr int kMaxRows = 2 * kMaxDrafts + 1;  // of a batch row
 constexpr int kMaxVocab = 1 << 24;
-constexpr int kChunk = 1024;                  // values that a wave of the second kernel takes at a time: 16 a lane
+constexpr int kChunk = 512;                   // values that a wave of the second kernel takes at a time: 8 a lane
 constexpr int kWhole = 4096;                  // of a batch of the first kernel, all threads
 constexpr int kMinSegment = 2048;             // values of a segment of the first kernel at least
 constexpr int kFill = 2048;                   // workgroups that the first kernel aims at, eight a CU
@@ -47,7 +48,7 @@ constexpr int kDrawFill = 1024;               // and the second
 constexpr double kSmall = 1e-4;
 constexpr double kLog2e = 1.4426950408889634074;
 constexpr double kLn2 = 0.69314718055994530942;
-constexpr double kFar = -1000.0;              // 2^kFar and below counts as 0
+constexpr double kFar = -1100.0;              // (2^-1100 is none of 64 bits)
 constexpr float kLowest = -3.402823466e38f;
 
 template <int kRows>
@@ -62,7 +63,7 @@ struct VerifyArgs {
     int32_t* count;       // [B]: workgroups of the second kernel that are done
     double2* part;        // [B][rows][segments]: the largest logit, and the sum of 2^(c (x - it))
     float2* best;         // [B][K + 1][segments] at T = 0: the largest logit, its index (as bits)
-    double* sums;         // [B][chunks][4]: sum p' and q' of the values with a weight, of all
+    double* sums;         // [B][chunks][4]: sum of p' - ratio q' and of q' where that is above 0, of p' and of q'
     int64_t ldb_x, ldt_x, ldb_y, ldt_y;
     double c;             // log2(e) / T
     float c_hi, c_lo;     // in two parts, both above 0 (a logit of -inf times either is -inf)
@@ -73,8 +74,9 @@ struct VerifyArgs {
     uint8_t n[kRows];     // drafts of each batch row
 };
 
-// 2^t to 10^-12 for t <= 1000, 0 below kFar; NaN stays. (2^f on [-1/2, 1/2] as its interpolation in nine Chebyshev points.)
+// 2^t to 10^-12 for t <= 1000, 0 for t <= kFar (and for NaN). (2^f on [-1/2, 1/2] as its interpolation in nine Chebyshev points.)
 __device__ __forceinline__ double exp2_64(double t) {
+    t = fmax(t, kFar);
     constexpr double kMagic = 6755399441055744.0;  // 1.5 2^52: the sum's low bits are the nearest whole number
     const double m = t + kMagic;
     const double f = t - (m - kMagic);
@@ -87,8 +89,7 @@ __device__ __forceinline__ double exp2_64(double t) {
     v = fma(v, f, 0x1.ebfbdff823cedp-3);
     v = fma(v, f, 0x1.62e42fef84cf0p-1);
     v = fma(v, f, 1.0);
-    v = __builtin_amdgcn_ldexp(v, static_cast<int>(__double_as_longlong(m)));
-    return t < kFar ? 0.0 : v;
+    return __builtin_amdgcn_ldexp(v, static_cast<int>(__double_as_longlong(m)));
 }
 
 template <bool kBf16>
@@ -332,20 +333,8 @@ __device__ __forceinline__ double log2_64(double s) {
     return y + (s * exp2_64(-y) - 1.0) * kLog2e;
 }
 
-// The two rows that the weights come from: p', 0 for a draft that nothing was drawn for, and q', 0 where there is no such row. Their
-// values go by twos through loops that are not unrolled: a kernel that runs once through its code waits for the code, too.
-struct Rows {
-    const void *px, *qx;  // qx: or NULL
-    double p_top, q_top, c;
-    int skip, V;
-    __device__ __forceinline__ void powers(float x, float y, int at, double& p, double& q) const {
-        p = exp2_64((static_cast<double>(x) - p_top) * c);
-        if (at == skip) p = 0.0;
-        q = 0.0;
-        if (qx) q = exp2_64((static_cast<double>(y) - q_top) * c);
-    }
-};
-// 8 values of a row as four pairs of words (bf16: two in a word)
+// 8 values of a row as four pairs of words, which the loops over them take one by one: a kernel that runs once through its code waits
+// for the code, too, so these loops are not unrolled.
 struct Eight {
     uint32_t lo[4], hi[4];
     template <bool kBf16>
@@ -362,10 +351,24 @@ struct Eight {
             }
         }
     }
+    __device__ __forceinline__ void hide(int i) {  // value i, if it is one of these, has no weight
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (2 * j == i) lo[j] = 0xff800000u;
+            if (2 * j + 1 == i) hi[j] = 0xff800000u;
+        }
+    }
     __device__ __forceinline__ void next() {
 #pragma unroll
         for (int i = 0; i < 3; ++i) lo[i] = lo[i + 1], hi[i] = hi[i + 1];
     }
+};
+// The two rows that the weights come from: p', and q', 0 where there is no such row.
+struct Rows {
+    const void *px, *qx;  // qx: or NULL
+    double p_top, q_top, c;
+    __device__ __forceinline__ double p(float x) const { return exp2_64((static_cast<double>(x) - p_top) * c); }
+    __device__ __forceinline__ double q(float y) const { return qx ? exp2_64((static_cast<double>(y) - q_top) * c) : 0.0; }
 };
 
 template <bool kBf16, bool kGreedy, int kRows>
@@ -467,42 +470,42 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs<kRows>
         token = best[acc];
     } else {
         const bool refused = acc < n;
-        Rows rows{row_of<kBf16>(a, b, acc), refused && a.y ? row_of<kBf16>(a, b, K + 1 + acc) : nullptr, tops[acc], 0.0, a.c,
-                  refused && !a.y ? drafts[acc] : -1, V};
+        Rows rows{row_of<kBf16>(a, b, acc), refused && a.y ? row_of<kBf16>(a, b, K + 1 + acc) : nullptr, tops[acc], 0.0, a.c};
+        const int skip = refused && !a.y ? drafts[acc] : -1;  // a draft that nothing was drawn for
         double near = 0.0;  // the ratio of the rows' sums, to 32 bits
         if (rows.qx) {
             rows.q_top = tops[K + 1 + acc];
             near = sums[acc] / sums[K + 1 + acc];
         }
+        const bool none = !(sum > 0.0) || !(near >= 0.0);  // a row that is none (the same for all of the batch row's workgroups)
+        if (none && blockIdx.x > 0) return;
         double* out = a.sums + static_cast<int64_t>(b) * a.chunks * 4;
         double h[4], p_sum = 0.0, ratio = 0.0, weight, before, all;
         int first = blockIdx.x * kWaves + wave, step = gridDim.x * kWaves;
-        for (bool again = false;; again = true) {
+        for (bool again = false; !none; again = true) {
 #pragma unroll 1
             for (int chunk = first; chunk < a.chunks; chunk += step) {
                 double pw = 0.0, qw = 0.0, pa = 0.0, qa = 0.0;
 #pragma unroll 1
                 for (int at = chunk * a.runs * kChunk + lane * 8, end = at + a.runs * kChunk; at < end; at += kChunk) {
-                    Eight x[2], y[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        x[i].load<kBf16>(rows.px, at + i * (kChunk / 2), V);
-                        if (rows.qx) y[i].load<kBf16>(rows.qx, at + i * (kChunk / 2), V);
-                    }
+                    Eight x, y;
+                    x.load<kBf16>(rows.px, at, V);
+                    if (rows.qx) y.load<kBf16>(rows.qx, at, V);
+                    if (static_cast<uint32_t>(skip - (at - lane * 8)) < kChunk) x.hide(skip - at);  // (the same for the whole wave)
 #pragma unroll 1
                     for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            double p, q;
-                            rows.powers(__uint_as_float(j & 1 ? x[j >> 1].hi[0] : x[j >> 1].lo[0]),
-                                        __uint_as_float(j & 1 ? y[j >> 1].hi[0] : y[j >> 1].lo[0]), at + (j >> 1) * (kChunk / 2) + 2 * i + (j & 1), p, q);
-                            const bool some = p > near * q;
+                        for (int j = 0; j < 2; ++j) {
+                            const double p = rows.p(__uint_as_float(j ? x.hi[0] : x.lo[0]));
                             pa += p;
-                            qa += q;
-                            pw += some ? p : 0.0;
-                            qw += some ? q : 0.0;
+                            if (rows.qx) {
+                                const double q = rows.q(__uint_as_float(j ? y.hi[0] : y.lo[0])), w = fma(-near, q, p);
+                                qa += q;
+                                pw += fmax(w, 0.0);
+                                qw += w > 0.0 ? q : 0.0;
+                            }
                         }
-                        x[0].next(), x[1].next(), y[0].next(), y[1].next();
+                        x.next(), y.next();
                     }
                 }
                 const double mine[4] = {pw, qw, pa, qa};
@@ -530,21 +533,20 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs<kRows>
                 p_sum = sum_all(h[2], red);
                 if (rows.qx) ratio = p_sum / sum_all(h[3], red);
             }
-            weight = rows.qx ? h[0] - ratio * h[1] : h[2];
-            if (weight < 0.0) weight = 0.0;  // (NaN stays)
+            weight = rows.qx ? fmax(h[0] - (ratio - near) * h[1], 0.0) : h[2];
             before = scan(weight, red, &all);
             if (again || !rows.qx || !(all < kSmall * p_sum)) break;  // (the same for the whole workgroup)
             near = ratio;
             first = wave, step = kWaves;
         }
-        if (all == 0.0 && rows.qx) {  // nothing is left: p itself
+        if (!none && all == 0.0 && rows.qx) {  // nothing is left: p itself
             rows.qx = nullptr;
             ratio = 0.0;
             weight = h[2];
             before = scan(weight, red, &all);
         }
-        if (rows.skip < 0) sum = p_sum;
-        if (all > 0.0) {
+        if (skip < 0) sum = p_sum;
+        if (!none && all > 0.0) {
             const double bound = last_u * all;
             // the first thread whose sum passes the border; where rounding leaves none, the last that has a weight (none: -1)
             bool passed = false;
@@ -574,12 +576,11 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs<kRows>
                 for (int i = 0; i < kOwn; ++i) {
                     x[i] = at + i < V ? load_one<kBf16>(rows.px, at + i) : -__builtin_huge_valf();
                     y[i] = rows.qx && at + i < V ? load_one<kBf16>(rows.qx, at + i) : -__builtin_huge_valf();
+                    if (at + i == skip) x[i] = -__builtin_huge_valf();
                 }
 #pragma unroll
                 for (int i = 0; i < kOwn; ++i) {
-                    double q;
-                    rows.powers(x[i], y[i], at + i, w[i], q);
-                    w[i] = fmax(w[i] - ratio * q, 0.0);
+                    w[i] = fmax(fma(-ratio, rows.q(y[i]), rows.p(x[i])), 0.0);
                     mine += w[i];
                 }
                 double upto = before + scan(mine, red, &all);
