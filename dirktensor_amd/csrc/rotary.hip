@@ -337,7 +337,7 @@ __global__ __launch_bounds__(kThreads) void head_norm_rotary_bwd_kernel(RotaryAr
             g.open(next_g);
             x.open(next_x);
             fetch(more ? token : next_token, more ? first + kGroupHeads : next_part * span);
-            if (!have) g.zero();
+            if (!have) g.zero(), x.zero();
             g.turn(cs[wave], lane, a.octets);
             const float inv = inverse_rms(x, a.eps);
             float dot = 0.0f;
@@ -436,9 +436,10 @@ int check_call(const dt_ctx* ctx, const Call& c) {
     if (c.D != DT_HEAD_DIM) return set_error(DT_ERR_UNSUPPORTED, "head_dim D=%d, kernels are built for D=%d", c.D, DT_HEAD_DIM);
     if (c.H + static_cast<int64_t>(c.Hk) > kMaxHeads) return set_error(DT_ERR_UNSUPPORTED, "%d and %d heads are more than %d", c.H, c.Hk, kMaxHeads);
     if (c.Hk > 0 && (!c.k || !c.ok)) return set_error(DT_ERR_INVALID_ARG, "k and its output must be non-NULL with Hk=%d", c.Hk);
-    // (indices of groups of heads stay within 31 bits)
-    if (static_cast<int64_t>(c.B) * c.T * ((c.H + 7) / 8 + (c.Hk + 7) / 8) > 0x7fffffff / 2)
-        return set_error(DT_ERR_UNSUPPORTED, "B*T = %lld tokens", (long long)c.B * c.T);
+    // (a launch's threads and the indices of groups of heads stay within 31 bits)
+    if (static_cast<int64_t>(c.B) * c.T > 0x7fffff) return set_error(DT_ERR_UNSUPPORTED, "B*T = %lld tokens", (long long)c.B * c.T);
+    if (c.Hk > 0 && (c.oq == c.ok || c.oq == c.k || c.ok == c.q || (c.xk && (c.oq == c.xk || c.ok == c.xq))))
+        return set_error(DT_ERR_INVALID_ARG, "an output is the other's, or the other's input");
     if (c.dtype != DT_FP32_EXACT && c.dtype != DT_BF16) return set_error(DT_ERR_INVALID_ARG, "unknown dtype %d", c.dtype);
     if (c.mem != DT_MEM_DEVICE && c.mem != DT_MEM_HOST) return set_error(DT_ERR_INVALID_ARG, "unknown mem %d", c.mem);
     if (c.positions && c.starts) return set_error(DT_ERR_INVALID_ARG, "positions and starts exclude each other");

@@ -515,9 +515,9 @@ typedef struct dt_rotary {
 int dt_rotary_init(dt_rotary* rotary, int dims, int layout, double theta, int scaling, double factor, double original_length,
                    double low, double high, double magnitude);
 /*
- * Rotates B x T tokens' queries (H heads) and keys (Hk heads; 0: none, k and k_out are ignored).
+ * Rotates B x T (<= 8388607) tokens' queries (H heads) and keys (Hk heads; 0: none, k and k_out are ignored).
  *   q, k, q_out, k_out : tokens of heads*128 values in dtype, ld* elements apart; an output may be its input (same address and
- *                        stride), and must not overlap it otherwise
+ *                        stride), and must not overlap it, the other input or the other output otherwise
  *   positions : [B, T] whole numbers of pos_bytes (4 or 8), in the same memory as q, or NULL: token (b, t) is at starts[b] + t
  *   starts    : B host values (B <= 256 then), or NULL: 0
  *   rotary    : host memory, read during the call

@@ -155,6 +155,31 @@ def test_nan_rows_reach_only_the_queries_that_see_them(gpu, tdt):
 
 
 @pytest.mark.parametrize("tdt", TYPES)
+def test_nan_rows_and_shared_heads(gpu, tdt):
+    """Several query tiles a wave, of which some see a row that is none and others do not."""
+    from dirktensor_amd import KVCache, cached_attention
+
+    T, L, H, Hk = 20, 150, 8, 2
+    k, v, q = attn.randn((1, L, Hk, D), 1), attn.randn((1, L, Hk, D), 2), attn.randn((1, T, H, D), 3, tdt)
+    clean, c = (KVCache(1, L + 40, Hk, format="fp4") for _ in range(2))
+    clean.append(k, v)
+    want = cached_attention(q, clean, attn.SCALE)
+    k, v = k.clone(), v.clone()
+    v[0, L - 7, 0, 5] = float("nan")   # seen by the last seven tokens, of the first four query heads
+    k[0, L - 12, 1, 7] = float("inf")  # by the last twelve, of the others
+    c.append(k, v)
+    junk = torch.full((1, 40, Hk, D), float("nan"), device="cuda")
+    c.append(junk, junk)
+    c.truncate([L])
+    r = cached_attention(q, c, attn.SCALE)
+    hit = torch.zeros((1, T, H), dtype=torch.bool, device="cuda")
+    hit[0, T - 7:, :4] = True
+    hit[0, T - 12:, 4:] = True
+    assert bool(torch.isnan(r.output[hit]).all())
+    assert torch.equal(r.output[~hit], want.output[~hit]) and torch.equal(r.softmax_l[~hit], want.softmax_l[~hit])
+
+
+@pytest.mark.parametrize("tdt", TYPES)
 @pytest.mark.parametrize("B,T,H,Hk,longest,P", [(64, 1, 16, 16, 500, 0), (64, 1, 16, 16, 100, 300), (33, 3, 16, 16, 120, 0)])
 def test_more_sequences_and_heads_than_workgroups(gpu, tdt, B, T, H, Hk, longest, P):
     attn.test_more_sequences_and_heads_than_workgroups("fp4", tdt, B, T, H, Hk, longest, P)

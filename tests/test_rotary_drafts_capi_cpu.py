@@ -70,6 +70,7 @@ ROWS = [
     (dict(positions=FAKE, pos_bytes=2), C.DT_ERR_INVALID_ARG, "pos_bytes"), (dict(positions=FAKE + 4, pos_bytes=8), C.DT_ERR_INVALID_ARG, "aligned"),
     (dict(B=257, starts=FAKE), C.DT_ERR_UNSUPPORTED, "starts"), (dict(ldq=255), C.DT_ERR_INVALID_ARG, "strides"),
     (dict(ldko=127), C.DT_ERR_INVALID_ARG, "strides"), (dict(ldq=260), C.DT_ERR_INVALID_ARG, "aligned"), (dict(oq=FAKE + 8), C.DT_ERR_INVALID_ARG, "aligned"),
+    (dict(ok=FAKE), C.DT_ERR_INVALID_ARG, "the other"), (dict(oq=FAKE + 4096, ok=FAKE + 8192), C.DT_ERR_INVALID_ARG, "the other"),
     ({}, C.DT_ERR_INVALID_ARG, "ctx is NULL"),
 ]
 
@@ -77,7 +78,7 @@ ROWS = [
 @pytest.mark.parametrize("kw,code,msg", ROWS + [(dict(backward=2), C.DT_ERR_INVALID_ARG, "backward")])
 def test_rotary_fwd(kw, code, msg):
     r, _ = rotary()
-    a = dict(ctx=None, q=FAKE, k=FAKE, oq=FAKE, ok=FAKE, B=1, T=4, H=2, Hk=1, D=128, ldq=256, ldk=128, ldqo=256, ldko=128, positions=None,
+    a = dict(ctx=None, q=FAKE, k=FAKE + 4096, oq=FAKE, ok=FAKE + 4096, B=1, T=4, H=2, Hk=1, D=128, ldq=256, ldk=128, ldqo=256, ldko=128, positions=None,
              pos_bytes=4, starts=None, rot=ctypes.addressof(r), backward=0, dtype=C.DT_BF16, mem=C.DT_MEM_DEVICE, stream=None)
     a.update(kw)
     refused(C.lib().dt_rotary_fwd(*a.values()), code, msg)
@@ -100,7 +101,7 @@ def test_a_rotary_filled_by_hand_is_checked():
     (dict(eps=0.0), C.DT_ERR_INVALID_ARG, "eps"), (dict(eps=float("inf")), C.DT_ERR_INVALID_ARG, "eps")])
 def test_head_norm_fwd(kw, code, msg):
     r, _ = rotary()
-    a = dict(ctx=None, q=FAKE, k=FAKE, wq=FAKE, wk=FAKE, oq=FAKE, ok=FAKE, B=1, T=4, H=2, Hk=1, D=128, ldq=256, ldk=128, ldqo=256, ldko=128,
+    a = dict(ctx=None, q=FAKE, k=FAKE + 4096, wq=FAKE, wk=FAKE + 4096, oq=FAKE, ok=FAKE + 4096, B=1, T=4, H=2, Hk=1, D=128, ldq=256, ldk=128, ldqo=256, ldko=128,
              positions=None, pos_bytes=4, starts=None, rot=ctypes.addressof(r), eps=1e-6, dtype=C.DT_BF16, mem=C.DT_MEM_DEVICE, stream=None)
     a.update(kw)
     refused(C.lib().dt_head_norm_rotary_fwd(*a.values()), code, msg)
@@ -111,7 +112,7 @@ def test_head_norm_fwd(kw, code, msg):
     (dict(ldxk=64), C.DT_ERR_INVALID_ARG, "strides"), (dict(xk=FAKE + 8), C.DT_ERR_INVALID_ARG, "aligned"), ({}, C.DT_ERR_INVALID_ARG, "ctx is NULL")])
 def test_head_norm_bwd(kw, code, msg):
     r, _ = rotary()
-    a = dict(ctx=None, q=FAKE, k=FAKE, xq=FAKE, xk=FAKE, wq=FAKE, wk=FAKE, oq=FAKE, ok=FAKE, dwq=FAKE, dwk=FAKE, B=1, T=4, H=2, Hk=1, D=128, ldq=256,
+    a = dict(ctx=None, q=FAKE, k=FAKE + 4096, xq=FAKE, xk=FAKE + 4096, wq=FAKE, wk=FAKE + 4096, oq=FAKE, ok=FAKE + 4096, dwq=FAKE, dwk=FAKE, B=1, T=4, H=2, Hk=1, D=128, ldq=256,
              ldk=128, ldxq=256, ldxk=128, ldqo=256, ldko=128, positions=None, pos_bytes=4, starts=None, rot=ctypes.addressof(r), eps=1e-6, ws=FAKE,
              ws_bytes=1 << 30, dtype=C.DT_BF16, mem=C.DT_MEM_DEVICE, stream=None)
     a.update(kw)

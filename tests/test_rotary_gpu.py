@@ -196,6 +196,19 @@ def test_head_norm_gradients(gpu, tdt, layout, dims, B, T, H, Hk):
         assert torch.equal(dx, dx2) and torch.equal(dw, dw2)
 
 
+def test_heads_that_are_none_do_not_reach_the_other_heads_weights(gpu):
+    """9 heads: the last group of eight has one. A NaN in a head of q makes q's weights' gradient NaN, not k's."""
+    rot = dt().Rotary()
+    q, k, dq, dk = randn((1, 3, 9, D), 1), randn((1, 3, 9, D), 2), randn((1, 3, 9, D), 3), randn((1, 3, 9, D), 4)
+    w = torch.ones(D, device="cuda")
+    want = dt().head_norm_rotary_backward(dq, dk, q, k, w, w, rot)
+    q[0, 1, 8, 5] = float("nan")
+    r = dt().head_norm_rotary_backward(dq, dk, q, k, w, w, rot)
+    assert torch.equal(r.d_K, want.d_K) and torch.equal(r.d_k_weight, want.d_k_weight)
+    assert torch.isnan(r.d_Q[0, 1, 8]).all() and int(torch.isnan(r.d_Q).sum()) == D
+    assert torch.isnan(r.d_q_weight).all()
+
+
 def test_gradients_against_differences(gpu):
     """<d, f(x + e v) - f(x - e v)> / 2e of the 64-bit formula against the kernel's gradients along v."""
     rot = dt().Rotary(dims=96, layout="interleaved")
@@ -363,6 +376,8 @@ def test_refusals(gpu):
         dt().rotary(q, k, rot, starts=[1])
     with pytest.raises(dt().DTError, match="T=0"):
         dt().rotary(q[:, :0], None, rot)
+    with pytest.raises(dt().DTError, match="other"):
+        dt().rotary(q, q, rot, inplace=True)
     with pytest.raises(ValueError, match="q_weight"):
         dt().head_norm_rotary(q, None, w[:64], None, rot)
     with pytest.raises(ValueError, match="k_weight"):
