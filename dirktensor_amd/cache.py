@@ -132,12 +132,13 @@ class KVCache:
         """Writes the rows of K and V [B, T, n_heads, 128] (both fp32 or both bf16; torch device tensors, views of a
         projection's output among them, or numpy arrays) behind what the B slots hold: slots[b], distinct, or 0 .. B-1.
         With ``counts`` batch row b appends its first counts[b] tokens. Raises DTError where a slot has no room."""
-        if K.shape != V.shape or len(K.shape) != 4 or tuple(K.shape[2:]) != (self.n_heads, C.HEAD_DIM):
-            raise ValueError(f"K and V must share a shape [B, T, {self.n_heads}, {C.HEAD_DIM}], got {tuple(K.shape)}, "
+        shape = K.shape
+        if shape != V.shape or len(shape) != 4 or shape[2] != self.n_heads or shape[3] != C.HEAD_DIM:
+            raise ValueError(f"K and V must share a shape [B, T, {self.n_heads}, {C.HEAD_DIM}], got {tuple(shape)}, "
                              f"{tuple(V.shape)}")
         if _is_torch(K) != _is_torch(V) or K.dtype != V.dtype:
             raise TypeError("K and V must be of one kind and dtype")
-        B, T = int(K.shape[0]), int(K.shape[1])
+        B, T = shape[0], shape[1]
         dtype = _mode_of(K, None)
         s, s_p = _per_row(slots, B, "slots")
         n, n_p = _per_row(counts, B, "counts")

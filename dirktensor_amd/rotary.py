@@ -150,28 +150,42 @@ def _inputs(x, host):
     return r, r.data_ptr(), ld
 
 
-def _outputs(x, rows, host, inplace):
-    """Where a result of x's shape goes: (the result, address, token stride)"""
+def _rows_and_result(x, host, inplace):
+    """The same, and where the result goes: (what to hold, address, token stride, the result, its address, its token stride)"""
     if x is None:
-        return None, None, 0
+        return None, None, 0, None, None, 0
+    r, p, ld = _inputs(x, host)
     if inplace:
-        if rows[0] is not x or (host and not x.flags.writeable):
+        if r is not x or (host and not x.flags.writeable):
             raise ValueError("in place needs writable rows of 128 contiguous values, 16-byte aligned, with one stride between tokens")
-        return x, rows[1], rows[2]
+        return r, p, ld, x, p, ld
     if host:
         o = np.empty(x.shape, x.dtype)
-        return o, o.ctypes.data, o.shape[2] * C.HEAD_DIM
-    o = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
-    return o, o.data_ptr(), x.shape[2] * C.HEAD_DIM
+        return r, p, ld, o, o.ctypes.data, o.shape[2] * C.HEAD_DIM
+    o = torch.empty_like(r) if r is x and x.is_contiguous() else x.new_empty(x.shape)
+    return r, p, ld, o, o.data_ptr(), x.shape[2] * C.HEAD_DIM
+
+
+_needs: dict = {}  # bytes by (B, T, H, Hk): they follow from these alone
+
+
+def _workspace_bytes(B: int, T: int, H: int, Hk: int) -> int:
+    n = _needs.get((B, T, H, Hk))
+    if n is None:
+        out = ctypes.c_int64()
+        C.call("dt_head_norm_rotary_bwd_workspace", B, T, H, Hk, ctypes.byref(out))
+        if len(_needs) >= 4096:
+            _needs.clear()
+        n = _needs[(B, T, H, Hk)] = out.value
+    return n
 
 
 def _weight(w, like, name):
     if _is_torch(like):
-        if not _is_torch(w) or w.device != like.device or w.dtype != torch.float32 or w.shape != (C.HEAD_DIM,):
+        if not _is_torch(w) or w.dtype != torch.float32 or w.dim() != 1 or w.numel() != C.HEAD_DIM or w.device != like.device:
             raise ValueError(f"{name} must be a [{C.HEAD_DIM}] fp32 tensor where the rows are")
-        w = w.contiguous()
-        if w.data_ptr() % 16:
-            w = w.clone()
+        if not w.is_contiguous() or w.data_ptr() % 16:
+            w = w.clone(memory_format=torch.contiguous_format)
         return w, w.data_ptr()
     w = np.ascontiguousarray(w)
     if w.dtype != np.float32 or w.shape != (C.HEAD_DIM,):
@@ -183,12 +197,13 @@ def _rotate(Q, K, rot, positions, starts, inplace, ctx, backward):
     B, T, H, Hk = _check_rows(Q, K, ("d_Q", "d_K") if backward else ("Q", "K"))
     ctx = _context_of(Q, ctx)
     dtype, host = _mode_of(Q, None), not _is_torch(Q)
-    pos = _positions_of(positions, starts, B, T, Q)
-    q, k = _inputs(Q, host), _inputs(K, host)
-    oq, ok = _outputs(Q, q, host, inplace), _outputs(K, k, host, inplace)
-    C.check(C.lib().dt_rotary_fwd(ctx.handle, q[1], k[1], oq[1], ok[1], B, T, H, Hk, C.HEAD_DIM, q[2], k[2], oq[2], ok[2], pos[1], pos[2],
-           pos[3], rot._p, backward, dtype, C.DT_MEM_HOST if host else C.DT_MEM_DEVICE, None if host else _stream_of(Q)))
-    return oq[0], ok[0]
+    _held, pos_p, pos_bytes, starts_p = _positions_of(positions, starts, B, T, Q)
+    _q, q_p, ldq, out_q, oq_p, ldoq = _rows_and_result(Q, host, inplace)
+    _k, k_p, ldk, out_k, ok_p, ldok = _rows_and_result(K, host, inplace)
+    mem, stream = (C.DT_MEM_HOST, None) if host else (C.DT_MEM_DEVICE, _stream_of(Q))
+    C.check(C.lib().dt_rotary_fwd(ctx.handle, q_p, k_p, oq_p, ok_p, B, T, H, Hk, C.HEAD_DIM, ldq, ldk, ldoq, ldok, pos_p, pos_bytes,
+                                  starts_p, rot._p, backward, dtype, mem, stream))
+    return out_q, out_k
 
 
 def rotary(Q, K, rot: Rotary, *, positions=None, starts=None, inplace: bool = False, ctx: Optional[Context] = None):
@@ -213,15 +228,15 @@ def head_norm_rotary(Q, K, q_weight, k_weight, rot: Rotary, *, positions=None, s
     B, T, H, Hk = _check_rows(Q, K)
     ctx = _context_of(Q, ctx)
     dtype, host = _mode_of(Q, None), not _is_torch(Q)
-    pos = _positions_of(positions, starts, B, T, Q)
-    wq = _weight(q_weight, Q, "q_weight")
-    wk = _weight(k_weight, Q, "k_weight") if Hk else (None, None)
-    q, k = _inputs(Q, host), _inputs(K, host)
-    oq, ok = _outputs(Q, q, host, inplace), _outputs(K, k, host, inplace)
-    C.call("dt_head_norm_rotary_fwd", ctx.handle, q[1], k[1], wq[1], wk[1], oq[1], ok[1], B, T, H, Hk, C.HEAD_DIM, q[2], k[2], oq[2],
-           ok[2], pos[1], pos[2], pos[3], rot._p, float(eps), dtype, C.DT_MEM_HOST if host else C.DT_MEM_DEVICE,
-           None if host else _stream_of(Q))
-    return oq[0], ok[0]
+    _held, pos_p, pos_bytes, starts_p = _positions_of(positions, starts, B, T, Q)
+    _wq, wq_p = _weight(q_weight, Q, "q_weight")
+    _wk, wk_p = _weight(k_weight, Q, "k_weight") if Hk else (None, None)
+    _q, q_p, ldq, out_q, oq_p, ldoq = _rows_and_result(Q, host, inplace)
+    _k, k_p, ldk, out_k, ok_p, ldok = _rows_and_result(K, host, inplace)
+    mem, stream = (C.DT_MEM_HOST, None) if host else (C.DT_MEM_DEVICE, _stream_of(Q))
+    C.check(C.lib().dt_head_norm_rotary_fwd(ctx.handle, q_p, k_p, wq_p, wk_p, oq_p, ok_p, B, T, H, Hk, C.HEAD_DIM, ldq, ldk, ldoq, ldok,
+                                            pos_p, pos_bytes, starts_p, rot._p, float(eps), dtype, mem, stream))
+    return out_q, out_k
 
 
 def head_norm_rotary_backward(d_Q, d_K, Q, K, q_weight, k_weight, rot: Rotary, *, positions=None, starts=None, eps: float = 1e-6,
@@ -236,24 +251,27 @@ def head_norm_rotary_backward(d_Q, d_K, Q, K, q_weight, k_weight, rot: Rotary, *
         raise TypeError("the gradients must be of the inputs' kind, dtype and device")
     ctx = _context_of(Q, ctx)
     dtype, host = _mode_of(Q, None), not _is_torch(Q)
-    pos = _positions_of(positions, starts, B, T, Q)
-    wq = _weight(q_weight, Q, "q_weight")
-    wk = _weight(k_weight, Q, "k_weight") if Hk else (None, None)
-    gq, gk, q, k = (_inputs(t, host) for t in (d_Q, d_K, Q, K))
-    oq, ok = _outputs(Q, q, host, False), _outputs(K, k, host, False)
+    _held, pos_p, pos_bytes, starts_p = _positions_of(positions, starts, B, T, Q)
+    _wq, wq_p = _weight(q_weight, Q, "q_weight")
+    _wk, wk_p = _weight(k_weight, Q, "k_weight") if Hk else (None, None)
+    _gq, gq_p, ldgq = _inputs(d_Q, host)
+    _gk, gk_p, ldgk = _inputs(d_K, host)
+    _q, q_p, ldq, out_q, oq_p, ldoq = _rows_and_result(Q, host, False)
+    _k, k_p, ldk, out_k, ok_p, ldok = _rows_and_result(K, host, False)
     n = 2 if Hk else 1
     if host:
         dw = np.empty((n, C.HEAD_DIM), np.float32)
         dw_p, ws, mem, stream = dw.ctypes.data, (None, 0), C.DT_MEM_HOST, None
+        d_w = list(dw)
     else:
         dw = Q.new_empty((n, C.HEAD_DIM), dtype=torch.float32)
         dw_p, mem, stream = dw.data_ptr(), C.DT_MEM_DEVICE, _stream_of(Q)
-        need = ctypes.c_int64()
-        C.call("dt_head_norm_rotary_bwd_workspace", B, T, H, Hk, ctypes.byref(need))
+        d_w = dw.unbind(0)
+        need = _workspace_bytes(B, T, H, Hk)
         ws = kept_workspace(ctx.device, stream)
-        if ws is None or ws[1] < need.value:
-            ws = new_workspace(Q, ctx.device, stream, need.value)
-    C.call("dt_head_norm_rotary_bwd", ctx.handle, gq[1], gk[1], q[1], k[1], wq[1], wk[1], oq[1], ok[1], dw_p,
-           dw_p + 4 * C.HEAD_DIM if Hk else None, B, T, H, Hk, C.HEAD_DIM, gq[2], gk[2], q[2], k[2], oq[2], ok[2], pos[1], pos[2],
-           pos[3], rot._p, float(eps), ws[0], ws[1], dtype, mem, stream)
-    return HeadNormRotaryGradients(oq[0], ok[0], dw[0], dw[1] if Hk else None)
+        if ws is None or ws[1] < need:
+            ws = new_workspace(Q, ctx.device, stream, need)
+    C.check(C.lib().dt_head_norm_rotary_bwd(ctx.handle, gq_p, gk_p, q_p, k_p, wq_p, wk_p, oq_p, ok_p, dw_p,
+                                            dw_p + 4 * C.HEAD_DIM if Hk else None, B, T, H, Hk, C.HEAD_DIM, ldgq, ldgk, ldq, ldk, ldoq,
+                                            ldok, pos_p, pos_bytes, starts_p, rot._p, float(eps), ws[0], ws[1], dtype, mem, stream))
+    return HeadNormRotaryGradients(out_q, out_k, d_w[0], d_w[1] if Hk else None)
