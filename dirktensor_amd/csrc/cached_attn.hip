@@ -5,7 +5,7 @@
 //   m = max_j s_j,  l = sum_j exp(s_j - m),  o = sum_j exp(s_j - m) v_j / l.
 //
 // What bounds it: a few query rows meet every held key once, so the cache's bytes (132 a key and head for K and for V
-// in 8 bits) are all that counts until about a hundred query rows share a key; arithmetic is far from its bound.
+// in 8 bits, 68 in 4) are all that counts until about a hundred query rows share a key; arithmetic is far from its bound.
 //
 // Work decomposition
 //   * Query rows that share a key/value head's keys go together, 16 to a matrix tile: the tokens and the query heads of
@@ -27,13 +27,17 @@
 // Measured at 16 heads, us: one sequence of 1000 in bf16 9.8 (latency: 16 workgroups); 16 sequences of up to 4096 in int8, 167 MB,
 // 28 and 4.4 for the join (6.0 TB/s); 32 of 8192 in fp8, 1.1 GB, 161 without a join (6.9 TB/s, what a read of this size reaches); 64 of
 // up to 512 behind a prefix of 4096 in int8 27 and 4.4 (94 MB, and the prefix's widening and products beside it); 12 by 5 tokens
-// behind 2777 in fp8 13 and 4; 4 of 1500 in exact mode, int8, 12 and 4.
+// behind 2777 in fp8 13 and 4; 4 of 1500 in exact mode, int8, 12 and 4. In 4 bits: 32 of 8192, 571 MB, 92 without a join (6.2 TB/s; about
+// 223 vector instructions a block, 64 % of what the CUs can issue); 12 by 5 tokens of 16 heads on 4 key/value heads, up to 1500 each behind 2777,
+// 18 and 5.7.
 //
 // Arithmetic: S^T = K Q^T with v_mfma_f32_16x16x32_bf16 on the held values, which bf16 holds exactly (int8 and e4m3
 // alike); the key's scale multiplies the 32-bit score. P times the value's scale is rounded to bf16 (at most half a step,
 // 2^-8 relative, for each term of the sum) for O^T += V^T P^T; m, l and O stay in 32 bits, l sums the unrounded probabilities.
 // In fp32 mode q (divided by 2^9 times the power of two below its row's largest magnitude) and P are split into three bf16 values
 // each, whose sum is the fp32 value, so every product is exact in the 32-bit accumulation.
+// In 4 bits a row has four scales, so they go into the operands: the conversion to bf16 multiplies by a power of two, exactly, and
+// no score or probability is. In exact mode the parts of q and P meet the same operands.
 
 #include "kv_cache.h"
 
@@ -73,7 +77,8 @@ constexpr float kLower = 0x1p-32f, kRaise = 0x1p32f;
 constexpr int kBufferDword3 = 0x00020000;  // raw buffer, 32-bit data format (gfx9 family)
 
 // blocks in flight a wave: what 256 registers a lane hold, which leave two workgroups a CU. Two of 8 bits with one query tile take 212;
-// two of bf16, in exact mode or with two tiles would spill 8, 19 and 79.
+// two of bf16, in exact mode or with two tiles would spill 8, 19 and 79. Two of 4 bits take 104; three and four of them gain nothing (32 of
+// 8192 94 and 99 us, profiled, where two take 92 to 98).
 constexpr int stages(int format, bool f32, int qt) { return format == DT_KV_BF16 || f32 || qt > 1 ? 1 : 2; }
 
 // The batch rows, by value in the kernel's arguments (kN places, 32 where these are enough: eager calls at 16 heads in int8, one
@@ -924,6 +929,8 @@ int query_waves_log(int64_t rows, int qt) { return rows <= 16 * qt ? 0 : rows <=
 
 // How a call is cut; fills rows' cum and the arguments that follow from the sizes. Returns the workspace's bytes.
 int64_t make_plan(CachedAttnArgs& a, AttnRows& rows, int format, bool f32, bool* join) {
+    // (in 4 bits the registers would hold three or four workgroups a CU: 32 of 8192 take 112 and 99 us then and 93 with two, 12 x 5 tokens
+    // of 4 key/value heads behind 2777 28, 28 and 21)
     constexpr int kResident = 2 * kCus;
     const int heads = a.own.heads;
     const int64_t own_rows = static_cast<int64_t>(a.T) * a.G, all_rows = own_rows * a.B;

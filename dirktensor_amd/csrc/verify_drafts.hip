@@ -21,6 +21,12 @@
 // corrects the chunks' weights by it. A value whose sign the first ratio got wrong has a weight below 2^-23 of its probability; only
 // where the weights' total is itself small (below kSmall) does that count: that workgroup then sums the weights again. Last it finds
 // the chunk that the border lies in, and in it the token.
+//
+// Measured at 100352 logits a row: 4 drafts of one sequence in fp32, 3.6 MB, 4.2 and 9.9 us in the two kernels: chains of one batch and of
+// one chunk, with about seven trips to memory in the second (the partial sums, the drafts' logits, a chunk, its sums out, the count, the sums
+// in, the border's chunk). Up to 5 drafts of 64 sequences in bf16, 72 MB, 20.7 and 26: the first is 3.5 TB/s, with 26 cycles a value and wave
+// for the powers and sums beside the reads; the second has 64 bits' arithmetic, 110 cycles a value and wave, 9 us were it spread evenly
+// (13 to 25 workgroups a batch row all take 24 to 27), and the chain around it.
 
 #include "dt_internal.h"
 
