@@ -423,13 +423,25 @@ struct Call {
     bool norm, backward;
 };
 
+bool good_magnitude(double m) {  // (the kernels have it in 32 bits)
+    const float f = static_cast<float>(m);
+    return std::isfinite(f) && f >= 0x1p-126f;
+}
+
 bool good_rotary(const dt_rotary* r) {
     if (r->dims < 16 || r->dims > DT_HEAD_DIM || r->dims % 16) return false;
     if (r->layout != DT_ROTARY_HALF && r->layout != DT_ROTARY_INTERLEAVED) return false;
-    if (!std::isfinite(r->magnitude) || !(r->magnitude > 0.0)) return false;
+    if (!good_magnitude(r->magnitude)) return false;
     for (int i = 0; i < r->dims / 2; ++i)
         if (!std::isfinite(r->frequency[i])) return false;
     return true;
+}
+
+int check_most(int B, int T, int H, int Hk) {
+    if (H + static_cast<int64_t>(Hk) > kMaxHeads) return set_error(DT_ERR_UNSUPPORTED, "%d and %d heads are more than %d", H, Hk, kMaxHeads);
+    // (a launch's threads and the indices of groups of heads stay within 31 bits)
+    if (static_cast<int64_t>(B) * T > 0x7fffff) return set_error(DT_ERR_UNSUPPORTED, "B*T = %lld tokens", (long long)B * T);
+    return DT_OK;
 }
 
 int check_call(const dt_ctx* ctx, const Call& c) {
@@ -440,10 +452,8 @@ int check_call(const dt_ctx* ctx, const Call& c) {
     if (!good_rotary(c.rot))
         return set_error(DT_ERR_INVALID_ARG, "the rotary needs dims of 16, 32 .. %d, a known layout, a magnitude above 0 and finite frequencies", DT_HEAD_DIM);
     if (c.D != DT_HEAD_DIM) return set_error(DT_ERR_UNSUPPORTED, "head_dim D=%d, kernels are built for D=%d", c.D, DT_HEAD_DIM);
-    if (c.H + static_cast<int64_t>(c.Hk) > kMaxHeads) return set_error(DT_ERR_UNSUPPORTED, "%d and %d heads are more than %d", c.H, c.Hk, kMaxHeads);
+    DT_TRY(check_most(c.B, c.T, c.H, c.Hk));
     if (c.Hk > 0 && (!c.k || !c.ok)) return set_error(DT_ERR_INVALID_ARG, "k and its output must be non-NULL with Hk=%d", c.Hk);
-    // (a launch's threads and the indices of groups of heads stay within 31 bits)
-    if (static_cast<int64_t>(c.B) * c.T > 0x7fffff) return set_error(DT_ERR_UNSUPPORTED, "B*T = %lld tokens", (long long)c.B * c.T);
     if (c.Hk > 0 && (c.oq == c.ok || c.oq == c.k || c.ok == c.q || (c.xk && (c.oq == c.xk || c.ok == c.xq))))
         return set_error(DT_ERR_INVALID_ARG, "an output is the other's, or the other's input");
     if (c.dtype != DT_FP32_EXACT && c.dtype != DT_BF16) return set_error(DT_ERR_INVALID_ARG, "unknown dtype %d", c.dtype);
@@ -470,6 +480,12 @@ int check_call(const dt_ctx* ctx, const Call& c) {
         if (c.positions && reinterpret_cast<uintptr_t>(c.positions) % c.pos_bytes)
             return set_error(DT_ERR_INVALID_ARG, "positions are not aligned to their size");
     }
+    // (rows that another row's results would overwrite)
+    const auto shifted = [&](const void* in, const void* out, int64_t ld_in, int64_t ld_out) { return in == out && ld_in != ld_out; };
+    if (static_cast<int64_t>(c.B) * c.T > 1 &&
+        (shifted(c.q, c.oq, c.ldq, c.ldoq) || (xs && shifted(c.xq, c.oq, c.ldxq, c.ldoq)) ||
+         (c.Hk > 0 && (shifted(c.k, c.ok, c.ldk, c.ldok) || (xs && shifted(c.xk, c.ok, c.ldxk, c.ldok))))))
+        return set_error(DT_ERR_INVALID_ARG, "an output in its input's place needs the same stride");
     if (!ctx) return set_error(DT_ERR_INVALID_ARG, "ctx is NULL");
     return DT_OK;
 }
@@ -643,7 +659,7 @@ int dt_rotary_init(dt_rotary* rot, int dims, int layout, double theta, int scali
     if (scaling == DT_ROTARY_RAMP &&
         (!std::isfinite(original_length) || !(original_length > 0.0) || !std::isfinite(low) || !std::isfinite(high) || !(low < high)))
         return set_error(DT_ERR_INVALID_ARG, "a ramp needs an original length above 0 and low < high, got %g, %g, %g", original_length, low, high);
-    if (!std::isfinite(magnitude) || !(magnitude > 0.0)) return set_error(DT_ERR_INVALID_ARG, "magnitude %g must be finite and above 0", magnitude);
+    if (!good_magnitude(magnitude)) return set_error(DT_ERR_INVALID_ARG, "magnitude %g must be above 0 and within fp32's range", magnitude);
     if (scaling == DT_ROTARY_THETA) theta *= std::pow(factor, static_cast<double>(dims) / (dims - 2));
     if (!std::isfinite(theta)) return set_error(DT_ERR_INVALID_ARG, "theta times the factor's power is past the range");
     *rot = {};
@@ -695,6 +711,7 @@ int dt_head_norm_rotary_bwd_workspace(int B, int T, int H, int Hk, int64_t* byte
     clear_error();
     if (!bytes) return set_error(DT_ERR_INVALID_ARG, "bytes is NULL");
     if (B < 1 || T < 1 || H < 1 || Hk < 0) return set_error(DT_ERR_INVALID_ARG, "B=%d, T=%d, H=%d must be >= 1, Hk=%d >= 0", B, T, H, Hk);
+    DT_TRY(check_most(B, T, H, Hk));
     Call c{};
     c.B = B, c.T = T, c.H = H, c.Hk = Hk, c.norm = c.backward = true;
     *bytes = workspace_bytes(c);

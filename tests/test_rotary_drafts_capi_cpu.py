@@ -50,7 +50,7 @@ def test_frequencies(dims, scaling):
     (dict(dims=0), "dims"), (dict(dims=24), "dims"), (dict(dims=144), "dims"), (dict(layout=2), "layout"), (dict(scaling=4), "scaling"),
     (dict(theta=1.0), "theta"), (dict(theta=float("inf")), "theta"), (dict(scaling=1, factor=0.5), "factor"),
     (dict(scaling=3, factor=2.0, low=4.0, high=4.0), "low"), (dict(scaling=3, factor=2.0, original=0.0), "ramp"),
-    (dict(magnitude=0.0), "magnitude"), (dict(magnitude=float("nan")), "magnitude"), (dict(scaling=2, factor=1e300), "theta"),
+    (dict(magnitude=0.0), "magnitude"), (dict(magnitude=float("nan")), "magnitude"), (dict(magnitude=1e39), "magnitude"), (dict(magnitude=1e-60), "magnitude"), (dict(scaling=2, factor=1e300), "theta"),
 ])
 def test_rotary_init_refusals(kw, msg):
     refused(rotary(**kw)[1], C.DT_ERR_INVALID_ARG, msg)
@@ -71,7 +71,8 @@ ROWS = [
     (dict(B=257, starts=FAKE), C.DT_ERR_UNSUPPORTED, "starts"), (dict(ldq=255), C.DT_ERR_INVALID_ARG, "strides"),
     (dict(ldko=127), C.DT_ERR_INVALID_ARG, "strides"), (dict(ldq=260), C.DT_ERR_INVALID_ARG, "aligned"), (dict(oq=FAKE + 8), C.DT_ERR_INVALID_ARG, "aligned"),
     (dict(ok=FAKE), C.DT_ERR_INVALID_ARG, "the other"), (dict(oq=FAKE + 4096, ok=FAKE + 8192), C.DT_ERR_INVALID_ARG, "the other"),
-    ({}, C.DT_ERR_INVALID_ARG, "ctx is NULL"),
+    (dict(ldqo=264), C.DT_ERR_INVALID_ARG, "same stride"), (dict(ldko=136), C.DT_ERR_INVALID_ARG, "same stride"),
+    (dict(T=1, ldqo=264), C.DT_ERR_INVALID_ARG, "ctx is NULL"), ({}, C.DT_ERR_INVALID_ARG, "ctx is NULL"),
 ]
 
 
@@ -109,7 +110,7 @@ def test_head_norm_fwd(kw, code, msg):
 
 @pytest.mark.parametrize("kw,code,msg", [r for r in ROWS if "ctx" not in r[2]] + [
     (dict(xq=None), C.DT_ERR_INVALID_ARG, "forward's inputs"), (dict(dwk=None), C.DT_ERR_INVALID_ARG, "forward's inputs"),
-    (dict(ldxk=64), C.DT_ERR_INVALID_ARG, "strides"), (dict(xk=FAKE + 8), C.DT_ERR_INVALID_ARG, "aligned"), ({}, C.DT_ERR_INVALID_ARG, "ctx is NULL")])
+    (dict(ldxk=64), C.DT_ERR_INVALID_ARG, "strides"), (dict(ldxk=136), C.DT_ERR_INVALID_ARG, "same stride"), (dict(xk=FAKE + 8), C.DT_ERR_INVALID_ARG, "aligned"), ({}, C.DT_ERR_INVALID_ARG, "ctx is NULL")])
 def test_head_norm_bwd(kw, code, msg):
     r, _ = rotary()
     a = dict(ctx=None, q=FAKE, k=FAKE + 4096, xq=FAKE, xk=FAKE + 4096, wq=FAKE, wk=FAKE + 4096, oq=FAKE, ok=FAKE + 4096, dwq=FAKE, dwk=FAKE, B=1, T=4, H=2, Hk=1, D=128, ldq=256,
@@ -125,6 +126,8 @@ def test_workspaces():
     assert lib.dt_head_norm_rotary_bwd_workspace(1, 1, 1, 0, ctypes.byref(n)) == C.DT_OK and n.value >= 512
     refused(lib.dt_head_norm_rotary_bwd_workspace(1, 1, 1, 0, None), C.DT_ERR_INVALID_ARG, "bytes")
     refused(lib.dt_head_norm_rotary_bwd_workspace(0, 1, 1, 0, ctypes.byref(n)), C.DT_ERR_INVALID_ARG, "B=0")
+    refused(lib.dt_head_norm_rotary_bwd_workspace(1, 1, 2**31 - 1, 2**31 - 1, ctypes.byref(n)), C.DT_ERR_UNSUPPORTED, "heads")
+    refused(lib.dt_head_norm_rotary_bwd_workspace(1 << 20, 1 << 20, 16, 16, ctypes.byref(n)), C.DT_ERR_UNSUPPORTED, "tokens")
     assert lib.dt_verify_drafts_workspace(4, 3, 1000, 1, 1.0, ctypes.byref(n)) == C.DT_OK and n.value > 0
     refused(lib.dt_verify_drafts_workspace(4, 3, 1000, 1, 1.0, None), C.DT_ERR_INVALID_ARG, "bytes")
     refused(lib.dt_verify_drafts_workspace(4, 65, 1000, 1, 1.0, ctypes.byref(n)), C.DT_ERR_UNSUPPORTED, "K=65")
