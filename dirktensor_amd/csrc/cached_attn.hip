@@ -1001,10 +1001,7 @@ int64_t make_plan(CachedAttnArgs& a, AttnRows& rows, int format, bool f32, bool*
         }
         a.head_places = static_cast<int>(cum);
         const int64_t places = cum * heads;
-        // (in 4 bits, whose steps are short, shares of two steps at least where there is no prefix: 12 x 5 tokens of 1500, 4 key/value heads,
-        // 16.9 us with one and 16.4 with two, 16 of 2000 12.4 and 12.0; ragged ones behind 2777 22.8 and 24.5)
-        const int64_t least = format == DT_KV_FP4 && a.pre_len == 0 ? 2 : 1;
-        a.own_groups = static_cast<int>(std::min<int64_t>((all + least - 1) / least, slots));
+        a.own_groups = static_cast<int>(std::min<int64_t>(all, slots));
         a.share = static_cast<int>(places / a.own_groups);
         a.extra = static_cast<int>(places % a.own_groups);
         own_parts = std::min(longest, (longest - 1) / a.share + 2);
