@@ -37,7 +37,7 @@
 // In fp32 mode q (divided by 2^9 times the power of two below its row's largest magnitude) and P are split into three bf16 values
 // each, whose sum is the fp32 value, so every product is exact in the 32-bit accumulation.
 // In 4 bits a row has four scales, so they go into the operands: the conversion to bf16 multiplies by a power of two, exactly, and
-// no score or probability is. In exact mode the parts of q and P meet the same operands.
+// no score or probability is multiplied. In exact mode the parts of q and P meet the same operands.
 
 #include "kv_cache.h"
 
