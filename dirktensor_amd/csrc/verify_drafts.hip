@@ -22,11 +22,12 @@
 // where the weights' total is itself small (below kSmall) does that count: that workgroup then sums the weights again. Last it finds
 // the chunk that the border lies in, and in it the token.
 //
-// Measured at 100352 logits a row: 4 drafts of one sequence in fp32, 3.6 MB, 4.2 and 9.9 us in the two kernels: chains of one batch and of
-// one chunk, with about seven trips to memory in the second (the partial sums, the drafts' logits, a chunk, its sums out, the count, the sums
-// in, the border's chunk). Up to 5 drafts of 64 sequences in bf16, 72 MB, 20.7 and 26: the first is 3.5 TB/s, with 26 cycles a value and wave
-// for the powers and sums beside the reads; the second has 64 bits' arithmetic, 110 cycles a value and wave, 9 us were it spread evenly
-// (13 to 25 workgroups a batch row all take 24 to 27), and the chain around it.
+// Measured at 100352 logits a row: 4 drafts of one sequence in fp32, 3.6 MB, 4.3 and 9.7 us in the two kernels: chains of one batch and of
+// one chunk, with six trips to memory in the second (the partial sums, a chunk, its sums out, the count, the sums in, the border's chunk),
+// of about 2.2, 2.5, 0.6, 1.1 and 1.5 us with what is done between them. Up to 5 drafts of 64 sequences in bf16, 72 MB, 20.9 and 20: the first
+// is 3.5 TB/s, with 26 cycles a value and wave for the powers and sums beside the reads; the second has the 64 bits' arithmetic, 7 us a
+// workgroup at the median and 12 where a CU's workgroups all have two rows, and the chain around it. (26 with powers by a longer
+// polynomial in place of the table, the next chunk's loads not ahead, the counts in one cache line and 13 workgroups a batch row.)
 
 #include "dt_internal.h"
 
@@ -50,7 +51,8 @@ constexpr int kChunk = 512;                   // values that a wave of the secon
 constexpr int kWhole = 4096;                  // of a batch of the first kernel, all threads
 constexpr int kMinSegment = 2048;             // values of a segment of the first kernel at least
 constexpr int kFill = 2048;                   // workgroups that the first kernel aims at, eight a CU
-constexpr int kDrawFill = 1024;               // and the second
+constexpr int kDrawFill = 1280;               // and the second: five a CU (64 sequences 21.4 us, 23.2 with 832, 22.5 with 1600)
+constexpr int kCountStride = 64;              // a cache line and more: counts of one line wait for each other
 constexpr double kSmall = 1e-4;
 constexpr double kLog2e = 1.4426950408889634074;
 constexpr double kLn2 = 0.69314718055994530942;
@@ -66,9 +68,10 @@ struct VerifyArgs {
     int32_t* accepted;    // [B]
     int32_t* tokens;      // [B, K + 1]
     float* logprob;       // [B, K + 1]
-    int32_t* count;       // [B]: workgroups of the second kernel that are done
+    int32_t* count;       // [B], kCountStride apart: workgroups of the second kernel that are done
     double2* part;        // [B][rows][segments]: the largest logit, and the sum of 2^(c (x - it))
     float2* best;         // [B][K + 1][segments] at T = 0: the largest logit, its index (as bits)
+    float* picked;        // [B][rows]: the draft's logit
     double* sums;         // [B][chunks][4]: sum of p' - ratio q' and of q' where that is above 0, of p' and of q'
     int64_t ldb_x, ldt_x, ldb_y, ldt_y;
     double c;             // log2(e) / T
@@ -96,6 +99,33 @@ __device__ __forceinline__ double exp2_64(double t) {
     v = fma(v, f, 0x1.62e42fef84cf0p-1);
     v = fma(v, f, 1.0);
     return __builtin_amdgcn_ldexp(v, static_cast<int>(__double_as_longlong(m)));
+}
+
+// The same for many of them, 2^(t/32): 2^(j/32) from a table, and 2^(f/32) on [-1/2, 1/2] as its interpolation in five points, to 10^-13.
+// The table lies in LDS, an entry in two of the 64 banks, so lanes read it without conflicts.
+constexpr int kRoots = 32;
+__device__ const double kRootsOfTwo[kRoots] = {
+    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
+    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
+    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
+    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
+    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0,
+};
+__device__ __forceinline__ double exp2_64(double t, const double* roots) {
+    t = fmax(t, kRoots * kFar);
+    constexpr double kMagic = 6755399441055744.0;
+    const double m = t + kMagic;
+    const double f = t - (m - kMagic);
+    const int i = static_cast<int>(__double_as_longlong(m));
+    double v = 0x1.3b2b1bee88b09p-27;
+    v = fma(v, f, 0x1.c6b167e571135p-20);
+    v = fma(v, f, 0x1.ebfbdff8131c3p-13);
+    v = fma(v, f, 0x1.62e42fef6d01ap-6);
+    v = fma(v, f, 1.0);
+    return __builtin_amdgcn_ldexp(v * roots[i & (kRoots - 1)], i >> 5);
 }
 
 template <bool kBf16>
@@ -153,6 +183,16 @@ __device__ __forceinline__ double sum16(double x) {
     x += moved<0x141, 0xf>(x);  // mirrored within 8
     return x + moved<0x140, 0xf>(x);  // and within 16
 }
+template <int kCtrl>
+__device__ __forceinline__ float moved32(float x) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, static_cast<int>(__float_as_uint(x)), kCtrl, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float max16(float x) {
+    x = fmaxf(x, moved32<0xb1>(x));
+    x = fmaxf(x, moved32<0x4e>(x));
+    x = fmaxf(x, moved32<0x141>(x));
+    return fmaxf(x, moved32<0x140>(x));
+}
 template <bool k32>
 __device__ __forceinline__ double sum_halves(double x) {
     const uint64_t u = static_cast<uint64_t>(__double_as_longlong(x));
@@ -163,6 +203,16 @@ __device__ __forceinline__ double sum_halves(double x) {
     return join(lo[0], hi[0]) + join(lo[1], hi[1]);
 }
 __device__ __forceinline__ double sum_wave(double x) { return sum_halves<true>(sum_halves<false>(sum16(x))); }
+// Four sums at once, sum (lane & 1) * 2 + (lane >> 1 & 1) in each lane: two steps leave a lane one of four values, which the others then add up.
+__device__ __forceinline__ double sum_four(double a, double b, double c, double d) {
+    const int lane = threadIdx.x;
+    const bool odd = lane & 1, upper = lane & 2;
+    const double x = (odd ? c : a) + moved<0xb1, 0xf>(odd ? a : c), y = (odd ? d : b) + moved<0xb1, 0xf>(odd ? b : d);
+    double s = (upper ? y : x) + moved<0x4e, 0xf>(upper ? x : y);
+    s += moved<0x124, 0xf>(s);  // from 4 lanes away, of 16
+    s += moved<0x128, 0xf>(s);  // and from 8
+    return sum_halves<true>(sum_halves<false>(s));
+}
 // the sums of a lane's and all lower lanes' values
 __device__ __forceinline__ double scan_wave(double x) {
     x += moved<0x111, 0xf>(x);
@@ -199,6 +249,14 @@ template <int kRows>
 __device__ __forceinline__ float power(const VerifyArgs<kRows>& a, float d) {
     return __builtin_amdgcn_exp2f(fmaf(d, a.c_hi, d * a.c_lo));
 }
+template <int kRows>
+__device__ __forceinline__ int draft_of(const VerifyArgs<kRows>& a, int b, int i) {
+    const int64_t at = static_cast<int64_t>(b) * a.K + i;
+    if (a.tok_bytes == 4) return static_cast<const int32_t*>(a.drafts)[at];
+    const int64_t t = static_cast<const int64_t*>(a.drafts)[at];
+    return t < 0 || t >= a.V ? -1 : static_cast<int>(t);
+}
+
 template <bool kBf16, bool kGreedy, int kRows>
 __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs<kRows> a) {
     constexpr int P = kPer<kBf16>;
@@ -207,9 +265,15 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs<kRows>
     __shared__ float red_top[kWaves];
     __shared__ float2 red_best[kWaves];
     const int b = blockIdx.z, r = blockIdx.y, seg = blockIdx.x, n = a.n[b];
-    if (seg == 0 && r == 0 && threadIdx.x == 0) a.count[b] = 0;
+    if (seg == 0 && r == 0 && threadIdx.x == 0) a.count[b * kCountStride] = 0;
     if (r <= a.K ? r > n : r - a.K - 1 >= n) return;
     const void* row = row_of<kBf16>(a, b, r);
+    // the draft's logit, for the second kernel (in the last segment, which may be the shortest)
+    const int i = r <= a.K ? r : r - a.K - 1;
+    if (seg == a.segments - 1 && threadIdx.x == kThreads - 1 && i < n) {
+        const int draft = draft_of(a, b, i);
+        a.picked[b * a.rows + r] = draft >= 0 && draft < a.V ? load_one<kBf16>(row, draft) : 0.0f;
+    }
     const int from = seg * a.segment, end = min(a.V, from + a.segment);
     float top = kLowest, best = -__builtin_huge_valf();
     double sum = 0.0;
@@ -297,14 +361,6 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs<kRows>
     }
 }
 
-template <int kRows>
-__device__ __forceinline__ int draft_of(const VerifyArgs<kRows>& a, int b, int i) {
-    const int64_t at = static_cast<int64_t>(b) * a.K + i;
-    if (a.tok_bytes == 4) return static_cast<const int32_t*>(a.drafts)[at];
-    const int64_t t = static_cast<const int64_t*>(a.drafts)[at];
-    return t < 0 || t >= a.V ? -1 : static_cast<int>(t);
-}
-
 // sums before a thread's own of the workgroup's, in the threads' order, and of all
 __device__ __forceinline__ double scan(double v, double (&red)[kWaves], double* all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -339,46 +395,64 @@ __device__ __forceinline__ double log2_64(double s) {
     return y + (s * exp2_64(-y) - 1.0) * kLog2e;
 }
 
-// 8 values of a row as four pairs of words, which the loops over them take one by one: a kernel that runs once through its code waits
-// for the code, too, so these loops are not unrolled.
+// 8 values of a row as they lie there, which the loop over them takes in four pairs: a kernel that runs once through its code waits for the
+// code, too, so that loop is not unrolled.
+template <bool kBf16>
 struct Eight {
-    uint32_t lo[4], hi[4];
-    template <bool kBf16>
-    __device__ __forceinline__ void load(const void* row, int at, int end) {
-        constexpr int P = kPer<kBf16>;
+    static constexpr int kWords = kBf16 ? 4 : 8;
+    uint32_t w[kWords];
+    // whole: none of the wave's values lie behind the row's end (these are -inf). Nothing is done with a whole one's words here, so the
+    // loads stay under way.
+    __device__ __forceinline__ void load(const void* row, int at, int end, bool whole) {
+        if (whole) {
 #pragma unroll
-        for (int i = 0; i < 8 / P; ++i) {
-            float x[P];
-            load_piece<kBf16>(row, at + i * P, end, x);
+            for (int i = 0; i < kWords / 4; ++i) {
+                u32x4 v;
+                if constexpr (kBf16) v = *reinterpret_cast<const u32x4_at2*>(static_cast<const uint16_t*>(row) + at);
+                else v = *reinterpret_cast<const u32x4_at4*>(static_cast<const float*>(row) + at + 4 * i);
 #pragma unroll
-            for (int j = 0; j < P / 2; ++j) {
-                lo[i * P / 2 + j] = __float_as_uint(x[2 * j]);
-                hi[i * P / 2 + j] = __float_as_uint(x[2 * j + 1]);
+                for (int j = 0; j < 4; ++j) w[4 * i + j] = v[j];
             }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            const auto one = [&](int to) {
+                const float v = load_one<kBf16>(row, min(to, end - 1));
+                return to < end ? __float_as_uint(v) : 0xff800000u;
+            };
+            if constexpr (kBf16) w[i] = one(at + 2 * i) >> 16 | one(at + 2 * i + 1);
+            else w[i] = one(at + i);
         }
     }
     __device__ __forceinline__ void hide(int i) {  // value i, if it is one of these, has no weight
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (2 * j == i) lo[j] = 0xff800000u;
-            if (2 * j + 1 == i) hi[j] = 0xff800000u;
-        }
+        for (int j = 0; j < 8; ++j)
+            if (j == i) {
+                if constexpr (kBf16) w[j >> 1] = j & 1 ? (w[j >> 1] & 0xffffu) | 0xff800000u : (w[j >> 1] & 0xffff0000u) | 0xff80u;
+                else w[j] = 0xff800000u;
+            }
     }
+    __device__ __forceinline__ float lo() const { return __uint_as_float(kBf16 ? w[0] << 16 : w[0]); }
+    __device__ __forceinline__ float hi() const { return __uint_as_float(kBf16 ? w[0] & 0xffff0000u : w[1]); }
     __device__ __forceinline__ void next() {
+        constexpr int kBy = kBf16 ? 1 : 2;
 #pragma unroll
-        for (int i = 0; i < 3; ++i) lo[i] = lo[i + 1], hi[i] = hi[i + 1];
+        for (int i = 0; i + kBy < kWords; ++i) w[i] = w[i + kBy];
     }
 };
 // The two rows that the weights come from: p', and q', 0 where there is no such row.
 struct Rows {
     const void *px, *qx;  // qx: or NULL
-    double p_top, q_top, c;
-    __device__ __forceinline__ double p(float x) const { return exp2_64((static_cast<double>(x) - p_top) * c); }
-    __device__ __forceinline__ double q(float y) const { return qx ? exp2_64((static_cast<double>(y) - q_top) * c) : 0.0; }
+    const double* roots;
+    double p_top, q_top, c;  // c: times kRoots
+    __device__ __forceinline__ double p(float x) const { return exp2_64((static_cast<double>(x) - p_top) * c, roots); }
+    __device__ __forceinline__ double q(float y) const { return exp2_64((static_cast<double>(y) - q_top) * c, roots); }
 };
 
 template <bool kBf16, bool kGreedy, int kRows>
 __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs<kRows> a) {
+    __shared__ double roots[kRoots];
     __shared__ float tops[kMaxRows];
     __shared__ double sums[kMaxRows];  // NaN of a row that has none
     __shared__ int best[kMaxDrafts + 1];
@@ -398,49 +472,59 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs<kRows>
     if (tid < n) {
         draft = draft_of(a, b, tid);
         if (!kGreedy) u = a.u[static_cast<int64_t>(b) * (K + 1) + tid];
-        if (draft >= 0 && draft < V) {
-            x = load_one<kBf16>(row_of<kBf16>(a, b, tid), draft);
-            if (a.y) y = load_one<kBf16>(row_of<kBf16>(a, b, K + 1 + tid), draft);
-        }
+        x = a.picked[b * a.rows + tid];
+        if (a.y) y = a.picked[b * a.rows + K + 1 + tid];
     }
+    if (!kGreedy && tid >= kThreads - kRoots) roots[tid - (kThreads - kRoots)] = kRootsOfTwo[tid - (kThreads - kRoots)];
     const double last_u = kGreedy ? 0.0 : a.u[static_cast<int64_t>(b) * (K + 1) + K];
     const int own_rows = n + 1 + (a.y ? n : 0);
     for (int i = tid >> 4; i < own_rows; i += kThreads / 16) {
         const int r = i <= n ? i : K + 1 + (i - n - 1);
         const double2* p = a.part + (static_cast<int64_t>(b) * a.rows + r) * a.segments;
-        // (four of a lane's segments at a time; rows of more are brought from one largest logit to the next)
-        float top = kLowest, most = -__builtin_huge_valf();
-        double sum = 0.0;
+        // The largest logit first (four of a lane's segments at a time; rows of more are read twice), then the sum brought to it.
+        float to = kLowest, most = -__builtin_huge_valf();
+        double2 v[4];
         int most_at = 0;
-        for (int s = tid & 15; s < a.segments; s += 64) {
-            double2 v[4];
-            float to = top;
+        const auto load = [&](int first) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                v[j] = s + 16 * j < a.segments ? p[s + 16 * j] : make_double2(kLowest, 0.0);
-                if (kGreedy && s + 16 * j < a.segments) {
-                    const float2 w = a.best[(static_cast<int64_t>(b) * (K + 1) + r) * a.segments + s + 16 * j];
+                const int s = first + 16 * j + (tid & 15);
+                v[j] = s < a.segments ? p[s] : make_double2(kLowest, 0.0);
+            }
+        };
+        for (int first = 0; first < a.segments; first += 64) {
+            load(first);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to = fmaxf(to, static_cast<float>(v[j].x));
+            if constexpr (kGreedy) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int s = first + 16 * j + (tid & 15);
+                    if (s >= a.segments) continue;
+                    const float2 w = a.best[(static_cast<int64_t>(b) * (K + 1) + r) * a.segments + s];
                     if (w.x > most) most = w.x, most_at = __float_as_int(w.y);
                 }
             }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) to = fmaxf(to, static_cast<float>(v[j].x));
-            sum *= exp2_64((static_cast<double>(top) - to) * a.c);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) sum += v[j].y * exp2_64((v[j].x - to) * a.c);
-            top = to;
         }
-        float to = top;
+        to = max16(to);
+        if constexpr (kGreedy) {
 #pragma unroll
-        for (int o = 8; o >= 1; o >>= 1) {
-            to = fmaxf(to, __shfl_xor(to, o, 16));
-            if (kGreedy) {
+            for (int o = 8; o >= 1; o >>= 1) {
                 const float t2 = __shfl_xor(most, o, 16);
                 const int a2 = __shfl_xor(most_at, o, 16);
                 if (t2 > most || (t2 == most && a2 < most_at)) most = t2, most_at = a2;
             }
         }
-        sum *= exp2_64((static_cast<double>(top) - to) * a.c);
+        double sum = 0.0;
+#pragma unroll 1
+        for (int first = 0; first < a.segments; first += 64) {
+            if (a.segments > 64) load(first);
+#pragma unroll 1
+            for (int s = first; s < min(first + 64, a.segments); s += 16) {  // (not unrolled, as below)
+                sum += v[0].y * exp2_64((v[0].x - to) * a.c);
+                v[0] = v[1], v[1] = v[2], v[2] = v[3];
+            }
+        }
         sum = sum16(sum);
         if ((tid & 15) == 0) {
             tops[r] = to;
@@ -476,7 +560,7 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs<kRows>
         token = best[acc];
     } else {
         const bool refused = acc < n;
-        Rows rows{row_of<kBf16>(a, b, acc), refused && a.y ? row_of<kBf16>(a, b, K + 1 + acc) : nullptr, tops[acc], 0.0, a.c};
+        Rows rows{row_of<kBf16>(a, b, acc), refused && a.y ? row_of<kBf16>(a, b, K + 1 + acc) : nullptr, roots, tops[acc], 0.0, kRoots * a.c};
         const int skip = refused && !a.y ? drafts[acc] : -1;  // a draft that nothing was drawn for
         double near = 0.0;  // the ratio of the rows' sums, to 32 bits
         if (rows.qx) {
@@ -489,46 +573,61 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs<kRows>
         double h[4], p_sum = 0.0, ratio = 0.0, weight, before, all;
         int first = blockIdx.x * kWaves + wave, step = gridDim.x * kWaves;
         for (bool again = false; !none; again = true) {
-#pragma unroll 1
-            for (int chunk = first; chunk < a.chunks; chunk += step) {
-                double pw = 0.0, qw = 0.0, pa = 0.0, qa = 0.0;
-#pragma unroll 1
-                for (int at = chunk * a.runs * kChunk + lane * 8, end = at + a.runs * kChunk; at < end; at += kChunk) {
-                    Eight x, y;
-                    x.load<kBf16>(rows.px, at, V);
-                    if (rows.qx) y.load<kBf16>(rows.qx, at, V);
-                    if (static_cast<uint32_t>(skip - (at - lane * 8)) < kChunk) x.hide(skip - at);  // (the same for the whole wave)
+            // Runs of kChunk values, the next one's under way while one is summed; behind a chunk's last its sums go out.
+            Eight<kBf16> px{}, qx{};
+            double pw = 0.0, qw = 0.0, pa = 0.0, qa = 0.0;
+            int chunk = first, run = 0, at = 0, of = 0;
+            bool more = false, last = false;
+#pragma clang loop unroll(disable)
+            do {
+                Eight<kBf16> x = px, y = qx;
+                const bool some = more, ends = last;
+                const int base = at, to = of;
+                more = chunk < a.chunks;
+                if (more) {
+                    of = chunk;
+                    at = (chunk * a.runs + run) * kChunk;
+                    last = ++run == a.runs;
+                    if (last) run = 0, chunk += step;
+                    const bool whole = at + kChunk <= V;
+                    px.load(rows.px, at + lane * 8, V, whole);
+                    if (rows.qx) qx.load(rows.qx, at + lane * 8, V, whole);
+                }
+                if (some) {
+                    if (static_cast<uint32_t>(skip - base) < kChunk) x.hide(skip - base - lane * 8);  // (the same for the whole wave)
 #pragma unroll 1
                     for (int i = 0; i < 4; ++i) {
+                        if (rows.qx) {  // (both branches whole: the powers' chains then go side by side)
+                            const double p[2] = {rows.p(x.lo()), rows.p(x.hi())}, q[2] = {rows.q(y.lo()), rows.q(y.hi())};
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const double p = rows.p(__uint_as_float(j ? x.hi[0] : x.lo[0]));
-                            pa += p;
-                            if (rows.qx) {
-                                const double q = rows.q(__uint_as_float(j ? y.hi[0] : y.lo[0])), w = fma(-near, q, p);
-                                qa += q;
+                            for (int j = 0; j < 2; ++j) {
+                                const double w = fma(-near, q[j], p[j]);
+                                pa += p[j];
+                                qa += q[j];
                                 pw += fmax(w, 0.0);
-                                qw += w > 0.0 ? q : 0.0;
+                                qw += w > 0.0 ? q[j] : 0.0;
                             }
+                            y.next();
+                        } else {
+                            const double p0 = rows.p(x.lo()), p1 = rows.p(x.hi());
+                            pa += p0;
+                            pa += p1;
                         }
-                        x.next(), y.next();
+                        x.next();
+                    }
+                    if (ends) {
+                        const double s = sum_four(pw, qw, pa, qa);
+                        if (lane < 4)  // through to the memory that all XCDs see
+                            __hip_atomic_store(out + to * 4 + (lane & 1) * 2 + (lane >> 1), s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                        pw = qw = pa = qa = 0.0;
                     }
                 }
-                const double mine[4] = {pw, qw, pa, qa};
-                double to = 0.0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const double s = sum_wave(mine[i]);
-                    if (lane == i) to = s;
-                }
-                if (lane < 4)  // through to the memory that all XCDs see
-                    __hip_atomic_store(out + chunk * 4 + lane, to, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
+            } while (more);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // and complete before they are counted
             __syncthreads();
             if (!again) {
                 if (tid == 0)
-                    sh_last = __hip_atomic_fetch_add(a.count + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == static_cast<int>(gridDim.x) - 1;
+                    sh_last = __hip_atomic_fetch_add(a.count + b * kCountStride, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == static_cast<int>(gridDim.x) - 1;
                 __syncthreads();
                 if (!sh_last) return;
             }
@@ -586,7 +685,7 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs<kRows>
                 }
 #pragma unroll
                 for (int i = 0; i < kOwn; ++i) {
-                    w[i] = fmax(fma(-ratio, rows.q(y[i]), rows.p(x[i])), 0.0);
+                    w[i] = rows.qx ? fmax(fma(-ratio, rows.q(y[i]), rows.p(x[i])), 0.0) : rows.p(x[i]);
                     mine += w[i];
                 }
                 double upto = before + scan(mine, red, &all);
@@ -644,7 +743,7 @@ struct Call {
 
 struct Plan {
     int rows, segments, segment, chunks, runs, groups;
-    int64_t part, best, sums, bytes;  // offsets
+    int64_t part, best, picked, sums, bytes;  // offsets
 };
 Plan make_plan(int B, int K, int V, bool drafts, bool greedy) {
     Plan p{};
@@ -658,12 +757,11 @@ Plan make_plan(int B, int K, int V, bool drafts, bool greedy) {
     p.runs = (V + kChunk * kThreads - 1) / (kChunk * kThreads);
     p.chunks = greedy ? 0 : (V + kChunk * p.runs - 1) / (kChunk * p.runs);
     // a chunk a wave, more where there would be many workgroups
-    const int groups = (p.chunks + kWaves - 1) / kWaves;
-    const int each = static_cast<int>((static_cast<int64_t>(groups) * B + kDrawFill - 1) / kDrawFill);
-    p.groups = greedy ? 1 : (groups + each - 1) / each;
-    p.part = (static_cast<int64_t>(B) * 4 + 255) / 256 * 256;
+    p.groups = greedy ? 1 : std::min((p.chunks + kWaves - 1) / kWaves, std::max(1, kDrawFill / B));
+    p.part = static_cast<int64_t>(B) * kCountStride * 4;
     p.best = p.part + rows * p.segments * 16;
-    p.sums = p.best + (greedy ? rows * p.segments * 8 : 0);
+    p.picked = p.best + (greedy ? rows * p.segments * 8 : 0);
+    p.sums = p.picked + (rows * 4 + 15) / 16 * 16;
     p.bytes = p.sums + static_cast<int64_t>(B) * p.chunks * 32;
     return p;
 }
@@ -692,6 +790,7 @@ int launch_rows(const Call& c, const Plan& p, void* ws, hipStream_t s) {
     a.count = reinterpret_cast<int32_t*>(w);
     a.part = reinterpret_cast<double2*>(w + p.part);
     a.best = reinterpret_cast<float2*>(w + p.best);
+    a.picked = reinterpret_cast<float*>(w + p.picked);
     a.sums = reinterpret_cast<double*>(w + p.sums);
     a.ldb_x = c.ldb_x, a.ldt_x = c.ldt_x, a.ldb_y = c.ldb_y, a.ldt_y = c.ldt_y;
     a.c = greedy ? kLog2e : kLog2e / c.temperature;
