@@ -158,12 +158,19 @@ def _rows_and_result(x, host, inplace):
     if inplace:
         if r is not x or (host and not x.flags.writeable):
             raise ValueError("in place needs writable rows of 128 contiguous values, 16-byte aligned, with one stride between tokens")
+        if not host and x.requires_grad and torch.is_grad_enabled():
+            raise ValueError("in place, a tensor that requires a gradient is only overwritten under torch.no_grad()")
         return r, p, ld, x, p, ld
     if host:
         o = np.empty(x.shape, x.dtype)
         return r, p, ld, o, o.ctypes.data, o.shape[2] * C.HEAD_DIM
     o = torch.empty_like(r) if r is x and x.is_contiguous() else x.new_empty(x.shape)
     return r, p, ld, o, o.data_ptr(), x.shape[2] * C.HEAD_DIM
+
+
+def _overwritten(*tensors):
+    """What torch's own operators do behind a write: a graph that saved such a tensor raises when it meets the new values."""
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
 
 
 _needs: dict = {}  # bytes by (B, T, H, Hk): they follow from these alone
@@ -203,6 +210,8 @@ def _rotate(Q, K, rot, positions, starts, inplace, ctx, backward):
     mem, stream = (C.DT_MEM_HOST, None) if host else (C.DT_MEM_DEVICE, _stream_of(Q))
     C.check(C.lib().dt_rotary_fwd(ctx.handle, q_p, k_p, oq_p, ok_p, B, T, H, Hk, C.HEAD_DIM, ldq, ldk, ldoq, ldok, pos_p, pos_bytes,
                                   starts_p, rot._p, backward, dtype, mem, stream))
+    if inplace and not host:
+        _overwritten(Q, K)
     return out_q, out_k
 
 
@@ -212,7 +221,8 @@ def rotary(Q, K, rot: Rotary, *, positions=None, starts=None, inplace: bool = Fa
 
     Token (b, t) is at ``positions`` [B, T] (int32 or int64, where the rows are), or at starts[b] + t for ``starts`` of B whole
     numbers on the host (such as a cache's lengths; a captured call repeats them), or at t. With ``inplace`` Q and K are
-    overwritten."""
+    overwritten (torch is told, as by its own operators; tensors that require a gradient are refused where gradients are
+    recorded)."""
     return _rotate(Q, K, rot, positions, starts, inplace, ctx, 0)
 
 
@@ -236,6 +246,8 @@ def head_norm_rotary(Q, K, q_weight, k_weight, rot: Rotary, *, positions=None, s
     mem, stream = (C.DT_MEM_HOST, None) if host else (C.DT_MEM_DEVICE, _stream_of(Q))
     C.check(C.lib().dt_head_norm_rotary_fwd(ctx.handle, q_p, k_p, wq_p, wk_p, oq_p, ok_p, B, T, H, Hk, C.HEAD_DIM, ldq, ldk, ldoq, ldok,
                                             pos_p, pos_bytes, starts_p, rot._p, float(eps), dtype, mem, stream))
+    if inplace and not host:
+        _overwritten(Q, K)
     return out_q, out_k
 
 
