@@ -259,7 +259,9 @@ __device__ __forceinline__ float inverse_rms(const Pieces<kBf16, kInter>& v, flo
     for (int i = 0; i < 16; ++i) ss += v.x[i / V::P][i % V::P] * v.x[i / V::P][i % V::P];
     ss = sum_head(ss);
     float inv = inverse_root(fmaf(ss, 1.0f / DT_HEAD_DIM, eps));
-    if (__any(ss == __builtin_huge_valf())) {  // squares past fp32's range: once more, of values 2^-70 times as large
+    // Squares past fp32's range: once more, of values 2^-70 times as large. (An infinity among the values has a sum that stays one, and
+    // the factor 0: finite values of its head become 0, as the formula has it, the infinity NaN.)
+    if (__any(ss == __builtin_huge_valf())) {
         float s2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -267,7 +269,7 @@ __device__ __forceinline__ float inverse_rms(const Pieces<kBf16, kInter>& v, flo
             s2 += y * y;
         }
         s2 = sum_head(s2);
-        if (ss == __builtin_huge_valf()) inv = 0x1p-70f * inverse_root(s2 * (1.0f / DT_HEAD_DIM));
+        if (ss == __builtin_huge_valf()) inv = s2 == __builtin_huge_valf() ? 0.0f : 0x1p-70f * inverse_root(s2 * (1.0f / DT_HEAD_DIM));
     }
     return inv;
 }

@@ -529,7 +529,7 @@ int dt_rotary_fwd(dt_ctx* ctx, const void* q, const void* k, void* q_out, void* 
 /*
  * RMSNorm of each head and the rotation in one pass (beside dt_qk_norm_rope_fwd, whose norm spans all heads):
  * x / sqrt(mean x^2 + eps) * weight over the head's 128 values, then as dt_rotary_fwd. q_weight, k_weight: [128] fp32,
- * eps >= 1e-30. Rounded to dtype once.
+ * eps >= 1e-30. Rounded to dtype once. A head with an infinity has NaN there (and in the value that turns with it) and zeros else.
  */
 int dt_head_norm_rotary_fwd(dt_ctx* ctx, const void* q, const void* k, const float* q_weight, const float* k_weight, void* q_out,
                             void* k_out, int B, int T, int H, int Hk, int D, int64_t ldq, int64_t ldk, int64_t ldq_out,
