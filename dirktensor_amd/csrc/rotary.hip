@@ -328,10 +328,11 @@ __global__ __launch_bounds__(kThreads) void head_norm_rotary_bwd_kernel(RotaryAr
         next_g.template load<kPast>(a.in[which], token * a.ld_in[which] + head * DT_HEAD_DIM, lane, a.octets);
         next_x.template load<kPast>(a.x[which], token * a.ld_x[which] + head * DT_HEAD_DIM, lane, a.octets);
     };
-    // token and part, row and place in the row: divided once
+    // token and part, row and place in the row: divided once (a step is 3072 tokens at most, and as many rows where these have one)
     const int item = block * kWaves + wave;
     int token = item / parts, part = item - token * parts, b = token / a.T, t = token - b * a.T;
     const int step_token = step / parts, step_part = step - step_token * parts;
+    const int step_b = step_token / a.T, step_t = step_token - step_b * a.T;
     if (token < a.tokens) fetch(token, part * span);
     while (token < a.tokens) {
         angles(a, position(a, b, t), lane, cs[wave]);
@@ -365,8 +366,9 @@ __global__ __launch_bounds__(kThreads) void head_norm_rotary_bwd_kernel(RotaryAr
                 for (int j = 0; j < V::P; ++j) g.x[i][j] = inv * (g.x[i][j] - x.x[i][j] * dot);
             if (have) g.template store<kPast>(a.out[which], token * a.ld_out[which] + head * DT_HEAD_DIM, lane, a.octets);
         }
-        t += next_token - token;
-        while (t >= a.T) t -= a.T, ++b;
+        b += step_b;
+        t += step_t + (next_token - token - step_token);  // (one more where the parts pass a token's end: less than 2 T)
+        if (t >= a.T) t -= a.T, ++b;
         token = next_token;
         part = next_part;
     }
