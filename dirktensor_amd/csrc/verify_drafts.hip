@@ -10,17 +10,19 @@
 //
 // A token is one side of a border or the other, and there are as many borders as tokens in the vocabulary: weights that are off by
 // 2^-24 of their probability would give another token about once in a few hundred calls. So the weights and their sums are held in
-// 64 bits, the terms to 10^-12. The rows' sums that decide on drafts (one border each) are of terms in 32 bits, summed in 64; the largest
+// 64 bits, the terms to 10^-13. The rows' sums that decide on drafts (one border each) are of terms in 32 bits, summed in 64; the largest
 // term is exact, so the log probability of a token that is almost certain is, too.
 //
 // Work: every row is read once for its sum (first kernel: a row in segments, as many as fill the CUs), and the one or two rows that the
 // weights come from once more, mostly from the caches (second kernel: each workgroup works out from the first kernel's sums which draft
 // was refused, and its waves take chunks of 512 values). The weights' difference needs the ratio of both rows' sums, which is known
-// to 2^-24 only: a chunk leaves sum (p' - ratio q') and sum q' over the values where that is above 0 (p', q': the powers, not divided
+// to 32 bits only: a chunk leaves sum (p' - ratio q') and sum q' over the values where that is above 0 (p', q': the powers, not divided
 // by their sums), and sum p' and sum q' over all; the last workgroup of a batch row to be done has the ratio to 64 bits then and
-// corrects the chunks' weights by it. A value whose sign the first ratio got wrong has a weight below 2^-23 of its probability; only
-// where the weights' total is itself small (below kSmall) does that count: that workgroup then sums the weights again. Last it finds
-// the chunk that the border lies in, and in it the token.
+// corrects the chunks' weights by it. What that leaves wrong are values whose sign the first ratio got wrong, each by the ratio's error
+// times q' at most. These are among the values with |p' - ratio q'| < kClose p' (the ratio's error, 10^-8 as a rule, is compared with
+// half of kClose), which are rare, and their q' are summed, too: where the ratio's error times that sum exceeds kSlack of the row's sum, as it
+// does for rows that agree almost everywhere, that workgroup sums the weights again. So a border is off by 2 10^-12 of the row's
+// sum at most, whatever the total of the weights. Last it finds the chunk that the border lies in, and in it the token.
 //
 // Measured at 100352 logits a row: 4 drafts of one sequence in fp32, 3.6 MB, 4.3 and 9.7 us in the two kernels: chains of one batch and of
 // one chunk, with six trips to memory in the second (the partial sums, a chunk, its sums out, the count, the sums in, the border's chunk),
@@ -53,7 +55,8 @@ constexpr int kMinSegment = 2048;             // values of a segment of the firs
 constexpr int kFill = 2048;                   // workgroups that the first kernel aims at, eight a CU
 constexpr int kDrawFill = 1280;               // and the second: five a CU (64 sequences 21.4 us, 23.2 with 832, 22.5 with 1600)
 constexpr int kCountStride = 64;              // a cache line and more: counts of one line wait for each other
-constexpr double kSmall = 1e-4;
+constexpr double kClose = 0x1p-20, kSlack = 0x1p-40;
+constexpr double kCloseUnit = 0x1p-38;        // of the sum of close values' q', which is 2^24 at most: whole units add up alike in any order
 constexpr double kLog2e = 1.4426950408889634074;
 constexpr double kLn2 = 0.69314718055994530942;
 constexpr double kFar = -1100.0;              // (2^-1100 is none of 64 bits)
@@ -68,7 +71,7 @@ struct VerifyArgs {
     int32_t* accepted;    // [B]
     int32_t* tokens;      // [B, K + 1]
     float* logprob;       // [B, K + 1]
-    int32_t* count;       // [B], kCountStride apart: workgroups of the second kernel that are done
+    int32_t* count;       // [B], kCountStride apart: workgroups of the second kernel that are done; 8 bytes behind it the sum of close values' q'
     double2* part;        // [B][rows][segments]: the largest logit, and the sum of 2^(c (x - it))
     float2* best;         // [B][K + 1][segments] at T = 0: the largest logit, its index (as bits)
     float* picked;        // [B][rows]: the draft's logit
@@ -83,7 +86,7 @@ struct VerifyArgs {
     uint8_t n[kRows];     // drafts of each batch row
 };
 
-// 2^t to 10^-12 for t <= 1000, 0 for t <= kFar (and for NaN). (2^f on [-1/2, 1/2] as its interpolation in nine Chebyshev points.)
+// 2^t to 1.1 10^-12 for t <= 1000, 0 for t <= kFar (and for NaN). (2^f on [-1/2, 1/2] as its interpolation in nine Chebyshev points.)
 __device__ __forceinline__ double exp2_64(double t) {
     t = fmax(t, kFar);
     constexpr double kMagic = 6755399441055744.0;  // 1.5 2^52: the sum's low bits are the nearest whole number
@@ -257,6 +260,11 @@ __device__ __forceinline__ int draft_of(const VerifyArgs<kRows>& a, int b, int i
     return t < 0 || t >= a.V ? -1 : static_cast<int>(t);
 }
 
+template <int kRows>
+__device__ __forceinline__ unsigned long long* close_sum(const VerifyArgs<kRows>& a, int b) {
+    return reinterpret_cast<unsigned long long*>(a.count + b * kCountStride + 2);
+}
+
 template <bool kBf16, bool kGreedy, int kRows>
 __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs<kRows> a) {
     constexpr int P = kPer<kBf16>;
@@ -265,7 +273,7 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs<kRows>
     __shared__ float red_top[kWaves];
     __shared__ float2 red_best[kWaves];
     const int b = blockIdx.z, r = blockIdx.y, seg = blockIdx.x, n = a.n[b];
-    if (seg == 0 && r == 0 && threadIdx.x == 0) a.count[b * kCountStride] = 0;
+    if (seg == 0 && r == 0 && threadIdx.x == 0) a.count[b * kCountStride] = 0, *close_sum(a, b) = 0;
     if (r <= a.K ? r > n : r - a.K - 1 >= n) return;
     const void* row = row_of<kBf16>(a, b, r);
     // the draft's logit, for the second kernel (in the last segment, which may be the shortest)
@@ -575,7 +583,7 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs<kRows>
         for (bool again = false; !none; again = true) {
             // Runs of kChunk values, the next one's under way while one is summed; behind a chunk's last its sums go out.
             Eight<kBf16> px{}, qx{};
-            double pw = 0.0, qw = 0.0, pa = 0.0, qa = 0.0;
+            double pw = 0.0, qw = 0.0, pa = 0.0, qa = 0.0, close = 0.0;
             int chunk = first, run = 0, at = 0, of = 0;
             bool more = false, last = false;
 #pragma clang loop unroll(disable)
@@ -599,6 +607,7 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs<kRows>
                     for (int i = 0; i < 4; ++i) {
                         if (rows.qx) {  // (both branches whole: the powers' chains then go side by side)
                             const double p[2] = {rows.p(x.lo()), rows.p(x.hi())}, q[2] = {rows.q(y.lo()), rows.q(y.hi())};
+                            bool some_close = false;
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
                                 const double w = fma(-near, q[j], p[j]);
@@ -606,7 +615,11 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs<kRows>
                                 qa += q[j];
                                 pw += fmax(w, 0.0);
                                 qw += w > 0.0 ? q[j] : 0.0;
+                                some_close |= fabs(w) < kClose * p[j];
                             }
+                            if (__builtin_expect(some_close, 0))
+#pragma unroll
+                                for (int j = 0; j < 2; ++j) close += fabs(fma(-near, q[j], p[j])) < kClose * p[j] ? q[j] : 0.0;
                             y.next();
                         } else {
                             const double p0 = rows.p(x.lo()), p1 = rows.p(x.hi());
@@ -620,6 +633,12 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs<kRows>
                         if (lane < 4)  // through to the memory that all XCDs see
                             __hip_atomic_store(out + to * 4 + (lane & 1) * 2 + (lane >> 1), s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                         pw = qw = pa = qa = 0.0;
+                        if (!again && __any(close > 0.0)) {
+                            const double c = ceil(sum_wave(close) / kCloseUnit);
+                            if (lane == 0)
+                                __hip_atomic_fetch_add(close_sum(a, b), static_cast<unsigned long long>(c), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                            close = 0.0;
+                        }
                     }
                 }
             } while (more);
@@ -640,7 +659,10 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs<kRows>
             }
             weight = rows.qx ? fmax(h[0] - (ratio - near) * h[1], 0.0) : h[2];
             before = scan(weight, red, &all);
-            if (again || !rows.qx || !(all < kSmall * p_sum)) break;  // (the same for the whole workgroup)
+            if (again || !rows.qx) break;  // (these are the same for the whole workgroup)
+            const double off = fabs(ratio - near);
+            const double close_q = static_cast<double>(__hip_atomic_load(close_sum(a, b), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) * kCloseUnit;
+            if (off <= 0.5 * kClose * near && off * close_q <= kSlack * p_sum) break;
             near = ratio;
             first = wave, step = kWaves;
         }
