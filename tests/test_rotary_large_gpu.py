@@ -6,7 +6,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_rotary_gpu import check, default_positions, grads64, norm64, randn, turn64
+from test_rotary_gpu import D, check, default_positions, grads64, norm64, randn, turn64
 from test_rotary_rows_gpu import dt, units, weights
 
 pytestmark = pytest.mark.gpu
