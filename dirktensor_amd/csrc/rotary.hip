@@ -76,12 +76,11 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 template <bool kBf16>
 constexpr int kPer = kBf16 ? 8 : 4;  // values of a piece
 
-// past the caches: nothing, what is written, or what is read too
-enum Past { kNothing, kWrites, kAll };
-template <bool kBf16, int kPast>
+// kPast: past the caches
+template <bool kBf16, bool kPast>
 __device__ __forceinline__ u32x4 load_piece(const void* p, int64_t at) {
     const u32x4* from = reinterpret_cast<const u32x4*>(static_cast<const char*>(p) + at * (kBf16 ? 2 : 4));
-    if constexpr (kPast == kAll) return __builtin_nontemporal_load(from);
+    if constexpr (kPast) return __builtin_nontemporal_load(from);
     else return *from;
 }
 template <bool kBf16>
@@ -96,7 +95,7 @@ __device__ __forceinline__ void open_piece(u32x4 w, float (&x)[kPer<kBf16>]) {
         }
     }
 }
-template <bool kBf16, int kPast>
+template <bool kBf16, bool kPast>
 __device__ __forceinline__ void store_piece(void* p, int64_t at, const float (&x)[kPer<kBf16>]) {
     u32x4 w;
     u32x4* to;
@@ -107,7 +106,7 @@ __device__ __forceinline__ void store_piece(void* p, int64_t at, const float (&x
         w = (u32x4){__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
         to = reinterpret_cast<u32x4*>(static_cast<float*>(p) + at);
     }
-    if constexpr (kPast != kNothing) __builtin_nontemporal_store(w, to);
+    if constexpr (kPast) __builtin_nontemporal_store(w, to);
     else *to = w;
 }
 
@@ -127,7 +126,7 @@ struct Pieces {
     // as loaded, and as values
     struct Raw {
         u32x4 w[kN];
-        template <int kPast>
+        template <bool kPast>
         __device__ __forceinline__ void load(const void* p, int64_t head, int lane, int octets) {
 #pragma unroll
             for (int i = 0; i < kN; ++i) w[i] = load_piece<kBf16, kPast>(p, head + offset(i, lane, octets));
@@ -137,13 +136,13 @@ struct Pieces {
 #pragma unroll
         for (int i = 0; i < kN; ++i) open_piece<kBf16>(r.w[i], x[i]);
     }
-    template <int kPast>
+    template <bool kPast>
     __device__ __forceinline__ void load(const void* p, int64_t head, int lane, int octets) {
         Raw r;
         r.template load<kPast>(p, head, lane, octets);
         open(r);
     }
-    template <int kPast>
+    template <bool kPast>
     __device__ __forceinline__ void store(void* p, int64_t head, int lane, int octets) const {
 #pragma unroll
         for (int i = 0; i < kN; ++i) store_piece<kBf16, kPast>(p, head + offset(i, lane, octets), x[i]);
@@ -275,7 +274,7 @@ __device__ __forceinline__ float inverse_rms(const Pieces<kBf16, kInter>& v, flo
 }
 
 // A workgroup takes a token, its waves the groups of eight heads: q's, then k's.
-template <bool kBf16, bool kNorm, bool kInter, int kPast, int kRows>
+template <bool kBf16, bool kNorm, bool kInter, bool kPast, int kRows>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs<kRows> a) {
     using V = Pieces<kBf16, kInter>;
     __shared__ float2 cs[kWaves][kPairs];
@@ -306,7 +305,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs<kRows> a) {
 
 // The norm's backward: workgroups of q (the first blocks[0]) or of k; their waves take tokens (or, where these are few, their groups of
 // eight heads) in turn, and each workgroup leaves the column sums of g n.
-template <bool kBf16, bool kInter, int kPast, int kRows>
+template <bool kBf16, bool kInter, bool kPast, int kRows>
 __global__ __launch_bounds__(kThreads) void head_norm_rotary_bwd_kernel(RotaryArgs<kRows> a) {
     using V = Pieces<kBf16, kInter>;
     __shared__ float2 cs[kWaves][kPairs];
@@ -529,10 +528,13 @@ int launch_rows(const Call& c, void* ws, hipStream_t s) {
     if (c.starts) std::copy_n(c.starts, c.B, a.start);
     const bool bf16 = c.dtype == DT_BF16, inter = c.rot->layout == DT_ROTARY_INTERLEAVED;
     const dim3 block(kThreads);
-    // Results that would push much else out of the last-level cache (256 MB) go past it, and so do reads of what cannot all be in it: 537
-    // MB moved in fp32 95 us, 88 with reads past it, too; 268 MB in bf16 with the norm 52 us, 49 with writes past it, 54 with reads as well.
+    // Rows that the last-level cache (256 MB) cannot hold go past it: 537 MB moved in fp32 95 us, 88 past it. Smaller results stay in it, as
+    // what follows reads them. With 67 to 168 MB stored past it the norm alone took 53.8 us in place of 55.9 (134 MB, calls back to back on
+    // new inputs) or 72 in place of 70 (one call); with an operator behind it that reads the results it was 91 in place of 86 (134 MB, elementwise),
+    // 175 in place of 171 (67 MB, attention), 42 in place of 39 (84 MB) and 62 in place of 63 (101 MB, keys into a cache); the gradient of
+    // 67 to 101 MB with such a reader 3 to 4 us more of 61 to 86.
     const int64_t bytes = static_cast<int64_t>(a.tokens) * (c.H + c.Hk) * DT_HEAD_DIM * (bf16 ? 2 : 4);
-    const int past = bytes * (c.norm && c.backward ? 2 : 1) >= kCacheBytes ? kAll : bytes >= kCacheBytes / 4 ? kWrites : kNothing;
+    const bool past = bytes * (c.norm && c.backward ? 2 : 1) >= kCacheBytes;
     constexpr std::true_type yes;
     constexpr std::false_type no;
     const auto choose = [&](bool which, auto go) {
@@ -542,9 +544,8 @@ int launch_rows(const Call& c, void* ws, hipStream_t s) {
     const int groups = (c.H + c.Hk + kGroupHeads - 1) / kGroupHeads;
     choose(bf16, [&](auto M) {
         choose(inter, [&](auto I) {
-            const auto go = [&](auto O) {
-                constexpr bool kM = decltype(M)::value, kI = decltype(I)::value;
-                constexpr int kO = decltype(O)::value;
+            choose(past, [&](auto O) {
+                constexpr bool kM = decltype(M)::value, kI = decltype(I)::value, kO = decltype(O)::value;
                 if (c.norm && c.backward) {
                     a.blocks[0] = bwd_blocks(a.tokens, c.H, c.Hk, &a.parts[0]);
                     a.blocks[1] = c.Hk > 0 ? bwd_blocks(a.tokens, c.Hk, c.H, &a.parts[1]) : 0;
@@ -555,10 +556,7 @@ int launch_rows(const Call& c, void* ws, hipStream_t s) {
                     if (c.norm) hipLaunchKernelGGL((rotary_kernel<kM, true, kI, kO, kRows>), grid, waves, 0, s, a);
                     else hipLaunchKernelGGL((rotary_kernel<kM, false, kI, kO, kRows>), grid, waves, 0, s, a);
                 }
-            };
-            if (past == kAll) go(std::integral_constant<int, kAll>());
-            else if (past == kWrites) go(std::integral_constant<int, kWrites>());
-            else go(std::integral_constant<int, kNothing>());
+            });
         });
     });
     DT_HIP_TRY(hipGetLastError());

@@ -12,8 +12,7 @@ from test_rotary_rows_gpu import dt, units, weights
 pytestmark = pytest.mark.gpu
 
 
-# (results of 105 MB, which are stored past the caches, of 180 MB, where the gradient's reads go past them as well, and of 300 MB, where
-# all do)
+# (results of 105 MB, which stay in the last-level cache, of 180 MB, where the gradient's rows go past it, and of 300 MB, where all do)
 @pytest.mark.parametrize("tdt", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("B,T,H,Hk", [(2, 5127, 16, 4), (1, 17579, 16, 4), (3, 9767, 16, 4)])
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
