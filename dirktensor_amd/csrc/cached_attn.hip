@@ -29,7 +29,7 @@
 // up to 512 behind a prefix of 4096 in int8 27 and 4.4 (94 MB, and the prefix's widening and products beside it); 12 by 5 tokens
 // behind 2777 in fp8 13 and 4; 4 of 1500 in exact mode, int8, 12 and 4. In 4 bits: 32 of 8192, 571 MB, 92 without a join (6.2 TB/s; about
 // 223 vector instructions a block, 64 % of what the CUs can issue); 12 by 5 tokens of 16 heads on 4 key/value heads, up to 1500 each behind 2777,
-// 18 and 5.7.
+// 18 and 5.7 (in exact mode 138 and 23 and 5.5); 64 and 256 tokens behind 131008 keys 545 and 631 TFLOP/s.
 //
 // Arithmetic: S^T = K Q^T with v_mfma_f32_16x16x32_bf16 on the held values, which bf16 holds exactly (int8 and e4m3
 // alike); the key's scale multiplies the 32-bit score. P times the value's scale is rounded to bf16 (at most half a step,
@@ -252,8 +252,8 @@ struct Block {
         to[0] = r[0].v;
         to[1] = r[1].v;
     }
-    // byte i of a key's scales as an exponent; the conversion takes nothing else of a scale (sign and fraction changed none of 2^20
-    // random ones' results)
+    // byte i of a key's scales as an exponent: the conversion's scale operand is a 32-bit number of which it takes the exponent field alone, so
+    // the neighbouring bytes that lie in its sign and fraction change nothing (nor did they in 2^20 random words)
     static __device__ __forceinline__ float scale4(uint32_t w, int i) { return __uint_as_float(i < 3 ? w << (23 - 8 * i) : w >> 1); }
     static __device__ __forceinline__ bf16x8 operand(const u32x4 (&w)[kPieces], int i) {
         if constexpr (kFormat == DT_KV_BF16) return __builtin_bit_cast(bf16x8, w[i]);

@@ -12,14 +12,15 @@
 // A wave takes eight heads of one token, eight lanes a head, 16 values a lane in pieces of 16 bytes: both values of each pair lie in one
 // lane, the eight lanes' pieces beside each other (in fp32 four pieces a lane; four of a lane behind each other took 198 in place of
 // 104 us past the caches), and a head's sums are three lane exchanges away. The angles need no table: lane i works out pair i's angle for the token, in 64
-// bits down to a fraction of a quarter turn, and the lanes read the pairs that they need from LDS; so positions are bounded by
-// nothing but their type, and nothing is fetched for them.
+// bits down to a fraction of a quarter turn, and the lanes read the pairs that they need from LDS; so no table bounds the positions, and
+// nothing is fetched for them. An angle is off by 3 2^-53 of itself and, from the fraction's rounding to 32 bits, by 2.4 10^-8 radians: the second is the
+// larger up to 2^26 radians, and near 2^53 nothing is left of a position's fraction.
 //
-// Measured, 128 values a head: 8 tokens of 16 heads, 4.1 us, a launch; 12 x 5 with the norm 4.2; 2 x 8192 tokens of 16 heads and 16 key
-// heads in fp32, 537 MB, 88 (6.1 TB/s, where the best copy reaches 6.25); 4 x 4096 of 16 and 16 in bf16 with the norm, 268 MB, 50 (5.4);
-// the gradients of 4 x 8192 of 16 and 4 in bf16, 503 MB, 90 (5.6) and 4.7 for the weights' columns; of 777 of 16 and 16 in fp32, 38 MB,
-// 11.6 and 3.8: a wave has one or two parts of a token there, so it is the chain of positions, angles, values, the columns' sums over lanes and
-// waves; adding the workgroups' columns in the same launch would need a counter that nothing has cleared.
+// Measured, 128 values a head: 8 tokens of 16 heads, 4.0 us, a launch; 12 x 5 with the norm 4.4; 2 x 8192 tokens of 16 heads and 16 key
+// heads in fp32, 537 MB, 88 (6.1 TB/s, where the best copy reaches 6.25); 4 x 4096 of 16 and 16 in bf16 with the norm, 268 MB, 54 (5.0);
+// the gradients of 4 x 8192 of 16 and 4 in bf16, 503 MB, 91 (5.5) and 5.0 for the weights' columns; of 777 of 16 and 16 in fp32, 38 MB,
+// 11.1 and 3.8: 1536 waves have one part of a token there and 18 of them a second one, so it is twice the chain of positions, angles, values, and the
+// columns' sums over lanes and waves; adding the workgroups' columns in the same launch would need a counter that nothing has cleared.
 
 #include "dt_internal.h"
 

@@ -490,7 +490,7 @@ int dt_token_logprobs_bwd(dt_ctx* ctx, const float* d_logprob, const float* d_en
  * layout of the pairs, scaled for contexts beyond the trained one): a pair (a, b) at position p goes to
  *   magnitude * (a cos t - b sin t),  magnitude * (b cos t + a sin t),  t = p * frequency[i],
  * and the values of the head from `dims` on stay. The angles are worked out in 64 bits where they are used: no table bounds the
- * positions, which may be negative.
+ * positions, which may be negative. An angle is off by 3 * 2^-53 of itself (less than fp32's rounding up to 2^26 radians) and 2.4e-8 radians.
  * dt_rotary is filled by dt_rotary_init, or by the caller:
  *   dims       values that turn, from the head's first on: 16, 32 .. 128
  *   layout     DT_ROTARY_HALF: pairs (d, d + dims/2); DT_ROTARY_INTERLEAVED: pairs (2i, 2i + 1)
