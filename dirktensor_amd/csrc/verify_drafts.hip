@@ -21,17 +21,18 @@
 // corrects the chunks' weights by it. What that leaves wrong are values whose sign the first ratio got wrong, each by the ratio's error
 // times q' at most. These are among the values with |p' - ratio q'| < kClose p' (the ratio's error, 10^-8 as a rule, is compared with
 // half of kClose), which are rare, and their q' are summed, too: where the ratio's error times that sum exceeds kSlack of the row's sum, as it
-// does for rows that agree almost everywhere, that workgroup sums the weights again (90 us more at 100352 values, 200 for 64 such rows). So a border is off by 3 10^-12 of the row's
-// sum at most, whatever the total of the weights. Last it finds the chunk that the border lies in, and in it the token.
+// does for rows that agree almost everywhere, that workgroup sums the weights again (90 us more at 100352 values, 200 for 64 such
+// rows). So a border is off by 3 10^-12 of the row's sum at most, whatever the total of the weights. Last it finds the chunk that the
+// border lies in, and in it the token.
 //
 // Measured at 100352 logits a row: 4 drafts of one sequence in fp32, 3.6 MB, 4.4 and 9.9 us in the two kernels: chains of one batch and of
 // one chunk, with six trips to memory in the second (the partial sums, a chunk, its sums out, the count, the sums in, the border's chunk),
 // of about 2.2, 2.5, 0.6, 1.1 and 1.5 us with what is done between them; without draft logits 3.9 and 8.5, at temperature 0 5.0 and 4.2. Up to 5
 // drafts of 64 sequences in bf16, 72 MB, 21.2 and 20.4: the first is 3.4 TB/s (where all have 5, 141 MB, 29.4, 4.8 TB/s: half of the workgroups
 // have nothing to do where drafts are ragged, and the others share the CUs unevenly), with 26 cycles a value and wave for the powers and
-// sums beside the reads; the second has the 64 bits' arithmetic, 7 us a
-// workgroup at the median and 12 where a CU's workgroups all have two rows, and the chain around it. (26 with powers by a longer
-// polynomial in place of the table, the next chunk's loads not ahead, the counts in one cache line and 13 workgroups a batch row.)
+// sums beside the reads; the second has the 64 bits' arithmetic, 7 us a workgroup at the median and 12 where a CU's workgroups all
+// have two rows, and the chain around it. (26 with powers by a longer polynomial in place of the table, the next chunk's loads not
+// ahead, the counts in one cache line and 13 workgroups a batch row.)
 // Without draft logits 18.8 and 15.0, without drafts 8.4 and 14.8, at temperature 0 22.8 and 4.0.
 
 #include "dt_internal.h"
